@@ -349,7 +349,7 @@ def _frequencies(rd, base, scaling):
     def where(turns):
         return rd * math.log(YARN["orig"] / (turns * 2 * math.pi)) / (2 * math.log(base))
 
-    low, high = max(math.floor(where(YARN["fast"])), 0), min(math.ceil(where(YARN["slow"])), rd // 2 - 1)
+    low, high = max(math.floor(where(YARN["fast"])), 0), min(math.ceil(where(YARN["slow"])), rd - 1)
     ramp = ((j - low) / max(high - low, 0.001)).clamp(0, 1)
     return f / YARN["factor"] * ramp + f * (1 - ramp)
 
@@ -475,7 +475,7 @@ def exact(case, seed):
             stretched = 0.0 if case["scaling"] == "none" else 1.0
             if case["scaling"] == "parts":           # the pair whose wave fits `turns` times into the original context
                 edge = [rd / 2 * math.log(YARN["orig"] / 2 / math.pi / turns) / math.log(base) for turns in (YARN["fast"], YARN["slow"])]
-                first, last = max(0, math.floor(edge[0])), min(rd // 2 - 1, math.ceil(edge[1]))
+                first, last = max(0, math.floor(edge[0])), min(rd - 1, math.ceil(edge[1]))
                 stretched = min(1.0, max(0.0, (j - first) / (last - first if last != first else 0.001)))
             f *= 1 - stretched + stretched / YARN["factor"]
             out[:, 2 * j], out[:, 2 * j + 1] = torch.cos(at * f) * _mscale(case["scaling"]), torch.sin(at * f) * _mscale(case["scaling"])
