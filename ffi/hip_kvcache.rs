@@ -426,6 +426,142 @@ launchers! {
         stream: *mut c_void,
     );
 
+    /// The rotation table of positions `first ..`: (cos, sin) pairs, the layout of
+    /// `CompFinish::freqs`, stretched as a whole or by parts for long contexts.
+    /// See `include/rivoli_kvcache.h` for the full contract.
+    launch_rope_table -> rivoli_rope_table, "rope_table" (
+        table: *mut f32,
+        first: i32,
+        n_positions: usize as i32,
+        rd: usize as i32,
+        base: f32,
+        factor: f32,
+        orig_ctx: usize as i32,
+        beta_fast: f32,
+        beta_slow: f32,
+        mscale: f32,
+        stream: *mut c_void,
+    );
+
+    /// Rotates `rd` values of every head by its token's row of the table, neighbouring pairs or
+    /// halves, in place or not.
+    /// See `include/rivoli_kvcache.h` for the full contract.
+    launch_rope_rows -> rivoli_rope_rows, "rope_rows" (
+        x: *const c_void,
+        out: *mut c_void,
+        table: *const f32,
+        positions: *const i32,
+        n_tokens: usize as i32,
+        n_heads: usize as i32,
+        rd: usize as i32,
+        n_positions: usize as i32,
+        x_token_stride: i64,
+        x_head_stride: i64,
+        out_token_stride: i64,
+        out_head_stride: i64,
+        half: i32,
+        bf16: i32,
+        bad_positions: *mut u32,
+        stream: *mut c_void,
+    );
+
+    /// Attention of a tree of drafted tokens over the fp8 pages: the cached prefix and, by mask,
+    /// the drafted rows behind it.
+    /// See `include/rivoli_kvcache.h` for the full contract.
+    launch_attend_tree_paged -> rivoli_mla_attend_tree_paged, "mla_attend_tree_paged" (
+        qabs: *const u16,
+        qrope: *const u16,
+        pool: *const u8,
+        block_table: *const i32,
+        ctx_lens: *const i32,
+        cu_nodes: *const i32,
+        masks: *const u32,
+        n_seqs: usize as i32,
+        H: usize as i32,
+        n_nodes: usize as i32,
+        max_nodes: usize as i32,
+        max_ctx: usize as i32,
+        max_blocks_per_seq: usize as i32,
+        kvl: usize as i32,
+        rope: usize as i32,
+        page_tokens: usize as i32,
+        n_pages: usize as i32,
+        scale: f32,
+        clat: *mut u16,
+        lse: *mut f32,
+        partial: *mut f32,
+        bad_rows: *mut u32,
+        stream: *mut c_void,
+    );
+
+    /// Which drafts stand, from the target's probabilities and given random numbers, and the token
+    /// after them.
+    /// See `include/rivoli_kvcache.h` for the full contract.
+    launch_draft_verify -> rivoli_draft_verify, "draft_verify" (
+        target_probs: *const c_void,
+        draft_probs: *const c_void,
+        tokens: *const i32,
+        parents: *const i32,
+        cu_nodes: *const i32,
+        uniforms: *const f32,
+        final_uniforms: *const f32,
+        n_seqs: usize as i32,
+        n_nodes: usize as i32,
+        max_nodes: usize as i32,
+        vocab: usize as i32,
+        target_stride: i64,
+        draft_stride: i64,
+        bf16: i32,
+        path: *mut i32,
+        n_path: *mut i32,
+        next_token: *mut i32,
+        workspace: *mut c_void,
+        bad_nodes: *mut u32,
+        stream: *mut c_void,
+    );
+
+    /// The kept drafts' rows moved to where the next step expects them, in every layer at once.
+    /// See `include/rivoli_kvcache.h` for the full contract.
+    launch_kv_commit_paged -> rivoli_kv_commit_paged, "kv_commit_paged" (
+        pool: *mut u8,
+        block_table: *const i32,
+        ctx_lens: *const i32,
+        path: *const i32,
+        n_path: *const i32,
+        n_seqs: usize as i32,
+        max_path: usize as i32,
+        max_blocks_per_seq: usize as i32,
+        width: usize as i32,
+        page_tokens: usize as i32,
+        n_pages: usize as i32,
+        n_layers: usize as i32,
+        layer_bytes: i64,
+        new_lens: *mut i32,
+        bad_rows: *mut u32,
+        stream: *mut c_void,
+    );
+
+    /// `launch_kv_commit_paged` for the paged index keys.
+    /// See `include/rivoli_kvcache.h` for the full contract.
+    launch_index_commit_paged -> rivoli_index_commit_paged, "index_commit_paged" (
+        kpool: *mut u16,
+        block_table: *const i32,
+        ctx_lens: *const i32,
+        path: *const i32,
+        n_path: *const i32,
+        n_seqs: usize as i32,
+        max_path: usize as i32,
+        max_blocks_per_seq: usize as i32,
+        hd: usize as i32,
+        page_tokens: usize as i32,
+        n_pages: usize as i32,
+        n_layers: usize as i32,
+        layer_keys: i64,
+        new_lens: *mut i32,
+        bad_rows: *mut u32,
+        stream: *mut c_void,
+    );
+
     /// Element codecs as launchers (what formats.hpp:42-57,99-106 and fwd.hip:20-45 are to the
     /// reference's kernels), for census tests of the device codecs on arbitrary inputs:
     /// e4m3_encode: out[i] = f32_to_e4m3(x[i]) (rule of crates/core/src/num.rs:128-152)
@@ -475,6 +611,8 @@ unsafe extern "C" {
     fn rivoli_mla_attend_paged_scratch_floats(n_seqs: i32, h: i32, max_rows: i32) -> usize;
     fn rivoli_sel_shape(win: i32, ratio: i32, index_topk: i32, seqlen: i32, start_pos: i32, rows: *mut i32, cols: *mut i32) -> i32;
     fn rivoli_gather_attn_scratch_floats(m: i32, h: i32, d: i32, topk: i32) -> usize;
+    fn rivoli_mla_attend_tree_paged_scratch_floats(n_seqs: i32, h: i32, n_nodes: i32, max_nodes: i32, max_ctx: i32) -> usize;
+    fn rivoli_draft_verify_workspace_bytes(n_seqs: i32, max_nodes: i32, vocab: i32) -> usize;
 }
 
 /// Bytes of one page: `page_tokens * width` codes followed by `page_tokens` f32 scales.
@@ -499,6 +637,20 @@ pub fn attend_paged_scratch_floats(n_seqs: usize, h: usize, max_rows: usize) -> 
 pub fn gather_attn_scratch_floats(m: usize, h: usize, d: usize, topk: usize) -> usize {
     // SAFETY: pure host function, no pointers.
     unsafe { rivoli_gather_attn_scratch_floats(m as i32, h as i32, d as i32, topk as i32) }
+}
+
+/// f32 elements of the partial buffer `launch_attend_tree_paged` wants for this shape (0 = none).
+pub fn attend_tree_paged_scratch_floats(n_seqs: usize, h: usize, n_nodes: usize, max_nodes: usize, max_ctx: usize) -> usize {
+    // SAFETY: pure host function, no pointers.
+    unsafe {
+        rivoli_mla_attend_tree_paged_scratch_floats(n_seqs as i32, h as i32, n_nodes as i32, max_nodes as i32, max_ctx as i32)
+    }
+}
+
+/// Bytes of the workspace `launch_draft_verify` wants for this shape (0 = none; nothing to be cleared).
+pub fn draft_verify_workspace_bytes(n_seqs: usize, max_nodes: usize, vocab: usize) -> usize {
+    // SAFETY: pure host function, no pointers.
+    unsafe { rivoli_draft_verify_workspace_bytes(n_seqs as i32, max_nodes as i32, vocab as i32) }
 }
 
 /// Rows and columns of a selection rectangle, or the guard code `Sel::shape` would refuse with.

@@ -501,6 +501,97 @@ int rivoli_kv_compress_prefill(const float* kv, const float* score, const float*
 int rivoli_kv_compress_decode(float* kv_state, float* score_state, const rivoli_comp_finish* ff,
                               const rivoli_comp_geom* pp, int start_pos, void* stream);
 
+/* ---- a step of drafted tokens over the paged cache: a sequence's drafted nodes are a tree in index order
+ * (a node's parent comes before it), node 0 the last token that is certain. Sequence s has the nodes
+ * cu_nodes[s] .. cu_nodes[s+1] of the step's n_nodes (exclusive prefix sum, n_seqs + 1 entries), node i's cache row is
+ * ctx_lens[s] + i (appended before the attention), its position ctx_lens[s] + depth. None of these calls
+ * has a counterpart in the reference. ---- */
+
+/* The rotation table: table[p - first][j] = (cos, sin)(p * f_j) * mscale for p in [first, first + n_positions) and
+ * j < rd / 2, [n_positions][rd] f32 - the layout of rivoli_comp_finish.freqs. f_j = base^(-2j/rd); `factor` stretches it
+ * for contexts longer than trained: every f_j / factor when orig_ctx is 0 (factor 1: none), else by parts - pairs that turn
+ * more than beta_fast times within orig_ctx positions keep f_j, those that turn less than beta_slow times have f_j /
+ * factor, a linear ramp over the pairs between (its ends floored and ceiled, within [0, rd - 1]). Angles
+ * are taken in 64 bits. Guards: 1001 null / non-positive sizes, negative first, base <= 1, factor <= 0, anything not finite, with
+ * orig_ctx betas not beta_fast > beta_slow > 0; 1002 rd > 1024 or positions past int; 1004 odd rd or table not 8-byte aligned. */
+int rivoli_rope_table(float* table, int first, int n_positions, int rd, float base, float factor, int orig_ctx,
+                      float beta_fast, float beta_slow, float mscale, void* stream);
+
+/* Rotates rd values of every head of every token by the table's row of its position: (x, y) -> (x c - y s, x s + y c), pairs
+ * being neighbours (half == 0: values 2j, 2j + 1) or half of rd apart (half != 0: j, j + rd / 2). Token t's head h has
+ * its rd values at x + t * x_token_stride + h * x_head_stride and gets them at out + t * out_token_stride + h * out_head_stride
+ * (strides in elements; for a part of a head pass the part's address); nothing else is written. bf16 != 0: bf16 values, else f32;
+ * products and sums in f32, rounded once. In place: out == x with the same strides; other overlaps are outside the contract. A token
+ * whose position is not in [0, n_positions) is left alone and counted in *bad_positions when non-null.
+ * 16-byte-aligned rows whose rd (half: rd / 2) values are whole 16 bytes go 16 bytes a lane, others a pair a lane.
+ * Guards: 1001 null / non-positive; 1002 rd > 1024 or more pieces than a launch has; 1004 odd rd, table not 8-byte aligned, rows not on an element. */
+int rivoli_rope_rows(const void* x, void* out, const float* table, const int* positions, int n_tokens, int n_heads,
+                     int rd, int n_positions, long long x_token_stride, long long x_head_stride,
+                     long long out_token_stride, long long out_head_stride, int half, int bf16,
+                     unsigned int* bad_positions, void* stream);
+
+/* Attention of the drafted nodes over the paged cache, in latent space (rivoli_mla_attend_paged's formula and cache, bf16 q
+ * and results): for node i of sequence s and head h
+ *   clat[n][h][:] = sum_t w_t L_t, w = softmax_t((qabs[n][h] . L_t + qrope[n][h] . R_t) * scale),  n = cu_nodes[s] + i,
+ * over the cached rows t < ctx_lens[s] and the drafted rows ctx_lens[s] + j that i sees: bit j & 31 of word j >> 5 of
+ * masks[n][(max_nodes + 31) / 32] (bits of nodes that the sequence does not have count for nothing), or j <= i when masks is
+ * null (a chain). lse[n][h] (nullable) = log of the softmax's denominator, natural logarithm. A node that attends nothing
+ * gets zeros and -inf. ctx_lens[s] <= max_ctx and at most max_nodes nodes a sequence: what is past either counts as absent.
+ * Rows of clat and lse of nodes that no sequence has are left as they were.
+ * Tokens whose page id is outside [0, n_pages) are left out and counted once in *bad_rows when non-null, tokens whose
+ * scale is not a positive number are left out. What a masked token's row holds (NaN codes, an infinite scale) reaches nobody.
+ * Weights are rounded to bf16 once for the value product; scores, statistics and sums are f32.
+ * `partial`: caller-owned scratch of rivoli_mla_attend_tree_paged_scratch_floats(same sizes) floats, null when that is 0;
+ * two calls in flight need one each. The plan depends on the sizes and the device-side lengths alone: equal calls give equal bits.
+ * Rows of 512 + 64 run on the matrix cores, other widths (kvl a multiple of 128 up to 512, rope a multiple of 8 up to 64) a slower kernel.
+ * Guards: 1001 null / non-positive (max_ctx may be 0), a null `partial` where one is needed; 1002 n_seqs > 65535, max_nodes > 4096, max_ctx >
+ * 2^31 - 8193, n_nodes * H > 2^30, H > 262140; 1004 widths as above, page_tokens % 4, qabs / qrope / pool / clat / partial not 16-byte aligned. */
+size_t rivoli_mla_attend_tree_paged_scratch_floats(int n_seqs, int H, int n_nodes, int max_nodes, int max_ctx);
+int rivoli_mla_attend_tree_paged(const unsigned short* qabs, const unsigned short* qrope, const unsigned char* pool,
+                                 const int* block_table, const int* ctx_lens, const int* cu_nodes,
+                                 const unsigned int* masks, int n_seqs, int H, int n_nodes, int max_nodes,
+                                 int max_ctx, int max_blocks_per_seq, int kvl, int rope, int page_tokens,
+                                 int n_pages, float scale, unsigned short* clat, float* lse, float* partial,
+                                 unsigned int* bad_rows, void* stream);
+
+/* Which drafts stand, from the target's probabilities and given random numbers in [0, 1), so that what is emitted is distributed
+ * as the target's. target_probs row n ([n_nodes][target_stride], f32 or with bf16 != 0 bf16) is the target's distribution AFTER node
+ * n over `vocab` tokens, draft_probs row n (nullable) the one that n's children were drawn from, independently; null: drafts
+ * were picked, not drawn. tokens[n], parents[n] (index within the sequence; node 0's is not read), uniforms[n]; final_uniforms[s].
+ * From cur = 0, w_0 = target row of cur, c_0 = 1, q = draft row of cur, over cur's children i in index order: accept i of token x when
+ * u_i * q(x) * c_k < w_k(x) (cur = i, k = 0), else w_{k+1} = max(w_k - c_k q, 0), c_{k+1} = its sum; picked drafts: q = 1 at x,
+ * w_{k+1} = w_k without x, c_{k+1} = c_k - w_k(x). After the last child next_token[s] = the first v whose running sum of w exceeds
+ * final_uniforms[s] times the whole (the last v with w > 0 when none does); a w that is all zero is replaced by cur's target row, and
+ * next_token is -1 when that is too. All in 64 bits. Probabilities that are NaN or negative count as 0, infinite ones as FLT_MAX; rows need not sum to one.
+ * path[s][max_nodes] = 0 and the accepted nodes in order, then -1; n_path[s] their number (0 and next_token -1 for a sequence
+ * without nodes). A node whose parent or token is out of range is nobody's child and counted in *bad_nodes when non-null.
+ * `workspace`: rivoli_draft_verify_workspace_bytes(n_seqs, max_nodes, vocab) bytes, 16-byte aligned, nothing to be cleared, null when
+ * that is 0; two calls in flight need one each. Guards: 1001 null / non-positive, a null workspace where one is needed; 1002 max_nodes > 1024, vocab > 2^21
+ * or above a stride; 1004 rows not on an element, workspace not 16-byte aligned. */
+size_t rivoli_draft_verify_workspace_bytes(int n_seqs, int max_nodes, int vocab);
+int rivoli_draft_verify(const void* target_probs, const void* draft_probs, const int* tokens, const int* parents,
+                        const int* cu_nodes, const float* uniforms, const float* final_uniforms, int n_seqs,
+                        int n_nodes, int max_nodes, int vocab, long long target_stride, long long draft_stride,
+                        int bf16, int* path, int* n_path, int* next_token, void* workspace,
+                        unsigned int* bad_nodes, void* stream);
+
+/* The kept rows where the next step expects them, in place: row ctx_lens[s] + path[s][k] (codes and scale, as they are) becomes row
+ * ctx_lens[s] + k for k < n_path[s] (path as rivoli_draft_verify writes it, [n_seqs][max_path]), in n_layers pools of the same layout
+ * that start layer_bytes apart (not read for one layer), as if all rows moved at once. new_lens[s] (nullable, not ctx_lens) = ctx_lens[s] +
+ * n_path[s]. An entry below k, or either of whose rows has no page, is left out and counted once in *bad_rows when non-null.
+ * Drafted rows must not share pages between sequences. Guards: 1001 null / non-positive, new_lens == ctx_lens; 1002 width > 1024,
+ * n_seqs > 65535, layer_bytes less than a pool; 1004 width % 16, page_tokens % 4, layer_bytes % 16, pool not 16-byte aligned.
+ * rivoli_index_commit_paged: the same for the paged index keys ([n_pages * page_tokens][hd] bf16, pools layer_keys keys apart);
+ * 1002 hd > 512, 1004 hd % 8. */
+int rivoli_kv_commit_paged(unsigned char* pool, const int* block_table, const int* ctx_lens, const int* path,
+                           const int* n_path, int n_seqs, int max_path, int max_blocks_per_seq, int width,
+                           int page_tokens, int n_pages, int n_layers, long long layer_bytes, int* new_lens,
+                           unsigned int* bad_rows, void* stream);
+int rivoli_index_commit_paged(unsigned short* kpool, const int* block_table, const int* ctx_lens, const int* path,
+                              const int* n_path, int n_seqs, int max_path, int max_blocks_per_seq, int hd,
+                              int page_tokens, int n_pages, int n_layers, long long layer_keys, int* new_lens,
+                              unsigned int* bad_rows, void* stream);
+
 /* Element codecs as launchers (what formats.hpp:42-57,99-106 and fwd.hip:20-45 are to the
  * reference's kernels), for census tests of the device codecs on arbitrary inputs:
  *   e4m3_encode: out[i] = f32_to_e4m3(x[i])            (rule of crates/core/src/num.rs:128-152)

@@ -69,6 +69,12 @@ RIVOLI_LAUNCHER(launch_sel_gather_scored, rivoli_sel_gather_scored, "sel_gather_
 RIVOLI_LAUNCHER(launch_kv_ring_write, rivoli_kv_ring_write, "kv_ring_write")
 RIVOLI_LAUNCHER(launch_gather_attn_shared_kv_bounded, rivoli_gather_attn_shared_kv_bounded, "gather_attn_shared_kv")
 RIVOLI_LAUNCHER(launch_gather_attn_shared_kv_split, rivoli_gather_attn_shared_kv_split, "gather_attn_shared_kv")
+RIVOLI_LAUNCHER(launch_rope_table, rivoli_rope_table, "rope_table")
+RIVOLI_LAUNCHER(launch_rope_rows, rivoli_rope_rows, "rope_rows")
+RIVOLI_LAUNCHER(launch_attend_tree_paged, rivoli_mla_attend_tree_paged, "mla_attend_tree_paged")
+RIVOLI_LAUNCHER(launch_draft_verify, rivoli_draft_verify, "draft_verify")
+RIVOLI_LAUNCHER(launch_kv_commit_paged, rivoli_kv_commit_paged, "kv_commit_paged")
+RIVOLI_LAUNCHER(launch_index_commit_paged, rivoli_index_commit_paged, "index_commit_paged")
 RIVOLI_LAUNCHER(launch_codec_e4m3_encode, rivoli_codec_e4m3_encode, "codec_e4m3_encode")
 RIVOLI_LAUNCHER(launch_codec_e4m3_dequant_bf16, rivoli_codec_e4m3_dequant_bf16, "codec_e4m3_dequant_bf16")
 RIVOLI_LAUNCHER(launch_codec_bf16_encode, rivoli_codec_bf16_encode, "codec_bf16_encode")
@@ -96,6 +102,13 @@ inline size_t attend_paged_scratch_floats(int n_seqs, int H, int max_rows) {
 inline size_t index_topk_workspace_bytes(int n_queries, int nt) { return rivoli_index_topk_workspace_bytes(n_queries, nt); }
 inline size_t gather_attn_scratch_floats(int m, int h, int d, int topk) {
     return rivoli_gather_attn_scratch_floats(m, h, d, topk);
+}
+
+inline size_t attend_tree_paged_scratch_floats(int n_seqs, int H, int n_nodes, int max_nodes, int max_ctx) {
+    return rivoli_mla_attend_tree_paged_scratch_floats(n_seqs, H, n_nodes, max_nodes, max_ctx);
+}
+inline size_t draft_verify_workspace_bytes(int n_seqs, int max_nodes, int vocab) {
+    return rivoli_draft_verify_workspace_bytes(n_seqs, max_nodes, vocab);
 }
 
 }  // namespace rivoli

@@ -76,6 +76,12 @@ _SIGNATURES = {
     "rivoli_kv_compress_deposit": [_VP] * 6 + [_I, _I, _VP],
     "rivoli_kv_compress_prefill": [_VP] * 5 + [_I, _VP],
     "rivoli_kv_compress_decode": [_VP] * 4 + [_I, _VP],
+    "rivoli_rope_table": [_VP] + [_I] * 3 + [_F, _F, _I, _F, _F, _F, _VP],
+    "rivoli_rope_rows": [_VP] * 4 + [_I] * 4 + [_LL] * 4 + [_I, _I, _VP, _VP],
+    "rivoli_mla_attend_tree_paged": [_VP] * 7 + [_I] * 10 + [_F] + [_VP] * 5,
+    "rivoli_draft_verify": [_VP] * 7 + [_I] * 4 + [_LL, _LL, _I] + [_VP] * 6,
+    "rivoli_kv_commit_paged": [_VP] * 5 + [_I] * 7 + [_LL] + [_VP] * 3,
+    "rivoli_index_commit_paged": [_VP] * 5 + [_I] * 7 + [_LL] + [_VP] * 3,
     "rivoli_codec_e4m3_encode": [_VP, _VP, _LL, _VP],
     "rivoli_codec_e4m3_dequant_bf16": [_VP, _F, _VP, _LL, _VP],
     "rivoli_codec_bf16_encode": [_VP, _VP, _LL, _VP],
@@ -89,6 +95,8 @@ _SIZE_SIGNATURES = {
     "rivoli_mla_attend_paged_scratch_floats": [_I, _I, _I],
     "rivoli_mla_attend_scratch_floats": [_I, _I],
     "rivoli_gather_attn_scratch_floats": [_I, _I, _I, _I],
+    "rivoli_mla_attend_tree_paged_scratch_floats": [_I] * 5,
+    "rivoli_draft_verify_workspace_bytes": [_I] * 3,
 }
 
 
@@ -121,9 +129,7 @@ def lib() -> C.CDLL:
 
 
 def exported_symbols() -> list[str]:
-    return sorted(list(_SIGNATURES) + ["rivoli_kv_page_bytes", "rivoli_index_topk_workspace_bytes",
-                                       "rivoli_mla_attend_paged_scratch_floats",
-                                       "rivoli_mla_attend_scratch_floats", "rivoli_gather_attn_scratch_floats"])
+    return sorted(list(_SIGNATURES) + list(_SIZE_SIGNATURES))
 
 
 def _p(x):
@@ -489,6 +495,74 @@ def launch_kv_compress_decode(kv_state, score_state, finish, geom, start_pos,
     ensure_hip_status(entry.rivoli_kv_compress_decode(
         kv_state, score_state, _addr_or_null(finish), _addr_or_null(geom), start_pos,
         stream), "kv_compress_decode")
+
+
+# ---- a step of drafted tokens ---------------------------------------------------------------
+
+def launch_rope_table(table, first, n_positions, rd, base, factor=1.0, orig_ctx=0, beta_fast=32.0, beta_slow=1.0,
+                      mscale=1.0, stream=NULL_STREAM) -> None:
+    """(cos, sin) pairs of positions first .. first + n_positions - 1, f32 [n_positions][rd]: what rope_rows
+    and the compressor's finish read. factor stretches the context: orig_ctx == 0 every frequency,
+    else by parts."""
+    ensure_hip_status(entry.rivoli_rope_table(table, first, n_positions, rd, base, factor, orig_ctx, beta_fast,
+                                              beta_slow, mscale, stream), "rope_table")
+
+
+def launch_rope_rows(x, out, table, positions, n_tokens, n_heads, rd, n_positions, x_token_stride, x_head_stride,
+                     out_token_stride, out_head_stride, half, bf16, bad_positions=None, stream=NULL_STREAM) -> None:
+    """Rotates rd values of every head (strides in elements; x and out may be the same rows) by its
+    token's row of the table; half: pairs are rd / 2 apart, else neighbours."""
+    ensure_hip_status(entry.rivoli_rope_rows(x, out, table, positions, n_tokens, n_heads, rd, n_positions,
+                                             x_token_stride, x_head_stride, out_token_stride, out_head_stride,
+                                             1 if half else 0, 1 if bf16 else 0, bad_positions, stream), "rope_rows")
+
+
+def mla_attend_tree_paged_scratch_floats(n_seqs: int, H: int, n_nodes: int, max_nodes: int, max_ctx: int) -> int:
+    return int(lib().rivoli_mla_attend_tree_paged_scratch_floats(n_seqs, H, n_nodes, max_nodes, max_ctx))
+
+
+def launch_mla_attend_tree_paged(qabs, qrope, pool, block_table, ctx_lens, cu_nodes, masks, n_seqs, H, n_nodes,
+                                 max_nodes, max_ctx, max_blocks_per_seq, kvl, rope, page_tokens, n_pages, scale, clat,
+                                 lse, partial, bad_rows=None, stream=NULL_STREAM) -> None:
+    """Attention of drafted nodes (bf16 q and results) over the cached rows and, by masks (None: a
+    chain), the drafted rows behind them."""
+    ensure_hip_status(entry.rivoli_mla_attend_tree_paged(
+        qabs, qrope, pool, block_table, ctx_lens, cu_nodes, masks, n_seqs, H, n_nodes, max_nodes, max_ctx,
+        max_blocks_per_seq, kvl, rope, page_tokens, n_pages, scale, clat, lse, partial, bad_rows, stream),
+        "mla_attend_tree_paged")
+
+
+def draft_verify_workspace_bytes(n_seqs: int, max_nodes: int, vocab: int) -> int:
+    return int(lib().rivoli_draft_verify_workspace_bytes(n_seqs, max_nodes, vocab))
+
+
+def launch_draft_verify(target_probs, draft_probs, tokens, parents, cu_nodes, uniforms, final_uniforms, n_seqs, n_nodes,
+                        max_nodes, vocab, target_stride, draft_stride, bf16, path, n_path, next_token, workspace=None,
+                        bad_nodes=None, stream=NULL_STREAM) -> None:
+    """Which drafted nodes stand (path, n_path: the root and the accepted ones) and the token that
+    follows them; draft_probs None: the drafts were picked, not drawn."""
+    ensure_hip_status(entry.rivoli_draft_verify(
+        target_probs, draft_probs, tokens, parents, cu_nodes, uniforms, final_uniforms, n_seqs, n_nodes, max_nodes,
+        vocab, target_stride, draft_stride, 1 if bf16 else 0, path, n_path, next_token, workspace, bad_nodes, stream),
+        "draft_verify")
+
+
+def launch_kv_commit_paged(pool, block_table, ctx_lens, path, n_path, n_seqs, max_path, max_blocks_per_seq, width,
+                           page_tokens, n_pages, n_layers=1, layer_bytes=0, new_lens=None, bad_rows=None,
+                           stream=NULL_STREAM) -> None:
+    """Moves the kept drafts' rows to ctx_lens[s] + 0, 1, ... in every layer's pool, in place."""
+    ensure_hip_status(entry.rivoli_kv_commit_paged(
+        pool, block_table, ctx_lens, path, n_path, n_seqs, max_path, max_blocks_per_seq, width, page_tokens, n_pages,
+        n_layers, layer_bytes, new_lens, bad_rows, stream), "kv_commit_paged")
+
+
+def launch_index_commit_paged(kpool, block_table, ctx_lens, path, n_path, n_seqs, max_path, max_blocks_per_seq, hd,
+                              page_tokens, n_pages, n_layers=1, layer_keys=0, new_lens=None, bad_rows=None,
+                              stream=NULL_STREAM) -> None:
+    """launch_kv_commit_paged for the paged index keys."""
+    ensure_hip_status(entry.rivoli_index_commit_paged(
+        kpool, block_table, ctx_lens, path, n_path, n_seqs, max_path, max_blocks_per_seq, hd, page_tokens, n_pages,
+        n_layers, layer_keys, new_lens, bad_rows, stream), "index_commit_paged")
 
 
 # ---- element codecs -----------------------------------------------------------------------
