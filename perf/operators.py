@@ -406,8 +406,8 @@ def _own_rope(s, hip):
     tokens, heads, rd, row = s["tokens"], s["heads"], s["rd"], s["head_row"]
     if "out" not in s:
         s["out"] = torch.empty(tokens, heads, rd, dtype=s["x"].dtype, device="cuda")
-    hip.launch_rope_rows(s["x"][..., row - rd:], s["out"], s["table"], s["positions"], tokens, heads, rd, s["table"].shape[0], row,
-                         heads * rd, rd, s["half"], s["bf16"], None, torch.cuda.current_stream())
+    hip.launch_rope_rows(s["x"][..., row - rd:], s["out"], s["table"], s["positions"], tokens, heads, rd, s["table"].shape[0],
+                         heads * row, row, heads * rd, rd, s["half"], s["bf16"], None, torch.cuda.current_stream())
     return s["out"]
 
 
