@@ -22,7 +22,8 @@ KERNELS = ["kv_append.hip", "kv_gather.hip", "index_topk.hip", "index_score.hip"
 # Matrix-instruction results in ordinary registers: the 8-bit attention kernel keeps its 128
 # accumulators there and its q terms in the accumulation registers (mla_attend_f8.hpp); the bf16
 # kernels of the same file time the same either way.
-EXTRA_FLAGS = {"mla_attend.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+EXTRA_FLAGS = {"mla_attend.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+               "mla_attend_tree.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 HOST_SOURCES = ["pagepool.cpp"]
 # Kernels whose design rests on "no scratch memory": source file -> (substring of the mangled
 # name, suffix of it) of each family. The 8-bit attention kernels and those of 16 and 32 heads a workgroup
@@ -33,7 +34,8 @@ HOST_SOURCES = ["pagepool.cpp"]
 NO_SCRATCH = {"mla_attend.hip": [("mla_attend_paged_kernel", "Lb1EEEvNS_10AttendArgsE"),
                                  ("mla_attend_heads16_kernel", "EEEvNS_10AttendArgsE"),
                                  ("mla_attend_few_kernel", "EEEvNS_10AttendArgsE"),
-                                 ("mla_attend_wide_kernel", "EEEvNS_10AttendArgsE")]}
+                                 ("mla_attend_wide_kernel", "EEEvNS_10AttendArgsE")],
+              "mla_attend_tree.hip": [("mla_attend_tree_kernel", "ENS_8TreeArgsE")]}
 
 
 def check_resources(k: str, report: str) -> None:

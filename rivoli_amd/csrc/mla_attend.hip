@@ -79,12 +79,6 @@ __device__ __forceinline__ int deal_item_of(long long t, long long n_items, long
     return (int)(((t + 1) * n_items - 1) / total);
 }
 
-// e4m3 codes -> bf16, exact: four codes (one dword) -> two dwords
-__device__ __forceinline__ void e4m3x4_to_bf16(uint32_t c, uint32_t& lo, uint32_t& hi) {
-    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, 1.0f, false));
-    hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, 1.0f, true));
-}
-
 struct AttendArgs {
     const float* qabs;            // [n_seqs][H][512]
     const float* qrope;           // [n_seqs][H][64]

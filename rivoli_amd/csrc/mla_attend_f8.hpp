@@ -39,7 +39,6 @@
 namespace rk {
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
-typedef int i32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kF8Threads = 256;              // four waves, one per SIMD, each with the full register file
 constexpr int kF8Waves = kF8Threads / kWave;

@@ -63,33 +63,6 @@ __device__ __forceinline__ float few_sum32(float x) {
     const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
-// Four bytes per lane from memory into LDS, as dma16.
-__device__ __forceinline__ void few_dma4(const void* src, lds_ptr<uint8_t> dst) {
-    const uint32_t base = (uint32_t)(uintptr_t)dst;
-    uint32_t keep;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %1, off\n\ts_mov_b32 m0, %0"
-                 : "=&s"(keep)
-                 : "v"(src), "s"(base)
-                 : "memory");
-}
-
-// A lane's four pieces of a row's codes, 128 bytes apart in memory and 1024 in LDS, and its fifth, of the roped codes, for the lanes of
-// `roped`. The instruction's offset counts in memory and in LDS, so m0 makes up the difference and the address is one. All lanes are here.
-__device__ __forceinline__ void few_dma_row(const uint8_t* src, lds_ptr<uint8_t> to, lds_ptr<uint8_t> to_rope, unsigned long long roped) {
-    const uint32_t base = (uint32_t)(uintptr_t)to, rope = (uint32_t)(uintptr_t)to_rope - 512u;
-    uint32_t keep;
-    unsigned long long all;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off\n\t"
-                 "s_add_u32 m0, m0, 896\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off offset:128\n\t"
-                 "s_add_u32 m0, m0, 896\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off offset:256\n\t"
-                 "s_add_u32 m0, m0, 896\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off offset:384\n\t"
-                 "s_mov_b32 m0, %4\n\ts_and_saveexec_b64 %1, %5\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off offset:512\n\t"
-                 "s_mov_b64 exec, %1\n\ts_mov_b32 m0, %0"
-                 : "=&s"(keep), "=&s"(all)
-                 : "v"(src), "s"(base), "s"(rope), "s"(roped)
-                 : "memory", "scc");
-}
-
 // A paged row, looked up: whether it is there, its codes and its scale (of one that is not there the first row's). bad: it should be.
 struct FewRow {
     bool there, bad;

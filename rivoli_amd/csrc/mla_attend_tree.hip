@@ -1,8 +1,10 @@
 // Attention of a tree of drafted tokens over the paged latent cache: node i of a sequence attends its ctx cached rows
 // and, of the drafted rows behind them, those its mask names. Launch-only.
 #include <climits>
+#include <type_traits>
 
 #include "attend_common.hpp"
+#include "mla_attend_tree_plan.hpp"
 
 namespace rk {
 
@@ -13,10 +15,13 @@ struct TreeArgs {
     const uint32_t* masks;  // [n_nodes][mask_words]; null: node i sees drafted rows 0 .. i
     int n_seqs, H, n_nodes, max_nodes, mask_words, max_ctx, max_blocks;
     int kvl, rope, row_w, page_tokens, n_pages;
+    int page_shift;         // log2(page_tokens) when that is a power of two, else -1
     size_t page_bytes;
     float qscale;           // softmax scale * log2(e)
     uint16_t* clat;
     float* lse;
+    int groups;             // TreePlan's
+    float* partial;
     unsigned int* bad_rows;
 };
 
@@ -138,9 +143,10 @@ __global__ __launch_bounds__(kTreeRowWaves* kWave) void mla_attend_tree_rowwise_
 
 }  // namespace rk
 
+#include "mla_attend_tree.hpp"
+
 extern "C" size_t rivoli_mla_attend_tree_paged_scratch_floats(int n_seqs, int H, int n_nodes, int max_nodes, int max_ctx) {
-    (void)n_seqs, (void)H, (void)n_nodes, (void)max_nodes, (void)max_ctx;
-    return 0;
+    return rk::tree_scratch_floats(rk::tree_plan(n_seqs, H, n_nodes, max_nodes, max_ctx));
 }
 
 extern "C" int rivoli_mla_attend_tree_paged(const unsigned short* qabs, const unsigned short* qrope,
@@ -158,11 +164,23 @@ extern "C" int rivoli_mla_attend_tree_paged(const unsigned short* qabs, const un
         return 1002;
     if (kvl % 128 != 0 || kvl > 512 || rope % 8 != 0 || rope > 64 || page_tokens % 4 != 0) return 1004;
     if (!rk::aligned16(qabs) || !rk::aligned16(qrope) || !rk::aligned16(pool) || !rk::aligned16(clat) || !rk::aligned16(partial)) return 1004;
+    const bool plain = kvl != 512 || rope != 64;
+    const rk::TreePlan plan = rk::tree_plan(n_seqs, H, n_nodes, max_nodes, max_ctx);
+    if (!plain && plan.groups && !partial) return 1001;
     const rk::TreeArgs a{qabs, qrope, pool, block_table, ctx_lens, cu_nodes, masks, n_seqs, H, n_nodes, max_nodes, (max_nodes + 31) / 32,
                          max_ctx, max_blocks_per_seq, kvl, rope, kvl + rope, page_tokens, n_pages,
-                         (size_t)page_tokens * (size_t)(kvl + rope + 4), scale * rk::kLog2e, clat, lse, bad_rows};
+                         (page_tokens & (page_tokens - 1)) == 0 ? __builtin_ctz((unsigned)page_tokens) : -1,
+                         (size_t)page_tokens * (size_t)(kvl + rope + 4), scale * rk::kLog2e, clat, lse, plan.groups, partial, bad_rows};
+    const hipStream_t st = (hipStream_t)stream;
     (void)hipGetLastError();
-    rk::launch_kernel(rk::mla_attend_tree_rowwise_kernel, dim3((unsigned)n_nodes, (unsigned)((H + rk::kTreeRowWaves - 1) / rk::kTreeRowWaves)),
-                      dim3(rk::kTreeRowWaves * rk::kWave), 0, (hipStream_t)stream, a);
+    if (plain) {
+        rk::launch_kernel(rk::mla_attend_tree_rowwise_kernel, dim3((unsigned)n_nodes, (unsigned)((H + rk::kTreeRowWaves - 1) / rk::kTreeRowWaves)),
+                          dim3(rk::kTreeRowWaves * rk::kWave), 0, st, a);
+        return rk::launch_status();
+    }
+    rk::launch_kernel(rk::mla_attend_tree_kernel, dim3((unsigned)(plan.groups ? plan.groups : plan.blocks)), dim3(rk::kTreeThreads), 0, st, a);
+    const int rc = rk::launch_status();
+    if (rc != 0 || plan.groups == 0) return rc;
+    rk::launch_kernel(rk::mla_attend_tree_merge_kernel, dim3((unsigned)plan.blocks, 32), dim3(256), 0, st, a);
     return rk::launch_status();
 }

@@ -1,0 +1,562 @@
+// Tree attention for rows of 512 + 64 codes on the matrix cores, included by mla_attend_tree.hip.
+//
+// What bounds it: of a tile of 64 tokens 64 rows of q need 64 * 64 * (576 + 512) multiply-adds, 2 176 cycles of a compute unit's four
+// matrix cores at 512 a cycle, while its LDS moves 128 bytes a cycle. So no operand may pass through LDS more often than
+// it must, and a fragment that is read has to serve many rows:
+//   - a workgroup is 64 rows (any mixture of nodes and heads of one sequence) and four waves, one per SIMD on the whole register file;
+//   - scores: wave (th, kh) has 32 tokens x all 64 rows over half of the dims, its q operands (144 registers) there for the whole
+//     call; every byte of a key is read out of LDS once for the workgroup. The two halves' partial scores meet through LDS: each wave sends
+//     32 rows and keeps the other 32, so that a score is handled once;
+//   - values: a wave has 128 of the 512 columns for all 64 rows (128 accumulators); every byte of a value is read once, by the transposing
+//     load, and only the weights (8 KB) are read by all four.
+// Codes go from memory into LDS as they are, three tiles in rotation, and become bf16 (exact) when an operand is read, once for the
+// workgroup. 32 x 32 matrix tiles: a fragment serves two of them.
+// An iteration has the scores of tile i + 1, then (partial scores having met at a barrier) the softmax of i + 1 under the values of
+// tile i; a second barrier ends it. The softmax's reference is that of the rows' first tile: weights are bf16 and sums f32, whose
+// exponents reach 2^127, so a row is rescaled only when a score grows by 2^kTreeGrow past its reference, which every wave learns
+// from a flag a tile late (regrow). Weights are rounded to bf16 once where they meet the values (2^-8 of a weight, at random, against the
+// 2^-8 of the rounded result); their sum, and so lse, is of the unrounded ones.
+#pragma once
+
+namespace rk {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int kTreeWaves = 4;
+constexpr int kTreeThreads = kTreeWaves * kWave;
+constexpr int kTreeBuffers = 3;
+// A tile in LDS: eight rows after the other, 4 KB each: their latent codes in four groups of 128 bytes, a group's rows next to each
+// other; then 1 KB of roped codes for each sixteen rows. A row's eight 16-byte pieces of a group change places by the row's number,
+// (row >> 1) & 7, so that reads of one piece of sixteen rows meet in no bank; of the roped codes the first eight rows of
+// sixteen have their four pieces in the lower 64 bytes then, the others in the upper.
+constexpr int kTreeRopeAt = 8 * 4096;
+constexpr int kTreeTileBytes = kTreeRopeAt + 4 * 1024;
+constexpr int kTreeSteps = 18;            // of 16 dims a wave: 16 of its 256 latent dims, two of its 32 roped ones
+constexpr float kTreeGrow = 24.0f;
+
+// A block of rows among a call's: its sequence, number and tiles, and the work units (tiles, or blocks where they are whole) before it.
+struct TreeBlock {
+    int seq, rb, blocks, tiles;
+    long long first;  // unit of the block's first tile
+};
+__device__ __forceinline__ void tree_units(const TreeArgs& a, int seq, int& blocks, int& tiles) {
+    blocks = tiles = 0;
+    if (seq >= a.n_seqs) return;
+    const TreeSeq s = tree_seq(a, seq);
+    blocks = (s.nodes * a.H + kTreeRows - 1) / kTreeRows;
+    tiles = (s.ctx + s.nodes + kTreeTokens - 1) / kTreeTokens;
+}
+__device__ __forceinline__ long long lanes_up_to(long long x) {
+#pragma unroll
+    for (int off = 1; off < kWave; off <<= 1) {
+        const long long y = __shfl_up(x, off, kWave);
+        if ((int)(threadIdx.x & 63) >= off) x += y;
+    }
+    return x;
+}
+__device__ __forceinline__ long long tree_total(const TreeArgs& a, bool whole) {
+    const int lane = threadIdx.x & 63;
+    long long sum = 0;
+    for (int s0 = 0; s0 < a.n_seqs; s0 += kWave) {
+        int blocks, tiles;
+        tree_units(a, s0 + lane, blocks, tiles);
+        sum += whole ? (long long)blocks : (long long)blocks * tiles;
+    }
+    return __shfl(lanes_up_to(sum), kWave - 1, kWave);
+}
+// The block that holds unit u of them.
+__device__ __forceinline__ TreeBlock tree_block(const TreeArgs& a, bool whole, long long u) {
+    const int lane = threadIdx.x & 63;
+    long long run = 0;
+    TreeBlock b{0, 0, 0, 0, 0};
+    for (int s0 = 0; s0 < a.n_seqs; s0 += kWave) {
+        int blocks, tiles;
+        tree_units(a, s0 + lane, blocks, tiles);
+        const long long mine = whole ? (long long)blocks : (long long)blocks * tiles;
+        const long long upto = run + lanes_up_to(mine);
+        const unsigned long long past = __builtin_amdgcn_ballot_w64(u < upto);
+        if (past) {
+            const int at = __builtin_ctzll(past);
+            const long long before = __shfl(upto - mine, at, kWave);
+            b.seq = s0 + at;
+            b.blocks = __builtin_amdgcn_readlane(blocks, at), b.tiles = __builtin_amdgcn_readlane(tiles, at);
+            const long long rel = u - before;
+            b.rb = (int)(whole ? rel : rel / b.tiles);
+            b.first = before + (whole ? (long long)b.rb : (long long)b.rb * b.tiles);
+            b.seq = __builtin_amdgcn_readfirstlane(b.seq), b.rb = __builtin_amdgcn_readfirstlane(b.rb);
+            return b;
+        }
+        run = __shfl(upto, kWave - 1, kWave);
+    }
+    b.seq = -1;
+    return b;
+}
+// The work items of a cut call: no more than have kTreeMinTiles each; eighths of them stay on one die.
+__device__ __forceinline__ int tree_items(const TreeArgs& a, long long total) {
+    const long long n = total / kTreeMinTiles;
+    int items = (int)(n < a.groups ? n : (long long)a.groups);
+    if (items > kTreeDies) items = items / kTreeDies * kTreeDies;
+    return max(items, 1);
+}
+__device__ __forceinline__ long long tree_item_lo(int item, int items, long long total) { return (long long)item * total / items; }
+__device__ __forceinline__ int tree_item_of(long long unit, int items, long long total) { return (int)(((unit + 1) * items - 1) / total); }
+
+struct TreeShared {
+    uint8_t tiles[kTreeBuffers * kTreeTileBytes];
+    f32x4 part[4][4][kWave];             // partial scores on their way to wave (th, kh)
+    uint8_t weights[2][kTreeRows * kTreeTokens * 2];  // by the tile's parity
+    float scale[kTreeBuffers][2][kTreeTokens];  // of a tile's tokens: the scale (0: not there), and times the softmax's
+    float top[2][kTreeRows], corr[kTreeRows], sum[2][kTreeRows], ref[kTreeRows];
+    int grown;                           // number of the tile some row of which outgrew its reference
+};
+static_assert(sizeof(TreeShared) <= 160 * 1024, "one workgroup per compute unit");
+
+// Codes that are no number as zeros.
+__device__ __forceinline__ uint32_t numbers_only(uint32_t c) {
+    const uint32_t nan = (((c & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
+    return c & ~(nan * 0xffu);
+}
+
+// Tiles [tile_lo, tile_hi) of rows 64 rb .. of a sequence. `whole`: they are all it has, results go out; else its record.
+// `number`: a count of the tiles the workgroup has had, for the flag.
+__device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeShared> sh, const TreeSeq& s, int seq, int rb, bool last_block,
+                                          int tile_lo, int tile_hi, bool whole, float* rec, int& number) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int half = lane >> 5, n32 = lane & 31;
+    const int th = wave & 1, kh = wave >> 1;  // its 32 tokens and its half of the dims, in the scores
+    const lds_ptr<uint8_t> tiles = (lds_ptr<uint8_t>)&sh->tiles[0];
+    const lds_ptr<uint8_t> weights = (lds_ptr<uint8_t>)&sh->weights[0][0];
+    const int rows = s.nodes * a.H;           // of the sequence
+    // what the block's last row may see: a chain's later nodes are nobody's business here
+    const int last_row = min(kTreeRows * rb + kTreeRows, rows) - 1;
+    const int len = a.masks ? s.ctx + s.nodes : s.ctx + last_row / a.H + 1;
+    const int n_tiles = min(tile_hi, (len + kTreeTokens - 1) / kTreeTokens) - tile_lo;
+
+    // ---- where a tile's rows are: eight lanes ask for rows 16 wave + 8 o + (lane >> 3) --------------------------
+    const int l8 = lane & 7, r8 = lane >> 3;
+    const int* const table = a.block_table + (size_t)seq * a.max_blocks;
+    auto block_of = [&](int t) -> unsigned { return a.page_shift >= 0 ? (unsigned)t >> a.page_shift : (unsigned)t / (unsigned)a.page_tokens; };
+    auto token_of = [&](int i, int o) -> int { return (tile_lo + i) * kTreeTokens + 16 * wave + 8 * o + r8; };
+    int page[2];
+    auto look_up = [&](int i) {
+#pragma unroll
+        for (int o = 0; o < 2; ++o) page[o] = table[min(block_of(min(token_of(i, o), len - 1)), (unsigned)a.max_blocks - 1)];
+    };
+    bool there[2];
+    float raw_scale[2];
+    auto scalar = [](lds_ptr<uint8_t> p) -> lds_ptr<uint8_t> {  // the transfers take their LDS base from a scalar register
+        return (lds_ptr<uint8_t>)(uintptr_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)p);
+    };
+    auto swap_of = [&](int o) -> int { return (4 * o + (r8 >> 1)) & 7; };
+    const unsigned long long roped[2] = {__builtin_amdgcn_ballot_w64((l8 ^ swap_of(0)) < 4), __builtin_amdgcn_ballot_w64((l8 ^ swap_of(1)) < 4)};
+    auto request = [&](int i, int buf) {  // of a tile looked up
+#pragma unroll
+        for (int o = 0; o < 2; ++o) {
+            const int t = token_of(i, o);
+            const unsigned blk = block_of(t);
+            unsigned off = a.page_shift >= 0 ? (unsigned)t & (unsigned)(a.page_tokens - 1) : (unsigned)t - blk * (unsigned)a.page_tokens;
+            const bool mine = t < len;
+            there[o] = mine & (blk < (unsigned)a.max_blocks) & ((unsigned)page[o] < (unsigned)a.n_pages);
+            if (a.bad_rows && last_block && __builtin_amdgcn_ballot_w64(mine & !there[o]) != 0) {
+                if (mine & !there[o] && l8 == 0) atomicAdd(a.bad_rows, 1u);
+            }
+            off = there[o] ? off : 0u;
+            const uint8_t* const base = a.pool + (unsigned long long)(unsigned)(there[o] ? page[o] : 0) * a.page_bytes;
+            raw_scale[o] = *reinterpret_cast<const float*>(base + (size_t)a.page_tokens * 576 + 4u * off);
+            few_dma_row(base + (size_t)off * 576u + 16 * (l8 ^ swap_of(o)), scalar(tiles + buf * kTreeTileBytes + (2 * wave + o) * 4096),
+                        scalar(tiles + buf * kTreeTileBytes + kTreeRopeAt + wave * 1024), roped[o]);
+        }
+    };
+    // The transfers asked for have landed: scales, and zeros for rows that are not there (codes must be finite, they meet
+    // a zero weight). A scale that is not a positive number cannot come from the append: such a row is not there.
+    auto arrived = [&](int buf) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int o = 0; o < 2; ++o) {
+            const bool ok = there[o] && raw_scale[o] > 0.0f;
+            if (__builtin_amdgcn_ballot_w64(!ok) != 0 && !ok) {
+                const lds_ptr<uint8_t> to = tiles + buf * kTreeTileBytes + 16 * lane;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) *(lds_ptr<u32x4>)(to + (2 * wave + o) * 4096 + 1024 * i) = u32x4{0, 0, 0, 0};
+                if ((l8 ^ swap_of(o)) < 4) *(lds_ptr<u32x4>)(to + kTreeRopeAt + wave * 1024) = u32x4{0, 0, 0, 0};
+            }
+            if (l8 == 0) {
+                const int row = 16 * wave + 8 * o + r8;
+                sh->scale[buf][0][row] = ok ? raw_scale[o] : 0.0f, sh->scale[buf][1][row] = ok ? raw_scale[o] * a.qscale : 0.0f;
+            }
+        }
+    };
+
+    f32x16 o[4][2];  // O^T: column tile c of 32, row block b: sixteen columns a lane, of row 32 b + n32
+    float m_ref = -INFINITY, l_sum = 0.0f, l_before = 0.0f;  // of row 32 kh + n32: the lane's share of the sum
+    const int own = 32 * kh + n32;
+    const int own_row = kTreeRows * rb + own;
+    const bool live = own_row < rows;
+    const int own_node = (live ? own_row : 0) / a.H;
+
+    if (n_tiles > 0) {
+        look_up(0);
+        u32x4 q[kTreeSteps][2];
+        request(0, 0);
+        if (n_tiles > 1) look_up(1);
+        // ---- the rows' operands: K-steps of 16 dims, eight a lane. Two K-steps share a 16-byte piece of codes. They live in the
+        // accumulation half of the register file, which the matrix instructions read as well; the sums are in the other --------
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const int r = kTreeRows * rb + 32 * b + n32;
+            const size_t at = (size_t)s.node0 * a.H + (r < rows ? r : 0);
+            u32x4 raw[kTreeSteps];
+#pragma unroll
+            for (int j = 0; j < kTreeSteps; ++j) {
+                const uint16_t* const src = j < 16 ? a.qabs + at * 512 + 256 * kh + 32 * (j >> 1) + 16 * half + 8 * (j & 1)
+                                                   : a.qrope + at * 64 + 32 * kh + 16 * half + 8 * (j & 1);
+                raw[j] = *reinterpret_cast<const u32x4*>(src);
+            }
+#pragma unroll
+            for (int j = 0; j < kTreeSteps; ++j)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    uint32_t kept;
+                    asm volatile("v_accvgpr_write_b32 %0, %1" : "=a"(kept) : "v"(raw[j][k]));
+                    q[j][b][k] = kept;
+                }
+        }
+
+        // ---- the lane's operands of a tile --------------------------------------------------------------------
+        const int k_swap = (n32 >> 1) & 7, e8 = (lane & 15) >> 1;
+        const int k_row = (4 * th + (n32 >> 3)) * 4096 + 2048 * kh + (n32 & 7) * 128;
+        const int k_rope = kTreeRopeAt + (2 * th + (n32 >> 4)) * 1024 + (n32 & 7) * 128 + 16 * ((2 * kh + half) ^ k_swap);
+        // values: of sixteen lanes, pair e addresses row 8 half + e of sixteen tokens; column tile c is piece c of group `wave` and, in
+        // the other sixteen lanes, c + 4, which keeps the two in different banks
+        const int v_swap = 4 * half + (e8 >> 1);
+        const int v_row = half * 4096 + wave * 1024 + e8 * 128 + 8 * (lane & 1);
+        const int v_piece = 4 * ((lane >> 4) & 1);
+        auto as_bf16 = [](uint32_t x, uint32_t y) -> bf16x8 {
+            uint32_t d0, d1, d2, d3;
+            e4m3x4_to_bf16(x, d0, d1), e4m3x4_to_bf16(y, d2, d3);
+            const u32x4 d = {d0, d1, d2, d3};
+            return __builtin_bit_cast(bf16x8, d);
+        };
+        // S^T[token][row] of the wave's tokens over its half of the dims, and 32 rows' of it on their way to the other half's wave
+        f32x16 sc;
+        auto scores = [&](int buf) {
+            const lds_ptr<uint8_t> codes = tiles + buf * kTreeTileBytes;
+            u32x4 k[9];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) k[i] = *(lds_ptr<u32x4>)(codes + k_row + 1024 * (i >> 2) + 16 * ((2 * (i & 3) + half) ^ k_swap));
+            k[8] = *(lds_ptr<u32x4>)(codes + k_rope);
+            f32x16 x[2] = {f32x16{}, f32x16{}};
+#pragma unroll
+            for (int i = 0; i < 9; ++i) {
+                const bf16x8 lo = as_bf16(k[i].x, k[i].y), hi = as_bf16(k[i].z, k[i].w);
+#pragma unroll
+                for (int b = 0; b < 2; ++b) x[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lo, __builtin_bit_cast(bf16x8, q[2 * i][b]), x[b], 0, 0, 0);
+#pragma unroll
+                for (int b = 0; b < 2; ++b) x[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(hi, __builtin_bit_cast(bf16x8, q[2 * i + 1][b]), x[b], 0, 0, 0);
+            }
+            const f32x16 send = kh ? x[0] : x[1];
+            sc = kh ? x[1] : x[0];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sh->part[2 * th + 1 - kh][i][lane] = f32x4{send[4 * i], send[4 * i + 1], send[4 * i + 2], send[4 * i + 3]};
+        };
+        // Which of the wave's 32 tokens of a tile the lane's row sees, a bit a token.
+        auto seen_of = [&](int i, int buf) -> uint32_t {
+            const uint32_t is_there = (uint32_t)__builtin_amdgcn_ballot_w64(sh->scale[buf][0][32 * th + n32] > 0.0f);
+            const int t0 = (tile_lo + i) * kTreeTokens + 32 * th;
+            if (t0 + 32 <= s.ctx) return is_there;
+            const int j0 = t0 - s.ctx;                  // drafted row of bit 0
+            const int most = (a.masks ? s.nodes : min(s.nodes, own_node + 1)) - j0;
+            uint32_t bits = most >= 32 ? ~0u : most > 0 ? (1u << most) - 1u : 0u;
+            if (a.masks) {
+                const uint32_t* const mask = a.masks + (size_t)(s.node0 + own_node) * a.mask_words;
+                const int w = j0 >> 5, shift = j0 & 31;  // (floors below zero)
+                const uint32_t lo = w < 0 ? ~0u : w < a.mask_words ? mask[w] : 0u;
+                const uint32_t hi = w + 1 < 0 ? ~0u : w + 1 < a.mask_words ? mask[w + 1] : 0u;
+                bits &= (uint32_t)((((unsigned long long)hi << 32) | lo) >> shift);
+            }
+            return bits & is_there;
+        };
+        uint32_t seen = ~0u;
+        // token of register r: 8 (r >> 2) + 4 half + (r & 3)
+        auto bit_of = [&](int r) -> bool { return seen >> (8 * (r >> 2) + 4 * half + (r & 3)) & 1; };
+        const lds_ptr<uint8_t> w_row = weights + own * (2 * kTreeTokens) + 8 * half;
+        const int w_swap = (own >> 1) & 7;
+        auto put_weights = [&](const float (&p)[16], int parity) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *(lds_ptr<u32x2>)(w_row + parity * (kTreeRows * kTreeTokens * 2) + 16 * ((4 * th + i) ^ w_swap)) = u32x2{pack_bf16x2(p[4 * i], p[4 * i + 1]), pack_bf16x2(p[4 * i + 2], p[4 * i + 3])};
+        };
+        // Weights of the tile under the row's reference; returns the largest exponent. Every tile goes unmasked first, in one piece with the
+        // values of the tile before; one with tokens that some row does not see has its weights again.
+        auto weigh = [&](auto masked, int buf, int parity) -> float {
+            constexpr bool MASKED = decltype(masked)::value;
+            const float mu = m_ref == -INFINITY ? 0.0f : m_ref;
+            float p[16], most = -INFINITY;
+            if (MASKED) l_sum = l_before;
+            else l_before = l_sum;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const f32x4 scale = *(lds_ptr<f32x4>)&sh->scale[buf][0][32 * th + 8 * i + 4 * half];
+                const f32x4 by = *(lds_ptr<f32x4>)&sh->scale[buf][1][32 * th + 8 * i + 4 * half];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    float y = __builtin_fmaf(sc[4 * i + k], by[k], -mu);
+                    if (MASKED) y = bit_of(4 * i + k) ? y : -INFINITY;
+                    most = fmaxf(most, y);
+                    const float e = __builtin_amdgcn_exp2f(y);
+                    l_sum += e;
+                    p[4 * i + k] = MASKED && !bit_of(4 * i + k) ? 0.0f : e * scale[k];
+                }
+            }
+            put_weights(p, parity);
+            return most;
+        };
+        // New references for the rows of tile i (the workgroup's decision): its weights again, everything before rescaled.
+        auto regrow = [&](int buf, int parity) {
+            float most = -INFINITY;
+            float x[16];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const f32x4 by = *(lds_ptr<f32x4>)&sh->scale[buf][1][32 * th + 8 * i + 4 * half];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    x[4 * i + k] = bit_of(4 * i + k) ? sc[4 * i + k] * by[k] : -INFINITY;
+                    most = fmaxf(most, x[4 * i + k]);
+                }
+            }
+            const auto other = __builtin_amdgcn_permlane32_swap(__float_as_uint(most), __float_as_uint(most), false, false);
+            most = fmaxf(__uint_as_float(other[0]), __uint_as_float(other[1]));
+            if (half == 0) sh->top[th][own] = most;
+            lds_barrier();
+            const float top = fmaxf(sh->top[0][own], sh->top[1][own]);
+            const bool grow = top > m_ref;
+            const float corr = grow ? __builtin_amdgcn_exp2f(m_ref - top) : 1.0f;  // 2^-inf = 0 at first
+            if (grow) m_ref = top;
+            if (th == 0 && half == 0) sh->corr[own] = corr;
+            const float mu = m_ref == -INFINITY ? 0.0f : m_ref;
+            l_sum = l_before * corr;
+            float p[16];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const f32x4 scale = *(lds_ptr<f32x4>)&sh->scale[buf][0][32 * th + 8 * i + 4 * half];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float e = __builtin_amdgcn_exp2f(x[4 * i + k] - mu);
+                    l_sum += e;
+                    p[4 * i + k] = bit_of(4 * i + k) ? e * scale[k] : 0.0f;
+                }
+            }
+            put_weights(p, parity);
+            lds_barrier();
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const float by = sh->corr[32 * b + n32];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) o[c][b] *= by;
+            }
+        };
+        // O^T[column][row] += V^T . P^T of a tile
+        auto values = [&](int buf, int parity) {
+            const lds_ptr<uint8_t> codes = tiles + buf * kTreeTileBytes + v_row;
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) {
+                bf16x8 w[2];
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+                    w[b] = *(lds_ptr<bf16x8>)(weights + parity * (kTreeRows * kTreeTokens * 2) + (32 * b + n32) * (2 * kTreeTokens) + 16 * ((2 * ks + half) ^ k_swap));
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const i32x2 r = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_ptr<i32x2>)(codes + 8192 * ks + 16 * ((v_piece + c) ^ v_swap)));
+                    const bf16x8 v = as_bf16((uint32_t)r[0], (uint32_t)r[1]);
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) o[c][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, w[b], o[c][b], 0, 0, 0);
+                }
+            }
+        };
+        // The wave's sixteen rows of a tile whose keys have all been read: codes that are no number become zeros, where some row does not
+        // see a token (its weight is zero, the product would not be). A row that does see it has no number for its weight.
+        auto clean = [&](int buf) {
+            const lds_ptr<uint8_t> to = tiles + buf * kTreeTileBytes + 2 * wave * 4096 + 16 * lane;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const u32x4 c = *(lds_ptr<u32x4>)(to + 1024 * i);
+                const u32x4 d = {numbers_only(c.x), numbers_only(c.y), numbers_only(c.z), numbers_only(c.w)};
+                if (((c.x ^ d.x) | (c.y ^ d.y) | (c.z ^ d.z) | (c.w ^ d.w)) != 0) *(lds_ptr<u32x4>)(to + 1024 * i) = d;
+            }
+        };
+        auto drafted = [&](int i) -> bool { return (tile_lo + i + 1) * kTreeTokens > s.ctx; };
+        auto meet = [&]() {  // the other half's partial scores of the rows that are the wave's
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const f32x4 x = sh->part[2 * th + kh][i][lane];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) sc[4 * i + k] += x[k];
+            }
+        };
+
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int b = 0; b < 2; ++b) o[c][b] = f32x16{};
+        // ---- the first tile, which sets the references -----------------------------------------------------------
+        arrived(0);
+        if (n_tiles > 1) request(1, 1);
+        if (n_tiles > 2) look_up(2);
+        lds_barrier();
+        scores(0);
+        seen = seen_of(0, 0);
+        lds_barrier();
+        meet();
+        regrow(0, 0);
+        if (drafted(0)) clean(0);
+        if (n_tiles > 1) arrived(1);
+        lds_barrier();
+        int buf = 0;  // of tile i
+        for (int i = 0; i + 1 < n_tiles; ++i) {
+            const int next = buf == 2 ? 0 : buf + 1, third = next == 2 ? 0 : next + 1, parity = i & 1;
+            const int grown = sh->grown;
+            if (i + 2 < n_tiles) request(i + 2, third);
+            if (i + 3 < n_tiles) look_up(i + 3);
+            if (__builtin_amdgcn_readfirstlane(grown) == number + i && i > 0) regrow(buf, parity);
+            scores(next);
+            seen = seen_of(i + 1, next);
+            lds_barrier();
+            meet();
+            values(buf, parity);
+            float most = weigh(std::false_type{}, next, parity ^ 1);
+            if (__builtin_amdgcn_ballot_w64(seen != ~0u) != 0) most = weigh(std::true_type{}, next, parity ^ 1);
+            if (drafted(i + 1)) clean(next);
+            if (__builtin_amdgcn_ballot_w64(most > (m_ref == -INFINITY ? -INFINITY : kTreeGrow)) != 0) sh->grown = number + i + 1;
+            if (i + 2 < n_tiles) arrived(third);
+            lds_barrier();
+            buf = next;
+        }
+        if (n_tiles > 1 && __builtin_amdgcn_readfirstlane(sh->grown) == number + n_tiles - 1) regrow(buf, (n_tiles - 1) & 1);
+        values(buf, (n_tiles - 1) & 1);
+        number += n_tiles;
+    }
+
+    if (n_tiles <= 0) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int b = 0; b < 2; ++b) o[c][b] = f32x16{};
+    }
+
+    // ---- results: of column tile c a lane's registers 4 i .. are columns of piece c, or four pieces further on (i >= 2), from
+    // 8 (i & 1) + 4 half on
+    const auto other = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_sum), __float_as_uint(l_sum), false, false);
+    l_sum = __uint_as_float(other[0]) + __uint_as_float(other[1]);
+    if (half == 0) {
+        sh->sum[th][own] = l_sum;
+        if (th == 0) sh->ref[own] = m_ref;
+    }
+    __syncthreads();
+    if (!whole) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (n_tiles > 0)
+                        reinterpret_cast<f32x4*>(rec)[(((wave * 4 + c) * 2 + b) * 4 + i) * kWave + lane] =
+                            f32x4{o[c][b][4 * i], o[c][b][4 * i + 1], o[c][b][4 * i + 2], o[c][b][4 * i + 3]};
+        if (tid < kTreeRows) {
+            rec[kTreeRows * 512 + 2 * tid] = sh->ref[tid];
+            rec[kTreeRows * 512 + 2 * tid + 1] = sh->sum[0][tid] + sh->sum[1][tid];
+        }
+    } else {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const int r = kTreeRows * rb + 32 * b + n32;
+            const float l = sh->sum[0][32 * b + n32] + sh->sum[1][32 * b + n32];
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            if (r < rows) {
+                uint16_t* const dst = a.clat + ((size_t)s.node0 * a.H + r) * 512 + 128 * wave + 4 * half;
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        *reinterpret_cast<u32x2*>(dst + 16 * c + 64 * (i >> 1) + 8 * (i & 1)) =
+                            u32x2{pack_bf16x2(o[c][b][4 * i] * inv, o[c][b][4 * i + 1] * inv), pack_bf16x2(o[c][b][4 * i + 2] * inv, o[c][b][4 * i + 3] * inv)};
+                if (a.lse && wave == 0 && half == 0)
+                    a.lse[(size_t)s.node0 * a.H + r] = l == 0.0f ? -INFINITY : (sh->ref[32 * b + n32] + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+            }
+        }
+    }
+    __syncthreads();
+}
+
+__global__ __launch_bounds__(kTreeThreads, 1) void mla_attend_tree_kernel(const TreeArgs a) {
+    __shared__ __attribute__((aligned(1024))) TreeShared shared;
+    const lds_ptr<TreeShared> sh = (lds_ptr<TreeShared>)&shared;
+    if (threadIdx.x == 0) sh->grown = -1;
+    const bool all = a.groups == 0;  // a block of rows is a work item
+    int item = blockIdx.x, number = 0;
+    long long u = item, end = u + 1;
+    if (!all) {
+        const long long total = tree_total(a, false);
+        const int items = tree_items(a, total);
+        if (item >= items || total == 0) return;
+        // an eighth of the items on each die: neighbours, which often read the same tokens
+        if (items % kTreeDies == 0) item = (item % kTreeDies) * (items / kTreeDies) + item / kTreeDies;
+        u = tree_item_lo(item, items, total), end = tree_item_lo(item + 1, items, total);
+    }
+    while (u < end) {
+        const TreeBlock b = tree_block(a, all, u);
+        if (b.seq < 0) return;
+        const int lo = all ? 0 : (int)(u - b.first), hi = all ? b.tiles : (int)min((long long)b.tiles, lo + end - u);
+        float* const rec = a.partial + (size_t)(2 * item + (lo == 0 ? 1 : 0)) * kTreeRecordFloats;
+        tree_part(a, sh, tree_seq(a, b.seq), b.seq, b.rb, b.rb == b.blocks - 1, lo, hi, lo == 0 && hi == b.tiles, rec, number);
+        u += all ? 1 : hi - lo;
+    }
+}
+
+// Blocks that several work items had: their records, in order, under the largest reference.
+__global__ __launch_bounds__(256) void mla_attend_tree_merge_kernel(const TreeArgs a) {
+    const long long total = tree_total(a, false);
+    if (total == 0) return;
+    const int items = tree_items(a, total);
+    // block number blockIdx.x: found among blocks, then its place among the tiles
+    const TreeBlock by_block = tree_block(a, true, blockIdx.x);
+    if (by_block.seq < 0) return;
+    long long before = 0;
+    {
+        const int lane = threadIdx.x & 63;
+        for (int s0 = 0; s0 < by_block.seq; s0 += kWave) {
+            int blocks = 0, tiles = 0;
+            if (s0 + lane < by_block.seq) tree_units(a, s0 + lane, blocks, tiles);
+            before += (long long)blocks * tiles;
+        }
+        before = __shfl(lanes_up_to(before), kWave - 1, kWave);
+    }
+    const long long first = before + (long long)by_block.rb * by_block.tiles;
+    const int g0 = tree_item_of(first, items, total), g1 = tree_item_of(first + by_block.tiles - 1, items, total);
+    if (g0 == g1) return;
+    const int at = blockIdx.y * 256 + threadIdx.x, lane = at & 63, idx = at >> 6;
+    const int i = idx & 3, b = (idx >> 2) & 1, c = (idx >> 3) & 3, wave = idx >> 5;
+    const int row = 32 * b + (lane & 31);
+    float m = -INFINITY, l = 0.0f;
+    f32x4 sum = {0, 0, 0, 0};
+    for (int g = g0; g <= g1; ++g) {
+        const float* const rec = a.partial + (size_t)(2 * g + (g == g0 ? 1 : 0)) * kTreeRecordFloats;
+        const float m_r = rec[kTreeRows * 512 + 2 * row], l_r = rec[kTreeRows * 512 + 2 * row + 1];
+        if (l_r == 0.0f) continue;  // nothing that the row sees
+        const f32x4 v = reinterpret_cast<const f32x4*>(rec)[at];
+        const float top = fmaxf(m, m_r);
+        const float keep = __builtin_amdgcn_exp2f(m - top), by = __builtin_amdgcn_exp2f(m_r - top);
+        m = top, l = l * keep + l_r * by;
+        sum = sum * keep + v * by;
+    }
+    const TreeSeq s = tree_seq(a, by_block.seq);
+    const int r = kTreeRows * by_block.rb + row;
+    if (r >= s.nodes * a.H) return;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const size_t out = (size_t)s.node0 * a.H + r;
+    *reinterpret_cast<u32x2*>(a.clat + out * 512 + 128 * wave + 16 * c + 64 * (i >> 1) + 8 * (i & 1) + 4 * (lane >> 5)) =
+        u32x2{pack_bf16x2(sum[0] * inv, sum[1] * inv), pack_bf16x2(sum[2] * inv, sum[3] * inv)};
+    if (a.lse && idx == 0 + 4 * b && lane < 32) a.lse[out] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+}
+
+}  // namespace rk
