@@ -15,7 +15,6 @@ struct TreeArgs {
     const uint32_t* masks;  // [n_nodes][mask_words]; null: node i sees drafted rows 0 .. i
     int n_seqs, H, n_nodes, max_nodes, mask_words, max_ctx, max_blocks;
     int kvl, rope, row_w, page_tokens, n_pages;
-    int page_shift;         // log2(page_tokens) when that is a power of two, else -1
     size_t page_bytes;
     float qscale;           // softmax scale * log2(e)
     uint16_t* clat;
@@ -160,7 +159,8 @@ extern "C" int rivoli_mla_attend_tree_paged(const unsigned short* qabs, const un
         n_nodes <= 0 || max_nodes <= 0 || max_ctx < 0 || max_blocks_per_seq <= 0 || kvl <= 0 || rope <= 0 ||
         page_tokens <= 0 || n_pages <= 0)
         return 1001;
-    if (n_seqs > 65535 || max_nodes > 4096 || max_ctx > INT_MAX - 8192 || (long long)n_nodes * H > 1 << 30 || H > 65535 * rk::kTreeRowWaves)
+    if (n_seqs > 65535 || max_nodes > 4096 || max_ctx > INT_MAX - 8192 || (long long)n_nodes * H > 1 << 30 || H > 65535 * rk::kTreeRowWaves ||
+        page_tokens > 1 << 22)
         return 1002;
     if (kvl % 128 != 0 || kvl > 512 || rope % 8 != 0 || rope > 64 || page_tokens % 4 != 0) return 1004;
     if (!rk::aligned16(qabs) || !rk::aligned16(qrope) || !rk::aligned16(pool) || !rk::aligned16(clat) || !rk::aligned16(partial)) return 1004;
@@ -169,7 +169,6 @@ extern "C" int rivoli_mla_attend_tree_paged(const unsigned short* qabs, const un
     if (!plain && plan.groups && !partial) return 1001;
     const rk::TreeArgs a{qabs, qrope, pool, block_table, ctx_lens, cu_nodes, masks, n_seqs, H, n_nodes, max_nodes, (max_nodes + 31) / 32,
                          max_ctx, max_blocks_per_seq, kvl, rope, kvl + rope, page_tokens, n_pages,
-                         (page_tokens & (page_tokens - 1)) == 0 ? __builtin_ctz((unsigned)page_tokens) : -1,
                          (size_t)page_tokens * (size_t)(kvl + rope + 4), scale * rk::kLog2e, clat, lse, plan.groups, partial, bad_rows};
     const hipStream_t st = (hipStream_t)stream;
     (void)hipGetLastError();

@@ -132,16 +132,22 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
     const int len = a.masks ? s.ctx + s.nodes : s.ctx + last_row / a.H + 1;
     const int n_tiles = min(tile_hi, (len + kTreeTokens - 1) / kTreeTokens) - tile_lo;
 
-    // ---- where a tile's rows are: eight lanes ask for rows 16 wave + 8 o + (lane >> 3) --------------------------
+    // ---- where a tile's rows are: eight lanes have rows 16 wave + 8 o + (lane >> 3) -----------------------------
+    // Lookups and transfers have no branches, so that they go between the matrix instructions: tiles past the end are asked for too (of
+    // the pool's first row), and a row's page and its place in it move on by a tile's tokens without a division.
     const int l8 = lane & 7, r8 = lane >> 3;
+    const int end_row = min(len, tile_hi * kTreeTokens);
     const int* const table = a.block_table + (size_t)seq * a.max_blocks;
-    auto block_of = [&](int t) -> unsigned { return a.page_shift >= 0 ? (unsigned)t >> a.page_shift : (unsigned)t / (unsigned)a.page_tokens; };
-    auto token_of = [&](int i, int o) -> int { return (tile_lo + i) * kTreeTokens + 16 * wave + 8 * o + r8; };
-    int page[2];
-    auto look_up = [&](int i) {
+    const unsigned page_tokens = (unsigned)a.page_tokens, on_pages = kTreeTokens / page_tokens, on_rows = kTreeTokens % page_tokens;
+    int token[2], page[2];        // of the tile to be asked for
+    unsigned block[2], place[2];  // of it; and of the next when that has been looked up
 #pragma unroll
-        for (int o = 0; o < 2; ++o) page[o] = table[min(block_of(min(token_of(i, o), len - 1)), (unsigned)a.max_blocks - 1)];
-    };
+    for (int o = 0; o < 2; ++o) {
+        token[o] = tile_lo * kTreeTokens + 16 * wave + 8 * o + r8;
+        block[o] = (unsigned)token[o] / page_tokens, place[o] = (unsigned)token[o] - block[o] * page_tokens;
+    }
+    auto look_up = [&](int o) { page[o] = table[min(block[o], (unsigned)a.max_blocks - 1)]; };
+    unsigned int missing = 0;     // rows of the block's that have no page
     bool there[2];
     float raw_scale[2];
     auto scalar = [](lds_ptr<uint8_t> p) -> lds_ptr<uint8_t> {  // the transfers take their LDS base from a scalar register
@@ -149,23 +155,27 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
     };
     auto swap_of = [&](int o) -> int { return (4 * o + (r8 >> 1)) & 7; };
     const unsigned long long roped[2] = {__builtin_amdgcn_ballot_w64((l8 ^ swap_of(0)) < 4), __builtin_amdgcn_ballot_w64((l8 ^ swap_of(1)) < 4)};
-    auto request = [&](int i, int buf) {  // of a tile looked up
-#pragma unroll
-        for (int o = 0; o < 2; ++o) {
-            const int t = token_of(i, o);
-            const unsigned blk = block_of(t);
-            unsigned off = a.page_shift >= 0 ? (unsigned)t & (unsigned)(a.page_tokens - 1) : (unsigned)t - blk * (unsigned)a.page_tokens;
-            const bool mine = t < len;
-            there[o] = mine & (blk < (unsigned)a.max_blocks) & ((unsigned)page[o] < (unsigned)a.n_pages);
-            if (a.bad_rows && last_block && __builtin_amdgcn_ballot_w64(mine & !there[o]) != 0) {
-                if (mine & !there[o] && l8 == 0) atomicAdd(a.bad_rows, 1u);
-            }
-            off = there[o] ? off : 0u;
-            const uint8_t* const base = a.pool + (unsigned long long)(unsigned)(there[o] ? page[o] : 0) * a.page_bytes;
-            raw_scale[o] = *reinterpret_cast<const float*>(base + (size_t)a.page_tokens * 576 + 4u * off);
-            few_dma_row(base + (size_t)off * 576u + 16 * (l8 ^ swap_of(o)), scalar(tiles + buf * kTreeTileBytes + (2 * wave + o) * 4096),
-                        scalar(tiles + buf * kTreeTileBytes + kTreeRopeAt + wave * 1024), roped[o]);
-        }
+    const uint32_t page_bytes = (uint32_t)a.page_bytes, codes_bytes = page_tokens * 576u;
+    const uint8_t* src[2];
+    auto find = [&](int o) {  // the lane's row of a tile looked up: its address, and its scale asked for
+        const bool mine = token[o] < end_row;
+        there[o] = mine & (block[o] < (unsigned)a.max_blocks) & ((unsigned)page[o] < (unsigned)a.n_pages);
+        missing += mine & !there[o];
+        const unsigned off = there[o] ? place[o] : 0u;
+        const uint8_t* const base = a.pool + (unsigned long long)(there[o] ? (unsigned)page[o] : 0u) * page_bytes;
+        raw_scale[o] = *reinterpret_cast<const float*>(base + (codes_bytes + 4u * off));
+        src[o] = base + (off * 576u + 16u * (unsigned)(l8 ^ swap_of(o)));
+    };
+    auto bring = [&](int o, int buf) {
+        few_dma_row(src[o], scalar(tiles + buf * kTreeTileBytes + (2 * wave + o) * 4096),
+                    scalar(tiles + buf * kTreeTileBytes + kTreeRopeAt + wave * 1024), roped[o]);
+    };
+    auto go_on = [&](int o) {
+        token[o] += kTreeTokens;
+        place[o] += on_rows;
+        const bool over = place[o] >= page_tokens;
+        place[o] -= over ? page_tokens : 0u;
+        block[o] += on_pages + (over ? 1u : 0u);
     };
     // The transfers asked for have landed: scales, and zeros for rows that are not there (codes must be finite, they meet
     // a zero weight). A scale that is not a positive number cannot come from the append: such a row is not there.
@@ -195,22 +205,22 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
     const int own_node = (live ? own_row : 0) / a.H;
 
     if (n_tiles > 0) {
-        look_up(0);
-        u32x4 q[kTreeSteps][2];
-        request(0, 0);
-        if (n_tiles > 1) look_up(1);
+        look_up(0), look_up(1);
+        u32x4 q[kTreeSteps][2];  // of the rows that are the wave's in the softmax, and of the others
+#pragma unroll
+        for (int o = 0; o < 2; ++o) find(o), bring(o, 0), go_on(o), look_up(o);
         // ---- the rows' operands: K-steps of 16 dims, eight a lane. Two K-steps share a 16-byte piece of codes. They live in the
         // accumulation half of the register file, which the matrix instructions read as well; the sums are in the other --------
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-            const int r = kTreeRows * rb + 32 * b + n32;
+            const int r = kTreeRows * rb + 32 * (b ^ kh) + n32;
             const size_t at = (size_t)s.node0 * a.H + (r < rows ? r : 0);
             u32x4 raw[kTreeSteps];
 #pragma unroll
             for (int j = 0; j < kTreeSteps; ++j) {
-                const uint16_t* const src = j < 16 ? a.qabs + at * 512 + 256 * kh + 32 * (j >> 1) + 16 * half + 8 * (j & 1)
-                                                   : a.qrope + at * 64 + 32 * kh + 16 * half + 8 * (j & 1);
-                raw[j] = *reinterpret_cast<const u32x4*>(src);
+                const uint16_t* const from = j < 16 ? a.qabs + at * 512 + 256 * kh + 32 * (j >> 1) + 16 * half + 8 * (j & 1)
+                                                    : a.qrope + at * 64 + 32 * kh + 16 * half + 8 * (j & 1);
+                raw[j] = *reinterpret_cast<const u32x4*>(from);
             }
 #pragma unroll
             for (int j = 0; j < kTreeSteps; ++j)
@@ -237,27 +247,44 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
             const u32x4 d = {d0, d1, d2, d3};
             return __builtin_bit_cast(bf16x8, d);
         };
-        // S^T[token][row] of the wave's tokens over its half of the dims, and 32 rows' of it on their way to the other half's wave
+        // S^T[token][row] of the wave's tokens over its half of the dims, the others' 32 rows' of it on their way to the other half's
+        // wave; and between its matrix instructions the next tile but one is asked for. A piece of codes is out of LDS two steps and converted
+        // one step before its matrix instructions; the fences keep that order.
         f32x16 sc;
-        auto scores = [&](int buf) {
+        auto scores = [&](int buf, auto ask, int third) {
             const lds_ptr<uint8_t> codes = tiles + buf * kTreeTileBytes;
-            u32x4 k[9];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) k[i] = *(lds_ptr<u32x4>)(codes + k_row + 1024 * (i >> 2) + 16 * ((2 * (i & 3) + half) ^ k_swap));
-            k[8] = *(lds_ptr<u32x4>)(codes + k_rope);
+            u32x4 k[3];
+            auto load = [&](int i) {
+                k[i % 3] = *(lds_ptr<u32x4>)(codes + (i < 8 ? k_row + 1024 * (i >> 2) + 16 * ((2 * (i & 3) + half) ^ k_swap) : k_rope));
+            };
+            load(0), load(1);
             f32x16 x[2] = {f32x16{}, f32x16{}};
+            bf16x8 lo = as_bf16(k[0].x, k[0].y), hi = as_bf16(k[0].z, k[0].w);
 #pragma unroll
             for (int i = 0; i < 9; ++i) {
-                const bf16x8 lo = as_bf16(k[i].x, k[i].y), hi = as_bf16(k[i].z, k[i].w);
-#pragma unroll
-                for (int b = 0; b < 2; ++b) x[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lo, __builtin_bit_cast(bf16x8, q[2 * i][b]), x[b], 0, 0, 0);
-#pragma unroll
-                for (int b = 0; b < 2; ++b) x[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(hi, __builtin_bit_cast(bf16x8, q[2 * i + 1][b]), x[b], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
+                if (i + 2 < 9) load(i + 2);
+                const u32x4 then = k[(i + 1) % 3];
+                x[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lo, __builtin_bit_cast(bf16x8, q[2 * i][0]), x[0], 0, 0, 0);
+                if (decltype(ask)::value) {
+                    if (i < 4 && i % 2 == 0) find(i / 2);
+                    if (i < 4 && i % 2 == 1) bring(i / 2, third);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                x[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lo, __builtin_bit_cast(bf16x8, q[2 * i][1]), x[1], 0, 0, 0);
+                if (i < 8) lo = as_bf16(then.x, then.y);
+                if (decltype(ask)::value && i >= 4 && i < 6) go_on(i - 4);
+                __builtin_amdgcn_sched_barrier(0);
+                x[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(hi, __builtin_bit_cast(bf16x8, q[2 * i + 1][0]), x[0], 0, 0, 0);
+                if (decltype(ask)::value && i >= 4 && i < 6) look_up(i - 4);
+                __builtin_amdgcn_sched_barrier(0);
+                x[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(hi, __builtin_bit_cast(bf16x8, q[2 * i + 1][1]), x[1], 0, 0, 0);
+                if (i < 8) hi = as_bf16(then.z, then.w);
             }
-            const f32x16 send = kh ? x[0] : x[1];
-            sc = kh ? x[1] : x[0];
+            __builtin_amdgcn_sched_barrier(0);
+            sc = x[0];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sh->part[2 * th + 1 - kh][i][lane] = f32x4{send[4 * i], send[4 * i + 1], send[4 * i + 2], send[4 * i + 3]};
+            for (int i = 0; i < 4; ++i) sh->part[2 * th + 1 - kh][i][lane] = f32x4{x[1][4 * i], x[1][4 * i + 1], x[1][4 * i + 2], x[1][4 * i + 3]};
         };
         // Which of the wave's 32 tokens of a tile the lane's row sees, a bit a token.
         auto seen_of = [&](int i, int buf) -> uint32_t {
@@ -286,26 +313,22 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
             for (int i = 0; i < 4; ++i)
                 *(lds_ptr<u32x2>)(w_row + parity * (kTreeRows * kTreeTokens * 2) + 16 * ((4 * th + i) ^ w_swap)) = u32x2{pack_bf16x2(p[4 * i], p[4 * i + 1]), pack_bf16x2(p[4 * i + 2], p[4 * i + 3])};
         };
-        // Weights of the tile under the row's reference; returns the largest exponent. Every tile goes unmasked first, in one piece with the
-        // values of the tile before; one with tokens that some row does not see has its weights again.
-        auto weigh = [&](auto masked, int buf, int parity) -> float {
-            constexpr bool MASKED = decltype(masked)::value;
+        // Weights of a tile with tokens that some row does not see, in place of those that step() made of it; the largest exponent.
+        auto weigh_seen = [&](int buf, int parity) -> float {
             const float mu = m_ref == -INFINITY ? 0.0f : m_ref;
             float p[16], most = -INFINITY;
-            if (MASKED) l_sum = l_before;
-            else l_before = l_sum;
+            l_sum = l_before;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const f32x4 scale = *(lds_ptr<f32x4>)&sh->scale[buf][0][32 * th + 8 * i + 4 * half];
                 const f32x4 by = *(lds_ptr<f32x4>)&sh->scale[buf][1][32 * th + 8 * i + 4 * half];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    float y = __builtin_fmaf(sc[4 * i + k], by[k], -mu);
-                    if (MASKED) y = bit_of(4 * i + k) ? y : -INFINITY;
+                    const float y = bit_of(4 * i + k) ? __builtin_fmaf(sc[4 * i + k], by[k], -mu) : -INFINITY;
                     most = fmaxf(most, y);
                     const float e = __builtin_amdgcn_exp2f(y);
                     l_sum += e;
-                    p[4 * i + k] = MASKED && !bit_of(4 * i + k) ? 0.0f : e * scale[k];
+                    p[4 * i + k] = bit_of(4 * i + k) ? e * scale[k] : 0.0f;
                 }
             }
             put_weights(p, parity);
@@ -355,23 +378,71 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
                 for (int c = 0; c < 4; ++c) o[c][b] *= by;
             }
         };
-        // O^T[column][row] += V^T . P^T of a tile
-        auto values = [&](int buf, int parity) {
+        // O^T[column][row] += V^T . P^T of a tile, sixteen units of a K-step and a column tile each; and, with NEXT, the softmax of the tile
+        // after it, a token a unit, from the partial scores' meeting to the weights: tile `next`'s, as if every row saw every
+        // token. A unit's codes are out of LDS three units and converted one unit before its matrix instructions.
+        auto step = [&](auto more, int buf, int parity, int next) -> float {
+            constexpr bool NEXT = decltype(more)::value;
             const lds_ptr<uint8_t> codes = tiles + buf * kTreeTileBytes + v_row;
+            const lds_ptr<uint8_t> w_from = weights + parity * (kTreeRows * kTreeTokens * 2) + n32 * (2 * kTreeTokens);
+            i32x2 raw[4];
+            bf16x8 w[2][2];
+            auto load = [&](int u) {
+                raw[u % 4] = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_ptr<i32x2>)(codes + 8192 * (u >> 2) + 16 * ((v_piece + (u & 3)) ^ v_swap)));
+            };
+            auto load_w = [&](int ks) {
 #pragma unroll
-            for (int ks = 0; ks < 4; ++ks) {
-                bf16x8 w[2];
+                for (int b = 0; b < 2; ++b) w[ks & 1][b] = *(lds_ptr<bf16x8>)(w_from + 32 * b * (2 * kTreeTokens) + 16 * ((2 * ks + half) ^ k_swap));
+            };
+            load(0), load_w(0), load(1), load(2);
+            f32x4 part[4], scale, by;
+            const float mu = m_ref == -INFINITY ? 0.0f : m_ref;
+            float most = -INFINITY, p[4];
+            if (NEXT) {
+                l_before = l_sum;
+                lds_barrier();  // the partial scores are there
 #pragma unroll
-                for (int b = 0; b < 2; ++b)
-                    w[b] = *(lds_ptr<bf16x8>)(weights + parity * (kTreeRows * kTreeTokens * 2) + (32 * b + n32) * (2 * kTreeTokens) + 16 * ((2 * ks + half) ^ k_swap));
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const i32x2 r = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_ptr<i32x2>)(codes + 8192 * ks + 16 * ((v_piece + c) ^ v_swap)));
-                    const bf16x8 v = as_bf16((uint32_t)r[0], (uint32_t)r[1]);
-#pragma unroll
-                    for (int b = 0; b < 2; ++b) o[c][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, w[b], o[c][b], 0, 0, 0);
-                }
+                for (int i = 0; i < 4; ++i) part[i] = sh->part[2 * th + kh][i][lane];
             }
+            auto scales = [&](int i) {
+                scale = *(lds_ptr<f32x4>)&sh->scale[next][0][32 * th + 8 * i + 4 * half];
+                by = *(lds_ptr<f32x4>)&sh->scale[next][1][32 * th + 8 * i + 4 * half];
+            };
+            float y;
+            auto first = [&](int r) {
+                if ((r & 3) == 0) scales(r >> 2);
+                sc[r] += part[r >> 2][r & 3];
+                y = __builtin_fmaf(sc[r], by[r & 3], -mu);
+                most = fmaxf(most, y);
+                y = __builtin_amdgcn_exp2f(y);
+            };
+            auto second = [&](int r) {
+                l_sum += y;
+                p[r & 3] = y * scale[r & 3];
+                if ((r & 3) == 3)
+                    *(lds_ptr<u32x2>)(w_row + (parity ^ 1) * (kTreeRows * kTreeTokens * 2) + 16 * ((4 * th + (r >> 2)) ^ w_swap)) =
+                        u32x2{pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3])};
+            };
+            bf16x8 v = as_bf16((uint32_t)raw[0][0], (uint32_t)raw[0][1]);
+#pragma unroll
+            for (int u = 0; u < 16; ++u) {
+                const int ks = u >> 2, c = u & 3;
+                __builtin_amdgcn_sched_barrier(0);
+                if (u + 3 < 16) load(u + 3);
+                if (c == 1 && ks < 3) load_w(ks + 1);
+                o[c][0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, w[ks & 1][0], o[c][0], 0, 0, 0);
+                if (NEXT && u >= 2) first(u - 2);
+                __builtin_amdgcn_sched_barrier(0);
+                o[c][1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, w[ks & 1][1], o[c][1], 0, 0, 0);
+                if (u < 15) v = as_bf16((uint32_t)raw[(u + 1) % 4][0], (uint32_t)raw[(u + 1) % 4][1]);
+                if (NEXT && u >= 2) second(u - 2);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if (NEXT) {
+#pragma unroll
+                for (int r = 14; r < 16; ++r) first(r), second(r);
+            }
+            return most;
         };
         // The wave's sixteen rows of a tile whose keys have all been read: codes that are no number become zeros, where some row does not
         // see a token (its weight is zero, the product would not be). A row that does see it has no number for its weight.
@@ -400,39 +471,34 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
             for (int b = 0; b < 2; ++b) o[c][b] = f32x16{};
         // ---- the first tile, which sets the references -----------------------------------------------------------
         arrived(0);
-        if (n_tiles > 1) request(1, 1);
-        if (n_tiles > 2) look_up(2);
+#pragma unroll
+        for (int o = 0; o < 2; ++o) find(o), bring(o, 1), go_on(o), look_up(o);
         lds_barrier();
-        scores(0);
+        scores(0, std::false_type{}, 0);
         seen = seen_of(0, 0);
         lds_barrier();
         meet();
         regrow(0, 0);
         if (drafted(0)) clean(0);
-        if (n_tiles > 1) arrived(1);
+        arrived(1);
         lds_barrier();
         int buf = 0;  // of tile i
         for (int i = 0; i + 1 < n_tiles; ++i) {
             const int next = buf == 2 ? 0 : buf + 1, third = next == 2 ? 0 : next + 1, parity = i & 1;
-            const int grown = sh->grown;
-            if (i + 2 < n_tiles) request(i + 2, third);
-            if (i + 3 < n_tiles) look_up(i + 3);
-            if (__builtin_amdgcn_readfirstlane(grown) == number + i && i > 0) regrow(buf, parity);
-            scores(next);
+            if (__builtin_amdgcn_readfirstlane(sh->grown) == number + i && i > 0) regrow(buf, parity);
+            scores(next, std::true_type{}, third);
             seen = seen_of(i + 1, next);
-            lds_barrier();
-            meet();
-            values(buf, parity);
-            float most = weigh(std::false_type{}, next, parity ^ 1);
-            if (__builtin_amdgcn_ballot_w64(seen != ~0u) != 0) most = weigh(std::true_type{}, next, parity ^ 1);
+            float most = step(std::true_type{}, buf, parity, next);
+            if (__builtin_amdgcn_ballot_w64(seen != ~0u) != 0) most = weigh_seen(next, parity ^ 1);
             if (drafted(i + 1)) clean(next);
             if (__builtin_amdgcn_ballot_w64(most > (m_ref == -INFINITY ? -INFINITY : kTreeGrow)) != 0) sh->grown = number + i + 1;
-            if (i + 2 < n_tiles) arrived(third);
+            arrived(third);
             lds_barrier();
             buf = next;
         }
         if (n_tiles > 1 && __builtin_amdgcn_readfirstlane(sh->grown) == number + n_tiles - 1) regrow(buf, (n_tiles - 1) & 1);
-        values(buf, (n_tiles - 1) & 1);
+        step(std::false_type{}, buf, (n_tiles - 1) & 1, 0);
+        if (a.bad_rows && last_block && l8 == 0 && missing) atomicAdd(a.bad_rows, missing);
         number += n_tiles;
     }
 
