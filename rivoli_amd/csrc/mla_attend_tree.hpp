@@ -107,9 +107,34 @@ struct TreeShared {
     uint8_t weights[2][kTreeRows * kTreeTokens * 2];  // by the tile's parity
     float scale[kTreeBuffers][2][kTreeTokens];  // of a tile's tokens: the scale (0: not there), and times the softmax's
     float top[2][kTreeRows], corr[kTreeRows], sum[2][kTreeRows], ref[kTreeRows];
-    int grown;                           // number of the tile some row of which outgrew its reference
+    // numbers of the latest tile of which some row outgrew its reference, and of which some token is not there
+    alignas(8) int grown;
+    int holed;
 };
 static_assert(sizeof(TreeShared) <= 160 * 1024, "one workgroup per compute unit");
+
+// A lane's pieces of a row's codes, in parts, so that the transfers go between matrix instructions one or two at a time: two of the four latent
+// groups (FIRST and the next), 128 bytes apart in memory and 1024 in LDS; the roped codes for the lanes of `roped`. As few_dma_row.
+template <int FIRST>
+__device__ __forceinline__ void tree_dma_latent(const uint8_t* src, lds_ptr<uint8_t> to) {
+    const uint32_t base = (uint32_t)(uintptr_t)to + (1024 - 128) * FIRST;
+    uint32_t keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off offset:%3\n\t"
+                 "s_add_u32 m0, m0, 896\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off offset:%4\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep)
+                 : "v"(src), "s"(base), "n"(128 * FIRST), "n"(128 * FIRST + 128)
+                 : "memory", "scc");
+}
+__device__ __forceinline__ void tree_dma_rope(const uint8_t* src, lds_ptr<uint8_t> to, unsigned long long roped) {
+    const uint32_t base = (uint32_t)(uintptr_t)to - 512u;
+    uint32_t keep;
+    unsigned long long all;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_and_saveexec_b64 %1, %4\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off offset:512\n\t"
+                 "s_mov_b64 exec, %1\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep), "=&s"(all)
+                 : "v"(src), "s"(base), "s"(roped)
+                 : "memory", "scc");
+}
 
 // Codes that are no number as zeros.
 __device__ __forceinline__ uint32_t numbers_only(uint32_t c) {
@@ -166,9 +191,11 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
         raw_scale[o] = *reinterpret_cast<const float*>(base + (codes_bytes + 4u * off));
         src[o] = base + (off * 576u + 16u * (unsigned)(l8 ^ swap_of(o)));
     };
-    auto bring = [&](int o, int buf) {
-        few_dma_row(src[o], scalar(tiles + buf * kTreeTileBytes + (2 * wave + o) * 4096),
-                    scalar(tiles + buf * kTreeTileBytes + kTreeRopeAt + wave * 1024), roped[o]);
+    auto bring = [&](int o, int part, int buf) {  // in three parts
+        const lds_ptr<uint8_t> to = scalar(tiles + buf * kTreeTileBytes + (2 * wave + o) * 4096);
+        if (part == 0) tree_dma_latent<0>(src[o], to);
+        if (part == 1) tree_dma_latent<2>(src[o], to);
+        if (part == 2) tree_dma_rope(src[o], scalar(tiles + buf * kTreeTileBytes + kTreeRopeAt + wave * 1024), roped[o]);
     };
     auto go_on = [&](int o) {
         token[o] += kTreeTokens;
@@ -177,14 +204,24 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
         place[o] -= over ? page_tokens : 0u;
         block[o] += on_pages + (over ? 1u : 0u);
     };
+    auto ask = [&](int buf) {
+#pragma unroll
+        for (int o = 0; o < 2; ++o) {
+            find(o);
+#pragma unroll
+            for (int part = 0; part < 3; ++part) bring(o, part, buf);
+            go_on(o), look_up(o);
+        }
+    };
     // The transfers asked for have landed: scales, and zeros for rows that are not there (codes must be finite, they meet
     // a zero weight). A scale that is not a positive number cannot come from the append: such a row is not there.
-    auto arrived = [&](int buf) {
+    auto arrived = [&](int buf, int of) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
         for (int o = 0; o < 2; ++o) {
             const bool ok = there[o] && raw_scale[o] > 0.0f;
             if (__builtin_amdgcn_ballot_w64(!ok) != 0 && !ok) {
+                sh->holed = of;
                 const lds_ptr<uint8_t> to = tiles + buf * kTreeTileBytes + 16 * lane;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) *(lds_ptr<u32x4>)(to + (2 * wave + o) * 4096 + 1024 * i) = u32x4{0, 0, 0, 0};
@@ -198,7 +235,7 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
     };
 
     f32x16 o[4][2];  // O^T: column tile c of 32, row block b: sixteen columns a lane, of row 32 b + n32
-    float m_ref = -INFINITY, l_sum = 0.0f, l_before = 0.0f;  // of row 32 kh + n32: the lane's share of the sum
+    float m_ref = -INFINITY, limit = -INFINITY, l_sum = 0.0f, l_before = 0.0f;  // of row 32 kh + n32: the lane's share of the sum
     const int own = 32 * kh + n32;
     const int own_row = kTreeRows * rb + own;
     const bool live = own_row < rows;
@@ -207,8 +244,7 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
     if (n_tiles > 0) {
         look_up(0), look_up(1);
         u32x4 q[kTreeSteps][2];  // of the rows that are the wave's in the softmax, and of the others
-#pragma unroll
-        for (int o = 0; o < 2; ++o) find(o), bring(o, 0), go_on(o), look_up(o);
+        ask(0);
         // ---- the rows' operands: K-steps of 16 dims, eight a lane. Two K-steps share a 16-byte piece of codes. They live in the
         // accumulation half of the register file, which the matrix instructions read as well; the sums are in the other --------
 #pragma unroll
@@ -251,13 +287,15 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
         // wave; and between its matrix instructions the next tile but one is asked for. A piece of codes is out of LDS two steps and converted
         // one step before its matrix instructions; the fences keep that order.
         f32x16 sc;
-        auto scores = [&](int buf, auto ask, int third) {
+        auto scores = [&](int buf, auto more, int third, auto before) {
+            constexpr bool MORE = decltype(more)::value;
             const lds_ptr<uint8_t> codes = tiles + buf * kTreeTileBytes;
             u32x4 k[3];
             auto load = [&](int i) {
                 k[i % 3] = *(lds_ptr<u32x4>)(codes + (i < 8 ? k_row + 1024 * (i >> 2) + 16 * ((2 * (i & 3) + half) ^ k_swap) : k_rope));
             };
             load(0), load(1);
+            before();
             f32x16 x[2] = {f32x16{}, f32x16{}};
             bf16x8 lo = as_bf16(k[0].x, k[0].y), hi = as_bf16(k[0].z, k[0].w);
 #pragma unroll
@@ -266,17 +304,14 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
                 if (i + 2 < 9) load(i + 2);
                 const u32x4 then = k[(i + 1) % 3];
                 x[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lo, __builtin_bit_cast(bf16x8, q[2 * i][0]), x[0], 0, 0, 0);
-                if (decltype(ask)::value) {
-                    if (i < 4 && i % 2 == 0) find(i / 2);
-                    if (i < 4 && i % 2 == 1) bring(i / 2, third);
-                }
+                if (MORE && (i == 0 || i == 4)) find(i / 4);
                 __builtin_amdgcn_sched_barrier(0);
                 x[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lo, __builtin_bit_cast(bf16x8, q[2 * i][1]), x[1], 0, 0, 0);
                 if (i < 8) lo = as_bf16(then.x, then.y);
-                if (decltype(ask)::value && i >= 4 && i < 6) go_on(i - 4);
+                if (MORE && i % 4 != 0) bring((i - 1) / 4, (i - 1) % 4, third);
                 __builtin_amdgcn_sched_barrier(0);
                 x[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(hi, __builtin_bit_cast(bf16x8, q[2 * i + 1][0]), x[0], 0, 0, 0);
-                if (decltype(ask)::value && i >= 4 && i < 6) look_up(i - 4);
+                if (MORE && i >= 5 && i < 7) go_on(i - 5), look_up(i - 5);
                 __builtin_amdgcn_sched_barrier(0);
                 x[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(hi, __builtin_bit_cast(bf16x8, q[2 * i + 1][1]), x[1], 0, 0, 0);
                 if (i < 8) hi = as_bf16(then.z, then.w);
@@ -355,6 +390,7 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
             const bool grow = top > m_ref;
             const float corr = grow ? __builtin_amdgcn_exp2f(m_ref - top) : 1.0f;  // 2^-inf = 0 at first
             if (grow) m_ref = top;
+            limit = m_ref == -INFINITY ? -INFINITY : kTreeGrow;
             if (th == 0 && half == 0) sh->corr[own] = corr;
             const float mu = m_ref == -INFINITY ? 0.0f : m_ref;
             l_sum = l_before * corr;
@@ -470,36 +506,42 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
 #pragma unroll
             for (int b = 0; b < 2; ++b) o[c][b] = f32x16{};
         // ---- the first tile, which sets the references -----------------------------------------------------------
-        arrived(0);
-#pragma unroll
-        for (int o = 0; o < 2; ++o) find(o), bring(o, 1), go_on(o), look_up(o);
+        arrived(0, number);
+        ask(1);
         lds_barrier();
-        scores(0, std::false_type{}, 0);
+        scores(0, std::false_type{}, 0, [] {});
         seen = seen_of(0, 0);
         lds_barrier();
         meet();
         regrow(0, 0);
         if (drafted(0)) clean(0);
-        arrived(1);
+        arrived(1, number + 1);
         lds_barrier();
         int buf = 0;  // of tile i
         for (int i = 0; i + 1 < n_tiles; ++i) {
             const int next = buf == 2 ? 0 : buf + 1, third = next == 2 ? 0 : next + 1, parity = i & 1;
-            if (__builtin_amdgcn_readfirstlane(sh->grown) == number + i && i > 0) regrow(buf, parity);
-            scores(next, std::true_type{}, third);
-            seen = seen_of(i + 1, next);
+            const i32x2 flags = *(lds_ptr<i32x2>)&sh->grown;
+            bool masked = false;  // some row may not see some token of tile i + 1
+            scores(next, std::true_type{}, third, [&] {
+                if (__builtin_amdgcn_readfirstlane(flags[0]) == number + i) regrow(buf, parity);
+                masked = drafted(i + 1) || __builtin_amdgcn_readfirstlane(flags[1]) == number + i + 1;
+                seen = ~0u;
+                if (masked) seen = seen_of(i + 1, next);
+            });
             float most = step(std::true_type{}, buf, parity, next);
-            if (__builtin_amdgcn_ballot_w64(seen != ~0u) != 0) most = weigh_seen(next, parity ^ 1);
-            if (drafted(i + 1)) clean(next);
-            if (__builtin_amdgcn_ballot_w64(most > (m_ref == -INFINITY ? -INFINITY : kTreeGrow)) != 0) sh->grown = number + i + 1;
-            arrived(third);
+            if (masked) {
+                most = weigh_seen(next, parity ^ 1);
+                if (drafted(i + 1)) clean(next);
+            }
+            if (__builtin_amdgcn_ballot_w64(most > limit) != 0) sh->grown = number + i + 1;
+            arrived(third, number + i + 2);
             lds_barrier();
             buf = next;
         }
         if (n_tiles > 1 && __builtin_amdgcn_readfirstlane(sh->grown) == number + n_tiles - 1) regrow(buf, (n_tiles - 1) & 1);
         step(std::false_type{}, buf, (n_tiles - 1) & 1, 0);
         if (a.bad_rows && last_block && l8 == 0 && missing) atomicAdd(a.bad_rows, missing);
-        number += n_tiles;
+        number += n_tiles + 2;  // (two tiles past the end were asked for)
     }
 
     if (n_tiles <= 0) {
@@ -557,7 +599,7 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
 __global__ __launch_bounds__(kTreeThreads, 1) void mla_attend_tree_kernel(const TreeArgs a) {
     __shared__ __attribute__((aligned(1024))) TreeShared shared;
     const lds_ptr<TreeShared> sh = (lds_ptr<TreeShared>)&shared;
-    if (threadIdx.x == 0) sh->grown = -1;
+    if (threadIdx.x == 0) sh->grown = sh->holed = -1;
     const bool all = a.groups == 0;  // a block of rows is a work item
     int item = blockIdx.x, number = 0;
     long long u = item, end = u + 1;
