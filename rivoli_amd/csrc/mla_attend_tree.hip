@@ -1,6 +1,7 @@
 // Attention of a tree of drafted tokens over the paged latent cache: node i of a sequence attends its ctx cached rows
 // and, of the drafted rows behind them, those its mask names. Launch-only.
 #include <climits>
+#include <cmath>
 #include <type_traits>
 
 #include "attend_common.hpp"
@@ -16,7 +17,7 @@ struct TreeArgs {
     int n_seqs, H, n_nodes, max_nodes, mask_words, max_ctx, max_blocks;
     int kvl, rope, row_w, page_tokens, n_pages;
     size_t page_bytes;
-    float qscale;           // softmax scale * log2(e)
+    float qscale;           // softmax scale * log2(e), kept from zero: results are divided by it
     uint16_t* clat;
     float* lse;
     int groups;             // TreePlan's
@@ -167,9 +168,11 @@ extern "C" int rivoli_mla_attend_tree_paged(const unsigned short* qabs, const un
     const bool plain = kvl != 512 || rope != 64;
     const rk::TreePlan plan = rk::tree_plan(n_seqs, H, n_nodes, max_nodes, max_ctx);
     if (!plain && plan.groups && !partial) return 1001;
+    float qscale = scale * rk::kLog2e;
+    if (std::fabs(qscale) < 1e-20f) qscale = std::copysign(1e-20f, qscale);  // as good as nothing to any softmax
     const rk::TreeArgs a{qabs, qrope, pool, block_table, ctx_lens, cu_nodes, masks, n_seqs, H, n_nodes, max_nodes, (max_nodes + 31) / 32,
                          max_ctx, max_blocks_per_seq, kvl, rope, kvl + rope, page_tokens, n_pages,
-                         (size_t)page_tokens * (size_t)(kvl + rope + 4), scale * rk::kLog2e, clat, lse, plan.groups, partial, bad_rows};
+                         (size_t)page_tokens * (size_t)(kvl + rope + 4), qscale, clat, lse, plan.groups, partial, bad_rows};
     const hipStream_t st = (hipStream_t)stream;
     (void)hipGetLastError();
     if (plain) {

@@ -33,6 +33,7 @@ constexpr int kTreeRopeAt = 8 * 4096;
 constexpr int kTreeTileBytes = kTreeRopeAt + 4 * 1024;
 constexpr int kTreeSteps = 18;            // of 16 dims a wave: 16 of its 256 latent dims, two of its 32 roped ones
 constexpr float kTreeGrow = 24.0f;
+constexpr uint32_t kTreeHole = 0x80000000u;  // the scale of a token that is not there: -0
 
 // A block of rows among a call's: its sequence, number and tiles, and the work units (tiles, or blocks where they are whole) before it.
 struct TreeBlock {
@@ -54,6 +55,11 @@ __device__ __forceinline__ long long lanes_up_to(long long x) {
     }
     return x;
 }
+// A value that is the same in every lane, as the compiler does not know: in scalar registers. What a workgroup's branches and loops go by is
+// kept there, so that none of them is a branch around masked lanes.
+__device__ __forceinline__ long long uniform(long long x) {
+    return ((long long)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)x);
+}
 __device__ __forceinline__ long long tree_total(const TreeArgs& a, bool whole) {
     const int lane = threadIdx.x & 63;
     long long sum = 0;
@@ -62,7 +68,7 @@ __device__ __forceinline__ long long tree_total(const TreeArgs& a, bool whole) {
         tree_units(a, s0 + lane, blocks, tiles);
         sum += whole ? (long long)blocks : (long long)blocks * tiles;
     }
-    return __shfl(lanes_up_to(sum), kWave - 1, kWave);
+    return uniform(__shfl(lanes_up_to(sum), kWave - 1, kWave));
 }
 // The block that holds unit u of them.
 __device__ __forceinline__ TreeBlock tree_block(const TreeArgs& a, bool whole, long long u) {
@@ -77,16 +83,15 @@ __device__ __forceinline__ TreeBlock tree_block(const TreeArgs& a, bool whole, l
         const unsigned long long past = __builtin_amdgcn_ballot_w64(u < upto);
         if (past) {
             const int at = __builtin_ctzll(past);
-            const long long before = __shfl(upto - mine, at, kWave);
+            const long long before = uniform(__shfl(upto - mine, at, kWave));
             b.seq = s0 + at;
             b.blocks = __builtin_amdgcn_readlane(blocks, at), b.tiles = __builtin_amdgcn_readlane(tiles, at);
             const long long rel = u - before;
             b.rb = (int)(whole ? rel : rel / b.tiles);
             b.first = before + (whole ? (long long)b.rb : (long long)b.rb * b.tiles);
-            b.seq = __builtin_amdgcn_readfirstlane(b.seq), b.rb = __builtin_amdgcn_readfirstlane(b.rb);
             return b;
         }
-        run = __shfl(upto, kWave - 1, kWave);
+        run = uniform(__shfl(upto, kWave - 1, kWave));
     }
     b.seq = -1;
     return b;
@@ -101,11 +106,13 @@ __device__ __forceinline__ int tree_items(const TreeArgs& a, long long total) {
 __device__ __forceinline__ long long tree_item_lo(int item, int items, long long total) { return (long long)item * total / items; }
 __device__ __forceinline__ int tree_item_of(long long unit, int items, long long total) { return (int)(((unit + 1) * items - 1) / total); }
 
+// (Weights carry their token's scale times the softmax's: one number a token for both products; results are divided by the softmax's.)
 struct TreeShared {
     uint8_t tiles[kTreeBuffers * kTreeTileBytes];
     f32x4 part[4][4][kWave];             // partial scores on their way to wave (th, kh)
     uint8_t weights[2][kTreeRows * kTreeTokens * 2];  // by the tile's parity
-    float scale[kTreeBuffers][2][kTreeTokens];  // of a tile's tokens: the scale (0: not there), and times the softmax's
+    float scale[kTreeBuffers][kTreeTokens];  // of a tile's tokens, times the softmax's; kTreeHole: not there
+    float spare[kWave];
     float top[2][kTreeRows], corr[kTreeRows], sum[2][kTreeRows], ref[kTreeRows];
     // numbers of the latest tile of which some row outgrew its reference, and of which some token is not there
     alignas(8) int grown;
@@ -217,20 +224,24 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
     // a zero weight). A scale that is not a positive number cannot come from the append: such a row is not there.
     auto arrived = [&](int buf, int of) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        bool ok[2];
 #pragma unroll
         for (int o = 0; o < 2; ++o) {
-            const bool ok = there[o] && raw_scale[o] > 0.0f;
-            if (__builtin_amdgcn_ballot_w64(!ok) != 0 && !ok) {
-                sh->holed = of;
-                const lds_ptr<uint8_t> to = tiles + buf * kTreeTileBytes + 16 * lane;
+            ok[o] = there[o] & (raw_scale[o] > 0.0f);
+            // (a row's eight lanes: the first has its place, the others a spare one, which costs less than a branch)
+            const lds_ptr<float> to = l8 == 0 ? &sh->scale[buf][16 * wave + 8 * o + r8] : &sh->spare[lane];
+            *to = ok[o] ? raw_scale[o] * a.qscale : __uint_as_float(kTreeHole);
+        }
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(ok[0] & ok[1])) != 0, 0)) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) *(lds_ptr<u32x4>)(to + (2 * wave + o) * 4096 + 1024 * i) = u32x4{0, 0, 0, 0};
-                if ((l8 ^ swap_of(o)) < 4) *(lds_ptr<u32x4>)(to + kTreeRopeAt + wave * 1024) = u32x4{0, 0, 0, 0};
-            }
-            if (l8 == 0) {
-                const int row = 16 * wave + 8 * o + r8;
-                sh->scale[buf][0][row] = ok ? raw_scale[o] : 0.0f, sh->scale[buf][1][row] = ok ? raw_scale[o] * a.qscale : 0.0f;
-            }
+            for (int o = 0; o < 2; ++o)
+                if (!ok[o]) {
+                    sh->holed = of;
+                    const lds_ptr<uint8_t> to = tiles + buf * kTreeTileBytes + 16 * lane;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) *(lds_ptr<u32x4>)(to + (2 * wave + o) * 4096 + 1024 * i) = u32x4{0, 0, 0, 0};
+                    if ((l8 ^ swap_of(o)) < 4) *(lds_ptr<u32x4>)(to + kTreeRopeAt + wave * 1024) = u32x4{0, 0, 0, 0};
+                }
         }
     };
 
@@ -304,11 +315,11 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
                 if (i + 2 < 9) load(i + 2);
                 const u32x4 then = k[(i + 1) % 3];
                 x[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lo, __builtin_bit_cast(bf16x8, q[2 * i][0]), x[0], 0, 0, 0);
-                if (MORE && (i == 0 || i == 4)) find(i / 4);
+                if (MORE && i < 2) find(i);
                 __builtin_amdgcn_sched_barrier(0);
                 x[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lo, __builtin_bit_cast(bf16x8, q[2 * i][1]), x[1], 0, 0, 0);
                 if (i < 8) lo = as_bf16(then.x, then.y);
-                if (MORE && i % 4 != 0) bring((i - 1) / 4, (i - 1) % 4, third);
+                if (MORE && i >= 2 && i < 8) bring((i - 2) / 3, (i - 2) % 3, third);
                 __builtin_amdgcn_sched_barrier(0);
                 x[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(hi, __builtin_bit_cast(bf16x8, q[2 * i + 1][0]), x[0], 0, 0, 0);
                 if (MORE && i >= 5 && i < 7) go_on(i - 5), look_up(i - 5);
@@ -323,7 +334,7 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
         };
         // Which of the wave's 32 tokens of a tile the lane's row sees, a bit a token.
         auto seen_of = [&](int i, int buf) -> uint32_t {
-            const uint32_t is_there = (uint32_t)__builtin_amdgcn_ballot_w64(sh->scale[buf][0][32 * th + n32] > 0.0f);
+            const uint32_t is_there = (uint32_t)__builtin_amdgcn_ballot_w64(__float_as_uint(sh->scale[buf][32 * th + n32]) != kTreeHole);
             const int t0 = (tile_lo + i) * kTreeTokens + 32 * th;
             if (t0 + 32 <= s.ctx) return is_there;
             const int j0 = t0 - s.ctx;                  // drafted row of bit 0
@@ -355,15 +366,14 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
             l_sum = l_before;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const f32x4 scale = *(lds_ptr<f32x4>)&sh->scale[buf][0][32 * th + 8 * i + 4 * half];
-                const f32x4 by = *(lds_ptr<f32x4>)&sh->scale[buf][1][32 * th + 8 * i + 4 * half];
+                const f32x4 by = *(lds_ptr<f32x4>)&sh->scale[buf][32 * th + 8 * i + 4 * half];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const float y = bit_of(4 * i + k) ? __builtin_fmaf(sc[4 * i + k], by[k], -mu) : -INFINITY;
                     most = fmaxf(most, y);
                     const float e = __builtin_amdgcn_exp2f(y);
                     l_sum += e;
-                    p[4 * i + k] = bit_of(4 * i + k) ? e * scale[k] : 0.0f;
+                    p[4 * i + k] = bit_of(4 * i + k) ? e * by[k] : 0.0f;
                 }
             }
             put_weights(p, parity);
@@ -375,7 +385,7 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
             float x[16];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const f32x4 by = *(lds_ptr<f32x4>)&sh->scale[buf][1][32 * th + 8 * i + 4 * half];
+                const f32x4 by = *(lds_ptr<f32x4>)&sh->scale[buf][32 * th + 8 * i + 4 * half];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     x[4 * i + k] = bit_of(4 * i + k) ? sc[4 * i + k] * by[k] : -INFINITY;
@@ -397,12 +407,12 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
             float p[16];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const f32x4 scale = *(lds_ptr<f32x4>)&sh->scale[buf][0][32 * th + 8 * i + 4 * half];
+                const f32x4 by = *(lds_ptr<f32x4>)&sh->scale[buf][32 * th + 8 * i + 4 * half];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const float e = __builtin_amdgcn_exp2f(x[4 * i + k] - mu);
                     l_sum += e;
-                    p[4 * i + k] = bit_of(4 * i + k) ? e * scale[k] : 0.0f;
+                    p[4 * i + k] = bit_of(4 * i + k) ? e * by[k] : 0.0f;
                 }
             }
             put_weights(p, parity);
@@ -431,7 +441,7 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
                 for (int b = 0; b < 2; ++b) w[ks & 1][b] = *(lds_ptr<bf16x8>)(w_from + 32 * b * (2 * kTreeTokens) + 16 * ((2 * ks + half) ^ k_swap));
             };
             load(0), load_w(0), load(1), load(2);
-            f32x4 part[4], scale, by;
+            f32x4 part[4], by;
             const float mu = m_ref == -INFINITY ? 0.0f : m_ref;
             float most = -INFINITY, p[4];
             if (NEXT) {
@@ -440,21 +450,18 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
 #pragma unroll
                 for (int i = 0; i < 4; ++i) part[i] = sh->part[2 * th + kh][i][lane];
             }
-            auto scales = [&](int i) {
-                scale = *(lds_ptr<f32x4>)&sh->scale[next][0][32 * th + 8 * i + 4 * half];
-                by = *(lds_ptr<f32x4>)&sh->scale[next][1][32 * th + 8 * i + 4 * half];
-            };
-            float y;
+            float y = -INFINITY, y_before;
             auto first = [&](int r) {
-                if ((r & 3) == 0) scales(r >> 2);
+                if ((r & 3) == 0) by = *(lds_ptr<f32x4>)&sh->scale[next][32 * th + 8 * (r >> 2) + 4 * half];
                 sc[r] += part[r >> 2][r & 3];
+                y_before = y;
                 y = __builtin_fmaf(sc[r], by[r & 3], -mu);
-                most = fmaxf(most, y);
-                y = __builtin_amdgcn_exp2f(y);
+                if (r & 1) most = fmaxf(most, fmaxf(y_before, y));
+                p[r & 3] = __builtin_amdgcn_exp2f(y);
             };
             auto second = [&](int r) {
-                l_sum += y;
-                p[r & 3] = y * scale[r & 3];
+                l_sum += p[r & 3];
+                p[r & 3] *= by[r & 3];
                 if ((r & 3) == 3)
                     *(lds_ptr<u32x2>)(w_row + (parity ^ 1) * (kTreeRows * kTreeTokens * 2) + 16 * ((4 * th + (r >> 2)) ^ w_swap)) =
                         u32x2{pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3])};
@@ -579,7 +586,7 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
         for (int b = 0; b < 2; ++b) {
             const int r = kTreeRows * rb + 32 * b + n32;
             const float l = sh->sum[0][32 * b + n32] + sh->sum[1][32 * b + n32];
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            const float inv = l == 0.0f ? 0.0f : 1.0f / (l * a.qscale);
             if (r < rows) {
                 uint16_t* const dst = a.clat + ((size_t)s.node0 * a.H + r) * 512 + 128 * wave + 4 * half;
 #pragma unroll
@@ -637,7 +644,7 @@ __global__ __launch_bounds__(256) void mla_attend_tree_merge_kernel(const TreeAr
             if (s0 + lane < by_block.seq) tree_units(a, s0 + lane, blocks, tiles);
             before += (long long)blocks * tiles;
         }
-        before = __shfl(lanes_up_to(before), kWave - 1, kWave);
+        before = uniform(__shfl(lanes_up_to(before), kWave - 1, kWave));
     }
     const long long first = before + (long long)by_block.rb * by_block.tiles;
     const int g0 = tree_item_of(first, items, total), g1 = tree_item_of(first + by_block.tiles - 1, items, total);
@@ -660,7 +667,7 @@ __global__ __launch_bounds__(256) void mla_attend_tree_merge_kernel(const TreeAr
     const TreeSeq s = tree_seq(a, by_block.seq);
     const int r = kTreeRows * by_block.rb + row;
     if (r >= s.nodes * a.H) return;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / (l * a.qscale);
     const size_t out = (size_t)s.node0 * a.H + r;
     *reinterpret_cast<u32x2*>(a.clat + out * 512 + 128 * wave + 16 * c + 64 * (i >> 1) + 8 * (i & 1) + 4 * (lane >> 5)) =
         u32x2{pack_bf16x2(sum[0] * inv, sum[1] * inv), pack_bf16x2(sum[2] * inv, sum[3] * inv)};
