@@ -35,7 +35,7 @@ NO_SCRATCH = {"mla_attend.hip": [("mla_attend_paged_kernel", "Lb1EEEvNS_10Attend
                                  ("mla_attend_heads16_kernel", "EEEvNS_10AttendArgsE"),
                                  ("mla_attend_few_kernel", "EEEvNS_10AttendArgsE"),
                                  ("mla_attend_wide_kernel", "EEEvNS_10AttendArgsE")],
-              "mla_attend_tree.hip": [("mla_attend_tree_kernel", "ENS_8TreeArgsE")]}
+              "mla_attend_tree.hip": [("mla_attend_tree_kernel", "EEEvNS_8TreeArgsE")]}
 
 
 def check_resources(k: str, report: str) -> None:

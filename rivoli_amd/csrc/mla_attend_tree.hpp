@@ -11,11 +11,14 @@
 //     load, and only the weights (8 KB) are read by all four.
 // Codes go from memory into LDS as they are, three tiles in rotation, and become bf16 (exact) when an operand is read, once for the
 // workgroup. 32 x 32 matrix tiles: a fragment serves two of them.
-// An iteration has the scores of tile i + 1, then (partial scores having met at a barrier) the softmax of i + 1 under the values of
-// tile i; a second barrier ends it. The softmax's reference is that of the rows' first tile: weights are bf16 and sums f32, whose
-// exponents reach 2^127, so a row is rescaled only when a score grows by 2^kTreeGrow past its reference, which every wave learns
-// from a flag a tile late (regrow). Weights are rounded to bf16 once where they meet the values (2^-8 of a weight, at random, against the
-// 2^-8 of the rounded result); their sum, and so lse, is of the unrounded ones.
+// An iteration has two halves, a barrier behind each: the scores of tile i + 1, with tile i's softmax and the transfers of tile i + 2
+// between their matrix instructions; then the values of tile i, with the partial scores of i + 1 meeting. The softmax's
+// reference is that of the rows' first tile: weights are bf16 and sums f32, whose exponents reach 2^127, so a row is rescaled only when
+// a score grows by 2^kTreeGrow past its reference, which every wave learns from a flag behind the first barrier (regrow). Weights are
+// rounded to bf16 once where they meet the values (2^-8 of a weight, at random, against the 2^-8 of the rounded result); their
+// sum, and so lse, is of the unrounded ones.
+// One wave a SIMD issues an instruction in four cycles at best, so what counts beside the matrix instructions is how many others there are and
+// what waits: fragments are asked for steps ahead of their use, control flow and a run's address are scalar, rare work sits behind flags.
 #pragma once
 
 namespace rk {
@@ -59,6 +62,15 @@ __device__ __forceinline__ long long lanes_up_to(long long x) {
 // kept there, so that none of them is a branch around masked lanes.
 __device__ __forceinline__ long long uniform(long long x) {
     return ((long long)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)x);
+}
+// f(0) .. f(N - 1), the numbers being constants of the compiler's.
+template <int N, class F, int... I>
+__device__ __forceinline__ void each_of(F&& f, std::integer_sequence<int, I...>) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, class F>
+__device__ __forceinline__ void each(F&& f) {
+    each_of<N>(static_cast<F&&>(f), std::make_integer_sequence<int, N>{});
 }
 __device__ __forceinline__ long long tree_total(const TreeArgs& a, bool whole) {
     const int lane = threadIdx.x & 63;
@@ -110,37 +122,43 @@ __device__ __forceinline__ int tree_item_of(long long unit, int items, long long
 struct TreeShared {
     uint8_t tiles[kTreeBuffers * kTreeTileBytes];
     f32x4 part[4][4][kWave];             // partial scores on their way to wave (th, kh)
-    uint8_t weights[2][kTreeRows * kTreeTokens * 2];  // by the tile's parity
+    uint8_t weights[kTreeRows * kTreeTokens * 2];
     float scale[kTreeBuffers][kTreeTokens];  // of a tile's tokens, times the softmax's; kTreeHole: not there
     float spare[kWave];
     float top[2][kTreeRows], corr[kTreeRows], sum[2][kTreeRows], ref[kTreeRows];
     // numbers of the latest tile of which some row outgrew its reference, and of which some token is not there
-    alignas(8) int grown;
-    int holed;
+    int grown, holed[2];                 // (the second by the tile's parity)
 };
 static_assert(sizeof(TreeShared) <= 160 * 1024, "one workgroup per compute unit");
 
-// A lane's pieces of a row's codes, in parts, so that the transfers go between matrix instructions one or two at a time: two of the four latent
-// groups (FIRST and the next), 128 bytes apart in memory and 1024 in LDS; the roped codes for the lanes of `roped`. As few_dma_row.
-template <int FIRST>
-__device__ __forceinline__ void tree_dma_latent(const uint8_t* src, lds_ptr<uint8_t> to) {
-    const uint32_t base = (uint32_t)(uintptr_t)to + (1024 - 128) * FIRST;
+// A lane's piece of a row's codes on its way to LDS, one of five, so that transfers go between matrix instructions one at a time: of the latent
+// groups 0 .. 3, 128 bytes apart in memory and 1024 in LDS, or (4) the roped codes, for the lanes of `roped`. `to` is the row's place
+// in the tile's latent codes, `to_rope` in its roped ones. The instruction's offset counts in memory and in LDS. As dma16_from: from a scalar
+// address and a lane's 32 bits, or (base null) a lane's 64.
+template <int PIECE, bool RUNS>
+__device__ __forceinline__ void tree_dma(unsigned long long base, uint32_t off, const uint8_t* src, lds_ptr<uint8_t> to, lds_ptr<uint8_t> to_rope,
+                                         unsigned long long roped) {
     uint32_t keep;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off offset:%3\n\t"
-                 "s_add_u32 m0, m0, 896\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off offset:%4\n\ts_mov_b32 m0, %0"
-                 : "=&s"(keep)
-                 : "v"(src), "s"(base), "n"(128 * FIRST), "n"(128 * FIRST + 128)
-                 : "memory", "scc");
-}
-__device__ __forceinline__ void tree_dma_rope(const uint8_t* src, lds_ptr<uint8_t> to, unsigned long long roped) {
-    const uint32_t base = (uint32_t)(uintptr_t)to - 512u;
-    uint32_t keep;
-    unsigned long long all;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_and_saveexec_b64 %1, %4\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off offset:512\n\t"
-                 "s_mov_b64 exec, %1\n\ts_mov_b32 m0, %0"
-                 : "=&s"(keep), "=&s"(all)
-                 : "v"(src), "s"(base), "s"(roped)
-                 : "memory", "scc");
+    if constexpr (PIECE < 4) {
+        const uint32_t at = (uint32_t)(uintptr_t)to + (1024 - 128) * PIECE;
+        if constexpr (RUNS)
+            asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:%4\n\ts_mov_b32 m0, %0"
+                         : "=&s"(keep) : "v"(off), "s"(base), "s"(at), "n"(128 * PIECE) : "memory");
+        else
+            asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off offset:%3\n\ts_mov_b32 m0, %0"
+                         : "=&s"(keep) : "v"(src), "s"(at), "n"(128 * PIECE) : "memory");
+    } else {
+        const uint32_t at = (uint32_t)(uintptr_t)to_rope - 512u;
+        unsigned long long all;
+        if constexpr (RUNS)
+            asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %4\n\ts_and_saveexec_b64 %1, %5\n\ts_nop 0\n\t"
+                         "global_load_lds_dwordx4 %2, %3 offset:512\n\ts_mov_b64 exec, %1\n\ts_mov_b32 m0, %0"
+                         : "=&s"(keep), "=&s"(all) : "v"(off), "s"(base), "s"(at), "s"(roped) : "memory", "scc");
+        else
+            asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_and_saveexec_b64 %1, %4\n\ts_nop 0\n\t"
+                         "global_load_lds_dwordx4 %2, off offset:512\n\ts_mov_b64 exec, %1\n\ts_mov_b32 m0, %0"
+                         : "=&s"(keep), "=&s"(all) : "v"(src), "s"(at), "s"(roped) : "memory", "scc");
+    }
 }
 
 // Codes that are no number as zeros.
@@ -151,13 +169,14 @@ __device__ __forceinline__ uint32_t numbers_only(uint32_t c) {
 
 // Tiles [tile_lo, tile_hi) of rows 64 rb .. of a sequence. `whole`: they are all it has, results go out; else its record.
 // `number`: a count of the tiles the workgroup has had, for the flag.
+template <bool RUNS>
 __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeShared> sh, const TreeSeq& s, int seq, int rb, bool last_block,
                                           int tile_lo, int tile_hi, bool whole, float* rec, int& number) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int half = lane >> 5, n32 = lane & 31;
     const int th = wave & 1, kh = wave >> 1;  // its 32 tokens and its half of the dims, in the scores
     const lds_ptr<uint8_t> tiles = (lds_ptr<uint8_t>)&sh->tiles[0];
-    const lds_ptr<uint8_t> weights = (lds_ptr<uint8_t>)&sh->weights[0][0];
+    const lds_ptr<uint8_t> weights = (lds_ptr<uint8_t>)&sh->weights[0];
     const int rows = s.nodes * a.H;           // of the sequence
     // what the block's last row may see: a chain's later nodes are nobody's business here
     const int last_row = min(kTreeRows * rb + kTreeRows, rows) - 1;
@@ -165,66 +184,79 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
     const int n_tiles = min(tile_hi, (len + kTreeTokens - 1) / kTreeTokens) - tile_lo;
 
     // ---- where a tile's rows are: eight lanes have rows 16 wave + 8 o + (lane >> 3) -----------------------------
-    // Lookups and transfers have no branches, so that they go between the matrix instructions: tiles past the end are asked for too (of
-    // the pool's first row), and a row's page and its place in it move on by a tile's tokens without a division.
+    // Lookups and transfers have no branches, so that they go between the matrix instructions: tiles past the end are asked for too,
+    // and a row's page and its place in it move on by a tile's tokens without a division. RUNS: pages are whole runs of 16 rows, so that the
+    // wave's rows have one page and one place, which are scalar.
     const int l8 = lane & 7, r8 = lane >> 3;
     const int end_row = min(len, tile_hi * kTreeTokens);
     const int* const table = a.block_table + (size_t)seq * a.max_blocks;
     const unsigned page_tokens = (unsigned)a.page_tokens, on_pages = kTreeTokens / page_tokens, on_rows = kTreeTokens % page_tokens;
-    int token[2], page[2];        // of the tile to be asked for
-    unsigned block[2], place[2];  // of it; and of the next when that has been looked up
+    constexpr int kRuns = RUNS ? 1 : 2;
+    int token[kRuns], page[kRuns];            // of the tile to be asked for
+    unsigned block[kRuns], place[kRuns];      // of it; and of the next when that has been looked up
 #pragma unroll
-    for (int o = 0; o < 2; ++o) {
-        token[o] = tile_lo * kTreeTokens + 16 * wave + 8 * o + r8;
+    for (int o = 0; o < kRuns; ++o) {
+        token[o] = tile_lo * kTreeTokens + 16 * wave + (RUNS ? 0 : 8 * o + r8);
         block[o] = (unsigned)token[o] / page_tokens, place[o] = (unsigned)token[o] - block[o] * page_tokens;
     }
-    auto look_up = [&](int o) { page[o] = table[min(block[o], (unsigned)a.max_blocks - 1)]; };
-    unsigned int missing = 0;     // rows of the block's that have no page
+    int no_lane = 0;                          // (a vector zero: the page is a load of every lane, not a scalar one, which LDS reads would wait for)
+    if (RUNS) asm volatile("" : "+v"(no_lane));
+    auto look_up = [&](int o) { page[o] = table[min(block[o], (unsigned)a.max_blocks - 1) + no_lane]; };
+    unsigned int missing = 0;                 // rows of the block's that have no page
     bool there[2];
     float raw_scale[2];
-    auto scalar = [](lds_ptr<uint8_t> p) -> lds_ptr<uint8_t> {  // the transfers take their LDS base from a scalar register
-        return (lds_ptr<uint8_t>)(uintptr_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)p);
-    };
     auto swap_of = [&](int o) -> int { return (4 * o + (r8 >> 1)) & 7; };
     const unsigned long long roped[2] = {__builtin_amdgcn_ballot_w64((l8 ^ swap_of(0)) < 4), __builtin_amdgcn_ballot_w64((l8 ^ swap_of(1)) < 4)};
     const uint32_t page_bytes = (uint32_t)a.page_bytes, codes_bytes = page_tokens * 576u;
-    const uint8_t* src[2];
+    const uint8_t* src[2] = {nullptr, nullptr};
+    unsigned long long base = 0;              // RUNS: of the wave's rows
+    const uint32_t lane_off[2] = {576u * (uint32_t)r8 + 16u * (uint32_t)(l8 ^ swap_of(0)), 576u * (uint32_t)(8 + r8) + 16u * (uint32_t)(l8 ^ swap_of(1))};
     auto find = [&](int o) {  // the lane's row of a tile looked up: its address, and its scale asked for
-        const bool mine = token[o] < end_row;
-        there[o] = mine & (block[o] < (unsigned)a.max_blocks) & ((unsigned)page[o] < (unsigned)a.n_pages);
-        missing += mine & !there[o];
-        const unsigned off = there[o] ? place[o] : 0u;
-        const uint8_t* const base = a.pool + (unsigned long long)(there[o] ? (unsigned)page[o] : 0u) * page_bytes;
-        raw_scale[o] = *reinterpret_cast<const float*>(base + (codes_bytes + 4u * off));
-        src[o] = base + (off * 576u + 16u * (unsigned)(l8 ^ swap_of(o)));
+        if constexpr (RUNS) {
+            const unsigned at = (unsigned)__builtin_amdgcn_readfirstlane(page[0]);
+            const bool has = block[0] < (unsigned)a.max_blocks && at < (unsigned)a.n_pages;
+            const bool mine = token[0] + 8 * o + r8 < end_row;
+            there[o] = mine & has;
+            missing += mine & !has;
+            const uint8_t* const run = a.pool + (unsigned long long)(has ? at : 0u) * page_bytes;
+            raw_scale[o] = *reinterpret_cast<const float*>(run + codes_bytes + 4u * place[0] + 4u * (8u * o + r8));
+            base = (unsigned long long)(uintptr_t)run + 576u * place[0];
+        } else {
+            const bool mine = token[o] < end_row;
+            there[o] = mine & (block[o] < (unsigned)a.max_blocks) & ((unsigned)page[o] < (unsigned)a.n_pages);
+            missing += mine & !there[o];
+            const unsigned off = there[o] ? place[o] : 0u;
+            const uint8_t* const from = a.pool + (unsigned long long)(there[o] ? (unsigned)page[o] : 0u) * page_bytes;
+            raw_scale[o] = *reinterpret_cast<const float*>(from + (codes_bytes + 4u * off));
+            src[o] = from + (off * 576u + 16u * (unsigned)(l8 ^ swap_of(o)));
+        }
     };
-    auto bring = [&](int o, int part, int buf) {  // in three parts
-        const lds_ptr<uint8_t> to = scalar(tiles + buf * kTreeTileBytes + (2 * wave + o) * 4096);
-        if (part == 0) tree_dma_latent<0>(src[o], to);
-        if (part == 1) tree_dma_latent<2>(src[o], to);
-        if (part == 2) tree_dma_rope(src[o], scalar(tiles + buf * kTreeTileBytes + kTreeRopeAt + wave * 1024), roped[o]);
+    // Of the tile found: piece k of ten, five an octet.
+    auto bring = [&](auto number_of, int buf) {
+        constexpr int k = decltype(number_of)::value, o = k / 5;
+        const lds_ptr<uint8_t> tile = tiles + buf * kTreeTileBytes;
+        tree_dma<k % 5, RUNS>(base, lane_off[o], src[o], tile + (2 * wave + o) * 4096, tile + kTreeRopeAt + wave * 1024, roped[o]);
     };
     auto go_on = [&](int o) {
+        if (o >= kRuns) return;
         token[o] += kTreeTokens;
         place[o] += on_rows;
         const bool over = place[o] >= page_tokens;
         place[o] -= over ? page_tokens : 0u;
         block[o] += on_pages + (over ? 1u : 0u);
+        look_up(o);
     };
     auto ask = [&](int buf) {
-#pragma unroll
-        for (int o = 0; o < 2; ++o) {
-            find(o);
-#pragma unroll
-            for (int part = 0; part < 3; ++part) bring(o, part, buf);
-            go_on(o), look_up(o);
-        }
+        find(0), find(1);
+        each<10>([&](auto k) { bring(k, buf); });
+        go_on(0), go_on(1);
     };
-    // The transfers asked for have landed: scales, and zeros for rows that are not there (codes must be finite, they meet
-    // a zero weight). A scale that is not a positive number cannot come from the append: such a row is not there.
-    auto arrived = [&](int buf, int of) {
+    // The transfers asked for have landed: scales, and (holes) zeros for rows that are not there: codes must be finite, they meet a zero
+    // weight. A scale that is not a positive number cannot come from the append: such a row is not there.
+    bool ok[2];
+    unsigned long long holes = 0;
+    auto arrived = [&](int buf) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        bool ok[2];
 #pragma unroll
         for (int o = 0; o < 2; ++o) {
             ok[o] = there[o] & (raw_scale[o] > 0.0f);
@@ -232,17 +264,19 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
             const lds_ptr<float> to = l8 == 0 ? &sh->scale[buf][16 * wave + 8 * o + r8] : &sh->spare[lane];
             *to = ok[o] ? raw_scale[o] * a.qscale : __uint_as_float(kTreeHole);
         }
-        if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(ok[0] & ok[1])) != 0, 0)) {
+        holes = __builtin_amdgcn_ballot_w64(!(ok[0] & ok[1]));
+    };
+    auto fill_holes = [&](int buf, int of) {
+        if (__builtin_expect(holes == 0, 1)) return;
+        sh->holed[of & 1] = of;
 #pragma unroll
-            for (int o = 0; o < 2; ++o)
-                if (!ok[o]) {
-                    sh->holed = of;
-                    const lds_ptr<uint8_t> to = tiles + buf * kTreeTileBytes + 16 * lane;
+        for (int o = 0; o < 2; ++o)
+            if (!ok[o]) {
+                const lds_ptr<uint8_t> to = tiles + buf * kTreeTileBytes + 16 * lane;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) *(lds_ptr<u32x4>)(to + (2 * wave + o) * 4096 + 1024 * i) = u32x4{0, 0, 0, 0};
-                    if ((l8 ^ swap_of(o)) < 4) *(lds_ptr<u32x4>)(to + kTreeRopeAt + wave * 1024) = u32x4{0, 0, 0, 0};
-                }
-        }
+                for (int i = 0; i < 4; ++i) *(lds_ptr<u32x4>)(to + (2 * wave + o) * 4096 + 1024 * i) = u32x4{0, 0, 0, 0};
+                if ((l8 ^ swap_of(o)) < 4) *(lds_ptr<u32x4>)(to + kTreeRopeAt + wave * 1024) = u32x4{0, 0, 0, 0};
+            }
     };
 
     f32x16 o[4][2];  // O^T: column tile c of 32, row block b: sixteen columns a lane, of row 32 b + n32
@@ -253,7 +287,8 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
     const int own_node = (live ? own_row : 0) / a.H;
 
     if (n_tiles > 0) {
-        look_up(0), look_up(1);
+        look_up(0);
+        if (!RUNS) look_up(1);
         u32x4 q[kTreeSteps][2];  // of the rows that are the wave's in the softmax, and of the others
         ask(0);
         // ---- the rows' operands: K-steps of 16 dims, eight a lane. Two K-steps share a 16-byte piece of codes. They live in the
@@ -294,44 +329,6 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
             const u32x4 d = {d0, d1, d2, d3};
             return __builtin_bit_cast(bf16x8, d);
         };
-        // S^T[token][row] of the wave's tokens over its half of the dims, the others' 32 rows' of it on their way to the other half's
-        // wave; and between its matrix instructions the next tile but one is asked for. A piece of codes is out of LDS two steps and converted
-        // one step before its matrix instructions; the fences keep that order.
-        f32x16 sc;
-        auto scores = [&](int buf, auto more, int third, auto before) {
-            constexpr bool MORE = decltype(more)::value;
-            const lds_ptr<uint8_t> codes = tiles + buf * kTreeTileBytes;
-            u32x4 k[3];
-            auto load = [&](int i) {
-                k[i % 3] = *(lds_ptr<u32x4>)(codes + (i < 8 ? k_row + 1024 * (i >> 2) + 16 * ((2 * (i & 3) + half) ^ k_swap) : k_rope));
-            };
-            load(0), load(1);
-            before();
-            f32x16 x[2] = {f32x16{}, f32x16{}};
-            bf16x8 lo = as_bf16(k[0].x, k[0].y), hi = as_bf16(k[0].z, k[0].w);
-#pragma unroll
-            for (int i = 0; i < 9; ++i) {
-                __builtin_amdgcn_sched_barrier(0);
-                if (i + 2 < 9) load(i + 2);
-                const u32x4 then = k[(i + 1) % 3];
-                x[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lo, __builtin_bit_cast(bf16x8, q[2 * i][0]), x[0], 0, 0, 0);
-                if (MORE && i < 2) find(i);
-                __builtin_amdgcn_sched_barrier(0);
-                x[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lo, __builtin_bit_cast(bf16x8, q[2 * i][1]), x[1], 0, 0, 0);
-                if (i < 8) lo = as_bf16(then.x, then.y);
-                if (MORE && i >= 2 && i < 8) bring((i - 2) / 3, (i - 2) % 3, third);
-                __builtin_amdgcn_sched_barrier(0);
-                x[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(hi, __builtin_bit_cast(bf16x8, q[2 * i + 1][0]), x[0], 0, 0, 0);
-                if (MORE && i >= 5 && i < 7) go_on(i - 5), look_up(i - 5);
-                __builtin_amdgcn_sched_barrier(0);
-                x[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(hi, __builtin_bit_cast(bf16x8, q[2 * i + 1][1]), x[1], 0, 0, 0);
-                if (i < 8) hi = as_bf16(then.z, then.w);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-            sc = x[0];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sh->part[2 * th + 1 - kh][i][lane] = f32x4{x[1][4 * i], x[1][4 * i + 1], x[1][4 * i + 2], x[1][4 * i + 3]};
-        };
         // Which of the wave's 32 tokens of a tile the lane's row sees, a bit a token.
         auto seen_of = [&](int i, int buf) -> uint32_t {
             const uint32_t is_there = (uint32_t)__builtin_amdgcn_ballot_w64(__float_as_uint(sh->scale[buf][32 * th + n32]) != kTreeHole);
@@ -349,88 +346,138 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
             }
             return bits & is_there;
         };
+        f32x16 sc;               // a tile's scores: of token 8 (r >> 2) + 4 half + (r & 3) in register r
         uint32_t seen = ~0u;
-        // token of register r: 8 (r >> 2) + 4 half + (r & 3)
         auto bit_of = [&](int r) -> bool { return seen >> (8 * (r >> 2) + 4 * half + (r & 3)) & 1; };
         const lds_ptr<uint8_t> w_row = weights + own * (2 * kTreeTokens) + 8 * half;
         const int w_swap = (own >> 1) & 7;
-        auto put_weights = [&](const float (&p)[16], int parity) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                *(lds_ptr<u32x2>)(w_row + parity * (kTreeRows * kTreeTokens * 2) + 16 * ((4 * th + i) ^ w_swap)) = u32x2{pack_bf16x2(p[4 * i], p[4 * i + 1]), pack_bf16x2(p[4 * i + 2], p[4 * i + 3])};
+        auto scales_of = [&](int buf, int i) -> f32x4 { return *(lds_ptr<f32x4>)&sh->scale[buf][32 * th + 8 * i + 4 * half]; };
+        auto put_weights = [&](int i, const float (&p)[4]) {
+            *(lds_ptr<u32x2>)(w_row + 16 * ((4 * th + i) ^ w_swap)) = u32x2{pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3])};
         };
-        // Weights of a tile with tokens that some row does not see, in place of those that step() made of it; the largest exponent.
-        auto weigh_seen = [&](int buf, int parity) -> float {
-            const float mu = m_ref == -INFINITY ? 0.0f : m_ref;
-            float p[16], most = -INFINITY;
-            l_sum = l_before;
+        // A tile's weights out of its scores, a token at a time; l_sum and the largest exponent go along. As if every row saw every token.
+        f32x4 by;
+        float mu = 0.0f, most = -INFINITY, y = 0.0f, p[4];
+        auto weigh_begin = [&](int buf) {
+            mu = m_ref == -INFINITY ? 0.0f : m_ref, most = -INFINITY, l_before = l_sum;
+            by = scales_of(buf, 0);
+        };
+        auto weigh = [&](int buf, int r) {
+            const float before = y;
+            y = __builtin_fmaf(sc[r], by[r & 3], -mu);
+            if (r & 1) most = fmaxf(most, fmaxf(before, y));
+            const float e = __builtin_amdgcn_exp2f(y);
+            l_sum += e;
+            p[r & 3] = e * by[r & 3];
+            if ((r & 3) == 3) {
+                put_weights(r >> 2, p);
+                if (r < 15) by = scales_of(buf, (r >> 2) + 1);
+            }
+        };
+        // The same of a tile with tokens that some row does not see, in place of what weigh() made of it.
+        auto weigh_seen = [&](int buf) {
+            most = -INFINITY, l_sum = l_before;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const f32x4 by = *(lds_ptr<f32x4>)&sh->scale[buf][32 * th + 8 * i + 4 * half];
+                const f32x4 s4 = scales_of(buf, i);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const float y = bit_of(4 * i + k) ? __builtin_fmaf(sc[4 * i + k], by[k], -mu) : -INFINITY;
-                    most = fmaxf(most, y);
-                    const float e = __builtin_amdgcn_exp2f(y);
+                    const float x = bit_of(4 * i + k) ? __builtin_fmaf(sc[4 * i + k], s4[k], -mu) : -INFINITY;
+                    most = fmaxf(most, x);
+                    const float e = __builtin_amdgcn_exp2f(x);
                     l_sum += e;
-                    p[4 * i + k] = bit_of(4 * i + k) ? e * by[k] : 0.0f;
+                    p[k] = bit_of(4 * i + k) ? e * s4[k] : 0.0f;
                 }
+                put_weights(i, p);
             }
-            put_weights(p, parity);
-            return most;
         };
-        // New references for the rows of tile i (the workgroup's decision): its weights again, everything before rescaled.
-        auto regrow = [&](int buf, int parity) {
-            float most = -INFINITY;
-            float x[16];
+        // New references for the rows of a tile (the workgroup's decision), and a factor for what came before.
+        auto refer = [&](int buf) -> float {
+            float top = -INFINITY;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const f32x4 by = *(lds_ptr<f32x4>)&sh->scale[buf][32 * th + 8 * i + 4 * half];
+                const f32x4 s4 = scales_of(buf, i);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    x[4 * i + k] = bit_of(4 * i + k) ? sc[4 * i + k] * by[k] : -INFINITY;
-                    most = fmaxf(most, x[4 * i + k]);
-                }
+                for (int k = 0; k < 4; ++k) top = fmaxf(top, bit_of(4 * i + k) ? sc[4 * i + k] * s4[k] : -INFINITY);
             }
-            const auto other = __builtin_amdgcn_permlane32_swap(__float_as_uint(most), __float_as_uint(most), false, false);
-            most = fmaxf(__uint_as_float(other[0]), __uint_as_float(other[1]));
-            if (half == 0) sh->top[th][own] = most;
+            const auto other = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+            top = fmaxf(__uint_as_float(other[0]), __uint_as_float(other[1]));
+            if (half == 0) sh->top[th][own] = top;
             lds_barrier();
-            const float top = fmaxf(sh->top[0][own], sh->top[1][own]);
+            top = fmaxf(sh->top[0][own], sh->top[1][own]);
             const bool grow = top > m_ref;
             const float corr = grow ? __builtin_amdgcn_exp2f(m_ref - top) : 1.0f;  // 2^-inf = 0 at first
             if (grow) m_ref = top;
             limit = m_ref == -INFINITY ? -INFINITY : kTreeGrow;
+            mu = m_ref == -INFINITY ? 0.0f : m_ref;
+            return corr;
+        };
+        auto regrow = [&](int buf) {
+            const float corr = refer(buf);
             if (th == 0 && half == 0) sh->corr[own] = corr;
-            const float mu = m_ref == -INFINITY ? 0.0f : m_ref;
-            l_sum = l_before * corr;
-            float p[16];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const f32x4 by = *(lds_ptr<f32x4>)&sh->scale[buf][32 * th + 8 * i + 4 * half];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const float e = __builtin_amdgcn_exp2f(x[4 * i + k] - mu);
-                    l_sum += e;
-                    p[4 * i + k] = bit_of(4 * i + k) ? e * by[k] : 0.0f;
-                }
-            }
-            put_weights(p, parity);
+            l_before *= corr;
+            weigh_seen(buf);
             lds_barrier();
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
-                const float by = sh->corr[32 * b + n32];
+                const float f = sh->corr[32 * b + n32];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) o[c][b] *= by;
+                for (int c = 0; c < 4; ++c) o[c][b] *= f;
             }
         };
-        // O^T[column][row] += V^T . P^T of a tile, sixteen units of a K-step and a column tile each; and, with NEXT, the softmax of the tile
-        // after it, a token a unit, from the partial scores' meeting to the weights: tile `next`'s, as if every row saw every
-        // token. A unit's codes are out of LDS three units and converted one unit before its matrix instructions.
-        auto step = [&](auto more, int buf, int parity, int next) -> float {
+        // ---- the first half of an iteration: S^T[token][row] of the wave's tokens of a tile over its half of the dims, x[0] of the rows that are the
+        // wave's, x[1] of the others on their way to the other half's wave. A piece of codes is out of LDS two steps and
+        // converted one step before its matrix instructions; the fences keep that order. With MORE the tile before is weighed and the next
+        // but one asked for in between.
+        f32x16 x[2];
+        auto scores = [&](int buf, auto more, int before, int third) {
+            constexpr bool MORE = decltype(more)::value;
+            const lds_ptr<uint8_t> codes = tiles + buf * kTreeTileBytes;
+            u32x4 k[3];
+            auto load = [&](int i) {
+                k[i % 3] = *(lds_ptr<u32x4>)(codes + (i < 8 ? k_row + 1024 * (i >> 2) + 16 * ((2 * (i & 3) + half) ^ k_swap) : k_rope));
+            };
+            load(0), load(1);
+            if (MORE) {
+                weigh_begin(before);
+                find(0), find(1);
+                weigh(before, 0), weigh(before, 1);
+            }
+            x[0] = f32x16{}, x[1] = f32x16{};
+            bf16x8 lo = as_bf16(k[0].x, k[0].y), hi = as_bf16(k[0].z, k[0].w);
+            each<9>([&](auto step) {
+                constexpr int i = decltype(step)::value;
+                __builtin_amdgcn_sched_barrier(0);
+                if (i + 2 < 9) load(i + 2);
+                const u32x4 then = k[(i + 1) % 3];
+                x[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lo, __builtin_bit_cast(bf16x8, q[2 * i][0]), x[0], 0, 0, 0);
+                if (MORE && i < 7) weigh(before, 2 + 2 * i);
+                __builtin_amdgcn_sched_barrier(0);
+                x[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lo, __builtin_bit_cast(bf16x8, q[2 * i][1]), x[1], 0, 0, 0);
+                if (i < 8) lo = as_bf16(then.x, then.y);
+                if constexpr (MORE) bring(std::integral_constant<int, i>{}, third);
+                __builtin_amdgcn_sched_barrier(0);
+                x[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(hi, __builtin_bit_cast(bf16x8, q[2 * i + 1][0]), x[0], 0, 0, 0);
+                if (MORE && i < 7) weigh(before, 3 + 2 * i);
+                __builtin_amdgcn_sched_barrier(0);
+                x[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(hi, __builtin_bit_cast(bf16x8, q[2 * i + 1][1]), x[1], 0, 0, 0);
+                if (i < 8) hi = as_bf16(then.z, then.w);
+                if constexpr (MORE) {
+                    if (i == 7) bring(std::integral_constant<int, 9>{}, third);
+                    if (i == 8) go_on(0), go_on(1);
+                }
+            });
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sh->part[2 * th + 1 - kh][i][lane] = f32x4{x[1][4 * i], x[1][4 * i + 1], x[1][4 * i + 2], x[1][4 * i + 3]};
+        };
+        // ---- the second half: O^T[column][row] += V^T . P^T of a tile, sixteen units of a K-step and a column tile each. With NEXT the
+        // partial scores of the next tile meet and the transfers asked for arrive in between. A unit's codes are out of LDS three units and
+        // converted one unit before its matrix instructions. `check` comes once every weight is there.
+        auto values = [&](auto more, int buf, int third, auto check) {
             constexpr bool NEXT = decltype(more)::value;
             const lds_ptr<uint8_t> codes = tiles + buf * kTreeTileBytes + v_row;
-            const lds_ptr<uint8_t> w_from = weights + parity * (kTreeRows * kTreeTokens * 2) + n32 * (2 * kTreeTokens);
+            const lds_ptr<uint8_t> w_from = weights + n32 * (2 * kTreeTokens);
             i32x2 raw[4];
             bf16x8 w[2][2];
             auto load = [&](int u) {
@@ -440,52 +487,32 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
 #pragma unroll
                 for (int b = 0; b < 2; ++b) w[ks & 1][b] = *(lds_ptr<bf16x8>)(w_from + 32 * b * (2 * kTreeTokens) + 16 * ((2 * ks + half) ^ k_swap));
             };
-            load(0), load_w(0), load(1), load(2);
-            f32x4 part[4], by;
-            const float mu = m_ref == -INFINITY ? 0.0f : m_ref;
-            float most = -INFINITY, p[4];
+            load(0), load(1), load(2);
+            lds_barrier();  // partial scores and weights are there
+            check();
+            load_w(0);
+            f32x4 part[4];
             if (NEXT) {
-                l_before = l_sum;
-                lds_barrier();  // the partial scores are there
 #pragma unroll
                 for (int i = 0; i < 4; ++i) part[i] = sh->part[2 * th + kh][i][lane];
             }
-            float y = -INFINITY, y_before;
-            auto first = [&](int r) {
-                if ((r & 3) == 0) by = *(lds_ptr<f32x4>)&sh->scale[next][32 * th + 8 * (r >> 2) + 4 * half];
-                sc[r] += part[r >> 2][r & 3];
-                y_before = y;
-                y = __builtin_fmaf(sc[r], by[r & 3], -mu);
-                if (r & 1) most = fmaxf(most, fmaxf(y_before, y));
-                p[r & 3] = __builtin_amdgcn_exp2f(y);
-            };
-            auto second = [&](int r) {
-                l_sum += p[r & 3];
-                p[r & 3] *= by[r & 3];
-                if ((r & 3) == 3)
-                    *(lds_ptr<u32x2>)(w_row + (parity ^ 1) * (kTreeRows * kTreeTokens * 2) + 16 * ((4 * th + (r >> 2)) ^ w_swap)) =
-                        u32x2{pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3])};
-            };
             bf16x8 v = as_bf16((uint32_t)raw[0][0], (uint32_t)raw[0][1]);
-#pragma unroll
-            for (int u = 0; u < 16; ++u) {
-                const int ks = u >> 2, c = u & 3;
+            each<16>([&](auto unit) {
+                constexpr int u = decltype(unit)::value, ks = u >> 2, c = u & 3;
                 __builtin_amdgcn_sched_barrier(0);
                 if (u + 3 < 16) load(u + 3);
                 if (c == 1 && ks < 3) load_w(ks + 1);
                 o[c][0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, w[ks & 1][0], o[c][0], 0, 0, 0);
-                if (NEXT && u >= 2) first(u - 2);
+                if (NEXT && u == 12) arrived(third);
                 __builtin_amdgcn_sched_barrier(0);
                 o[c][1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, w[ks & 1][1], o[c][1], 0, 0, 0);
                 if (u < 15) v = as_bf16((uint32_t)raw[(u + 1) % 4][0], (uint32_t)raw[(u + 1) % 4][1]);
-                if (NEXT && u >= 2) second(u - 2);
-            }
+                if (NEXT && u >= 2 && u < 10) {
+                    constexpr int r = 2 * (u - 2) & 15;
+                    sc[r] = x[0][r] + part[r >> 2][r & 3], sc[r + 1] = x[0][r + 1] + part[r >> 2][(r & 3) + 1];
+                }
+            });
             __builtin_amdgcn_sched_barrier(0);
-            if (NEXT) {
-#pragma unroll
-                for (int r = 14; r < 16; ++r) first(r), second(r);
-            }
-            return most;
         };
         // The wave's sixteen rows of a tile whose keys have all been read: codes that are no number become zeros, where some row does not
         // see a token (its weight is zero, the product would not be). A row that does see it has no number for its weight.
@@ -499,54 +526,54 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
             }
         };
         auto drafted = [&](int i) -> bool { return (tile_lo + i + 1) * kTreeTokens > s.ctx; };
-        auto meet = [&]() {  // the other half's partial scores of the rows that are the wave's
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const f32x4 x = sh->part[2 * th + kh][i][lane];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) sc[4 * i + k] += x[k];
-            }
-        };
 
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
             for (int b = 0; b < 2; ++b) o[c][b] = f32x16{};
         // ---- the first tile, which sets the references -----------------------------------------------------------
-        arrived(0, number);
+        arrived(0), fill_holes(0, number);
         ask(1);
         lds_barrier();
-        scores(0, std::false_type{}, 0, [] {});
+        scores(0, std::false_type{}, 0, 0);
         seen = seen_of(0, 0);
+        bool masked = __builtin_amdgcn_ballot_w64(seen != ~0u) != 0;  // some row may not see some token of tile i
         lds_barrier();
-        meet();
-        regrow(0, 0);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sc[r] = x[0][r] + sh->part[2 * th + kh][r >> 2][lane][r & 3];
+        refer(0);
         if (drafted(0)) clean(0);
-        arrived(1, number + 1);
+        arrived(1), fill_holes(1, number + 1);
         lds_barrier();
         int buf = 0;  // of tile i
         for (int i = 0; i + 1 < n_tiles; ++i) {
-            const int next = buf == 2 ? 0 : buf + 1, third = next == 2 ? 0 : next + 1, parity = i & 1;
-            const i32x2 flags = *(lds_ptr<i32x2>)&sh->grown;
-            bool masked = false;  // some row may not see some token of tile i + 1
-            scores(next, std::true_type{}, third, [&] {
-                if (__builtin_amdgcn_readfirstlane(flags[0]) == number + i) regrow(buf, parity);
-                masked = drafted(i + 1) || __builtin_amdgcn_readfirstlane(flags[1]) == number + i + 1;
-                seen = ~0u;
-                if (masked) seen = seen_of(i + 1, next);
+            const int next = buf == 2 ? 0 : buf + 1, third = next == 2 ? 0 : next + 1;
+            scores(next, std::true_type{}, buf, third);
+            if (__builtin_expect(masked, 0)) weigh_seen(buf);
+            if (__builtin_amdgcn_ballot_w64(most > limit) != 0) sh->grown = number + i;
+            bool holed = false;
+            values(std::true_type{}, buf, third, [&] {
+                const int grown = sh->grown, hole = sh->holed[(number + i + 1) & 1];
+                if (__builtin_expect(__builtin_amdgcn_readfirstlane(grown) == number + i, 0)) regrow(buf);
+                holed = __builtin_amdgcn_readfirstlane(hole) == number + i + 1;
             });
-            float most = step(std::true_type{}, buf, parity, next);
-            if (masked) {
-                most = weigh_seen(next, parity ^ 1);
+            fill_holes(third, number + i + 2);
+            masked = drafted(i + 1) || holed;
+            seen = ~0u;
+            if (__builtin_expect(masked, 0)) {
+                seen = seen_of(i + 1, next);
                 if (drafted(i + 1)) clean(next);
             }
-            if (__builtin_amdgcn_ballot_w64(most > limit) != 0) sh->grown = number + i + 1;
-            arrived(third, number + i + 2);
             lds_barrier();
             buf = next;
         }
-        if (n_tiles > 1 && __builtin_amdgcn_readfirstlane(sh->grown) == number + n_tiles - 1) regrow(buf, (n_tiles - 1) & 1);
-        step(std::false_type{}, buf, (n_tiles - 1) & 1, 0);
+        weigh_begin(buf);
+        seen = seen_of(n_tiles - 1, buf);
+        weigh_seen(buf);
+        if (__builtin_amdgcn_ballot_w64(most > limit) != 0) sh->grown = number + n_tiles - 1;
+        values(std::false_type{}, buf, 0, [&] {
+            if (__builtin_amdgcn_readfirstlane(sh->grown) == number + n_tiles - 1) regrow(buf);
+        });
         if (a.bad_rows && last_block && l8 == 0 && missing) atomicAdd(a.bad_rows, missing);
         number += n_tiles + 2;  // (two tiles past the end were asked for)
     }
@@ -603,10 +630,12 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
     __syncthreads();
 }
 
+// RUNS: pages are whole runs of 16 rows.
+template <bool RUNS>
 __global__ __launch_bounds__(kTreeThreads, 1) void mla_attend_tree_kernel(const TreeArgs a) {
     __shared__ __attribute__((aligned(1024))) TreeShared shared;
     const lds_ptr<TreeShared> sh = (lds_ptr<TreeShared>)&shared;
-    if (threadIdx.x == 0) sh->grown = sh->holed = -1;
+    if (threadIdx.x == 0) sh->grown = sh->holed[0] = sh->holed[1] = -1;
     const bool all = a.groups == 0;  // a block of rows is a work item
     int item = blockIdx.x, number = 0;
     long long u = item, end = u + 1;
@@ -623,7 +652,7 @@ __global__ __launch_bounds__(kTreeThreads, 1) void mla_attend_tree_kernel(const 
         if (b.seq < 0) return;
         const int lo = all ? 0 : (int)(u - b.first), hi = all ? b.tiles : (int)min((long long)b.tiles, lo + end - u);
         float* const rec = a.partial + (size_t)(2 * item + (lo == 0 ? 1 : 0)) * kTreeRecordFloats;
-        tree_part(a, sh, tree_seq(a, b.seq), b.seq, b.rb, b.rb == b.blocks - 1, lo, hi, lo == 0 && hi == b.tiles, rec, number);
+        tree_part<RUNS>(a, sh, tree_seq(a, b.seq), b.seq, b.rb, b.rb == b.blocks - 1, lo, hi, lo == 0 && hi == b.tiles, rec, number);
         u += all ? 1 : hi - lo;
     }
 }

@@ -10,7 +10,7 @@ from tests.exec_joins import early_vector_work
 
 
 def test_the_build_refuses_a_kernel_that_spills():
-    block = ("remark: Function Name: _ZN2rk22mla_attend_tree_kernelENS_8TreeArgsE\n ScratchSize [bytes/lane]: %d\n LDS Size [bytes/block]: %d\n")
+    block = ("remark: Function Name: _ZN2rk22mla_attend_tree_kernelILb1EEEvNS_8TreeArgsE\n ScratchSize [bytes/lane]: %d\n LDS Size [bytes/block]: %d\n")
     build.check_resources("mla_attend_tree.hip", block % (0, 146448))
     for scratch, lds in ((4, 146448), (0, 163841)):
         with pytest.raises(RuntimeError):
