@@ -38,31 +38,74 @@ constexpr int kTreeSteps = 18;            // of 16 dims a wave: 16 of its 256 la
 constexpr float kTreeGrow = 24.0f;
 constexpr uint32_t kTreeHole = 0x80000000u;  // the scale of a token that is not there: -0
 
-// A block of rows among a call's: its sequence, number and tiles, and the work units (tiles, or blocks where they are whole) before it.
-struct TreeBlock {
-    int seq, rb, blocks, tiles;
-    long long first;  // unit of the block's first tile
+// A call's blocks of rows are numbered by sequence, and so are its work units: their tiles, block after block, or the blocks themselves where a
+// workgroup has a whole one. A lane has the lengths of the sequences lane, lane + 64, ...; counts fit 32 bits (tree_plan).
+struct TreeLane {
+    TreeSeq s;
+    unsigned blocks, tiles;
 };
-__device__ __forceinline__ void tree_units(const TreeArgs& a, int seq, int& blocks, int& tiles) {
-    blocks = tiles = 0;
-    if (seq >= a.n_seqs) return;
-    const TreeSeq s = tree_seq(a, seq);
-    blocks = (s.nodes * a.H + kTreeRows - 1) / kTreeRows;
-    tiles = (s.ctx + s.nodes + kTreeTokens - 1) / kTreeTokens;
-}
-__device__ __forceinline__ long long lanes_up_to(long long x) {
-#pragma unroll
-    for (int off = 1; off < kWave; off <<= 1) {
-        const long long y = __shfl_up(x, off, kWave);
-        if ((int)(threadIdx.x & 63) >= off) x += y;
+__device__ __forceinline__ TreeLane tree_lane(const TreeArgs& a, int seq) {
+    TreeLane l{tree_seq(a, min(seq, a.n_seqs - 1)), 0u, 0u};
+    if (seq < a.n_seqs) {
+        l.blocks = ((unsigned)l.s.nodes * (unsigned)a.H + kTreeRows - 1) / kTreeRows;
+        l.tiles = ((unsigned)l.s.ctx + (unsigned)l.s.nodes + kTreeTokens - 1) / kTreeTokens;
     }
-    return x;
+    return l;
 }
-// A value that is the same in every lane, as the compiler does not know: in scalar registers. What a workgroup's branches and loops go by is
-// kept there, so that none of them is a branch around masked lanes.
-__device__ __forceinline__ long long uniform(long long x) {
-    return ((long long)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)x);
-}
+struct TreeWalk {
+    const TreeArgs& a;
+    const TreeLane first;  // of the first 64 sequences
+    __device__ __forceinline__ explicit TreeWalk(const TreeArgs& args) : a(args), first(tree_lane(args, threadIdx.x & 63)) {}
+    __device__ __forceinline__ TreeLane lane_of(int s0) const { return s0 == 0 ? first : tree_lane(a, s0 + (int)(threadIdx.x & 63)); }
+    static __device__ __forceinline__ unsigned units(const TreeLane& l, bool whole) { return whole ? l.blocks : l.blocks * l.tiles; }
+    __device__ __forceinline__ unsigned total(bool whole) const {
+        unsigned sum = 0;
+        for (int s0 = 0; s0 < a.n_seqs; s0 += kWave) sum += units(lane_of(s0), whole);
+        return wave_total(wave_inclusive_sum(sum));
+    }
+    // The block that unit u is of: its sequence, number and tiles in it, and the tiles before it in all.
+    struct Block {
+        TreeSeq s;
+        int seq, rb;
+        unsigned blocks, tiles, before;
+    };
+    __device__ __forceinline__ bool block(bool whole, unsigned u, Block& b) const {
+        unsigned run = 0, tiles_run = 0;
+        for (int s0 = 0; s0 < a.n_seqs; s0 += kWave) {
+            const TreeLane l = lane_of(s0);
+            const unsigned mine = units(l, whole), upto = wave_inclusive_sum(mine), all = wave_total(upto);
+            if (u < run + all) {
+                const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(u < run + upto));
+                auto of = [&](unsigned v) -> unsigned { return (unsigned)__builtin_amdgcn_readlane((int)v, at); };
+                b.s.ctx = (int)of((unsigned)l.s.ctx), b.s.node0 = (int)of((unsigned)l.s.node0), b.s.nodes = (int)of((unsigned)l.s.nodes);
+                b.seq = s0 + at, b.blocks = of(l.blocks), b.tiles = of(l.tiles);
+                const unsigned rel = u - run - of(upto - mine);
+                b.rb = (int)(whole ? rel : rel / b.tiles);
+                const unsigned tiles_of = l.blocks * l.tiles;
+                b.before = tiles_run + of(wave_inclusive_sum(tiles_of) - tiles_of) + (unsigned)b.rb * b.tiles;
+                return true;
+            }
+            run += all;
+            tiles_run += wave_total(wave_inclusive_sum(l.blocks * l.tiles));
+        }
+        return false;
+    }
+};
+// The work items of a cut call, none with less than kTreeMinTiles, the first `more` of them with a tile more than the others.
+struct TreeItems {
+    unsigned items, each, more;
+    __device__ __forceinline__ TreeItems(const TreeArgs& a, unsigned total) {
+        items = min(max(total / kTreeMinTiles, 1u), (unsigned)a.groups);
+        if (items > kTreeDies) items = items / kTreeDies * kTreeDies;  // eighths of them stay on one die
+        each = total / items, more = total - each * items;
+    }
+    __device__ __forceinline__ unsigned lo(unsigned item) const { return item * each + min(item, more); }
+    __device__ __forceinline__ unsigned of(unsigned unit) const {
+        const unsigned large = more * (each + 1);
+        return unit < large ? unit / (each + 1) : more + (unit - large) / each;
+    }
+};
+
 // f(0) .. f(N - 1), the numbers being constants of the compiler's.
 template <int N, class F, int... I>
 __device__ __forceinline__ void each_of(F&& f, std::integer_sequence<int, I...>) {
@@ -72,52 +115,6 @@ template <int N, class F>
 __device__ __forceinline__ void each(F&& f) {
     each_of<N>(static_cast<F&&>(f), std::make_integer_sequence<int, N>{});
 }
-__device__ __forceinline__ long long tree_total(const TreeArgs& a, bool whole) {
-    const int lane = threadIdx.x & 63;
-    long long sum = 0;
-    for (int s0 = 0; s0 < a.n_seqs; s0 += kWave) {
-        int blocks, tiles;
-        tree_units(a, s0 + lane, blocks, tiles);
-        sum += whole ? (long long)blocks : (long long)blocks * tiles;
-    }
-    return uniform(__shfl(lanes_up_to(sum), kWave - 1, kWave));
-}
-// The block that holds unit u of them.
-__device__ __forceinline__ TreeBlock tree_block(const TreeArgs& a, bool whole, long long u) {
-    const int lane = threadIdx.x & 63;
-    long long run = 0;
-    TreeBlock b{0, 0, 0, 0, 0};
-    for (int s0 = 0; s0 < a.n_seqs; s0 += kWave) {
-        int blocks, tiles;
-        tree_units(a, s0 + lane, blocks, tiles);
-        const long long mine = whole ? (long long)blocks : (long long)blocks * tiles;
-        const long long upto = run + lanes_up_to(mine);
-        const unsigned long long past = __builtin_amdgcn_ballot_w64(u < upto);
-        if (past) {
-            const int at = __builtin_ctzll(past);
-            const long long before = uniform(__shfl(upto - mine, at, kWave));
-            b.seq = s0 + at;
-            b.blocks = __builtin_amdgcn_readlane(blocks, at), b.tiles = __builtin_amdgcn_readlane(tiles, at);
-            const long long rel = u - before;
-            b.rb = (int)(whole ? rel : rel / b.tiles);
-            b.first = before + (whole ? (long long)b.rb : (long long)b.rb * b.tiles);
-            return b;
-        }
-        run = uniform(__shfl(upto, kWave - 1, kWave));
-    }
-    b.seq = -1;
-    return b;
-}
-// The work items of a cut call: no more than have kTreeMinTiles each; eighths of them stay on one die.
-__device__ __forceinline__ int tree_items(const TreeArgs& a, long long total) {
-    const long long n = total / kTreeMinTiles;
-    int items = (int)(n < a.groups ? n : (long long)a.groups);
-    if (items > kTreeDies) items = items / kTreeDies * kTreeDies;
-    return max(items, 1);
-}
-__device__ __forceinline__ long long tree_item_lo(int item, int items, long long total) { return (long long)item * total / items; }
-__device__ __forceinline__ int tree_item_of(long long unit, int items, long long total) { return (int)(((unit + 1) * items - 1) / total); }
-
 // (Weights carry their token's scale times the softmax's: one number a token for both products; results are divided by the softmax's.)
 struct TreeShared {
     uint8_t tiles[kTreeBuffers * kTreeTileBytes];
@@ -637,70 +634,77 @@ __global__ __launch_bounds__(kTreeThreads, 1) void mla_attend_tree_kernel(const 
     const lds_ptr<TreeShared> sh = (lds_ptr<TreeShared>)&shared;
     if (threadIdx.x == 0) sh->grown = sh->holed[0] = sh->holed[1] = -1;
     const bool all = a.groups == 0;  // a block of rows is a work item
-    int item = blockIdx.x, number = 0;
-    long long u = item, end = u + 1;
-    if (!all) {
-        const long long total = tree_total(a, false);
-        const int items = tree_items(a, total);
-        if (item >= items || total == 0) return;
-        // an eighth of the items on each die: neighbours, which often read the same tokens
-        if (items % kTreeDies == 0) item = (item % kTreeDies) * (items / kTreeDies) + item / kTreeDies;
-        u = tree_item_lo(item, items, total), end = tree_item_lo(item + 1, items, total);
+    unsigned item = blockIdx.x, u = item, end = u + 1;
+    TreeWalk::Block b;
+    {
+        const TreeWalk walk(a);
+        if (!all) {
+            const unsigned total = walk.total(false);
+            if (total == 0) return;
+            const TreeItems items(a, total);
+            if (item >= items.items) return;
+            // an eighth of the items on each die: neighbours, which often read the same tokens
+            if (items.items % kTreeDies == 0) item = (item % kTreeDies) * (items.items / kTreeDies) + item / kTreeDies;
+            u = items.lo(item), end = items.lo(item + 1);
+        }
+        if (!walk.block(all, u, b)) return;
     }
-    while (u < end) {
-        const TreeBlock b = tree_block(a, all, u);
-        if (b.seq < 0) return;
-        const int lo = all ? 0 : (int)(u - b.first), hi = all ? b.tiles : (int)min((long long)b.tiles, lo + end - u);
+    for (int number = 0;;) {
+        const int lo = all ? 0 : (int)(u - b.before), hi = all ? (int)b.tiles : (int)min(b.tiles, lo + end - u);
         float* const rec = a.partial + (size_t)(2 * item + (lo == 0 ? 1 : 0)) * kTreeRecordFloats;
-        tree_part<RUNS>(a, sh, tree_seq(a, b.seq), b.seq, b.rb, b.rb == b.blocks - 1, lo, hi, lo == 0 && hi == b.tiles, rec, number);
+        tree_part<RUNS>(a, sh, b.s, b.seq, b.rb, b.rb == (int)b.blocks - 1, lo, hi, lo == 0 && hi == (int)b.tiles, rec, number);
         u += all ? 1 : hi - lo;
+        if (u >= end) return;
+        const TreeWalk walk(a);  // (looked up again: what it has would keep registers through the tiles)
+        if (!walk.block(false, u, b)) return;
     }
 }
 
-// Blocks that several work items had: their records, in order, under the largest reference.
+// Blocks that several work items had: their records, in order, under the largest reference. Bound by memory's round trips where
+// there are few: records go eight at a time, every load of a batch in front of the first use.
 __global__ __launch_bounds__(256) void mla_attend_tree_merge_kernel(const TreeArgs a) {
-    const long long total = tree_total(a, false);
-    if (total == 0) return;
-    const int items = tree_items(a, total);
-    // block number blockIdx.x: found among blocks, then its place among the tiles
-    const TreeBlock by_block = tree_block(a, true, blockIdx.x);
-    if (by_block.seq < 0) return;
-    long long before = 0;
-    {
-        const int lane = threadIdx.x & 63;
-        for (int s0 = 0; s0 < by_block.seq; s0 += kWave) {
-            int blocks = 0, tiles = 0;
-            if (s0 + lane < by_block.seq) tree_units(a, s0 + lane, blocks, tiles);
-            before += (long long)blocks * tiles;
-        }
-        before = uniform(__shfl(lanes_up_to(before), kWave - 1, kWave));
-    }
-    const long long first = before + (long long)by_block.rb * by_block.tiles;
-    const int g0 = tree_item_of(first, items, total), g1 = tree_item_of(first + by_block.tiles - 1, items, total);
+    const TreeWalk walk(a);
+    TreeWalk::Block block;
+    if (!walk.block(true, blockIdx.x, block)) return;
+    const TreeItems items(a, walk.total(false));
+    const unsigned g0 = items.of(block.before), g1 = items.of(block.before + block.tiles - 1);
     if (g0 == g1) return;
     const int at = blockIdx.y * 256 + threadIdx.x, lane = at & 63, idx = at >> 6;
     const int i = idx & 3, b = (idx >> 2) & 1, c = (idx >> 3) & 3, wave = idx >> 5;
-    const int row = 32 * b + (lane & 31);
+    const int row = 32 * b + (lane & 31), r = kTreeRows * block.rb + row;
+    if (r >= block.s.nodes * a.H) return;
     float m = -INFINITY, l = 0.0f;
     f32x4 sum = {0, 0, 0, 0};
-    for (int g = g0; g <= g1; ++g) {
-        const float* const rec = a.partial + (size_t)(2 * g + (g == g0 ? 1 : 0)) * kTreeRecordFloats;
-        const float m_r = rec[kTreeRows * 512 + 2 * row], l_r = rec[kTreeRows * 512 + 2 * row + 1];
-        if (l_r == 0.0f) continue;  // nothing that the row sees
-        const f32x4 v = reinterpret_cast<const f32x4*>(rec)[at];
-        const float top = fmaxf(m, m_r);
-        const float keep = __builtin_amdgcn_exp2f(m - top), by = __builtin_amdgcn_exp2f(m_r - top);
-        m = top, l = l * keep + l_r * by;
-        sum = sum * keep + v * by;
+    constexpr int kBatch = 8;
+    for (unsigned g = g0; g <= g1; g += kBatch) {
+        f32x2 ml[kBatch];
+        f32x4 v[kBatch];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {  // (a record past the last re-reads the last, and is left out)
+            const unsigned rec_of = min(g + k, g1);
+            const float* const rec = a.partial + (size_t)(2 * rec_of + (rec_of == g0 ? 1 : 0)) * kTreeRecordFloats;
+            ml[k] = *reinterpret_cast<const f32x2*>(rec + kTreeRows * 512 + 2 * row);
+            v[k] = reinterpret_cast<const f32x4*>(rec)[at];
+        }
+        float top = m;
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) top = fmaxf(top, ml[k].x);
+        if (top == -INFINITY) continue;         // nothing yet that the row sees
+        const float keep = __builtin_amdgcn_exp2f(m - top);
+        m = top, l *= keep, sum *= keep;
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            if (g + k > g1 || ml[k].y == 0.0f) continue;
+            const float by = __builtin_amdgcn_exp2f(ml[k].x - top);
+            l += ml[k].y * by;
+            sum += v[k] * by;
+        }
     }
-    const TreeSeq s = tree_seq(a, by_block.seq);
-    const int r = kTreeRows * by_block.rb + row;
-    if (r >= s.nodes * a.H) return;
     const float inv = l == 0.0f ? 0.0f : 1.0f / (l * a.qscale);
-    const size_t out = (size_t)s.node0 * a.H + r;
+    const size_t out = (size_t)block.s.node0 * a.H + r;
     *reinterpret_cast<u32x2*>(a.clat + out * 512 + 128 * wave + 16 * c + 64 * (i >> 1) + 8 * (i & 1) + 4 * (lane >> 5)) =
         u32x2{pack_bf16x2(sum[0] * inv, sum[1] * inv), pack_bf16x2(sum[2] * inv, sum[3] * inv)};
-    if (a.lse && idx == 0 + 4 * b && lane < 32) a.lse[out] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+    if (a.lse && idx == 4 * b && lane < 32) a.lse[out] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
 }
 
 }  // namespace rk

@@ -26,7 +26,7 @@ static inline TreePlan tree_plan(int n_seqs, int H, int n_nodes, int max_nodes, 
     const long long by_node = (long long)n_nodes * H / kTreeRows + (n_seqs < n_nodes ? n_seqs : n_nodes);
     p.blocks = by_seq < by_node ? by_seq : by_node;
     const long long tiles = ((long long)max_ctx + max_nodes + kTreeTokens - 1) / kTreeTokens;
-    if (tiles <= kTreeWholeTiles) return p;
+    if (tiles <= kTreeWholeTiles || p.blocks * tiles >= 1ll << 31) return p;  // (cut calls count their tiles in 32 bits)
     const long long groups = (p.blocks * tiles + kTreeMinTiles - 1) / kTreeMinTiles;
     p.groups = (int)(groups < kTreeGroups ? groups : kTreeGroups);
     return p;
