@@ -42,8 +42,35 @@ __device__ __forceinline__ void e4m3x4_to_bf16(uint32_t c, uint32_t& lo, uint32_
     hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, 1.0f, true));
 }
 
-// Four bytes per lane from memory into LDS, lane L's at dst + 4 L (dst is wave-uniform). Issued as text,
-// as dma16 (mla_attend_f8.hpp): the caller waits (vmcnt) before the data is used.
+// Sixteen bytes per lane from memory straight into LDS: lane L's land at dst + 16 L (dst is
+// wave-uniform). Issued as text: through the builtin the compiler makes every later LDS read wait
+// for the transfer, whichever buffer it reads. The caller waits (vmcnt) before the data is used.
+__device__ __forceinline__ void dma16(const uint8_t* src, lds_ptr<uint8_t> dst) {
+    const uint32_t base = (uint32_t)(uintptr_t)dst;
+    uint32_t keep;  // m0 is the instruction's LDS base; the compiler's own value of it is put back
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep)
+                 : "v"(src), "s"(base)
+                 : "memory");
+}
+
+// The same from a wave-uniform address plus a 32-bit offset per lane (the instruction's scalar
+// base form: no 64-bit add, and offsets kept across a loop cost one register each). The base is
+// made scalar here: an operand that reaches the statement through a loop-carried value may
+// otherwise sit in vector registers, which the assembler accepts and the instruction misreads.
+__device__ __forceinline__ void dma16_from(const uint8_t* base_uniform, uint32_t off, lds_ptr<uint8_t> dst) {
+    const uint32_t lds_base = (uint32_t)(uintptr_t)dst;
+    const uint64_t b = (uint64_t)(uintptr_t)base_uniform;
+    const uint64_t sb = ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(b >> 32)) << 32) |
+                        (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)b);
+    uint32_t keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep)
+                 : "v"(off), "s"(sb), "s"(lds_base)
+                 : "memory");
+}
+
+// Four bytes per lane from memory into LDS, as dma16.
 __device__ __forceinline__ void few_dma4(const void* src, lds_ptr<uint8_t> dst) {
     const uint32_t base = (uint32_t)(uintptr_t)dst;
     uint32_t keep;

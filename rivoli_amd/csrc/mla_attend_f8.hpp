@@ -108,34 +108,6 @@ __device__ __forceinline__ uint32_t e4m3x4_term(float (&x)[4], float (&val)[4]) 
     return u;
 }
 
-// Sixteen bytes per lane from memory straight into LDS: lane L's land at dst + 16 L (dst is
-// wave-uniform). Issued as text: through the builtin the compiler makes every later LDS read wait
-// for the transfer, whichever buffer it reads. The caller waits (vmcnt) before the data is used.
-__device__ __forceinline__ void dma16(const uint8_t* src, lds_ptr<uint8_t> dst) {
-    const uint32_t base = (uint32_t)(uintptr_t)dst;
-    uint32_t keep;  // m0 is the instruction's LDS base; the compiler's own value of it is put back
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
-                 : "=&s"(keep)
-                 : "v"(src), "s"(base)
-                 : "memory");
-}
-
-// The same from a wave-uniform address plus a 32-bit offset per lane (the instruction's scalar
-// base form: no 64-bit add, and offsets kept across a loop cost one register each). The base is
-// made scalar here: an operand that reaches the statement through a loop-carried value may
-// otherwise sit in vector registers, which the assembler accepts and the instruction misreads.
-__device__ __forceinline__ void dma16_from(const uint8_t* base_uniform, uint32_t off, lds_ptr<uint8_t> dst) {
-    const uint32_t lds_base = (uint32_t)(uintptr_t)dst;
-    const uint64_t b = (uint64_t)(uintptr_t)base_uniform;
-    const uint64_t sb = ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(b >> 32)) << 32) |
-                        (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)b);
-    uint32_t keep;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
-                 : "=&s"(keep)
-                 : "v"(off), "s"(sb), "s"(lds_base)
-                 : "memory");
-}
-
 template <int TQ, int TP, bool SPARSE, int TILE>
 __device__ __forceinline__ void attend_part_f8(const AttendArgs& a, int seq, int hb, int r_begin, int r_end,
                                                bool whole, float* pa, float* pml) {

@@ -123,8 +123,8 @@ struct TreeShared {
     float scale[kTreeBuffers][kTreeTokens];  // of a tile's tokens, times the softmax's; kTreeHole: not there
     float spare[kWave];
     float top[2][kTreeRows], corr[kTreeRows], sum[2][kTreeRows], ref[kTreeRows];
-    // numbers of the latest tile of which some row outgrew its reference, and of which some token is not there
-    int grown, holed[2];                 // (the second by the tile's parity)
+    // numbers of the latest tile of which some row outgrew its reference, some score is no number, some token is not there
+    int grown, dirty, holed[2];          // (the last by the tile's parity)
 };
 static_assert(sizeof(TreeShared) <= 160 * 1024, "one workgroup per compute unit");
 
@@ -284,23 +284,38 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
     const int own_node = (live ? own_row : 0) / a.H;
 
     if (n_tiles > 0) {
-        look_up(0);
-        if (!RUNS) look_up(1);
-        u32x4 q[kTreeSteps][2];  // of the rows that are the wave's in the softmax, and of the others
-        ask(0);
         // ---- the rows' operands: K-steps of 16 dims, eight a lane. Two K-steps share a 16-byte piece of codes. They live in the
-        // accumulation half of the register file, which the matrix instructions read as well; the sums are in the other --------
+        // accumulation half of the register file, which the matrix instructions read as well; the sums are in the other. They come through the
+        // second and third tile's LDS, a row a transfer (a lane's own loads of 32 rows each took 9 600 cycles, this 3 700): a row's 16-byte pieces change
+        // places by its number. The first page is asked for in front of them, where it can be by the scalar cache's way, which they are not waited for with.
+        const lds_ptr<uint8_t> q_at = tiles + kTreeTileBytes;
+        static_assert(kTreeRows * (1024 + 128) == 2 * kTreeTileBytes, "the rows fill two tiles");
+        if constexpr (RUNS) page[0] = ((const __attribute__((address_space(4))) int*)(uintptr_t)table)[min(block[0], (unsigned)a.max_blocks - 1)];
+        else look_up(0), look_up(1), ask(0);
+#pragma unroll 1
+        for (int i = 0; i < 16; ++i) {
+            const int r = kTreeRows * rb + 16 * wave + i;
+            dma16_from(reinterpret_cast<const uint8_t*>(a.qabs + ((size_t)s.node0 * a.H + (r < rows ? r : 0)) * 512), 16u * (uint32_t)(lane ^ i),
+                       q_at + 1024 * (16 * wave + i));
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int r = kTreeRows * rb + 16 * wave + 8 * i + r8;
+            dma16(reinterpret_cast<const uint8_t*>(a.qrope + ((size_t)s.node0 * a.H + (r < rows ? r : 0)) * 64) + 16 * (l8 ^ r8),
+                  (lds_ptr<uint8_t>)(uintptr_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)(q_at + 1024 * kTreeRows + 128 * (16 * wave + 8 * i))));
+        }
+        if constexpr (RUNS) ask(0);
+        arrived(0);
+        lds_barrier();
+        u32x4 q[kTreeSteps][2];  // of the rows that are the wave's in the softmax, and of the others
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-            const int r = kTreeRows * rb + 32 * (b ^ kh) + n32;
-            const size_t at = (size_t)s.node0 * a.H + (r < rows ? r : 0);
+            const int r = 32 * (b ^ kh) + n32;
             u32x4 raw[kTreeSteps];
 #pragma unroll
-            for (int j = 0; j < kTreeSteps; ++j) {
-                const uint16_t* const from = j < 16 ? a.qabs + at * 512 + 256 * kh + 32 * (j >> 1) + 16 * half + 8 * (j & 1)
-                                                    : a.qrope + at * 64 + 32 * kh + 16 * half + 8 * (j & 1);
-                raw[j] = *reinterpret_cast<const u32x4*>(from);
-            }
+            for (int j = 0; j < kTreeSteps; ++j)
+                raw[j] = j < 16 ? *(lds_ptr<u32x4>)(q_at + 1024 * r + 16 * ((32 * kh + 4 * (j >> 1) + 2 * half + (j & 1)) ^ (r & 15)))
+                                : *(lds_ptr<u32x4>)(q_at + 1024 * kTreeRows + 128 * r + 16 * ((4 * kh + 2 * half + (j & 1)) ^ (r & 7)));
 #pragma unroll
             for (int j = 0; j < kTreeSteps; ++j)
 #pragma unroll
@@ -310,6 +325,8 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
                     q[j][b][k] = kept;
                 }
         }
+        fill_holes(0, number);
+        lds_barrier();  // (the next tile comes where they were)
 
         // ---- the lane's operands of a tile --------------------------------------------------------------------
         const int k_swap = (n32 >> 1) & 7, e8 = (lane & 15) >> 1;
@@ -344,8 +361,8 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
             return bits & is_there;
         };
         f32x16 sc;               // a tile's scores: of token 8 (r >> 2) + 4 half + (r & 3) in register r
-        uint32_t seen = ~0u;
-        auto bit_of = [&](int r) -> bool { return seen >> (8 * (r >> 2) + 4 * half + (r & 3)) & 1; };
+        uint32_t seen = ~0u, seen_half = ~0u;  // (the second from the lane's first token on)
+        auto bit_of = [&](int r) -> bool { return (int)(seen_half << (31 - 8 * (r >> 2) - (r & 3))) < 0; };
         const lds_ptr<uint8_t> w_row = weights + own * (2 * kTreeTokens) + 8 * half;
         const int w_swap = (own >> 1) & 7;
         auto scales_of = [&](int buf, int i) -> f32x4 { return *(lds_ptr<f32x4>)&sh->scale[buf][32 * th + 8 * i + 4 * half]; };
@@ -371,14 +388,17 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
                 if (r < 15) by = scales_of(buf, (r >> 2) + 1);
             }
         };
-        // The same of a tile with tokens that some row does not see, in place of what weigh() made of it.
-        auto weigh_seen = [&](int buf) {
+        // The same of a tile with tokens that some row does not see, in place of what weigh() made of it. Whether a score is no number: then some code of
+        // the tile may be none, and its product with a weight of zero would be none either (clean).
+        auto weigh_seen = [&](int buf) -> bool {
             most = -INFINITY, l_sum = l_before;
+            bool nan = false;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const f32x4 s4 = scales_of(buf, i);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
+                    nan |= sc[4 * i + k] != sc[4 * i + k];
                     const float x = bit_of(4 * i + k) ? __builtin_fmaf(sc[4 * i + k], s4[k], -mu) : -INFINITY;
                     most = fmaxf(most, x);
                     const float e = __builtin_amdgcn_exp2f(x);
@@ -387,6 +407,7 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
                 }
                 put_weights(i, p);
             }
+            return __builtin_amdgcn_ballot_w64(nan) != 0;
         };
         // New references for the rows of a tile (the workgroup's decision), and a factor for what came before.
         auto refer = [&](int buf) -> float {
@@ -470,7 +491,8 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
         };
         // ---- the second half: O^T[column][row] += V^T . P^T of a tile, sixteen units of a K-step and a column tile each. With NEXT the
         // partial scores of the next tile meet and the transfers asked for arrive in between. A unit's codes are out of LDS three units and
-        // converted one unit before its matrix instructions. `check` comes once every weight is there.
+        // converted one unit before its matrix instructions. `check` comes once every weight is there, and says whether it changed the
+        // tile's codes.
         auto values = [&](auto more, int buf, int third, auto check) {
             constexpr bool NEXT = decltype(more)::value;
             const lds_ptr<uint8_t> codes = tiles + buf * kTreeTileBytes + v_row;
@@ -486,7 +508,7 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
             };
             load(0), load(1), load(2);
             lds_barrier();  // partial scores and weights are there
-            check();
+            if (__builtin_expect(check(), 0)) load(0), load(1), load(2);
             load_w(0);
             f32x4 part[4];
             if (NEXT) {
@@ -511,16 +533,17 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
             });
             __builtin_amdgcn_sched_barrier(0);
         };
-        // The wave's sixteen rows of a tile whose keys have all been read: codes that are no number become zeros, where some row does not
-        // see a token (its weight is zero, the product would not be). A row that does see it has no number for its weight.
+        // A tile whose keys have all been read, the wave's sixteen rows of it: codes that are no number become zeros. A row that does see such a
+        // token has no number for its weight.
         auto clean = [&](int buf) {
             const lds_ptr<uint8_t> to = tiles + buf * kTreeTileBytes + 2 * wave * 4096 + 16 * lane;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const u32x4 c = *(lds_ptr<u32x4>)(to + 1024 * i);
                 const u32x4 d = {numbers_only(c.x), numbers_only(c.y), numbers_only(c.z), numbers_only(c.w)};
-                if (((c.x ^ d.x) | (c.y ^ d.y) | (c.z ^ d.z) | (c.w ^ d.w)) != 0) *(lds_ptr<u32x4>)(to + 1024 * i) = d;
+                *(lds_ptr<u32x4>)(to + 1024 * i) = d;
             }
+            lds_barrier();
         };
         auto drafted = [&](int i) -> bool { return (tile_lo + i + 1) * kTreeTokens > s.ctx; };
 
@@ -529,47 +552,49 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
 #pragma unroll
             for (int b = 0; b < 2; ++b) o[c][b] = f32x16{};
         // ---- the first tile, which sets the references -----------------------------------------------------------
-        arrived(0), fill_holes(0, number);
         ask(1);
-        lds_barrier();
         scores(0, std::false_type{}, 0, 0);
-        seen = seen_of(0, 0);
+        seen = seen_of(0, 0), seen_half = seen >> 4 * half;
         bool masked = __builtin_amdgcn_ballot_w64(seen != ~0u) != 0;  // some row may not see some token of tile i
         lds_barrier();
 #pragma unroll
         for (int r = 0; r < 16; ++r) sc[r] = x[0][r] + sh->part[2 * th + kh][r >> 2][lane][r & 3];
         refer(0);
-        if (drafted(0)) clean(0);
         arrived(1), fill_holes(1, number + 1);
         lds_barrier();
         int buf = 0;  // of tile i
         for (int i = 0; i + 1 < n_tiles; ++i) {
             const int next = buf == 2 ? 0 : buf + 1, third = next == 2 ? 0 : next + 1;
             scores(next, std::true_type{}, buf, third);
-            if (__builtin_expect(masked, 0)) weigh_seen(buf);
+            if (__builtin_expect(masked, 0) && weigh_seen(buf)) sh->dirty = number + i;
             if (__builtin_amdgcn_ballot_w64(most > limit) != 0) sh->grown = number + i;
             bool holed = false;
             values(std::true_type{}, buf, third, [&] {
                 const int grown = sh->grown, hole = sh->holed[(number + i + 1) & 1];
+                const bool dirty = __builtin_amdgcn_readfirstlane(sh->dirty) == number + i;
+                if (__builtin_expect(dirty, 0)) clean(buf);
                 if (__builtin_expect(__builtin_amdgcn_readfirstlane(grown) == number + i, 0)) regrow(buf);
                 holed = __builtin_amdgcn_readfirstlane(hole) == number + i + 1;
+                return dirty;
             });
             fill_holes(third, number + i + 2);
             masked = drafted(i + 1) || holed;
-            seen = ~0u;
+            seen = seen_half = ~0u;
             if (__builtin_expect(masked, 0)) {
-                seen = seen_of(i + 1, next);
-                if (drafted(i + 1)) clean(next);
+                seen = seen_of(i + 1, next), seen_half = seen >> 4 * half;
             }
             lds_barrier();
             buf = next;
         }
         weigh_begin(buf);
-        seen = seen_of(n_tiles - 1, buf);
-        weigh_seen(buf);
+        seen = seen_of(n_tiles - 1, buf), seen_half = seen >> 4 * half;
+        if (weigh_seen(buf)) sh->dirty = number + n_tiles - 1;
         if (__builtin_amdgcn_ballot_w64(most > limit) != 0) sh->grown = number + n_tiles - 1;
         values(std::false_type{}, buf, 0, [&] {
+            const bool dirty = __builtin_amdgcn_readfirstlane(sh->dirty) == number + n_tiles - 1;
+            if (dirty) clean(buf);
             if (__builtin_amdgcn_readfirstlane(sh->grown) == number + n_tiles - 1) regrow(buf);
+            return dirty;
         });
         if (a.bad_rows && last_block && l8 == 0 && missing) atomicAdd(a.bad_rows, missing);
         number += n_tiles + 2;  // (two tiles past the end were asked for)
@@ -590,41 +615,53 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
         sh->sum[th][own] = l_sum;
         if (th == 0) sh->ref[own] = m_ref;
     }
-    __syncthreads();
+    lds_barrier();
     if (!whole) {
+        if (n_tiles > 0) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+            for (int c = 0; c < 4; ++c)
 #pragma unroll
-            for (int b = 0; b < 2; ++b)
+                for (int b = 0; b < 2; ++b)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (n_tiles > 0)
+                    for (int i = 0; i < 4; ++i)
                         reinterpret_cast<f32x4*>(rec)[(((wave * 4 + c) * 2 + b) * 4 + i) * kWave + lane] =
                             f32x4{o[c][b][4 * i], o[c][b][4 * i + 1], o[c][b][4 * i + 2], o[c][b][4 * i + 3]};
+        }
         if (tid < kTreeRows) {
             rec[kTreeRows * 512 + 2 * tid] = sh->ref[tid];
             rec[kTreeRows * 512 + 2 * tid + 1] = sh->sum[0][tid] + sh->sum[1][tid];
         }
     } else {
+        // through LDS, a row a store: the same places as the rows' operands had
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-            const int r = kTreeRows * rb + 32 * b + n32;
-            const float l = sh->sum[0][32 * b + n32] + sh->sum[1][32 * b + n32];
+            const int row = 32 * b + n32, r = kTreeRows * rb + row;
+            const float l = sh->sum[0][row] + sh->sum[1][row];
             const float inv = l == 0.0f ? 0.0f : 1.0f / (l * a.qscale);
-            if (r < rows) {
-                uint16_t* const dst = a.clat + ((size_t)s.node0 * a.H + r) * 512 + 128 * wave + 4 * half;
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
+            for (int c = 0; c < 4; ++c)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        *reinterpret_cast<u32x2*>(dst + 16 * c + 64 * (i >> 1) + 8 * (i & 1)) =
-                            u32x2{pack_bf16x2(o[c][b][4 * i] * inv, o[c][b][4 * i + 1] * inv), pack_bf16x2(o[c][b][4 * i + 2] * inv, o[c][b][4 * i + 3] * inv)};
-                if (a.lse && wave == 0 && half == 0)
-                    a.lse[(size_t)s.node0 * a.H + r] = l == 0.0f ? -INFINITY : (sh->ref[32 * b + n32] + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
-            }
+                for (int i = 0; i < 4; ++i)
+                    *(lds_ptr<u32x2>)(tiles + 1024 * row + 16 * ((16 * wave + c * 2 + 8 * (i >> 1) + (i & 1)) ^ (row & 15)) + 8 * half) =
+                        u32x2{pack_bf16x2(o[c][b][4 * i] * inv, o[c][b][4 * i + 1] * inv), pack_bf16x2(o[c][b][4 * i + 2] * inv, o[c][b][4 * i + 3] * inv)};
+            if (a.lse && wave == 0 && half == 0 && r < rows)
+                a.lse[(size_t)s.node0 * a.H + r] = l == 0.0f ? -INFINITY : (sh->ref[row] + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+        }
+        lds_barrier();
+        const int first = kTreeRows * rb + 16 * wave;  // the wave's
+        uint8_t* const out = reinterpret_cast<uint8_t*>(a.clat) + ((size_t)s.node0 * a.H + first) * 1024;
+        const lds_ptr<uint8_t> from = tiles + 1024 * 16 * wave;
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            u32x4 v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = *(lds_ptr<u32x4>)(from + 1024 * (i + k) + 16 * (lane ^ (i + k)));
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (first + i + k < rows) *reinterpret_cast<u32x4*>(out + (1024u * (unsigned)(i + k) + 16u * (unsigned)lane)) = v[k];
         }
     }
-    __syncthreads();
+    lds_barrier();
 }
 
 // RUNS: pages are whole runs of 16 rows.
@@ -632,7 +669,7 @@ template <bool RUNS>
 __global__ __launch_bounds__(kTreeThreads, 1) void mla_attend_tree_kernel(const TreeArgs a) {
     __shared__ __attribute__((aligned(1024))) TreeShared shared;
     const lds_ptr<TreeShared> sh = (lds_ptr<TreeShared>)&shared;
-    if (threadIdx.x == 0) sh->grown = sh->holed[0] = sh->holed[1] = -1;
+    if (threadIdx.x == 0) sh->grown = sh->dirty = sh->holed[0] = sh->holed[1] = -1;
     const bool all = a.groups == 0;  // a block of rows is a work item
     unsigned item = blockIdx.x, u = item, end = u + 1;
     TreeWalk::Block b;
