@@ -183,7 +183,8 @@ extern "C" int rivoli_mla_attend_tree_paged(const unsigned short* qabs, const un
     }
     rk::launch_kernel(page_tokens % 16 == 0 ? rk::mla_attend_tree_kernel<true> : rk::mla_attend_tree_kernel<false>, dim3((unsigned)(plan.groups ? plan.groups : plan.blocks)), dim3(rk::kTreeThreads), 0, st, a);
     const int rc = rk::launch_status();
-    if (rc != 0 || plan.groups == 0) return rc;
-    rk::launch_kernel(rk::mla_attend_tree_merge_kernel, dim3((unsigned)plan.blocks, 32), dim3(256), 0, st, a);
+    if (rc != 0 || plan.groups < 2) return rc;
+    if (plan.blocks < plan.groups) rk::launch_kernel(rk::mla_attend_tree_merge_kernel<false>, dim3((unsigned)plan.blocks, 32), dim3(256), 0, st, a);
+    else rk::launch_kernel(rk::mla_attend_tree_merge_kernel<true>, dim3((unsigned)plan.groups - 1, 32), dim3(256), 0, st, a);
     return rk::launch_status();
 }

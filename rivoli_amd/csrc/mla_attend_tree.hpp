@@ -91,11 +91,11 @@ struct TreeWalk {
         return false;
     }
 };
-// The work items of a cut call, none with less than kTreeMinTiles, the first `more` of them with a tile more than the others.
+// The work items of a cut call, the first `more` of them with a tile more than the others.
 struct TreeItems {
     unsigned items, each, more;
     __device__ __forceinline__ TreeItems(const TreeArgs& a, unsigned total) {
-        items = min(max(total / kTreeMinTiles, 1u), (unsigned)a.groups);
+        items = min(total <= kTreeFewTiles ? total : max(total / kTreeMinTiles, (unsigned)kTreeFewTiles), (unsigned)a.groups);
         if (items > kTreeDies) items = items / kTreeDies * kTreeDies;  // eighths of them stay on one die
         each = total / items, more = total - each * items;
     }
@@ -697,14 +697,28 @@ __global__ __launch_bounds__(kTreeThreads, 1) void mla_attend_tree_kernel(const 
     }
 }
 
-// Blocks that several work items had: their records, in order, under the largest reference. Bound by memory's round trips where
-// there are few: records go eight at a time, every load of a batch in front of the first use.
+// Blocks that several work items had: their records, in order, under the largest reference. A workgroup's column of the launch has a block,
+// or, where there are more blocks than work items (BY_ITEM), the block inside of which its work item begins, the first one of that
+// block. Bound by memory's round trips where there are few: records go eight at a time, every load of a batch in front of the first use.
+template <bool BY_ITEM>
 __global__ __launch_bounds__(256) void mla_attend_tree_merge_kernel(const TreeArgs a) {
     const TreeWalk walk(a);
+    const unsigned total = walk.total(false);
+    if (total == 0) return;
+    const TreeItems items(a, total);
     TreeWalk::Block block;
-    if (!walk.block(true, blockIdx.x, block)) return;
-    const TreeItems items(a, walk.total(false));
-    const unsigned g0 = items.of(block.before), g1 = items.of(block.before + block.tiles - 1);
+    unsigned g0;
+    if (BY_ITEM) {
+        const unsigned g = blockIdx.x + 1;
+        if (g >= items.items) return;
+        const unsigned u = items.lo(g);
+        g0 = g - 1;
+        if (!walk.block(false, u, block) || u == block.before || items.lo(g0) > block.before) return;
+    } else {
+        if (!walk.block(true, blockIdx.x, block)) return;
+        g0 = items.of(block.before);
+    }
+    const unsigned g1 = items.of(block.before + block.tiles - 1);
     if (g0 == g1) return;
     const int at = blockIdx.y * 256 + threadIdx.x, lane = at & 63, idx = at >> 6;
     const int i = idx & 3, b = (idx >> 2) & 1, c = (idx >> 3) & 3, wave = idx >> 5;
@@ -713,12 +727,12 @@ __global__ __launch_bounds__(256) void mla_attend_tree_merge_kernel(const TreeAr
     float m = -INFINITY, l = 0.0f;
     f32x4 sum = {0, 0, 0, 0};
     constexpr int kBatch = 8;
-    for (unsigned g = g0; g <= g1; g += kBatch) {
+    for (unsigned from = g0; from <= g1; from += kBatch) {
         f32x2 ml[kBatch];
         f32x4 v[kBatch];
 #pragma unroll
         for (int k = 0; k < kBatch; ++k) {  // (a record past the last re-reads the last, and is left out)
-            const unsigned rec_of = min(g + k, g1);
+            const unsigned rec_of = min(from + k, g1);
             const float* const rec = a.partial + (size_t)(2 * rec_of + (rec_of == g0 ? 1 : 0)) * kTreeRecordFloats;
             ml[k] = *reinterpret_cast<const f32x2*>(rec + kTreeRows * 512 + 2 * row);
             v[k] = reinterpret_cast<const f32x4*>(rec)[at];
@@ -731,7 +745,7 @@ __global__ __launch_bounds__(256) void mla_attend_tree_merge_kernel(const TreeAr
         m = top, l *= keep, sum *= keep;
 #pragma unroll
         for (int k = 0; k < kBatch; ++k) {
-            if (g + k > g1 || ml[k].y == 0.0f) continue;
+            if (from + k > g1 || ml[k].y == 0.0f) continue;
             const float by = __builtin_amdgcn_exp2f(ml[k].x - top);
             l += ml[k].y * by;
             sum += v[k] * by;

@@ -8,8 +8,13 @@ constexpr int kTreeRows = 64;             // of q (node, head) a workgroup
 constexpr int kTreeTokens = 64;           // of a tile
 constexpr int kTreeGroups = 256;          // workgroups, one per compute unit
 constexpr int kTreeDies = 8;
-constexpr int kTreeMinTiles = 4;          // a work item's least, but for what lengths leave
-constexpr int kTreeWholeTiles = 8;        // up to these a block of rows is one workgroup's
+// A work item's least tiles, but for what the lengths leave. Fewer are not worth their records: 8 blocks of 32 tiles 19.6 us by two, 24.9 by
+// one, 21.6 by four; 1 block of 126 tiles 27.6, 42.5, 26.8. Calls of up to kTreeFewTiles are cut to single tiles: 1 block of 4 or 9 tiles 14.3 us,
+// by two 16.3.
+constexpr int kTreeMinTiles = 2, kTreeFewTiles = 64;
+// Blocks of up to this many tiles are a workgroup's each, where there are kTreeWholeBlocks of them or two tiles at most: 32 blocks of 5 tiles 20.0 us,
+// cut 24.6; 64 of 6 22.7 and 29.4; but 8 of 16 28.1 and 17.2, 1 of 9 25.0 and 14.3.
+constexpr int kTreeWholeTiles = 8, kTreeWholeBlocks = 32;
 constexpr int kTreeRecordFloats = kTreeRows * (512 + 2);
 
 // `blocks`: most blocks of 64 rows. `groups` > 0: that many workgroups share the tiles of all blocks evenly, each leaving up to
@@ -26,8 +31,10 @@ static inline TreePlan tree_plan(int n_seqs, int H, int n_nodes, int max_nodes, 
     const long long by_node = (long long)n_nodes * H / kTreeRows + (n_seqs < n_nodes ? n_seqs : n_nodes);
     p.blocks = by_seq < by_node ? by_seq : by_node;
     const long long tiles = ((long long)max_ctx + max_nodes + kTreeTokens - 1) / kTreeTokens;
-    if (tiles <= kTreeWholeTiles || p.blocks * tiles >= 1ll << 31) return p;  // (cut calls count their tiles in 32 bits)
-    const long long groups = (p.blocks * tiles + kTreeMinTiles - 1) / kTreeMinTiles;
+    const long long most = p.blocks * tiles;
+    if (tiles <= 2 || (tiles <= kTreeWholeTiles && p.blocks >= kTreeWholeBlocks)) return p;
+    if (most >= 1ll << 31) return p;  // (cut calls count their tiles in 32 bits; nor is there anything to gain)
+    const long long groups = most <= kTreeFewTiles ? most : most / kTreeMinTiles > kTreeFewTiles ? most / kTreeMinTiles : kTreeFewTiles;
     p.groups = (int)(groups < kTreeGroups ? groups : kTreeGroups);
     return p;
 }
