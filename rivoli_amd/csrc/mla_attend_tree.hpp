@@ -38,8 +38,8 @@ constexpr int kTreeSteps = 18;            // of 16 dims a wave: 16 of its 256 la
 constexpr float kTreeGrow = 24.0f;
 constexpr uint32_t kTreeHole = 0x80000000u;  // the scale of a token that is not there: -0
 
-// A call's blocks of rows are numbered by sequence, and so are its work units: their tiles, block after block, or the blocks themselves where a
-// workgroup has a whole one. A lane has the lengths of the sequences lane, lane + 64, ...; counts fit 32 bits (tree_plan).
+// A call's blocks of rows are numbered by sequence, and so are its work units: block after block what a block costs to begin with, counted in tiles,
+// and its tiles; or the blocks themselves where a workgroup has a whole one. A lane has the lengths of the sequences lane, lane + 64, ...; counts fit 32 bits (tree_plan).
 struct TreeLane {
     TreeSeq s;
     unsigned blocks, tiles;
@@ -57,20 +57,27 @@ struct TreeWalk {
     const TreeLane first;  // of the first 64 sequences
     __device__ __forceinline__ explicit TreeWalk(const TreeArgs& args) : a(args), first(tree_lane(args, threadIdx.x & 63)) {}
     __device__ __forceinline__ TreeLane lane_of(int s0) const { return s0 == 0 ? first : tree_lane(a, s0 + (int)(threadIdx.x & 63)); }
-    static __device__ __forceinline__ unsigned units(const TreeLane& l, bool whole) { return whole ? l.blocks : l.blocks * l.tiles; }
-    __device__ __forceinline__ unsigned total(bool whole) const {
-        unsigned sum = 0;
-        for (int s0 = 0; s0 < a.n_seqs; s0 += kWave) sum += units(lane_of(s0), whole);
-        return wave_total(wave_inclusive_sum(sum));
+    unsigned begin = 0;    // what a block costs to begin with
+    __device__ __forceinline__ unsigned units(const TreeLane& l, bool whole) const { return whole ? l.blocks : l.blocks * (l.tiles + begin); }
+    // Units in all of a cut call; sets `begin`.
+    __device__ __forceinline__ unsigned total() {
+        unsigned tiles = 0, blocks = 0;
+        for (int s0 = 0; s0 < a.n_seqs; s0 += kWave) {
+            const TreeLane l = lane_of(s0);
+            tiles += l.blocks * l.tiles, blocks += l.blocks;
+        }
+        tiles = wave_total(wave_inclusive_sum(tiles)), blocks = wave_total(wave_inclusive_sum(blocks));
+        begin = tiles <= kTreeGroups ? 0u : kTreeBeginTiles;
+        return tiles + begin * blocks;
     }
-    // The block that unit u is of: its sequence, number and tiles in it, and the tiles before it in all.
+    // The block that unit u is of: its sequence, number and tiles in it, and the unit of its first tile in a cut call.
     struct Block {
         TreeSeq s;
         int seq, rb;
-        unsigned blocks, tiles, before;
+        unsigned blocks, tiles, first_tile;
     };
     __device__ __forceinline__ bool block(bool whole, unsigned u, Block& b) const {
-        unsigned run = 0, tiles_run = 0;
+        unsigned run = 0, cut_run = 0;
         for (int s0 = 0; s0 < a.n_seqs; s0 += kWave) {
             const TreeLane l = lane_of(s0);
             const unsigned mine = units(l, whole), upto = wave_inclusive_sum(mine), all = wave_total(upto);
@@ -80,18 +87,18 @@ struct TreeWalk {
                 b.s.ctx = (int)of((unsigned)l.s.ctx), b.s.node0 = (int)of((unsigned)l.s.node0), b.s.nodes = (int)of((unsigned)l.s.nodes);
                 b.seq = s0 + at, b.blocks = of(l.blocks), b.tiles = of(l.tiles);
                 const unsigned rel = u - run - of(upto - mine);
-                b.rb = (int)(whole ? rel : rel / b.tiles);
-                const unsigned tiles_of = l.blocks * l.tiles;
-                b.before = tiles_run + of(wave_inclusive_sum(tiles_of) - tiles_of) + (unsigned)b.rb * b.tiles;
+                b.rb = (int)(whole ? rel : rel / (b.tiles + begin));
+                const unsigned cut = units(l, false);
+                b.first_tile = cut_run + of(wave_inclusive_sum(cut) - cut) + (unsigned)b.rb * (b.tiles + begin) + begin;
                 return true;
             }
             run += all;
-            tiles_run += wave_total(wave_inclusive_sum(l.blocks * l.tiles));
+            cut_run += wave_total(wave_inclusive_sum(units(l, false)));
         }
         return false;
     }
 };
-// The work items of a cut call, the first `more` of them with a tile more than the others.
+// The work items of a cut call, the first `more` of them with a unit more than the others.
 struct TreeItems {
     unsigned items, each, more;
     __device__ __forceinline__ TreeItems(const TreeArgs& a, unsigned total) {
@@ -619,13 +626,14 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
     if (!whole) {
         if (n_tiles > 0) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
+            for (int b = 0; b < 2; ++b)
+                if (kTreeRows * rb + 32 * b + n32 < rows) {
 #pragma unroll
-                for (int b = 0; b < 2; ++b)
+                    for (int c = 0; c < 4; ++c)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        reinterpret_cast<f32x4*>(rec)[(((wave * 4 + c) * 2 + b) * 4 + i) * kWave + lane] =
+                        for (int i = 0; i < 4; ++i) reinterpret_cast<f32x4*>(rec)[(((wave * 4 + c) * 2 + b) * 4 + i) * kWave + lane] =
                             f32x4{o[c][b][4 * i], o[c][b][4 * i + 1], o[c][b][4 * i + 2], o[c][b][4 * i + 3]};
+                }
         }
         if (tid < kTreeRows) {
             rec[kTreeRows * 512 + 2 * tid] = sh->ref[tid];
@@ -671,12 +679,13 @@ __global__ __launch_bounds__(kTreeThreads, 1) void mla_attend_tree_kernel(const 
     const lds_ptr<TreeShared> sh = (lds_ptr<TreeShared>)&shared;
     if (threadIdx.x == 0) sh->grown = sh->dirty = sh->holed[0] = sh->holed[1] = -1;
     const bool all = a.groups == 0;  // a block of rows is a work item
-    unsigned item = blockIdx.x, u = item, end = u + 1;
+    unsigned item = blockIdx.x, u = item, end = u + 1, begin = 0;
     TreeWalk::Block b;
     {
-        const TreeWalk walk(a);
+        TreeWalk walk(a);
         if (!all) {
-            const unsigned total = walk.total(false);
+            const unsigned total = walk.total();
+            begin = walk.begin;
             if (total == 0) return;
             const TreeItems items(a, total);
             if (item >= items.items) return;
@@ -687,12 +696,13 @@ __global__ __launch_bounds__(kTreeThreads, 1) void mla_attend_tree_kernel(const 
         if (!walk.block(all, u, b)) return;
     }
     for (int number = 0;;) {
-        const int lo = all ? 0 : (int)(u - b.before), hi = all ? (int)b.tiles : (int)min(b.tiles, lo + end - u);
+        const int lo = all ? 0 : max((int)(u - b.first_tile), 0), hi = all ? (int)b.tiles : min((int)b.tiles, (int)(end - b.first_tile));
         float* const rec = a.partial + (size_t)(2 * item + (lo == 0 ? 1 : 0)) * kTreeRecordFloats;
-        tree_part<RUNS>(a, sh, b.s, b.seq, b.rb, b.rb == (int)b.blocks - 1, lo, hi, lo == 0 && hi == (int)b.tiles, rec, number);
-        u += all ? 1 : hi - lo;
+        if (hi > lo) tree_part<RUNS>(a, sh, b.s, b.seq, b.rb, b.rb == (int)b.blocks - 1, lo, hi, lo == 0 && hi == (int)b.tiles, rec, number);
+        u = all ? end : b.first_tile + b.tiles;
         if (u >= end) return;
-        const TreeWalk walk(a);  // (looked up again: what it has would keep registers through the tiles)
+        TreeWalk walk(a);  // (looked up again: what it has would keep registers through the tiles)
+        walk.begin = begin;
         if (!walk.block(false, u, b)) return;
     }
 }
@@ -702,8 +712,8 @@ __global__ __launch_bounds__(kTreeThreads, 1) void mla_attend_tree_kernel(const 
 // block. Bound by memory's round trips where there are few: records go eight at a time, every load of a batch in front of the first use.
 template <bool BY_ITEM>
 __global__ __launch_bounds__(256) void mla_attend_tree_merge_kernel(const TreeArgs a) {
-    const TreeWalk walk(a);
-    const unsigned total = walk.total(false);
+    TreeWalk walk(a);
+    const unsigned total = walk.total();
     if (total == 0) return;
     const TreeItems items(a, total);
     TreeWalk::Block block;
@@ -713,12 +723,12 @@ __global__ __launch_bounds__(256) void mla_attend_tree_merge_kernel(const TreeAr
         if (g >= items.items) return;
         const unsigned u = items.lo(g);
         g0 = g - 1;
-        if (!walk.block(false, u, block) || u == block.before || items.lo(g0) > block.before) return;
+        if (!walk.block(false, u, block) || u <= block.first_tile || items.lo(g0) > block.first_tile) return;
     } else {
         if (!walk.block(true, blockIdx.x, block)) return;
-        g0 = items.of(block.before);
+        g0 = items.of(block.first_tile);
     }
-    const unsigned g1 = items.of(block.before + block.tiles - 1);
+    const unsigned g1 = items.of(block.first_tile + block.tiles - 1);
     if (g0 == g1) return;
     const int at = blockIdx.y * 256 + threadIdx.x, lane = at & 63, idx = at >> 6;
     const int i = idx & 3, b = (idx >> 2) & 1, c = (idx >> 3) & 3, wave = idx >> 5;

@@ -12,6 +12,9 @@ constexpr int kTreeDies = 8;
 // one, 21.6 by four; 1 block of 126 tiles 27.6, 42.5, 26.8. Calls of up to kTreeFewTiles are cut to single tiles: 1 block of 4 or 9 tiles 14.3 us,
 // by two 16.3.
 constexpr int kTreeMinTiles = 2, kTreeFewTiles = 64;
+// What a block costs a work item to begin with and end, in tiles: 13 ragged sequences of up to 79 tiles, 3 blocks each, 32.9 us, as nothing 44.8;
+// 1 of 513, 8 blocks, 58.0 and 65.9. Nothing in calls of less than a tile a workgroup: 8 blocks of 16 17.1 us, and 20.1.
+constexpr unsigned kTreeBeginTiles = 3;
 // Blocks of up to this many tiles are a workgroup's each, where there are kTreeWholeBlocks of them or two tiles at most: 32 blocks of 5 tiles 20.0 us,
 // cut 24.6; 64 of 6 22.7 and 29.4; but 8 of 16 28.1 and 17.2, 1 of 9 25.0 and 14.3.
 constexpr int kTreeWholeTiles = 8, kTreeWholeBlocks = 32;
@@ -33,7 +36,7 @@ static inline TreePlan tree_plan(int n_seqs, int H, int n_nodes, int max_nodes, 
     const long long tiles = ((long long)max_ctx + max_nodes + kTreeTokens - 1) / kTreeTokens;
     const long long most = p.blocks * tiles;
     if (tiles <= 2 || (tiles <= kTreeWholeTiles && p.blocks >= kTreeWholeBlocks)) return p;
-    if (most >= 1ll << 31) return p;  // (cut calls count their tiles in 32 bits; nor is there anything to gain)
+    if (most >= 1ll << 29) return p;  // (cut calls count their tiles in 32 bits; nor is there anything to gain)
     const long long groups = most <= kTreeFewTiles ? most : most / kTreeMinTiles > kTreeFewTiles ? most / kTreeMinTiles : kTreeFewTiles;
     p.groups = (int)(groups < kTreeGroups ? groups : kTreeGroups);
     return p;
