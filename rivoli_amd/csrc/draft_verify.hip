@@ -16,10 +16,24 @@
 
 namespace rk {
 
+//
+// What bounds it. The walk is a chain of short steps in LDS by one wave, some 7 us with the launch and the nodes' scattered loads; a row's sum reads it once,
+// and a rejected draft whose sibling is still to be judged reads target and draft rows once more, by the sequence's own workgroup: 131 072 tokens
+// of f32 and a draft are 1 MB, some 16 us for a compute unit, as much its conversions and sums in 64 bits as its loads. 256 sequences of 8 drawn nodes
+// of that size take 94 us where one read of two rows each is 54, the rest being second and third siblings; 32 of 16 picked nodes 14 us; one of 4 over 32 001 tokens 8.4.
+// A wave's loads of a block are all on their way before the first is used, and picked tokens that were rejected are looked for once a block:
+// testing each weight against each of them took 28 us where the row's sum now takes 14.
 constexpr int kVerifyThreads = 1024, kVerifyWaves = kVerifyThreads / kWave;
 constexpr int kVerifyNodes = 1024;             // of a sequence, held in LDS
-constexpr int kVerifyBlock = 8 * kWave;        // tokens of a block: eight a lane
-constexpr int kVerifyBlocks = 4096;            // block sums in LDS: up to 2^21 tokens
+constexpr int kVerifyChunk = 8 * kWave;        // tokens a wave's loads bring at once: eight a lane
+constexpr int kVerifyChunks = 2;               // of a block: four of them spill in a workgroup of 16 waves, and are no faster
+constexpr int kVerifyBlock = kVerifyChunks * kVerifyChunk;
+constexpr int kVerifyBlocks = 2048;            // block sums in LDS: up to 2^21 tokens
+// Calls of few sequences and long rows have the last pass over a row, the only one that most have, by many workgroups in a launch of its own, and the draw in a third. In
+// us, one launch and three: 1 sequence of 131 072 picked bf16 tokens 14.6 and 11.8, 32 of them 15.2 and 12.5, 32 of f32 with drafts 45 and 39; 64 of those
+// 40 and 45; 32 of 65 536 picked 11.0 and 12.1.
+constexpr int kVerifySplitSeqs = 32, kVerifySplitVocab = 98304;
+constexpr int kVerifySumThreads = 256, kVerifySumBlocks = 4;  // a workgroup of the split form: a block a wave
 
 struct VerifyArgs {
     const void *target, *draft;
@@ -28,37 +42,65 @@ struct VerifyArgs {
     int n_nodes, max_nodes, vocab;
     long long target_stride, draft_stride;  // in elements
     int *path, *n_path, *next;
+    // the split form's, by sequence: the walk's end (node and rejections), its levels and rejected tokens, the blocks' sums
+    int* end;
+    double* levels;
+    int* gone;
+    double* sums;
     unsigned int* bad;
 };
 
-// A probability as it counts: what is no number, or negative, as zero.
-__device__ __forceinline__ float counted(float x) { return x > 0.0f ? fminf(x, FLT_MAX) : 0.0f; }
+// A probability as it counts: what is no number, or negative, as zero, infinity as the largest. (The median of three with a quiet NaN among
+// them is the least of the others; a signalling one it would pass on.)
+__device__ __forceinline__ float counted(float x) { return __builtin_amdgcn_fmed3f(__builtin_canonicalizef(x), 0.0f, FLT_MAX); }
 
 template <bool BF16>
 __device__ __forceinline__ float prob(const void* rows, long long at) {
     if constexpr (BF16) return counted(__uint_as_float((uint32_t) static_cast<const uint16_t*>(rows)[at] << 16));
     else return counted(static_cast<const float*>(rows)[at]);
 }
-// Eight of a row from `at`, of which `n` are there.
+// Eight of a row from `at`, as loaded, and as they count. A row starts where its stride puts it: on an element.
 template <bool BF16>
-__device__ __forceinline__ void prob8(const void* rows, long long at, int n, float (&p)[8]) {
-    if (n >= 8) {  // (a row starts where its stride puts it: on an element)
-        if constexpr (BF16) {
-            typedef u32x4 words __attribute__((aligned(2)));
-            const u32x4 v = *reinterpret_cast<const words*>(static_cast<const uint16_t*>(rows) + at);
+struct Eight;
+template <>
+struct Eight<true> {
+    u32x4 v;
+    __device__ __forceinline__ void load(const void* rows, long long at) {
+        typedef u32x4 words __attribute__((aligned(2)));
+        v = *reinterpret_cast<const words*>(static_cast<const uint16_t*>(rows) + at);
+    }
+    __device__ __forceinline__ float operator[](int i) const { return counted(i & 1 ? bf16_hi_to_f32(v[i >> 1]) : bf16_lo_to_f32(v[i >> 1])); }
+};
+template <>
+struct Eight<false> {
+    typedef float f32x4v __attribute__((ext_vector_type(4)));
+    f32x4v lo, hi;
+    __device__ __forceinline__ void load(const void* rows, long long at) {
+        typedef f32x4v words __attribute__((aligned(4)));
+        const words* const src = reinterpret_cast<const words*>(static_cast<const float*>(rows) + at);
+        lo = src[0], hi = src[1];
+    }
+    __device__ __forceinline__ float operator[](int i) const { return counted(i < 4 ? lo[i] : hi[i - 4]); }
+};
+
+// The same with `left` tokens from there on, of which some may not be (they count as zero).
+template <bool BF16>
+__device__ __forceinline__ void load_some(Eight<BF16>& x, const void* rows, long long at, int left) {
+    x = Eight<BF16>{};
+    if (left >= 8) {
+        x.load(rows, at);
+    } else if (left > 0) {
+        for (int i = 0; i < left; ++i) {
+            if constexpr (BF16) {
+                const uint32_t v = static_cast<const uint16_t*>(rows)[at + i];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) p[2 * i] = counted(bf16_lo_to_f32(v[i])), p[2 * i + 1] = counted(bf16_hi_to_f32(v[i]));
-        } else {
-            typedef float f32x4v __attribute__((ext_vector_type(4)));
-            typedef f32x4v words __attribute__((aligned(4)));
-            const words* src = reinterpret_cast<const words*>(static_cast<const float*>(rows) + at);
-            const f32x4v lo = src[0], hi = src[1];
+                for (int j = 0; j < 4; ++j) x.v[j] |= j == i >> 1 ? v << (16 * (i & 1)) : 0u;
+            } else {
+                const float v = static_cast<const float*>(rows)[at + i];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) p[i] = counted(lo[i]), p[4 + i] = counted(hi[i]);
+                for (int j = 0; j < 4; ++j) x.lo[j] = j == i ? v : x.lo[j], x.hi[j] = j + 4 == i ? v : x.hi[j];
+            }
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) p[i] = i < n ? prob<BF16>(rows, at + i) : 0.0f;
     }
 }
 
@@ -73,19 +115,159 @@ __device__ __forceinline__ double lanes_before(double x, double& total) {
     total = __shfl(sum, kWave - 1, kWave);
     return sum - x;
 }
+// The same over all of them alone, by rotations within sixteen lanes and swaps of those rows: no trip through LDS, which a shuffle is.
+template <int CTRL>
+__device__ __forceinline__ double rotated(double x) {
+    const long long v = __builtin_bit_cast(long long, x);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xf, 0xf, true), hi = (uint32_t)__builtin_amdgcn_mov_dpp((int)(v >> 32), CTRL, 0xf, 0xf, true);
+    return __builtin_bit_cast(double, ((unsigned long long)hi << 32) | lo);
+}
 __device__ __forceinline__ double lanes_sum(double x) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, kWave);
-    return x;
+    x += rotated<0x128>(x), x += rotated<0x124>(x), x += rotated<0x122>(x), x += rotated<0x121>(x);
+    const auto both = [](uint32_t lo, uint32_t hi) -> double { return __builtin_bit_cast(double, ((unsigned long long)hi << 32) | lo); };
+    unsigned long long v = __builtin_bit_cast(unsigned long long, x);
+    auto l = __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false);
+    auto h = __builtin_amdgcn_permlane16_swap((uint32_t)(v >> 32), (uint32_t)(v >> 32), false, false);
+    x = both(l[0], h[0]) + both(l[1], h[1]);
+    v = __builtin_bit_cast(unsigned long long, x);
+    l = __builtin_amdgcn_permlane32_swap((uint32_t)v, (uint32_t)v, false, false);
+    h = __builtin_amdgcn_permlane32_swap((uint32_t)(v >> 32), (uint32_t)(v >> 32), false, false);
+    return both(l[0], h[0]) + both(l[1], h[1]);
 }
 
+// A node's row after k rejections.
 template <bool BF16>
+struct Row {
+    const VerifyArgs& a;
+    long long p_at, q_at;
+    int k;
+    const double* level;  // in LDS, as is gone
+    const int* gone;
+    __device__ __forceinline__ Row(const VerifyArgs& args, int node, int rejections, const double* levels, const int* tokens)
+        : a(args), p_at(node * args.target_stride), q_at(node * args.draft_stride), k(rejections), level(levels), gone(tokens) {}
+    static __device__ __forceinline__ double eights(const double (&w)[8]) { return ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])); }
+    // Calls f(first token, weights of eight) for this lane's part of each of block b's chunks, whose loads are on their way before the first is used.
+    template <class F>
+    __device__ __forceinline__ void chunks(int b, F f) const {
+        const int v = b * kVerifyBlock + 8 * (int)(threadIdx.x & 63);
+        const bool drafted = a.draft && k > 0;
+        bool less = false;  // whether picked tokens that were rejected lie here: they are few
+        if (!a.draft) {
+            for (int j = 0; j < k; j += kWave)
+                less |= __builtin_amdgcn_ballot_w64((unsigned)(gone[min(j + (int)(threadIdx.x & 63), k - 1)] - b * kVerifyBlock) < (unsigned)kVerifyBlock) != 0;
+        }
+        Eight<BF16> p[kVerifyChunks], q[kVerifyChunks];
+        if ((b + 1) * kVerifyBlock <= a.vocab) {
+#pragma unroll
+            for (int c = 0; c < kVerifyChunks; ++c) p[c].load(a.target, p_at + v + c * kVerifyChunk);
+            if (drafted) {
+#pragma unroll
+                for (int c = 0; c < kVerifyChunks; ++c) q[c].load(a.draft, q_at + v + c * kVerifyChunk);
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < kVerifyChunks; ++c) load_some<BF16>(p[c], a.target, p_at + v + c * kVerifyChunk, a.vocab - v - c * kVerifyChunk);
+            if (drafted) {
+#pragma unroll
+                for (int c = 0; c < kVerifyChunks; ++c) load_some<BF16>(q[c], a.draft, q_at + v + c * kVerifyChunk, a.vocab - v - c * kVerifyChunk);
+            }
+        }
+        double w[kVerifyChunks][8];
+#pragma unroll
+        for (int i = 0; i < 8 * kVerifyChunks; ++i) w[i / 8][i % 8] = (double)p[i / 8][i % 8];
+        if (drafted) {
+            for (int j = 0; j < k; ++j) {
+                const double c = level[j];
+#pragma unroll
+                for (int i = 0; i < 8 * kVerifyChunks; ++i) w[i / 8][i % 8] = fmax(w[i / 8][i % 8] - c * (double)q[i / 8][i % 8], 0.0);
+            }
+        } else if (less) {
+            for (int j = 0; j < k; ++j) {
+                const int x = gone[j] - v;
+#pragma unroll
+                for (int i = 0; i < 8 * kVerifyChunks; ++i) w[i / 8][i % 8] = x == i / 8 * kVerifyChunk + i % 8 ? 0.0 : w[i / 8][i % 8];
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < kVerifyChunks; ++c) f(v + c * kVerifyChunk, w[c]);
+    }
+    // The sum of block b, by a wave.
+    __device__ __forceinline__ double block(int b) const {
+        double sum = 0.0;
+        chunks(b, [&](int, const double(&w)[8]) { sum += eights(w); });
+        return lanes_sum(sum);
+    }
+};
+
+// The sums of every block of a row by a workgroup, and of all of them.
+template <class R>
+__device__ __forceinline__ void sum_row(const R& row, int blocks, double* sums, double* all) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int b = wave; b < blocks; b += kVerifyWaves) {
+        const double s = row.block(b);
+        if (lane == 0) sums[b] = s;
+    }
+    __syncthreads();
+    if (wave == 0) {
+        double s = 0.0;
+        for (int b = lane; b < blocks; b += kWave) s += sums[b];
+        s = lanes_sum(s);
+        if (lane == 0) *all = s;
+    }
+    __syncthreads();
+}
+
+// The first token whose running sum is past `goal`, by a wave, from the blocks' sums, some of which is positive.
+template <class R>
+__device__ __forceinline__ int drawn(const R& row, int blocks, const double* sums, double goal) {
+    const int lane = threadIdx.x & 63;
+    // the block: a lane has `each` of them in a row
+    const int each = (blocks + kWave - 1) / kWave;
+    double mine = 0.0, total;
+    int some = -1;  // the lane's last block with anything in it
+    for (int i = 0; i < each; ++i) {
+        const int b = lane * each + i;
+        if (b < blocks && sums[b] > 0.0) mine += sums[b], some = b;
+    }
+    double run = lanes_before(mine, total);
+    const unsigned long long past = __builtin_amdgcn_ballot_w64(run + mine > goal && some >= 0);
+    const unsigned long long any = __builtin_amdgcn_ballot_w64(some >= 0);
+    const int holder = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(any);
+    run = __shfl(run, holder, kWave), some = __shfl(some, holder, kWave);
+    int block = holder * each;
+    for (; block < some; ++block) {
+        if (run + sums[block] > goal) break;
+        run += sums[block];
+    }
+    // and in it: the first past the goal, or the last with anything in it where the sums' roundings leave none
+    int answer = -1, found = -1;
+    row.chunks(block, [&](int v, const double(&w)[8]) {
+        double upto = run + lanes_before(R::eights(w), total);
+        int first = -1, held = -1;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            upto += w[i];
+            if (w[i] > 0.0) {
+                held = v + i;
+                if (first < 0 && upto > goal) first = v + i;
+            }
+        }
+        const unsigned long long past = __builtin_amdgcn_ballot_w64(first >= 0), left = __builtin_amdgcn_ballot_w64(held >= 0);
+        if (left) answer = __shfl(held, 63 - __builtin_clzll(left), kWave);
+        if (past && found < 0) found = __shfl(first, __builtin_ctzll(past), kWave);
+        run += total;
+    });
+    return found >= 0 ? found : answer;
+}
+
+// The walk of a sequence's tree, a workgroup each; and, unless SPLIT, the next token.
+template <bool BF16, bool SPLIT>
 __global__ __launch_bounds__(kVerifyThreads) void draft_verify_kernel(const VerifyArgs a) {
     __shared__ int parent[kVerifyNodes], token[kVerifyNodes], gone[kVerifyNodes];  // gone: tokens rejected at cur
     __shared__ float share[kVerifyNodes], p_of[kVerifyNodes], q_of[kVerifyNodes];
     __shared__ double level[kVerifyNodes];  // c_0 .. c_k at cur
     __shared__ double sums[kVerifyBlocks];
-    __shared__ int state[4];
+    __shared__ int state[3];
     __shared__ double all;
     const int seq = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int node0 = min(max(a.cu[seq], 0), a.n_nodes);
@@ -94,6 +276,7 @@ __global__ __launch_bounds__(kVerifyThreads) void draft_verify_kernel(const Veri
     if (n == 0) {
         for (int i = tid; i < a.max_nodes; i += kVerifyThreads) path[i] = -1;
         if (tid == 0) a.n_path[seq] = 0, a.next[seq] = -1;
+        if (SPLIT && tid == 0) a.end[2 * seq] = -1;
         return;
     }
     for (int i = tid; i < n; i += kVerifyThreads) {
@@ -108,47 +291,7 @@ __global__ __launch_bounds__(kVerifyThreads) void draft_verify_kernel(const Veri
         p_of[i] = there ? prob<BF16>(a.target, (long long)(node0 + up) * a.target_stride + x) : 0.0f;
         q_of[i] = there && a.draft ? prob<BF16>(a.draft, (long long)(node0 + up) * a.draft_stride + x) : 1.0f;
     }
-    __syncthreads();
-
     const int blocks = (a.vocab + kVerifyBlock - 1) / kVerifyBlock;
-    // w of eight tokens from v on, after `k` rejections at `cur`
-    auto weights = [&](int cur, int k, int v, double (&w)[8]) {
-        float p[8], q[8];
-        prob8<BF16>(a.target, (long long)(node0 + cur) * a.target_stride + v, a.vocab - v, p);
-        if (a.draft && k > 0) prob8<BF16>(a.draft, (long long)(node0 + cur) * a.draft_stride + v, a.vocab - v, q);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = (double)p[i];
-        if (a.draft) {
-            for (int j = 0; j < k; ++j) {
-                const double c = level[j];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) w[i] = fmax(w[i] - c * (double)q[i], 0.0);
-            }
-        } else {
-            for (int j = 0; j < k; ++j) {
-                const int x = gone[j] - v;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) w[i] = x == i ? 0.0 : w[i];
-            }
-        }
-    };
-    // The sums of every block, and of all of them.
-    auto sum_row = [&](int cur, int k) {
-        for (int b = wave; b < blocks; b += kVerifyWaves) {
-            double w[8];
-            weights(cur, k, b * kVerifyBlock + 8 * lane, w);
-            const double s = lanes_sum(((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])));
-            if (lane == 0) sums[b] = s;
-        }
-        __syncthreads();
-        if (wave == 0) {
-            double s = 0.0;
-            for (int b = lane; b < blocks; b += kWave) s += sums[b];
-            s = lanes_sum(s);
-            if (lane == 0) all = s;
-        }
-        __syncthreads();
-    };
 
     // ---- the walk: wave 0 goes on until it is done or needs the sum of a residual ------------------------------
     auto child_after = [&](int cur, int last) -> int {
@@ -197,7 +340,7 @@ __global__ __launch_bounds__(kVerifyThreads) void draft_verify_kernel(const Veri
         __syncthreads();
         const int at = state[0], after = state[1], need = state[2];
         if (!need) break;
-        sum_row(at, after);
+        sum_row(Row<BF16>(a, node0 + at, after, level, gone), blocks, sums, &all);
         if (tid == 0) level[after] = all;
         __syncthreads();
     }
@@ -206,67 +349,107 @@ __global__ __launch_bounds__(kVerifyThreads) void draft_verify_kernel(const Veri
         for (int i = count + lane; i < a.max_nodes; i += kWave) path[i] = -1;
         if (lane == 0) a.n_path[seq] = count;
     }
-
-    // ---- the next token ----------------------------------------------------------------------------------------
-    sum_row(cur, k);
+    if (SPLIT) {
+        if (tid == 0) a.end[2 * seq] = node0 + cur, a.end[2 * seq + 1] = k;
+        for (int j = tid; j < k; j += kVerifyThreads) {
+            a.levels[(size_t)seq * a.max_nodes + j] = a.draft ? level[j] : 0.0;
+            a.gone[(size_t)seq * a.max_nodes + j] = gone[j];
+        }
+        return;
+    }
+    sum_row(Row<BF16>(a, node0 + cur, k, level, gone), blocks, sums, &all);
     if (!(all > 0.0) && k > 0) {  // nothing is left of it: the node's own row
         k = 0;
         __syncthreads();
-        sum_row(cur, 0);
+        sum_row(Row<BF16>(a, node0 + cur, 0, level, gone), blocks, sums, &all);
     }
     if (wave != 0) return;
-    if (!(all > 0.0)) {
-        if (lane == 0) a.next[seq] = -1;
-        return;
+    const int next = all > 0.0 ? drawn(Row<BF16>(a, node0 + cur, k, level, gone), blocks, sums, (double)a.u_final[seq] * all) : -1;
+    if (lane == 0) a.next[seq] = next;
+}
+
+// The split form's second launch, a wave a block of the row that a sequence's walk ended with, and its third, which draws from their sums.
+template <bool BF16>
+__global__ __launch_bounds__(kVerifySumThreads) void draft_sums_kernel(const VerifyArgs a) {
+    __shared__ double level[kVerifyNodes];
+    __shared__ int gone[kVerifyNodes];
+    const int seq = blockIdx.y, node = a.end[2 * seq], k = a.end[2 * seq + 1];
+    if (node < 0) return;
+    for (int j = threadIdx.x; j < k; j += kVerifySumThreads)
+        level[j] = a.levels[(size_t)seq * a.max_nodes + j], gone[j] = a.gone[(size_t)seq * a.max_nodes + j];
+    __syncthreads();
+    const int blocks = (a.vocab + kVerifyBlock - 1) / kVerifyBlock, b = blockIdx.x * kVerifySumBlocks + (int)(threadIdx.x >> 6);
+    if (b >= blocks) return;
+    const double s = Row<BF16>(a, node, k, level, gone).block(b);
+    if ((threadIdx.x & 63) == 0) a.sums[(size_t)seq * blocks + b] = s;
+}
+
+template <bool BF16>
+__global__ __launch_bounds__(kVerifyThreads) void draft_draw_kernel(const VerifyArgs a) {
+    __shared__ double level[kVerifyNodes];
+    __shared__ int gone[kVerifyNodes];
+    __shared__ double sums[kVerifyBlocks];
+    __shared__ double all;
+    const int seq = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, node = a.end[2 * seq];
+    int k = a.end[2 * seq + 1];
+    if (node < 0) return;
+    const int blocks = (a.vocab + kVerifyBlock - 1) / kVerifyBlock;
+    for (int j = threadIdx.x; j < k; j += kVerifyThreads)
+        level[j] = a.levels[(size_t)seq * a.max_nodes + j], gone[j] = a.gone[(size_t)seq * a.max_nodes + j];
+    for (int b = threadIdx.x; b < blocks; b += kVerifyThreads) sums[b] = a.sums[(size_t)seq * blocks + b];
+    __syncthreads();
+    if (wave == 0) {
+        double s = 0.0;
+        for (int b = lane; b < blocks; b += kWave) s += sums[b];
+        s = lanes_sum(s);
+        if (lane == 0) all = s;
     }
-    // the block: a lane has `each` of them in a row
-    const double goal = (double)a.u_final[seq] * all;
-    const int each = (blocks + kWave - 1) / kWave;
-    double mine = 0.0, total;
-    int some = -1;  // the lane's last block with anything in it
-    for (int i = 0; i < each; ++i) {
-        const int b = lane * each + i;
-        if (b < blocks && sums[b] > 0.0) mine += sums[b], some = b;
+    __syncthreads();
+    if (!(all > 0.0) && k > 0) {
+        k = 0;
+        __syncthreads();
+        sum_row(Row<BF16>(a, node, 0, level, gone), blocks, sums, &all);
     }
-    double run = lanes_before(mine, total);
-    const unsigned long long past = __builtin_amdgcn_ballot_w64(run + mine > goal && some >= 0);
-    const unsigned long long any = __builtin_amdgcn_ballot_w64(some >= 0);
-    const int holder = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(any);
-    run = __shfl(run, holder, kWave), some = __shfl(some, holder, kWave);
-    int block = some;
-    for (int i = 0; i < each; ++i) {
-        const int b = holder * each + i;
-        if (b >= blocks || b >= some) break;
-        if (run + sums[b] > goal) {
-            block = b;
-            break;
-        }
-        run += sums[b];
+    if (wave != 0) return;
+    const int next = all > 0.0 ? drawn(Row<BF16>(a, node, k, level, gone), blocks, sums, (double)a.u_final[seq] * all) : -1;
+    if (lane == 0) a.next[seq] = next;
+}
+
+// Whether a call takes the split form, and the pieces of its workspace (from 16-byte boundaries on).
+struct VerifySplit {
+    bool on;
+    size_t levels, sums, gone, end, bytes;
+};
+static VerifySplit verify_split(int n_seqs, int max_nodes, int vocab) {
+    VerifySplit s{n_seqs > 0 && n_seqs <= kVerifySplitSeqs && max_nodes > 0 && vocab >= kVerifySplitVocab, 0, 0, 0, 0, 0};
+    if (!s.on) return s;
+    const size_t blocks = ((size_t)vocab + kVerifyBlock - 1) / kVerifyBlock, n = (size_t)n_seqs;
+    s.sums = n * max_nodes * 8;
+    s.gone = s.sums + n * blocks * 8;
+    s.end = s.gone + n * max_nodes * 4;
+    s.bytes = (s.end + n * 8 + 15) / 16 * 16;
+    return s;
+}
+
+template <bool BF16>
+static int draft_verify(const VerifyArgs& a, bool split, int n_seqs, hipStream_t st) {
+    (void)hipGetLastError();
+    const dim3 grid((unsigned)n_seqs), block(kVerifyThreads);
+    if (!split) {
+        launch_kernel(draft_verify_kernel<BF16, false>, grid, block, 0, st, a);
+        return launch_status();
     }
-    // and in it: the first past the goal, or the last with anything in it where the sums' roundings leave none
-    double w[8];
-    const int v = block * kVerifyBlock + 8 * lane;
-    weights(cur, k, v, w);
-    double upto = run + lanes_before(((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])), total);
-    int first = -1, held = -1;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        upto += w[i];
-        if (w[i] > 0.0) {
-            held = v + i;
-            if (first < 0 && upto > goal) first = v + i;
-        }
-    }
-    const unsigned long long found = __builtin_amdgcn_ballot_w64(first >= 0), left = __builtin_amdgcn_ballot_w64(held >= 0);
-    const int answer = found ? __shfl(first, __builtin_ctzll(found), kWave) : __shfl(held, 63 - __builtin_clzll(left), kWave);
-    if (lane == 0) a.next[seq] = answer;
+    const unsigned blocks = (unsigned)((a.vocab + kVerifyBlock - 1) / kVerifyBlock);
+    launch_kernel(draft_verify_kernel<BF16, true>, grid, block, 0, st, a);
+    launch_kernel(draft_sums_kernel<BF16>, dim3((blocks + kVerifySumBlocks - 1) / kVerifySumBlocks, (unsigned)n_seqs), dim3(kVerifySumThreads), 0, st, a);
+    launch_kernel(draft_draw_kernel<BF16>, grid, block, 0, st, a);
+    return launch_status();
 }
 
 }  // namespace rk
 
 extern "C" size_t rivoli_draft_verify_workspace_bytes(int n_seqs, int max_nodes, int vocab) {
-    (void)n_seqs, (void)max_nodes, (void)vocab;
-    return 0;
+    return rk::verify_split(n_seqs, max_nodes, vocab).bytes;
 }
 
 extern "C" int rivoli_draft_verify(const void* target_probs, const void* draft_probs, const int* tokens,
@@ -274,20 +457,20 @@ extern "C" int rivoli_draft_verify(const void* target_probs, const void* draft_p
                                    const float* final_uniforms, int n_seqs, int n_nodes, int max_nodes, int vocab,
                                    long long target_stride, long long draft_stride, int bf16, int* path, int* n_path,
                                    int* next_token, void* workspace, unsigned int* bad_nodes, void* stream) {
-    (void)workspace;
     if (!target_probs || !tokens || !parents || !cu_nodes || !uniforms || !final_uniforms || !path || !n_path ||
         !next_token || n_seqs <= 0 || n_nodes <= 0 || max_nodes <= 0 || vocab <= 0)
         return 1001;
     if (max_nodes > rk::kVerifyNodes || vocab > rk::kVerifyBlocks * rk::kVerifyBlock || target_stride < vocab ||
         (draft_probs && draft_stride < vocab))
         return 1002;
+    const rk::VerifySplit split = rk::verify_split(n_seqs, max_nodes, vocab);
+    if (split.on && !workspace) return 1001;
     const uintptr_t size = bf16 ? 2 : 4;
-    if ((uintptr_t)target_probs % size != 0 || (uintptr_t)draft_probs % size != 0) return 1004;
+    if ((uintptr_t)target_probs % size != 0 || (uintptr_t)draft_probs % size != 0 || !rk::aligned16(workspace)) return 1004;
+    unsigned char* const work = static_cast<unsigned char*>(workspace);
     const rk::VerifyArgs a{target_probs, draft_probs, tokens, parents, cu_nodes, uniforms, final_uniforms, n_nodes, max_nodes, vocab,
-                           target_stride, draft_stride, path, n_path, next_token, bad_nodes};
-    (void)hipGetLastError();
-    const dim3 grid((unsigned)n_seqs), block(rk::kVerifyThreads);
-    if (bf16) rk::launch_kernel(rk::draft_verify_kernel<true>, grid, block, 0, (hipStream_t)stream, a);
-    else rk::launch_kernel(rk::draft_verify_kernel<false>, grid, block, 0, (hipStream_t)stream, a);
-    return rk::launch_status();
+                           target_stride, draft_stride, path, n_path, next_token, reinterpret_cast<int*>(work + split.end),
+                           reinterpret_cast<double*>(work + split.levels), reinterpret_cast<int*>(work + split.gone),
+                           reinterpret_cast<double*>(work + split.sums), bad_nodes};
+    return bf16 ? rk::draft_verify<true>(a, split.on, n_seqs, (hipStream_t)stream) : rk::draft_verify<false>(a, split.on, n_seqs, (hipStream_t)stream);
 }

@@ -45,7 +45,7 @@ def test_tree_attention_refusals():
     changes += [(dict([(name, 0)]), 1001) for name in ("n_seqs", "H", "n_nodes", "max_nodes", "max_blocks_per_seq", "kvl", "rope",
                                                       "page_tokens", "n_pages")]
     changes += [(dict(max_ctx=-1), 1001), (dict(n_seqs=65536), 1002), (dict(max_nodes=4097), 1002), (dict(max_ctx=2 ** 31 - 8192), 1002),
-                (dict(n_nodes=2 ** 27), 1002), (dict(kvl=640), 1004), (dict(kvl=192), 1004), (dict(rope=12), 1004), (dict(rope=72), 1004),
+                (dict(n_nodes=2 ** 27), 1002), (dict(page_tokens=2 ** 22 + 4), 1002), (dict(kvl=640), 1004), (dict(kvl=192), 1004), (dict(rope=12), 1004), (dict(rope=72), 1004),
                 (dict(page_tokens=6), 1004)]
     changes += [(dict([(name, B.data_ptr() + 8)]), 1004) for name in ("qabs", "qrope", "pool", "clat", "partial")]
     refused(hip.launch_mla_attend_tree_paged, good, changes)
@@ -63,8 +63,13 @@ def test_verify_refusals():
     changes += [(dict([(name, 0)]), 1001) for name in ("n_seqs", "n_nodes", "max_nodes", "vocab")]
     changes += [(dict(max_nodes=1025), 1002), (dict(vocab=2 ** 21 + 1, target_stride=2 ** 22, draft_stride=2 ** 22), 1002),
                 (dict(target_stride=31), 1002), (dict(draft_stride=31), 1002), (dict(target_probs=B.data_ptr() + 2), 1004),
-                (dict(draft_probs=B.data_ptr() + 1, bf16=True), 1004)]
+                (dict(draft_probs=B.data_ptr() + 1, bf16=True), 1004), (dict(workspace=B.data_ptr() + 8), 1004)]
     refused(hip.launch_draft_verify, good, changes)
+    # where rows are shared among workgroups a call without room for their sums is refused
+    wide = dict(n_seqs=2, max_nodes=4, vocab=131072)
+    assert hip.draft_verify_workspace_bytes(**wide) > 0
+    refused(hip.launch_draft_verify, dict(good, target_stride=131072, draft_stride=131072, **wide), [(dict(workspace=None), 1001)])
+    assert hip.draft_verify_workspace_bytes(1, 4, 32) == hip.draft_verify_workspace_bytes(0, 4, 131072) == 0
 
 
 @pytest.mark.parametrize("call,width,stride", [(hip.launch_kv_commit_paged, "width", "layer_bytes"),

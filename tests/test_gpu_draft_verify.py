@@ -201,3 +201,78 @@ def test_replayed_from_a_graph_and_on_two_streams():
         graph.replay()
         torch.cuda.synchronize()
         cases[0].check(cases[0].results())
+
+
+WIDE = 98304 + 1029  # rows that many workgroups share in a call of few sequences; the last block is a part of one
+
+
+def test_wide_rows_take_a_workspace_in_calls_of_few_sequences():
+    assert hip.draft_verify_workspace_bytes(4, 5, WIDE) > 0
+
+
+@pytest.mark.parametrize("draft", [False, True])
+@pytest.mark.parametrize("bf16", [False, True])
+def test_wide_rows(draft, bf16):
+    Case(60, [3, 0, 4, 1, 2], WIDE, draft, bf16=bf16, pad=1, peaked=3.0).check()
+
+
+@pytest.mark.parametrize("draft", [False, True])
+def test_wide_rows_of_siblings(draft):
+    case = Case(61, [6] * 4, WIDE, draft, near=3.0)
+    case.parents = np.concatenate([[-1] + [0] * 5] * 4).astype(np.int32)
+    case.u[:] = np.float32(1 - 2.0 ** -24)
+    _, n_path, _ = case.check()
+    assert (n_path == 1).any()
+
+
+def test_wide_rows_with_nothing_left():
+    case = Case(62, [2] * 3, WIDE, True)
+    case.draft[:] = np.maximum(case.draft, case.target)
+    case.tokens[:] = 7
+    case.u[:] = np.float32(1 - 2.0 ** -24)
+    case.draft[:, 7] = 2 * case.target[:, 7]
+    case.check()
+    case.target[-2:] = 0
+    _, _, token = case.check()
+    assert (token >= 0).tolist() == [True, True, False]
+
+
+def test_wide_rows_replayed_from_a_graph_and_on_two_streams():
+    torch = torch_cuda()
+    cases = [Case(63 + i, [3] * 3, WIDE, i == 0) for i in range(2)]
+    for c in cases:
+        c.buffers()
+        c.launch()
+    torch.cuda.synchronize()
+    want = [c.results() for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(4):
+        for c, st in zip(cases, streams):
+            c.launch(st)
+    torch.cuda.synchronize()
+    for c, w in zip(cases, want):
+        assert all(np.array_equal(x, y) for x, y in zip(c.results()[:3], w[:3]))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cases[0].launch(torch.cuda.current_stream())
+    rng = np.random.default_rng(3)
+    for _ in range(3):
+        cases[0].u[:], cases[0].u_final[:] = rng.random(cases[0].n), rng.random(3)
+        cases[0].dev[5].copy_(dev(cases[0].u))
+        cases[0].dev[6].copy_(dev(cases[0].u_final))
+        graph.replay()
+        torch.cuda.synchronize()
+        cases[0].check(cases[0].results())
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_infinities_and_signalling_nans(bf16):
+    """Infinity counts as the largest number of 32 bits, every NaN as nothing, also where conversions would quieten it."""
+    case = Case(65, [2] * 8, 500, False, bf16=bf16)
+    rows = case.rows(case.target)
+    rng = np.random.default_rng(4)
+    odd = rng.random(rows.shape) < 0.2
+    bits = rows.view(np.uint32) if not bf16 else rows
+    bits[odd] = rng.choice([0x7F81, 0x7FFF, 0xFF81, 0xFFC0, 0x7F80, 0xFF80, 0x8000], int(odd.sum())).astype(bits.dtype) << (0 if bf16 else 16)
+    case.rows = lambda x: rows if x is not None else None
+    case.check()
