@@ -88,7 +88,7 @@ def tree_attention(qabs, qrope, pool, tables, ctx, cu, masks, page, scale):
     token's row is never used.
 
     The bounds. A product of a bf16 and a code is exact in f32 (8 + 4 bits); a dot of `width` of them in f32, in any order, is off by at
-    most width half steps of the sum of magnitudes, the two scalings by three more: d = (width + 3) 2^-24 max_t sum |q k| scale. A weight is then
+    most width half steps of the sum of magnitudes, the two scalings by three more: d = (width + 3) 2^-24 max_t sum |q k| |scale|. A weight is then
     off by d relative, by 8 steps of its exponential and exponent's argument (|x| < 2^7 in powers of two: 2^-17 relative), and by half a bf16 step where
     it meets the values; sums of n weights by n half steps. Against mass = sum_t w_t |L_t|:
     |clat error| <= 2^-8 |clat| + (2^-8 + 2 (d + 2^-16 + n 2^-24)) mass;   |lse error| <= d + 2^-16 + n 2^-24 + 2^-22 |lse|."""
@@ -117,7 +117,7 @@ def tree_attention(qabs, qrope, pool, tables, ctx, cu, masks, page, scale):
                 total = e.sum(1, keepdims=True)
                 out[node] = e @ rows[at, :kvl] / total
                 lse[node] = (top + np.log(total))[:, 0]
-                d = (width + 3) * F32 * scale * (np.abs(q[node]) @ np.abs(rows[at]).T).max(1) + 2.0 ** -16 + len(at) * F32
+                d = (width + 3) * F32 * abs(scale) * (np.abs(q[node]) @ np.abs(rows[at]).T).max(1) + 2.0 ** -16 + len(at) * F32
                 far[node] = BF16 * np.abs(out[node]) + (BF16 + 2 * d[:, None]) * (e @ np.abs(rows[at, :kvl]) / total)
                 lse_far[node] = d + 2.0 ** -22 * np.abs(lse[node])
     return out, lse, far, lse_far

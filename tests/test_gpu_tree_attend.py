@@ -218,3 +218,41 @@ def test_pool_past_four_gigabytes():
     case.launch()
     got = case.results()
     assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("seqs,span,H", [(100, 900, 24), (150, 700, 40), (300, 640, 16)])
+def test_more_sequences_than_lanes_cut_among_workgroups(seqs, span, H):
+    """Ragged batches whose blocks of rows are cut: fewer blocks than workgroups and more, sequences without nodes or rows among them."""
+    rng = np.random.default_rng(seqs)
+    ctx = rng.integers(0, span, seqs) * (rng.random(seqs) < 0.8)
+    nodes = rng.integers(0, 5, seqs)
+    ctx[0], nodes[-1], nodes[0] = span, 4, 1
+    case = Case(seqs, [int(x) for x in ctx], [int(x) for x in nodes], H, masks="tree" if seqs % 100 else "chain")
+    assert hip.mla_attend_tree_paged_scratch_floats(seqs, H, case.n, case.max_nodes, span) > 0
+    case.check()
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.0, -0.07, 3.0])
+def test_softmax_scales(scale):
+    """Nothing, less than nothing and a lot: even weights, the smallest score first, one row's."""
+    case = Case(50, [300, 70], [5, 3], 20)
+    case.scale = scale
+    case.check()
+
+
+def test_scores_that_go_up_and_down():
+    """Rows' scales that swing by 2^12 from page to page, larger ones later: references are replaced again and again, in some rows only."""
+    case = Case(51, [1500, 640], [6, 2], 24, q_scale=1.0)
+    scales = case.pool[:, 64 * 576:].view(np.float32)
+    for s in range(2):
+        for b, page in enumerate(case.tables[s]):
+            scales[page] *= np.float32((1.0 if b % 3 else 2.0 ** -12) * (1.0 + b))
+    case.qabs[::2] ^= 0x8000                             # every other node's scores have the other sign
+    case.check()
+
+
+def test_cached_rows_without_a_scale_are_left_out():
+    case = Case(52, [260], [4], 16)
+    for t, bad in ((0, 0.0), (1, -1.0), (63, np.nan), (64, -0.0), (130, -np.inf), (259, 0.0), (261, 0.0)):
+        case.pool[case.tables[0][t // 64]][64 * 576:].view(np.float32)[t % 64] = bad
+    case.check()

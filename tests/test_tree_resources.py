@@ -49,7 +49,10 @@ def test_work_in_front_of_a_restore_is_found():
 
 def test_scratch_covers_every_record_and_no_more_than_two_a_workgroup():
     record = 64 * (512 + 2)
-    assert hip.mla_attend_tree_paged_scratch_floats(1, 16, 4, 4, 200) == 0            # whole blocks
+    # whole blocks: two tiles, and enough blocks of a few
+    assert hip.mla_attend_tree_paged_scratch_floats(1, 16, 4, 4, 124) == hip.mla_attend_tree_paged_scratch_floats(32, 16, 128, 4, 508) == 0
+    assert hip.mla_attend_tree_paged_scratch_floats(1, 16, 4, 4, 125) == 3 * 2 * record        # one block of three tiles, a workgroup each
+    assert hip.mla_attend_tree_paged_scratch_floats(65535, 128, 2 ** 23, 128, 2 ** 31 - 8193) == 0  # too many to count in 32 bits: whole
     assert hip.mla_attend_tree_paged_scratch_floats(32, 64, 256, 8, 32768) == 256 * 2 * record
     small = hip.mla_attend_tree_paged_scratch_floats(1, 16, 4, 4, 2000)
     assert 0 < small < 256 * 2 * record and small % (2 * record) == 0
