@@ -19,6 +19,9 @@
 // sum, and so lse, is of the unrounded ones.
 // One wave a SIMD issues an instruction in four cycles at best, so what counts beside the matrix instructions is how many others there are and
 // what waits: fragments are asked for steps ahead of their use, control flow and a run's address are scalar, rare work sits behind flags.
+// Measured: 32 sequences of 32 768 tokens, 8 nodes of 64 heads 1 100 us, 1.06 PFLOP/s; 131 072 tokens, 64 nodes of 128 heads 2 110 us, 1.11 PFLOP/s, where
+// a large bf16 product reaches 1.36 (and these instructions alone, every load and all of the softmax taken out, 1.5: the clock follows the power). Short calls are bound by
+// what a block costs to begin with and end (kTreeBeginTiles): 4 nodes of 16 heads over 200 tokens 14 us, 11 of them here.
 #pragma once
 
 namespace rk {
@@ -709,7 +712,8 @@ __global__ __launch_bounds__(kTreeThreads, 1) void mla_attend_tree_kernel(const 
 
 // Blocks that several work items had: their records, in order, under the largest reference. A workgroup's column of the launch has a block,
 // or, where there are more blocks than work items (BY_ITEM), the block inside of which its work item begins, the first one of that
-// block. Bound by memory's round trips where there are few: records go eight at a time, every load of a batch in front of the first use.
+// block. Bound by memory's round trips where there are few: records go eight at a time, every load of a batch in front of the first use. 39 blocks of some 8 records
+// 12 us, 3.2 TB/s; in an eighth of the workgroups with four pieces a thread, rows stored whole, 16.
 template <bool BY_ITEM>
 __global__ __launch_bounds__(256) void mla_attend_tree_merge_kernel(const TreeArgs a) {
     TreeWalk walk(a);

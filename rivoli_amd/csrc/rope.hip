@@ -13,7 +13,8 @@ namespace rk {
 // (f_j / factor) or by parts: pairs that turn often within the original context keep f_j, pairs that turn
 // hardly ever have f_j / factor, a ramp over the pairs between (the published NTK-by-parts rule).
 // An angle is taken in turns and in 64 bits: at position 10^6 the product's 24 bits would leave 0.06 of a radian.
-// Its whole turns go before it is rounded, so that sine and cosine are f32 functions of |x| <= 1.
+// Its whole turns go before it is rounded, so that sine and cosine are f32 functions of |x| <= 1. 163 840 positions of 32 pairs, 42 MB, 10.8 us
+// (6.1 at a fill's rate): vector instructions, 64-bit ones and the sine's and cosine's.
 struct RopeTableArgs {
     float* table;
     int first, n, pairs;
@@ -48,8 +49,8 @@ __global__ __launch_bounds__(256) void rope_table_kernel(const RopeTableArgs a) 
 // ---- the rows ---------------------------------------------------------------------------------------------
 // (x, y) -> (x c - y s, x s + y c) for the pairs of a head's rd values: neighbours, or half of them apart. Memory
 // bound: every value is read and written once, a token's table row serves all of its heads. A thread has one
-// piece of up to kHeads heads: 16 bytes of neighbouring pairs, or the 16 bytes of either half that belong together, so
-// that rows may be rotated in place.
+// piece of up to kRopeHeads heads: 16 bytes of neighbouring pairs, or the 16 bytes of either half that belong together, so
+// that rows may be rotated in place. 8 192 tokens of 128 heads, the last 64 of 192 values, 53 us: 270 MB at a large copy's rate.
 struct RopeArgs {
     const void* x;
     void* out;
