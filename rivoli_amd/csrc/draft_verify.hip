@@ -236,7 +236,7 @@ __device__ __forceinline__ int drawn(const R& row, int blocks, const double* sum
     run = __shfl(run, holder, kWave), some = __shfl(some, holder, kWave);
     int block = holder * each;
     for (; block < some; ++block) {
-        if (run + sums[block] > goal) break;
+        if (sums[block] > 0.0 && run + sums[block] > goal) break;
         run += sums[block];
     }
     // and in it: the first past the goal, or the last with anything in it where the sums' roundings leave none

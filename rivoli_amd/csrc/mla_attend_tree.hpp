@@ -702,8 +702,9 @@ __global__ __launch_bounds__(kTreeThreads, 1) void mla_attend_tree_kernel(const 
         const int lo = all ? 0 : max((int)(u - b.first_tile), 0), hi = all ? (int)b.tiles : min((int)b.tiles, (int)(end - b.first_tile));
         float* const rec = a.partial + (size_t)(2 * item + (lo == 0 ? 1 : 0)) * kTreeRecordFloats;
         if (hi > lo) tree_part<RUNS>(a, sh, b.s, b.seq, b.rb, b.rb == (int)b.blocks - 1, lo, hi, lo == 0 && hi == (int)b.tiles, rec, number);
-        u = all ? end : b.first_tile + b.tiles;
-        if (u >= end) return;
+        const unsigned next = all ? end : b.first_tile + b.tiles;
+        if (next >= end || next <= u) return;  // (the second: prefix sums that are none, whose units pass 32 bits)
+        u = next;
         TreeWalk walk(a);  // (looked up again: what it has would keep registers through the tiles)
         walk.begin = begin;
         if (!walk.block(false, u, b)) return;
