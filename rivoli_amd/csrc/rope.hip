@@ -12,16 +12,17 @@ namespace rk {
 // Pair j turns by p * f_j at position p, f_j = base^(-2j / rd), stretched for a longer context either as a whole
 // (f_j / factor) or by parts: pairs that turn often within the original context keep f_j, pairs that turn
 // hardly ever have f_j / factor, a ramp over the pairs between (the published NTK-by-parts rule).
-// An angle is taken in turns and in 64 bits: at position 10^6 the product's 24 bits would leave 0.06 of a radian.
-// Its whole turns go before it is rounded, so that sine and cosine are f32 functions of |x| <= 1. 163 840 positions of 32 pairs, 42 MB, 10.8 us
-// (6.1 at a fill's rate): vector instructions, 64-bit ones and the sine's and cosine's.
+// Angles are taken in turns and in 64 bits: at position 10^6 a product's 24 bits would leave 0.06 of a radian. A thread has a pair at
+// kTableRun positions at even distances and takes two sines and cosines, of the first angle and of the distance; the others come by
+// turning, (c + is)(dc + ids), four 64-bit operations a step whose error, some 10^-16 a step, is nothing to f32.
+// 163 840 positions of 32 pairs, 42 MB, 8.7 us (6.1 at a fill's rate; 9.2 by 32 positions a thread; 10.8 with a 32-bit sine and cosine of every reduced angle).
 struct RopeTableArgs {
     float* table;
     int first, n, pairs;
     double log2_base, factor, low, high;  // ramp over pairs low .. high; high < 0: every pair is stretched
     float mscale;
 };
-constexpr int kTableRun = 16;  // positions a thread: its frequency (a 64-bit power) once
+constexpr int kTableRun = 16;
 
 __global__ __launch_bounds__(256) void rope_table_kernel(const RopeTableArgs a) {
     const unsigned at = blockIdx.x * 256u + threadIdx.x;
@@ -34,15 +35,21 @@ __global__ __launch_bounds__(256) void rope_table_kernel(const RopeTableArgs a) 
     if (a.high >= 0.0) stretched = fmin(1.0, fmax(0.0, ((double)j - a.low) / (a.high - a.low)));
     f = f / a.factor * stretched + f * (1.0 - stretched);
     const double turns = f * 0.15915494309189533577;  // 1 / (2 pi)
+    const auto angle = [&](double p, double& s, double& c) {
+        double t = p * turns;
+        t -= rint(t);  // its whole turns
+        sincospi(2.0 * t, &s, &c);
+    };
+    double s, c, ds, dc;
+    angle((double)a.first + (double)run, s, c);
+    angle((double)runs, ds, dc);
 #pragma unroll 4
     for (int i = 0; i < kTableRun; ++i) {
         const unsigned p = run + (unsigned)i * runs;
         if (p >= (unsigned)a.n) return;
-        double t = ((double)a.first + (double)p) * turns;
-        t -= rint(t);
-        float s, c;
-        sincospif((float)(2.0 * t), &s, &c);
-        reinterpret_cast<f32x2*>(a.table)[(size_t)p * a.pairs + j] = f32x2{c * a.mscale, s * a.mscale};
+        reinterpret_cast<f32x2*>(a.table)[(size_t)p * a.pairs + j] = f32x2{(float)c * a.mscale, (float)s * a.mscale};
+        const double was = c;
+        c = c * dc - s * ds, s = was * ds + s * dc;
     }
 }
 
