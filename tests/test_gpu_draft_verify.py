@@ -276,3 +276,20 @@ def test_infinities_and_signalling_nans(bf16):
     bits[odd] = rng.choice([0x7F81, 0x7FFF, 0xFF81, 0xFFC0, 0x7F80, 0xFF80, 0x8000], int(odd.sum())).astype(bits.dtype) << (0 if bf16 else 16)
     case.rows = lambda x: rows if x is not None else None
     case.check()
+
+
+@pytest.mark.parametrize("draft", [False, True])
+def test_the_most_nodes(draft):
+    """1024 nodes, the root's children all but one of them and all rejected: as many rejections as there can be."""
+    case = Case(66, [1024, 5], 300, draft)
+    case.parents[:1024] = [-1] + [0] * 1023
+    case.u[:1024] = np.float32(1 - 2.0 ** -24)
+    if not draft:                                        # the likeliest token is nobody's
+        case.tokens[:1024] = np.where(case.tokens[:1024] == case.target[0, :300].argmax(), 0, case.tokens[:1024])
+    _, n_path, _ = case.check()
+    assert draft or n_path[0] == 1
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_the_longest_rows(bf16):
+    Case(67, [2], 2 ** 21, False, bf16=bf16, peaked=2.0).check()

@@ -256,3 +256,15 @@ def test_cached_rows_without_a_scale_are_left_out():
     for t, bad in ((0, 0.0), (1, -1.0), (63, np.nan), (64, -0.0), (130, -np.inf), (259, 0.0), (261, 0.0)):
         case.pool[case.tables[0][t // 64]][64 * 576:].view(np.float32)[t % 64] = bad
     case.check()
+
+
+@pytest.mark.parametrize("masks", ["chain", "tree"])
+def test_many_nodes(masks):
+    """A prompt's worth of nodes behind a prefix that ends inside a page: many words of masks, many blocks of rows."""
+    Case(53, [70, 0, 9], [700, 1, 333], 2, masks=masks).check()
+
+
+def test_a_batch_of_nothing_but_prefixes_and_of_single_tokens():
+    case = Case(54, [5000, 0, 1], [0, 0, 1], 16)         # one node in all
+    case.check()
+    Case(55, [0] * 200, [1] * 200, 128, masks="chain").check()
