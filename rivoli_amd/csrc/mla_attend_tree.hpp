@@ -14,13 +14,16 @@
 // An iteration has two halves, a barrier behind each: the scores of tile i + 1, with tile i's softmax and the transfers of tile i + 2
 // between their matrix instructions; then the values of tile i, with the partial scores of i + 1 meeting. The softmax's
 // reference is that of the rows' first tile: weights are bf16 and sums f32, whose exponents reach 2^127, so a row is rescaled only when
-// a score grows by 2^kTreeGrow past its reference, which every wave learns from a flag behind the first barrier (regrow). Weights are
+// a lane's weights of a tile come to more than kTreeGrow, which every wave learns from a flag behind the first barrier (regrow). Weights are
 // rounded to bf16 once where they meet the values (2^-8 of a weight, at random, against the 2^-8 of the rounded result); their
 // sum, and so lse, is of the unrounded ones.
-// One wave a SIMD issues an instruction in four cycles at best, so what counts beside the matrix instructions is how many others there are and
-// what waits: fragments are asked for steps ahead of their use, control flow and a run's address are scalar, rare work sits behind flags.
-// Measured: 32 sequences of 32 768 tokens, 8 nodes of 64 heads 1 100 us, 1.06 PFLOP/s; 131 072 tokens, 64 nodes of 128 heads 2 110 us, 1.11 PFLOP/s, where
-// a large bf16 product reaches 1.36 (and these instructions alone, every load and all of the softmax taken out, 1.5: the clock follows the power). Short calls are bound by
+// One wave a SIMD issues an instruction in four cycles at best and a matrix instruction of 32 cycles in sixteen, which leaves room for four
+// others under each. So what counts beside the matrix instructions is how many others there are and what waits: fragments are asked for steps
+// ahead of their use, control flow and a run's address are scalar, rare work sits behind flags. An iteration is 68 matrix instructions and some 430 others a
+// wave, 4 100 cycles (2 176 of matrix instructions; 70 more others took 4 680).
+// Measured: 32 sequences of 32 768 tokens, 8 nodes of 64 heads 1 057 us, 1.11 PFLOP/s; 131 072 tokens, 64 nodes of 128 heads 2 040 us, 1.15 PFLOP/s, where
+// a large bf16 product reaches 1.36. The clock follows the power: 2.33 GHz at 4 680 cycles a tile, 2.08 at 4 100, 1.8 in a loop of nothing but these
+// matrix instructions (1.86 PFLOP/s), so that an instruction saved gives about a quarter of its cycles. Short calls are bound by
 // what a block costs to begin with and end (kTreeBeginTiles): 4 nodes of 16 heads over 200 tokens 14 us, 11 of them here.
 #pragma once
 
@@ -38,7 +41,7 @@ constexpr int kTreeBuffers = 3;
 constexpr int kTreeRopeAt = 8 * 4096;
 constexpr int kTreeTileBytes = kTreeRopeAt + 4 * 1024;
 constexpr int kTreeSteps = 18;            // of 16 dims a wave: 16 of its 256 latent dims, two of its 32 roped ones
-constexpr float kTreeGrow = 24.0f;
+constexpr float kTreeGrow = 16777216.0f;  // 2^24: of sixteen weights
 constexpr uint32_t kTreeHole = 0x80000000u;  // the scale of a token that is not there: -0
 
 // A call's blocks of rows are numbered by sequence, and so are its work units: block after block what a block costs to begin with, counted in tiles,
@@ -136,36 +139,22 @@ struct TreeShared {
     // numbers of the latest tile of which some row outgrew its reference, some score is no number, some token is not there
     int grown, dirty, holed[2];          // (the last by the tile's parity)
 };
+struct TreeFlags {
+    int grown, dirty, holed;
+};
 static_assert(sizeof(TreeShared) <= 160 * 1024, "one workgroup per compute unit");
 
-// A lane's piece of a row's codes on its way to LDS, one of five, so that transfers go between matrix instructions one at a time: of the latent
-// groups 0 .. 3, 128 bytes apart in memory and 1024 in LDS, or (4) the roped codes, for the lanes of `roped`. `to` is the row's place
-// in the tile's latent codes, `to_rope` in its roped ones. The instruction's offset counts in memory and in LDS. As dma16_from: from a scalar
-// address and a lane's 32 bits, or (base null) a lane's 64.
+// A lane's sixteen bytes on their way to LDS, at `to` for the wave's first lane: from a scalar address and a lane's 32 bits, or (RUNS false) a lane's 64.
+// PIECE: 128 bytes further in memory a piece (the instruction's offset, which counts in LDS as well) and 1024 in LDS. m0, the
+// instruction's LDS base, is nobody else's here.
 template <int PIECE, bool RUNS>
-__device__ __forceinline__ void tree_dma(unsigned long long base, uint32_t off, const uint8_t* src, lds_ptr<uint8_t> to, lds_ptr<uint8_t> to_rope,
-                                         unsigned long long roped) {
-    uint32_t keep;
-    if constexpr (PIECE < 4) {
-        const uint32_t at = (uint32_t)(uintptr_t)to + (1024 - 128) * PIECE;
-        if constexpr (RUNS)
-            asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:%4\n\ts_mov_b32 m0, %0"
-                         : "=&s"(keep) : "v"(off), "s"(base), "s"(at), "n"(128 * PIECE) : "memory");
-        else
-            asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off offset:%3\n\ts_mov_b32 m0, %0"
-                         : "=&s"(keep) : "v"(src), "s"(at), "n"(128 * PIECE) : "memory");
-    } else {
-        const uint32_t at = (uint32_t)(uintptr_t)to_rope - 512u;
-        unsigned long long all;
-        if constexpr (RUNS)
-            asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %4\n\ts_and_saveexec_b64 %1, %5\n\ts_nop 0\n\t"
-                         "global_load_lds_dwordx4 %2, %3 offset:512\n\ts_mov_b64 exec, %1\n\ts_mov_b32 m0, %0"
-                         : "=&s"(keep), "=&s"(all) : "v"(off), "s"(base), "s"(at), "s"(roped) : "memory", "scc");
-        else
-            asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_and_saveexec_b64 %1, %4\n\ts_nop 0\n\t"
-                         "global_load_lds_dwordx4 %2, off offset:512\n\ts_mov_b64 exec, %1\n\ts_mov_b32 m0, %0"
-                         : "=&s"(keep), "=&s"(all) : "v"(src), "s"(at), "s"(roped) : "memory", "scc");
-    }
+__device__ __forceinline__ void tree_dma(unsigned long long base, uint32_t off, const uint8_t* src, uint32_t to) {
+    if constexpr (RUNS)
+        asm volatile("s_add_i32 m0, %2, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 offset:%4"
+                     :: "v"(off), "s"(base), "s"(to), "n"((1024 - 128) * PIECE), "n"(128 * PIECE) : "memory", "m0", "scc");
+    else
+        asm volatile("s_add_i32 m0, %1, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off offset:%3"
+                     :: "v"(src), "s"(to), "n"((1024 - 128) * PIECE), "n"(128 * PIECE) : "memory", "m0", "scc");
 }
 
 // Codes that are no number as zeros.
@@ -213,11 +202,13 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
     bool there[2];
     float raw_scale[2];
     auto swap_of = [&](int o) -> int { return (4 * o + (r8 >> 1)) & 7; };
-    const unsigned long long roped[2] = {__builtin_amdgcn_ballot_w64((l8 ^ swap_of(0)) < 4), __builtin_amdgcn_ballot_w64((l8 ^ swap_of(1)) < 4)};
+    // of the roped codes a lane has the piece that its place asks for, of the first or the second eight rows
+    const bool roped_second = (l8 ^ swap_of(0)) >= 4;
     const uint32_t page_bytes = (uint32_t)a.page_bytes, codes_bytes = page_tokens * 576u;
     const uint8_t* src[2] = {nullptr, nullptr};
     unsigned long long base = 0;              // RUNS: of the wave's rows
     const uint32_t lane_off[2] = {576u * (uint32_t)r8 + 16u * (uint32_t)(l8 ^ swap_of(0)), 576u * (uint32_t)(8 + r8) + 16u * (uint32_t)(l8 ^ swap_of(1))};
+    const uint32_t roped_off = (roped_second ? lane_off[1] : lane_off[0]) + 512u;
     auto find = [&](int o) {  // the lane's row of a tile looked up: its address, and its scale asked for
         if constexpr (RUNS) {
             const unsigned at = (unsigned)__builtin_amdgcn_readfirstlane(page[0]);
@@ -238,11 +229,12 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
             src[o] = from + (off * 576u + 16u * (unsigned)(l8 ^ swap_of(o)));
         }
     };
-    // Of the tile found: piece k of ten, five an octet.
+    // Of the tile found: piece k of nine, four of either octet's latent codes and the roped ones.
     auto bring = [&](auto number_of, int buf) {
-        constexpr int k = decltype(number_of)::value, o = k / 5;
-        const lds_ptr<uint8_t> tile = tiles + buf * kTreeTileBytes;
-        tree_dma<k % 5, RUNS>(base, lane_off[o], src[o], tile + (2 * wave + o) * 4096, tile + kTreeRopeAt + wave * 1024, roped[o]);
+        constexpr int k = decltype(number_of)::value, o = k / 4;
+        const uint32_t tile = (uint32_t)(uintptr_t)(tiles + buf * kTreeTileBytes);
+        if constexpr (k < 8) tree_dma<k % 4, RUNS>(base, lane_off[o], src[o], tile + (2 * wave + o) * 4096);
+        else tree_dma<0, RUNS>(base, roped_off, (roped_second ? src[1] : src[0]) + 512, tile + kTreeRopeAt + wave * 1024);
     };
     auto go_on = [&](int o) {
         if (o >= kRuns) return;
@@ -255,7 +247,7 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
     };
     auto ask = [&](int buf) {
         find(0), find(1);
-        each<10>([&](auto k) { bring(k, buf); });
+        each<9>([&](auto k) { bring(k, buf); });
         go_on(0), go_on(1);
     };
     // The transfers asked for have landed: scales, and (holes) zeros for rows that are not there: codes must be finite, they meet a zero
@@ -287,7 +279,7 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
     };
 
     f32x16 o[4][2];  // O^T: column tile c of 32, row block b: sixteen columns a lane, of row 32 b + n32
-    float m_ref = -INFINITY, limit = -INFINITY, l_sum = 0.0f, l_before = 0.0f;  // of row 32 kh + n32: the lane's share of the sum
+    float m_ref = -INFINITY, limit = -1.0f, l_sum = 0.0f, l_before = 0.0f;  // of row 32 kh + n32: the lane's share of the sum
     const int own = 32 * kh + n32;
     const int own_row = kTreeRows * rb + own;
     const bool live = own_row < rows;
@@ -375,23 +367,23 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
         auto bit_of = [&](int r) -> bool { return (int)(seen_half << (31 - 8 * (r >> 2) - (r & 3))) < 0; };
         const lds_ptr<uint8_t> w_row = weights + own * (2 * kTreeTokens) + 8 * half;
         const int w_swap = (own >> 1) & 7;
-        auto scales_of = [&](int buf, int i) -> f32x4 { return *(lds_ptr<f32x4>)&sh->scale[buf][32 * th + 8 * i + 4 * half]; };
+        lds_ptr<float> scale_row = (lds_ptr<float>)&sh->scale[0][32 * th + 4 * half];
+        asm volatile("" : "+v"(scale_row));  // (one address: its part of the layout is past an instruction's offset)
+        auto scales_of = [&](int buf, int i) -> f32x4 { return *(lds_ptr<f32x4>)(scale_row + buf * kTreeTokens + 8 * i); };
         auto put_weights = [&](int i, const float (&p)[4]) {
             *(lds_ptr<u32x2>)(w_row + 16 * ((4 * th + i) ^ w_swap)) = u32x2{pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3])};
         };
         // A tile's weights out of its scores, a token at a time; l_sum and the largest exponent go along. As if every row saw every token.
         f32x4 by;
-        float mu = 0.0f, most = -INFINITY, y = 0.0f, p[4];
+        float mu = 0.0f, p[4];
         auto weigh_begin = [&](int buf) {
-            mu = m_ref == -INFINITY ? 0.0f : m_ref, most = -INFINITY, l_before = l_sum;
+            mu = m_ref == -INFINITY ? 0.0f : m_ref, l_before = l_sum;
             by = scales_of(buf, 0);
         };
         auto weigh = [&](int buf, int r) {
-            const float before = y;
-            y = __builtin_fmaf(sc[r], by[r & 3], -mu);
-            if (r & 1) most = fmaxf(most, fmaxf(before, y));
-            const float e = __builtin_amdgcn_exp2f(y);
+            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], by[r & 3], -mu));
             l_sum += e;
+            asm volatile("" : "+v"(l_sum));  // (here, under the matrix instructions, though weigh_seen() may replace it)
             p[r & 3] = e * by[r & 3];
             if ((r & 3) == 3) {
                 put_weights(r >> 2, p);
@@ -401,7 +393,7 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
         // The same of a tile with tokens that some row does not see, in place of what weigh() made of it. Whether a score is no number: then some code of
         // the tile may be none, and its product with a weight of zero would be none either (clean).
         auto weigh_seen = [&](int buf) -> bool {
-            most = -INFINITY, l_sum = l_before;
+            l_sum = l_before;
             bool nan = false;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -410,7 +402,6 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
                 for (int k = 0; k < 4; ++k) {
                     nan |= sc[4 * i + k] != sc[4 * i + k];
                     const float x = bit_of(4 * i + k) ? __builtin_fmaf(sc[4 * i + k], s4[k], -mu) : -INFINITY;
-                    most = fmaxf(most, x);
                     const float e = __builtin_amdgcn_exp2f(x);
                     l_sum += e;
                     p[k] = bit_of(4 * i + k) ? e * s4[k] : 0.0f;
@@ -436,7 +427,7 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
             const bool grow = top > m_ref;
             const float corr = grow ? __builtin_amdgcn_exp2f(m_ref - top) : 1.0f;  // 2^-inf = 0 at first
             if (grow) m_ref = top;
-            limit = m_ref == -INFINITY ? -INFINITY : kTreeGrow;
+            limit = m_ref == -INFINITY ? -1.0f : kTreeGrow;
             mu = m_ref == -INFINITY ? 0.0f : m_ref;
             return corr;
         };
@@ -473,7 +464,7 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
             }
             x[0] = f32x16{}, x[1] = f32x16{};
             bf16x8 lo = as_bf16(k[0].x, k[0].y), hi = as_bf16(k[0].z, k[0].w);
-            each<9>([&](auto step) {
+            each<8>([&](auto step) {
                 constexpr int i = decltype(step)::value;
                 __builtin_amdgcn_sched_barrier(0);
                 if (i + 2 < 9) load(i + 2);
@@ -482,19 +473,26 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
                 if (MORE && i < 7) weigh(before, 2 + 2 * i);
                 __builtin_amdgcn_sched_barrier(0);
                 x[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lo, __builtin_bit_cast(bf16x8, q[2 * i][1]), x[1], 0, 0, 0);
-                if (i < 8) lo = as_bf16(then.x, then.y);
+                lo = as_bf16(then.x, then.y);
                 if constexpr (MORE) bring(std::integral_constant<int, i>{}, third);
                 __builtin_amdgcn_sched_barrier(0);
                 x[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(hi, __builtin_bit_cast(bf16x8, q[2 * i + 1][0]), x[0], 0, 0, 0);
                 if (MORE && i < 7) weigh(before, 3 + 2 * i);
                 __builtin_amdgcn_sched_barrier(0);
                 x[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(hi, __builtin_bit_cast(bf16x8, q[2 * i + 1][1]), x[1], 0, 0, 0);
-                if (i < 8) hi = as_bf16(then.z, then.w);
-                if constexpr (MORE) {
-                    if (i == 7) bring(std::integral_constant<int, 9>{}, third);
-                    if (i == 8) go_on(0), go_on(1);
-                }
+                hi = as_bf16(then.z, then.w);
             });
+            // (the last step: the rows that are sent first, so that they go out while the others are made)
+            __builtin_amdgcn_sched_barrier(0);
+            x[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lo, __builtin_bit_cast(bf16x8, q[16][1]), x[1], 0, 0, 0);
+            if constexpr (MORE) bring(std::integral_constant<int, 8>{}, third);
+            __builtin_amdgcn_sched_barrier(0);
+            x[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(hi, __builtin_bit_cast(bf16x8, q[17][1]), x[1], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            x[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lo, __builtin_bit_cast(bf16x8, q[16][0]), x[0], 0, 0, 0);
+            if constexpr (MORE) go_on(0), go_on(1);
+            __builtin_amdgcn_sched_barrier(0);
+            x[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(hi, __builtin_bit_cast(bf16x8, q[17][0]), x[0], 0, 0, 0);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int i = 0; i < 4; ++i) sh->part[2 * th + 1 - kh][i][lane] = f32x4{x[1][4 * i], x[1][4 * i + 1], x[1][4 * i + 2], x[1][4 * i + 3]};
@@ -503,7 +501,7 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
         // partial scores of the next tile meet and the transfers asked for arrive in between. A unit's codes are out of LDS three units and
         // converted one unit before its matrix instructions. `check` comes once every weight is there, and says whether it changed the
         // tile's codes.
-        auto values = [&](auto more, int buf, int third, auto check) {
+        auto values = [&](auto more, int buf, int third, int number_of, auto check) {
             constexpr bool NEXT = decltype(more)::value;
             const lds_ptr<uint8_t> codes = tiles + buf * kTreeTileBytes + v_row;
             const lds_ptr<uint8_t> w_from = weights + n32 * (2 * kTreeTokens);
@@ -518,27 +516,37 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
             };
             load(0), load(1), load(2);
             lds_barrier();  // partial scores and weights are there
-            if (__builtin_expect(check(), 0)) load(0), load(1), load(2);
+            const TreeFlags flags{sh->grown, sh->dirty, sh->holed[(number_of + 1) & 1]};
             load_w(0);
             f32x4 part[4];
             if (NEXT) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) part[i] = sh->part[2 * th + kh][i][lane];
             }
-            bf16x8 v = as_bf16((uint32_t)raw[0][0], (uint32_t)raw[0][1]);
+            if (__builtin_expect(check(flags), 0)) load(0), load(1), load(2), load_w(0);
+            u32x4 v[2];
+            auto convert = [&](int u, int side) {
+                uint32_t lo, hi;
+                e4m3x4_to_bf16((uint32_t)raw[u % 4][side], lo, hi);
+                v[u & 1][2 * side] = lo, v[u & 1][2 * side + 1] = hi;
+            };
+            convert(0, 0), convert(0, 1);
             each<16>([&](auto unit) {
                 constexpr int u = decltype(unit)::value, ks = u >> 2, c = u & 3;
                 __builtin_amdgcn_sched_barrier(0);
                 if (u + 3 < 16) load(u + 3);
                 if (c == 1 && ks < 3) load_w(ks + 1);
-                o[c][0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, w[ks & 1][0], o[c][0], 0, 0, 0);
+                o[c][0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v[u & 1]), w[ks & 1][0], o[c][0], 0, 0, 0);
+                if (u < 15) convert(u + 1, 0);
                 if (NEXT && u == 12) arrived(third);
                 __builtin_amdgcn_sched_barrier(0);
-                o[c][1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, w[ks & 1][1], o[c][1], 0, 0, 0);
-                if (u < 15) v = as_bf16((uint32_t)raw[(u + 1) % 4][0], (uint32_t)raw[(u + 1) % 4][1]);
+                o[c][1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v[u & 1]), w[ks & 1][1], o[c][1], 0, 0, 0);
+                if (u < 15) convert(u + 1, 1);
                 if (NEXT && u >= 2 && u < 10) {
                     constexpr int r = 2 * (u - 2) & 15;
-                    sc[r] = x[0][r] + part[r >> 2][r & 3], sc[r + 1] = x[0][r + 1] + part[r >> 2][(r & 3) + 1];
+                    float s0 = x[0][r] + part[r >> 2][r & 3], s1 = x[0][r + 1] + part[r >> 2][(r & 3) + 1];
+                    asm volatile("" : "+v"(s0), "+v"(s1));  // (here, under the matrix instructions, though a later tile's)
+                    sc[r] = s0, sc[r + 1] = s1;
                 }
             });
             __builtin_amdgcn_sched_barrier(0);
@@ -577,15 +585,14 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
             const int next = buf == 2 ? 0 : buf + 1, third = next == 2 ? 0 : next + 1;
             scores(next, std::true_type{}, buf, third);
             if (__builtin_expect(masked, 0) && weigh_seen(buf)) sh->dirty = number + i;
-            if (__builtin_amdgcn_ballot_w64(most > limit) != 0) sh->grown = number + i;
+            if (__builtin_amdgcn_ballot_w64(l_sum - l_before > limit) != 0) sh->grown = number + i;
             bool holed = false;
-            values(std::true_type{}, buf, third, [&] {
-                const int grown = sh->grown, hole = sh->holed[(number + i + 1) & 1];
-                const bool dirty = __builtin_amdgcn_readfirstlane(sh->dirty) == number + i;
+            values(std::true_type{}, buf, third, number + i, [&](const TreeFlags& f) {
+                const bool dirty = __builtin_amdgcn_readfirstlane(f.dirty) == number + i, grown = __builtin_amdgcn_readfirstlane(f.grown) == number + i;
+                holed = __builtin_amdgcn_readfirstlane(f.holed) == number + i + 1;
                 if (__builtin_expect(dirty, 0)) clean(buf);
-                if (__builtin_expect(__builtin_amdgcn_readfirstlane(grown) == number + i, 0)) regrow(buf);
-                holed = __builtin_amdgcn_readfirstlane(hole) == number + i + 1;
-                return dirty;
+                if (__builtin_expect(grown, 0)) regrow(buf);
+                return dirty || grown;
             });
             fill_holes(third, number + i + 2);
             masked = drafted(i + 1) || holed;
@@ -599,12 +606,12 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
         weigh_begin(buf);
         seen = seen_of(n_tiles - 1, buf), seen_half = seen >> 4 * half;
         if (weigh_seen(buf)) sh->dirty = number + n_tiles - 1;
-        if (__builtin_amdgcn_ballot_w64(most > limit) != 0) sh->grown = number + n_tiles - 1;
-        values(std::false_type{}, buf, 0, [&] {
-            const bool dirty = __builtin_amdgcn_readfirstlane(sh->dirty) == number + n_tiles - 1;
+        if (__builtin_amdgcn_ballot_w64(l_sum - l_before > limit) != 0) sh->grown = number + n_tiles - 1;
+        values(std::false_type{}, buf, 0, number + n_tiles - 1, [&](const TreeFlags& f) {
+            const bool dirty = __builtin_amdgcn_readfirstlane(f.dirty) == number + n_tiles - 1, grown = __builtin_amdgcn_readfirstlane(f.grown) == number + n_tiles - 1;
             if (dirty) clean(buf);
-            if (__builtin_amdgcn_readfirstlane(sh->grown) == number + n_tiles - 1) regrow(buf);
-            return dirty;
+            if (grown) regrow(buf);
+            return dirty || grown;
         });
         if (a.bad_rows && last_block && l8 == 0 && missing) atomicAdd(a.bad_rows, missing);
         number += n_tiles + 2;  // (two tiles past the end were asked for)
