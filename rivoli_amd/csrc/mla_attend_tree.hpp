@@ -12,16 +12,16 @@
 // Codes go from memory into LDS as they are, three tiles in rotation, and become bf16 (exact) when an operand is read, once for the
 // workgroup. 32 x 32 matrix tiles: a fragment serves two of them.
 // An iteration has two halves, a barrier behind each: the scores of tile i + 1, with tile i's softmax and the transfers of tile i + 2
-// between their matrix instructions; then the values of tile i, with the partial scores of i + 1 meeting. The softmax's
-// reference is that of the rows' first tile: weights are bf16 and sums f32, whose exponents reach 2^127, so a row is rescaled only when
-// a lane's weights of a tile come to more than kTreeGrow, which every wave learns from a flag behind the first barrier (regrow). Weights are
-// rounded to bf16 once where they meet the values (2^-8 of a weight, at random, against the 2^-8 of the rounded result); their
-// sum, and so lse, is of the unrounded ones.
+// between their matrix instructions; then the values of tile i, with the partial scores of i + 1 meeting.
+// A weight is its exponential times its token's scale, rounded once to f16, which codes are exact in as well. A row's reference makes the
+// largest of these products one in its first tile; the row is rescaled only when some weight has grown to kTreeGrown, which every wave learns from a flag behind
+// the first barrier (regrow). So a weight has 11 bits down to 2^-14 of that largest one and is off by 2^-25 of it at most below: against 64 bits results are
+// off by 1.6e-3 of the norm, all of it their own rounding to bf16 (by bf16 weights 2.4e-3). Their sum, and so lse, is of the unrounded ones, in f32.
 // One wave a SIMD issues an instruction in four cycles at best and a matrix instruction of 32 cycles in sixteen, which leaves room for four
 // others under each. So what counts beside the matrix instructions is how many others there are and what waits: fragments are asked for steps
 // ahead of their use, control flow and a run's address are scalar, rare work sits behind flags. An iteration is 68 matrix instructions and some 430 others a
 // wave, 4 100 cycles (2 176 of matrix instructions; 70 more others took 4 680).
-// Measured: 32 sequences of 32 768 tokens, 8 nodes of 64 heads 1 057 us, 1.11 PFLOP/s; 131 072 tokens, 64 nodes of 128 heads 2 040 us, 1.15 PFLOP/s, where
+// Measured: 32 sequences of 32 768 tokens, 8 nodes of 64 heads 1 024 us, 1.14 PFLOP/s; 131 072 tokens, 64 nodes of 128 heads 1 941 us, 1.20 PFLOP/s, where
 // a large bf16 product reaches 1.36. The clock follows the power: 2.33 GHz at 4 680 cycles a tile, 2.08 at 4 100, 1.8 in a loop of nothing but these
 // matrix instructions (1.86 PFLOP/s), so that an instruction saved gives about a quarter of its cycles. Short calls are bound by
 // what a block costs to begin with and end (kTreeBeginTiles): 4 nodes of 16 heads over 200 tokens 14 us, 11 of them here.
@@ -30,6 +30,7 @@
 namespace rk {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kTreeWaves = 4;
 constexpr int kTreeThreads = kTreeWaves * kWave;
@@ -41,7 +42,9 @@ constexpr int kTreeBuffers = 3;
 constexpr int kTreeRopeAt = 8 * 4096;
 constexpr int kTreeTileBytes = kTreeRopeAt + 4 * 1024;
 constexpr int kTreeSteps = 18;            // of 16 dims a wave: 16 of its 256 latent dims, two of its 32 roped ones
-constexpr float kTreeGrow = 16777216.0f;  // 2^24: of sixteen weights
+// A row's largest weight of its first tile is one, later ones may grow to 2^15 (65 504 is the largest of 16 bits, 2^-14 the least with all of its bits).
+constexpr uint16_t kTreeGrown = 0x7800;  // 2^15; a number with a sign bit counts as more (negative softmax scales)
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 constexpr uint32_t kTreeHole = 0x80000000u;  // the scale of a token that is not there: -0
 
 // A call's blocks of rows are numbered by sequence, and so are its work units: block after block what a block costs to begin with, counted in tiles,
@@ -155,6 +158,17 @@ __device__ __forceinline__ void tree_dma(unsigned long long base, uint32_t off, 
     else
         asm volatile("s_add_i32 m0, %1, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off offset:%3"
                      :: "v"(src), "s"(to), "n"((1024 - 128) * PIECE), "n"(128 * PIECE) : "memory", "m0", "scc");
+}
+
+// Four codes as f16, exact.
+__device__ __forceinline__ void e4m3x4_to_f16(uint32_t c, uint32_t& lo, uint32_t& hi) {
+    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c, 1.0f, false));
+    hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c, 1.0f, true));
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float x, float y) {
+    typedef float f32x2v __attribute__((ext_vector_type(2)));
+    typedef _Float16 f16x2v __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2v{x, y}), f16x2v));
 }
 
 // Codes that are no number as zeros.
@@ -279,7 +293,7 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
     };
 
     f32x16 o[4][2];  // O^T: column tile c of 32, row block b: sixteen columns a lane, of row 32 b + n32
-    float m_ref = -INFINITY, limit = -1.0f, l_sum = 0.0f, l_before = 0.0f;  // of row 32 kh + n32: the lane's share of the sum
+    float m_ref = -INFINITY, l_sum = 0.0f, l_before = 0.0f;  // of row 32 kh + n32: the lane's share of the sum
     const int own = 32 * kh + n32;
     const int own_row = kTreeRows * rb + own;
     const bool live = own_row < rows;
@@ -370,14 +384,17 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
         lds_ptr<float> scale_row = (lds_ptr<float>)&sh->scale[0][32 * th + 4 * half];
         asm volatile("" : "+v"(scale_row));  // (one address: its part of the layout is past an instruction's offset)
         auto scales_of = [&](int buf, int i) -> f32x4 { return *(lds_ptr<f32x4>)(scale_row + buf * kTreeTokens + 8 * i); };
+        u16x2 high = {0, 0};     // the largest of a tile's weights
         auto put_weights = [&](int i, const float (&p)[4]) {
-            *(lds_ptr<u32x2>)(w_row + 16 * ((4 * th + i) ^ w_swap)) = u32x2{pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3])};
+            const uint32_t lo = pack_f16x2(p[0], p[1]), hi = pack_f16x2(p[2], p[3]);
+            high = __builtin_elementwise_max(high, __builtin_elementwise_max(__builtin_bit_cast(u16x2, lo), __builtin_bit_cast(u16x2, hi)));
+            *(lds_ptr<u32x2>)(w_row + 16 * ((4 * th + i) ^ w_swap)) = u32x2{lo, hi};
         };
         // A tile's weights out of its scores, a token at a time; l_sum and the largest exponent go along. As if every row saw every token.
         f32x4 by;
         float mu = 0.0f, p[4];
         auto weigh_begin = [&](int buf) {
-            mu = m_ref == -INFINITY ? 0.0f : m_ref, l_before = l_sum;
+            mu = m_ref == -INFINITY ? 0.0f : m_ref, high.x = m_ref == -INFINITY ? kTreeGrown : (uint16_t)0, high.y = 0, l_before = l_sum;
             by = scales_of(buf, 0);
         };
         auto weigh = [&](int buf, int r) {
@@ -393,7 +410,7 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
         // The same of a tile with tokens that some row does not see, in place of what weigh() made of it. Whether a score is no number: then some code of
         // the tile may be none, and its product with a weight of zero would be none either (clean).
         auto weigh_seen = [&](int buf) -> bool {
-            l_sum = l_before;
+            l_sum = l_before, high.x = m_ref == -INFINITY ? kTreeGrown : (uint16_t)0, high.y = 0;
             bool nan = false;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -410,14 +427,16 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
             }
             return __builtin_amdgcn_ballot_w64(nan) != 0;
         };
-        // New references for the rows of a tile (the workgroup's decision), and a factor for what came before.
+        // New references for the rows of a tile (the workgroup's decision), and a factor for what came before. (The exponent of a scale is held to 2^-90, so
+        // that a sum of exponentials alone stays a number.)
         auto refer = [&](int buf) -> float {
             float top = -INFINITY;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const f32x4 s4 = scales_of(buf, i);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) top = fmaxf(top, bit_of(4 * i + k) ? sc[4 * i + k] * s4[k] : -INFINITY);
+                for (int k = 0; k < 4; ++k)
+                    top = fmaxf(top, bit_of(4 * i + k) ? __builtin_fmaf(sc[4 * i + k], s4[k], fmaxf(__builtin_amdgcn_logf(fabsf(s4[k])), -90.0f)) : -INFINITY);
             }
             const auto other = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
             top = fmaxf(__uint_as_float(other[0]), __uint_as_float(other[1]));
@@ -427,7 +446,6 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
             const bool grow = top > m_ref;
             const float corr = grow ? __builtin_amdgcn_exp2f(m_ref - top) : 1.0f;  // 2^-inf = 0 at first
             if (grow) m_ref = top;
-            limit = m_ref == -INFINITY ? -1.0f : kTreeGrow;
             mu = m_ref == -INFINITY ? 0.0f : m_ref;
             return corr;
         };
@@ -506,13 +524,13 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
             const lds_ptr<uint8_t> codes = tiles + buf * kTreeTileBytes + v_row;
             const lds_ptr<uint8_t> w_from = weights + n32 * (2 * kTreeTokens);
             i32x2 raw[4];
-            bf16x8 w[2][2];
+            f16x8 w[2][2];
             auto load = [&](int u) {
                 raw[u % 4] = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_ptr<i32x2>)(codes + 8192 * (u >> 2) + 16 * ((v_piece + (u & 3)) ^ v_swap)));
             };
             auto load_w = [&](int ks) {
 #pragma unroll
-                for (int b = 0; b < 2; ++b) w[ks & 1][b] = *(lds_ptr<bf16x8>)(w_from + 32 * b * (2 * kTreeTokens) + 16 * ((2 * ks + half) ^ k_swap));
+                for (int b = 0; b < 2; ++b) w[ks & 1][b] = *(lds_ptr<f16x8>)(w_from + 32 * b * (2 * kTreeTokens) + 16 * ((2 * ks + half) ^ k_swap));
             };
             load(0), load(1), load(2);
             lds_barrier();  // partial scores and weights are there
@@ -527,7 +545,7 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
             u32x4 v[2];
             auto convert = [&](int u, int side) {
                 uint32_t lo, hi;
-                e4m3x4_to_bf16((uint32_t)raw[u % 4][side], lo, hi);
+                e4m3x4_to_f16((uint32_t)raw[u % 4][side], lo, hi);
                 v[u & 1][2 * side] = lo, v[u & 1][2 * side + 1] = hi;
             };
             convert(0, 0), convert(0, 1);
@@ -536,11 +554,11 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
                 __builtin_amdgcn_sched_barrier(0);
                 if (u + 3 < 16) load(u + 3);
                 if (c == 1 && ks < 3) load_w(ks + 1);
-                o[c][0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v[u & 1]), w[ks & 1][0], o[c][0], 0, 0, 0);
+                o[c][0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, v[u & 1]), w[ks & 1][0], o[c][0], 0, 0, 0);
                 if (u < 15) convert(u + 1, 0);
                 if (NEXT && u == 12) arrived(third);
                 __builtin_amdgcn_sched_barrier(0);
-                o[c][1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v[u & 1]), w[ks & 1][1], o[c][1], 0, 0, 0);
+                o[c][1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, v[u & 1]), w[ks & 1][1], o[c][1], 0, 0, 0);
                 if (u < 15) convert(u + 1, 1);
                 if (NEXT && u >= 2 && u < 10) {
                     constexpr int r = 2 * (u - 2) & 15;
@@ -585,7 +603,7 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
             const int next = buf == 2 ? 0 : buf + 1, third = next == 2 ? 0 : next + 1;
             scores(next, std::true_type{}, buf, third);
             if (__builtin_expect(masked, 0) && weigh_seen(buf)) sh->dirty = number + i;
-            if (__builtin_amdgcn_ballot_w64(l_sum - l_before > limit) != 0) sh->grown = number + i;
+            if (__builtin_amdgcn_ballot_w64(max(high.x, high.y) >= kTreeGrown) != 0) sh->grown = number + i;
             bool holed = false;
             values(std::true_type{}, buf, third, number + i, [&](const TreeFlags& f) {
                 const bool dirty = __builtin_amdgcn_readfirstlane(f.dirty) == number + i, grown = __builtin_amdgcn_readfirstlane(f.grown) == number + i;
@@ -606,7 +624,7 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
         weigh_begin(buf);
         seen = seen_of(n_tiles - 1, buf), seen_half = seen >> 4 * half;
         if (weigh_seen(buf)) sh->dirty = number + n_tiles - 1;
-        if (__builtin_amdgcn_ballot_w64(l_sum - l_before > limit) != 0) sh->grown = number + n_tiles - 1;
+        if (__builtin_amdgcn_ballot_w64(max(high.x, high.y) >= kTreeGrown) != 0) sh->grown = number + n_tiles - 1;
         values(std::false_type{}, buf, 0, number + n_tiles - 1, [&](const TreeFlags& f) {
             const bool dirty = __builtin_amdgcn_readfirstlane(f.dirty) == number + n_tiles - 1, grown = __builtin_amdgcn_readfirstlane(f.grown) == number + n_tiles - 1;
             if (dirty) clean(buf);

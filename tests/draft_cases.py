@@ -89,8 +89,8 @@ def tree_attention(qabs, qrope, pool, tables, ctx, cu, masks, page, scale):
 
     The bounds. A product of a bf16 and a code is exact in f32 (8 + 4 bits); a dot of `width` of them in f32, in any order, is off by at
     most width half steps of the sum of magnitudes, the two scalings by three more: d = (width + 3) 2^-24 max_t sum |q k| |scale|. A weight is then
-    off by d relative, by 8 steps of its exponential and exponent's argument (|x| < 2^7 in powers of two: 2^-17 relative), and by half a bf16 step where
-    it meets the values; sums of n weights by n half steps. Against mass = sum_t w_t |L_t|:
+    off by d relative, by 8 steps of its exponential and exponent's argument (|x| < 2^7 in powers of two: 2^-17 relative), and by half a step of 16 bits where
+    it meets the values (2^-8, bf16's, is the most that is allowed; fp16's is 2^-11, or 2^-25 of the row's largest); sums of n weights by n half steps. Against mass = sum_t w_t |L_t|:
     |clat error| <= 2^-8 |clat| + (2^-8 + 2 (d + 2^-16 + n 2^-24)) mass;   |lse error| <= d + 2^-16 + n 2^-24 + 2^-22 |lse|."""
     n, H, kvl = qabs.shape
     width = kvl + qrope.shape[2]
