@@ -268,3 +268,13 @@ def test_a_batch_of_nothing_but_prefixes_and_of_single_tokens():
     case = Case(54, [5000, 0, 1], [0, 0, 1], 16)         # one node in all
     case.check()
     Case(55, [0] * 200, [1] * 200, 128, masks="chain").check()
+
+
+@pytest.mark.parametrize("ctx,nodes,H", [([700, 300], [6, 3], 16), ([2500], [2], 8)])
+def test_scales_of_very_different_rows(ctx, nodes, H):
+    """Rows whose scales lie up to 2^16 apart: weights carry them."""
+    case = Case(56 + H, ctx, nodes, H)
+    rng = np.random.default_rng(9)
+    scales = case.pool[:, 64 * 576:].view(np.float32)
+    scales *= np.exp2(rng.uniform(-16, 0, scales.shape)).astype(np.float32)
+    case.check()
