@@ -20,19 +20,21 @@ namespace rk {
 // What bounds it. The walk is a chain of short steps in LDS by one wave, some 7 us with the launch and the nodes' scattered loads; a row's sum reads it once,
 // and a rejected draft whose sibling is still to be judged reads target and draft rows once more, by the sequence's own workgroup: 131 072 tokens
 // of f32 and a draft are 1 MB, some 16 us for a compute unit, as much its conversions and sums in 64 bits as its loads. 256 sequences of 8 drawn nodes
-// of that size take 94 us where one read of two rows each is 54, the rest being second and third siblings; 32 of 16 picked nodes 14 us; one of 4 over 32 001 tokens 8.4.
+// of that size take 94 us where one read of two rows each is 54, the rest being second and third siblings; 32 of 16 picked nodes 11 us; one of 4 over 32 001 tokens 8.4.
 // A wave's loads of a block are all on their way before the first is used, and picked tokens that were rejected are looked for once a block:
-// testing each weight against each of them took 28 us where the row's sum now takes 14.
+// testing each weight against each of them took 28 us where one launch now takes 16.
 constexpr int kVerifyThreads = 1024, kVerifyWaves = kVerifyThreads / kWave;
 constexpr int kVerifyNodes = 1024;             // of a sequence, held in LDS
 constexpr int kVerifyChunk = 8 * kWave;        // tokens a wave's loads bring at once: eight a lane
 constexpr int kVerifyChunks = 2;               // of a block: four of them spill in a workgroup of 16 waves, and are no faster
 constexpr int kVerifyBlock = kVerifyChunks * kVerifyChunk;
 constexpr int kVerifyBlocks = 2048;            // block sums in LDS: up to 2^21 tokens
-// Calls of few sequences and long rows have the last pass over a row, the only one that most have, by many workgroups in a launch of its own, and the draw in a third. In
-// us, one launch and three: 1 sequence of 131 072 picked bf16 tokens 14.6 and 11.8, 32 of them 15.2 and 12.5, 32 of f32 with drafts 45 and 39; 64 of those
-// 40 and 45; 32 of 65 536 picked 11.0 and 12.1.
+// Calls of few sequences and long rows have the last pass over a row, the only one that most have, by many workgroups, and the draw in a launch of its
+// own. Picked drafts' walk takes no sums, so that every workgroup makes it for itself: two launches. In us, in one launch and in two: 1 sequence of 131 072
+// bf16 tokens 15.6 and 9.3, 32 of them 16.0 and 9.9, 64 16.3 and 14.6, 128 16.9 and 21.3; 64 of 65 536 11.4 and 10.1, 32 of 32 768 9.3 and 9.5. Drawn drafts have the
+// walk in front in a launch of its own, three launches: 32 of 131 072 f32 tokens 45 and 39, 64 of them 40 and 45.
 constexpr int kVerifySplitSeqs = 32, kVerifySplitVocab = 98304;
+constexpr int kPickedSplitSeqs = 64, kPickedSplitVocab = 49152;
 constexpr int kVerifySumThreads = 256, kVerifySumBlocks = 4;  // a workgroup of the split form: a block a wave
 
 struct VerifyArgs {
@@ -260,36 +262,42 @@ __device__ __forceinline__ int drawn(const R& row, int blocks, const double* sum
     return found >= 0 ? found : answer;
 }
 
-// The walk of a sequence's tree, a workgroup each; and, unless SPLIT, the next token.
-template <bool BF16, bool SPLIT>
-__global__ __launch_bounds__(kVerifyThreads) void draft_verify_kernel(const VerifyArgs a) {
+// The walk of a sequence's tree, a workgroup each, and the next token (kWhole); of the split forms the walk alone (kWalk), or (kPicked) the walk of picked
+// drafts, which takes no sums, by every workgroup of a sequence, and then the sums of the blocks that are the workgroup's, a wave each.
+enum VerifyForm { kWhole, kWalk, kPicked };
+template <bool BF16, VerifyForm FORM>
+__global__ __launch_bounds__(FORM == kPicked ? kVerifySumThreads : kVerifyThreads) void draft_verify_kernel(const VerifyArgs a) {
+    constexpr int kThreads = FORM == kPicked ? kVerifySumThreads : kVerifyThreads;
+    const bool drawn_drafts = FORM != kPicked && a.draft;
+    const bool writes = FORM != kPicked || blockIdx.x == 0;
     __shared__ int parent[kVerifyNodes], token[kVerifyNodes], gone[kVerifyNodes];  // gone: tokens rejected at cur
     __shared__ float share[kVerifyNodes], p_of[kVerifyNodes], q_of[kVerifyNodes];
     __shared__ double level[kVerifyNodes];  // c_0 .. c_k at cur
     __shared__ double sums[kVerifyBlocks];
     __shared__ int state[3];
     __shared__ double all;
-    const int seq = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int seq = FORM == kPicked ? blockIdx.y : blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int node0 = min(max(a.cu[seq], 0), a.n_nodes);
     const int n = min(max(a.cu[seq + 1] - node0, 0), min(a.max_nodes, a.n_nodes - node0));
     int* const path = a.path + (size_t)seq * a.max_nodes;
     if (n == 0) {
-        for (int i = tid; i < a.max_nodes; i += kVerifyThreads) path[i] = -1;
+        if (!writes) return;
+        for (int i = tid; i < a.max_nodes; i += kThreads) path[i] = -1;
         if (tid == 0) a.n_path[seq] = 0, a.next[seq] = -1;
-        if (SPLIT && tid == 0) a.end[2 * seq] = -1;
+        if (FORM != kWhole && tid == 0) a.end[2 * seq] = -1;
         return;
     }
-    for (int i = tid; i < n; i += kVerifyThreads) {
+    for (int i = tid; i < n; i += kThreads) {
         int up = i > 0 ? a.parents[node0 + i] : -1;
         const int x = a.tokens[node0 + i];
         if (i > 0 && !((unsigned)up < (unsigned)i && (unsigned)x < (unsigned)a.vocab)) {
             up = -1;  // no node's child
-            if (a.bad) atomicAdd(a.bad, 1u);
+            if (a.bad && writes) atomicAdd(a.bad, 1u);
         }
         parent[i] = up, token[i] = x, share[i] = a.u[node0 + i];
         const bool there = up >= 0;
         p_of[i] = there ? prob<BF16>(a.target, (long long)(node0 + up) * a.target_stride + x) : 0.0f;
-        q_of[i] = there && a.draft ? prob<BF16>(a.draft, (long long)(node0 + up) * a.draft_stride + x) : 1.0f;
+        q_of[i] = there && drawn_drafts ? prob<BF16>(a.draft, (long long)(node0 + up) * a.draft_stride + x) : 1.0f;
     }
     const int blocks = (a.vocab + kVerifyBlock - 1) / kVerifyBlock;
 
@@ -302,7 +310,8 @@ __global__ __launch_bounds__(kVerifyThreads) void draft_verify_kernel(const Veri
         return -1;
     };
     int cur = 0, last = 0, k = 0, count = 1;
-    if (tid == 0) path[0] = 0, level[0] = 1.0;
+    if (tid == 0 && writes) path[0] = 0;
+    if (tid == 0) level[0] = 1.0;
     __syncthreads();
     for (;;) {
         if (wave == 0) {
@@ -314,7 +323,7 @@ __global__ __launch_bounds__(kVerifyThreads) void draft_verify_kernel(const Veri
                 const int x = token[child];
                 const double c = level[k], q = (double)q_of[child];
                 double w = (double)p_of[child];
-                if (a.draft) {
+                if (drawn_drafts) {
                     for (int j = 0; j < k; ++j) w = fmax(w - level[j] * q, 0.0);
                 } else {
                     for (int j = 0; j < k; j += kWave)
@@ -322,15 +331,15 @@ __global__ __launch_bounds__(kVerifyThreads) void draft_verify_kernel(const Veri
                 }
                 if ((double)share[child] * q * c < w) {
                     cur = child, k = 0;
-                    if (lane == 0) path[count] = child;
+                    if (lane == 0 && writes) path[count] = child;
                     ++count;
                     continue;
                 }
                 if (lane == 0) gone[k] = x;
-                if (lane == 0 && !a.draft && k + 1 < kVerifyNodes) level[k + 1] = c - w;
+                if (lane == 0 && !drawn_drafts && k + 1 < kVerifyNodes) level[k + 1] = c - w;
                 __builtin_amdgcn_wave_barrier();
                 ++k;
-                if (a.draft && child_after(cur, last) >= 0) {  // (the sum is for a sibling's test)
+                if (drawn_drafts && child_after(cur, last) >= 0) {  // (the sum is for a sibling's test)
                     need = 1;
                     break;
                 }
@@ -339,21 +348,28 @@ __global__ __launch_bounds__(kVerifyThreads) void draft_verify_kernel(const Veri
         }
         __syncthreads();
         const int at = state[0], after = state[1], need = state[2];
-        if (!need) break;
+        if (FORM == kPicked || !need) break;
         sum_row(Row<BF16>(a, node0 + at, after, level, gone), blocks, sums, &all);
         if (tid == 0) level[after] = all;
         __syncthreads();
     }
     cur = state[0], k = state[1];
-    if (wave == 0) {
+    if (wave == 0 && writes) {
         for (int i = count + lane; i < a.max_nodes; i += kWave) path[i] = -1;
         if (lane == 0) a.n_path[seq] = count;
     }
-    if (SPLIT) {
-        if (tid == 0) a.end[2 * seq] = node0 + cur, a.end[2 * seq + 1] = k;
-        for (int j = tid; j < k; j += kVerifyThreads) {
-            a.levels[(size_t)seq * a.max_nodes + j] = a.draft ? level[j] : 0.0;
-            a.gone[(size_t)seq * a.max_nodes + j] = gone[j];
+    if (FORM != kWhole) {
+        if (tid == 0 && writes) a.end[2 * seq] = node0 + cur, a.end[2 * seq + 1] = k;
+        if (writes)
+            for (int j = tid; j < k; j += kThreads) {
+                a.levels[(size_t)seq * a.max_nodes + j] = drawn_drafts ? level[j] : 0.0;
+                a.gone[(size_t)seq * a.max_nodes + j] = gone[j];
+            }
+        if (FORM == kPicked) {
+            const int b = blockIdx.x * kVerifySumBlocks + wave;
+            if (b >= blocks) return;
+            const double s = Row<BF16>(a, node0 + cur, k, level, gone).block(b);
+            if (lane == 0) a.sums[(size_t)seq * blocks + b] = s;
         }
         return;
     }
@@ -368,7 +384,7 @@ __global__ __launch_bounds__(kVerifyThreads) void draft_verify_kernel(const Veri
     if (lane == 0) a.next[seq] = next;
 }
 
-// The split form's second launch, a wave a block of the row that a sequence's walk ended with, and its third, which draws from their sums.
+// The split form's second launch after kWalk, a wave a block of the row that a sequence's walk ended with; and the last one, which draws from their sums.
 template <bool BF16>
 __global__ __launch_bounds__(kVerifySumThreads) void draft_sums_kernel(const VerifyArgs a) {
     __shared__ double level[kVerifyNodes];
@@ -415,14 +431,16 @@ __global__ __launch_bounds__(kVerifyThreads) void draft_draw_kernel(const Verify
     if (lane == 0) a.next[seq] = next;
 }
 
-// Whether a call takes the split form, and the pieces of its workspace (from 16-byte boundaries on).
+// Whether a call of picked or drawn drafts takes a split form, and the pieces of its workspace (from 16-byte boundaries on).
 struct VerifySplit {
-    bool on;
+    bool picked, drawn;
     size_t levels, sums, gone, end, bytes;
 };
 static VerifySplit verify_split(int n_seqs, int max_nodes, int vocab) {
-    VerifySplit s{n_seqs > 0 && n_seqs <= kVerifySplitSeqs && max_nodes > 0 && vocab >= kVerifySplitVocab, 0, 0, 0, 0, 0};
-    if (!s.on) return s;
+    const bool some = n_seqs > 0 && max_nodes > 0;
+    VerifySplit s{some && n_seqs <= kPickedSplitSeqs && vocab >= kPickedSplitVocab, some && n_seqs <= kVerifySplitSeqs && vocab >= kVerifySplitVocab,
+                  0, 0, 0, 0, 0};
+    if (!s.picked && !s.drawn) return s;
     const size_t blocks = ((size_t)vocab + kVerifyBlock - 1) / kVerifyBlock, n = (size_t)n_seqs;
     s.sums = n * max_nodes * 8;
     s.gone = s.sums + n * blocks * 8;
@@ -436,12 +454,17 @@ static int draft_verify(const VerifyArgs& a, bool split, int n_seqs, hipStream_t
     (void)hipGetLastError();
     const dim3 grid((unsigned)n_seqs), block(kVerifyThreads);
     if (!split) {
-        launch_kernel(draft_verify_kernel<BF16, false>, grid, block, 0, st, a);
+        launch_kernel(draft_verify_kernel<BF16, kWhole>, grid, block, 0, st, a);
         return launch_status();
     }
     const unsigned blocks = (unsigned)((a.vocab + kVerifyBlock - 1) / kVerifyBlock);
-    launch_kernel(draft_verify_kernel<BF16, true>, grid, block, 0, st, a);
-    launch_kernel(draft_sums_kernel<BF16>, dim3((blocks + kVerifySumBlocks - 1) / kVerifySumBlocks, (unsigned)n_seqs), dim3(kVerifySumThreads), 0, st, a);
+    const dim3 shares((blocks + kVerifySumBlocks - 1) / kVerifySumBlocks, (unsigned)n_seqs), some(kVerifySumThreads);
+    if (a.draft) {
+        launch_kernel(draft_verify_kernel<BF16, kWalk>, grid, block, 0, st, a);
+        launch_kernel(draft_sums_kernel<BF16>, shares, some, 0, st, a);
+    } else {
+        launch_kernel(draft_verify_kernel<BF16, kPicked>, shares, some, 0, st, a);
+    }
     launch_kernel(draft_draw_kernel<BF16>, grid, block, 0, st, a);
     return launch_status();
 }
@@ -464,7 +487,8 @@ extern "C" int rivoli_draft_verify(const void* target_probs, const void* draft_p
         (draft_probs && draft_stride < vocab))
         return 1002;
     const rk::VerifySplit split = rk::verify_split(n_seqs, max_nodes, vocab);
-    if (split.on && !workspace) return 1001;
+    const bool shared = draft_probs ? split.drawn : split.picked;
+    if (shared && !workspace) return 1001;
     const uintptr_t size = bf16 ? 2 : 4;
     if ((uintptr_t)target_probs % size != 0 || (uintptr_t)draft_probs % size != 0 || !rk::aligned16(workspace)) return 1004;
     unsigned char* const work = static_cast<unsigned char*>(workspace);
@@ -472,5 +496,5 @@ extern "C" int rivoli_draft_verify(const void* target_probs, const void* draft_p
                            target_stride, draft_stride, path, n_path, next_token, reinterpret_cast<int*>(work + split.end),
                            reinterpret_cast<double*>(work + split.levels), reinterpret_cast<int*>(work + split.gone),
                            reinterpret_cast<double*>(work + split.sums), bad_nodes};
-    return bf16 ? rk::draft_verify<true>(a, split.on, n_seqs, (hipStream_t)stream) : rk::draft_verify<false>(a, split.on, n_seqs, (hipStream_t)stream);
+    return bf16 ? rk::draft_verify<true>(a, shared, n_seqs, (hipStream_t)stream) : rk::draft_verify<false>(a, shared, n_seqs, (hipStream_t)stream);
 }

@@ -207,13 +207,20 @@ WIDE = 98304 + 1029  # rows that many workgroups share in a call of few sequence
 
 
 def test_wide_rows_take_a_workspace_in_calls_of_few_sequences():
-    assert hip.draft_verify_workspace_bytes(4, 5, WIDE) > 0
+    assert hip.draft_verify_workspace_bytes(5, 5, WIDE) > 0 and hip.draft_verify_workspace_bytes(64, 3, 49152) > 0
 
 
 @pytest.mark.parametrize("draft", [False, True])
 @pytest.mark.parametrize("bf16", [False, True])
 def test_wide_rows(draft, bf16):
     Case(60, [3, 0, 4, 1, 2], WIDE, draft, bf16=bf16, pad=1, peaked=3.0).check()
+
+
+def test_rows_shared_by_workgroups_that_walk_for_themselves():
+    """Picked drafts: bad nodes counted once, sequences without nodes, a last workgroup with less than a block a wave."""
+    case = Case(68, [7, 0, 5, 9, 1], 49152 + 5 * 1024 + 3, False, bf16=True, pad=2)
+    case.parents[3], case.tokens[15] = 6, -1
+    case.check(bad=2)
 
 
 @pytest.mark.parametrize("draft", [False, True])
