@@ -588,7 +588,7 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
 #pragma unroll
             for (int b = 0; b < 2; ++b) o[c][b] = f32x16{};
         // ---- the first tile, which sets the references -----------------------------------------------------------
-        ask(1);
+        if (n_tiles > 1) ask(1);
         scores(0, std::false_type{}, 0, 0);
         seen = seen_of(0, 0), seen_half = seen >> 4 * half;
         bool masked = __builtin_amdgcn_ballot_w64(seen != ~0u) != 0;  // some row may not see some token of tile i
@@ -596,7 +596,7 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
 #pragma unroll
         for (int r = 0; r < 16; ++r) sc[r] = x[0][r] + sh->part[2 * th + kh][r >> 2][lane][r & 3];
         refer(0);
-        arrived(1), fill_holes(1, number + 1);
+        if (n_tiles > 1) arrived(1), fill_holes(1, number + 1);
         lds_barrier();
         int buf = 0;  // of tile i
         for (int i = 0; i + 1 < n_tiles; ++i) {
