@@ -9,8 +9,8 @@
 //     32 rows and keeps the other 32, so that a score is handled once;
 //   - values: a wave has 128 of the 512 columns for all 64 rows (128 accumulators); every byte of a value is read once, by the transposing
 //     load, and only the weights (8 KB) are read by all four.
-// Codes go from memory into LDS as they are, three tiles in rotation, and become bf16 (exact) when an operand is read, once for the
-// workgroup. 32 x 32 matrix tiles: a fragment serves two of them.
+// Codes go from memory into LDS as they are, three tiles in rotation, and become bf16 for the scores and f16 for the values (both exact) when an
+// operand is read, once for the workgroup. 32 x 32 matrix tiles: a fragment serves two of them.
 // An iteration has two halves, a barrier behind each: the scores of tile i + 1, with tile i's softmax and the transfers of tile i + 2
 // between their matrix instructions; then the values of tile i, with the partial scores of i + 1 meeting.
 // A weight is its exponential times its token's scale, rounded once to f16, which codes are exact in as well. A row's reference makes the
@@ -21,10 +21,11 @@
 // others under each. So what counts beside the matrix instructions is how many others there are and what waits: fragments are asked for steps
 // ahead of their use, control flow and a run's address are scalar, rare work sits behind flags. An iteration is 68 matrix instructions and some 430 others a
 // wave, 4 100 cycles (2 176 of matrix instructions; 70 more others took 4 680).
-// Measured: 32 sequences of 32 768 tokens, 8 nodes of 64 heads 1 024 us, 1.14 PFLOP/s; 131 072 tokens, 64 nodes of 128 heads 1 941 us, 1.20 PFLOP/s, where
+// Measured: 32 sequences of 32 768 tokens, 8 nodes of 64 heads 1 020 us, 1.14 PFLOP/s; 131 072 tokens, 64 nodes of 128 heads 1 930 us, 1.21 PFLOP/s, where
 // a large bf16 product reaches 1.36. The clock follows the power: 2.33 GHz at 4 680 cycles a tile, 2.08 at 4 100, 1.8 in a loop of nothing but these
 // matrix instructions (1.86 PFLOP/s), so that an instruction saved gives about a quarter of its cycles. Short calls are bound by
-// what a block costs to begin with and end (kTreeBeginTiles): 4 nodes of 16 heads over 200 tokens 14 us, 11 of them here.
+// what a block costs to begin with and end (kTreeBeginTiles): 4 nodes of 16 heads over 200 tokens 13.5 us, 10 of them here (of some 20 000 cycles, 6 500 until the first tile and q are there, 2 000 until q is
+// in its registers, 3 000 for the record).
 #pragma once
 
 namespace rk {

@@ -12,9 +12,10 @@ constexpr int kTreeDies = 8;
 // one, 21.6 by four; 1 block of 126 tiles 27.6, 42.5, 26.8. Calls of up to kTreeFewTiles are cut to single tiles: 1 block of 4 or 9 tiles 14.3 us,
 // by two 16.3.
 constexpr int kTreeMinTiles = 2, kTreeFewTiles = 64;
-// What a block costs a work item to begin with and end, in tiles: 13 ragged sequences of up to 79 tiles, 3 blocks each, 32.9 us, as nothing 44.8;
-// 1 of 513, 8 blocks, 58.0 and 65.9. Nothing in calls of less than a tile a workgroup: 8 blocks of 16 17.1 us, and 20.1.
-constexpr unsigned kTreeBeginTiles = 3;
+// What a block costs a work item to begin with and end, in tiles: 13 ragged sequences of up to 79 tiles, 3 blocks each, 33.6 us, by three tiles 35.7, as
+// nothing over 44; 8 of 63 tiles, 8 blocks each, 60.1 and 65.5; 1 of 513, 8 blocks, 61.7 and 65.8; but 64 ragged of up to 32, 4 blocks, 52.9 and 51.8. Seven or nine
+// lose more there. Nothing in calls of less than a tile a workgroup: 8 blocks of 16 17.1 us, and 20.1.
+constexpr unsigned kTreeBeginTiles = 5;
 // Blocks of up to this many tiles are a workgroup's each, where there are kTreeWholeBlocks of them or two tiles at most: 32 blocks of 5 tiles 20.0 us,
 // cut 24.6; 64 of 6 22.7 and 29.4; but 8 of 16 28.1 and 17.2, 1 of 9 25.0 and 14.3.
 constexpr int kTreeWholeTiles = 8, kTreeWholeBlocks = 32;
