@@ -540,8 +540,8 @@ int rivoli_rope_rows(const void* x, void* out, const float* table, const int* po
  * Rows of clat and lse of nodes that no sequence has are left as they were.
  * Tokens whose page id is outside [0, n_pages) are left out and counted once in *bad_rows when non-null, tokens whose
  * scale is not a positive number are left out. What a masked token's row holds (NaN codes, an infinite scale) reaches nobody.
- * Weights (a token's exponential times its scale) are rounded to fp16 once for the value product, under a reference of their own row;
- * scores, statistics and sums are f32.
+ * Weights (a token's exponential times its scale) are rounded to fp16 once for the value product, 2^-11 of each at most; the smallest
+ * ones, below fp16's range under a reference of their own row, lose together at most 2^-13 of the sum of all (2^-39 a token past 2^26 tokens). Scores, statistics and sums are f32.
  * `partial`: caller-owned scratch of rivoli_mla_attend_tree_paged_scratch_floats(same sizes) floats, null when that is 0;
  * two calls in flight need one each. The plan depends on the sizes and the device-side lengths alone: equal calls give equal bits.
  * Rows of 512 + 64 run on the matrix cores, other widths (kvl a multiple of 128 up to 512, rope a multiple of 8 up to 64) a slower kernel.

@@ -14,9 +14,13 @@
 // An iteration has two halves, a barrier behind each: the scores of tile i + 1, with tile i's softmax and the transfers of tile i + 2
 // between their matrix instructions; then the values of tile i, with the partial scores of i + 1 meeting.
 // A weight is its exponential times its token's scale, rounded once to f16, which codes are exact in as well. A row's reference makes the
-// largest of these products one in its first tile; the row is rescaled only when some weight has grown to kTreeGrown, which every wave learns from a flag behind
-// the first barrier (regrow). So a weight has 11 bits down to 2^-14 of that largest one and is off by 2^-25 of it at most below: against 64 bits results are
-// off by 1.6e-3 of the norm, all of it their own rounding to bf16 (by bf16 weights 2.4e-3). Their sum, and so lse, is of the unrounded ones, in f32.
+// largest of these products 2^lift in its first tile; the row is rescaled only when some weight has grown to kTreeGrown, which every wave learns from a flag behind
+// the first barrier (regrow). A weight below 2^-14 there is off by up to 2^-25, one below 2^-25 gone, so that the small weights of n tokens lose at most n 2^-25: where
+// one early token outweighs a long flat rest that is a part of the result (with a lift of none 2^17 tokens of 2^-25 each lost 3.8e-3 of it). So the lift grows with a work
+// item's tiles, floor(log2(tiles)) - 5, and n 2^-(25 + lift) stays below 2^-13 of that weight, a thirty-second of a result's half step; past 2^26 tokens, where the lift
+// is held to 14 (2^15 is kTreeGrown), n 2^-39. Higher lifts leave less room to grow and rescale more often: 64 nodes of 128 heads over 131 072 tokens take 1 930 us by
+// none, 1 954 by this one, 1 976 by two more; 32 sequences of 32 768 1 042, 1 031 and 1 067.
+// Against 64 bits results are off by 1.6e-3 of the norm, their own rounding to bf16 (by bf16 weights 2.4e-3). The sum of the weights, and so lse, is of the unrounded ones, in f32.
 // One wave a SIMD issues an instruction in four cycles at best and a matrix instruction of 32 cycles in sixteen, which leaves room for four
 // others under each. So what counts beside the matrix instructions is how many others there are and what waits: fragments are asked for steps
 // ahead of their use, control flow and a run's address are scalar, rare work sits behind flags. An iteration is 68 matrix instructions and some 430 others a
@@ -43,8 +47,9 @@ constexpr int kTreeBuffers = 3;
 constexpr int kTreeRopeAt = 8 * 4096;
 constexpr int kTreeTileBytes = kTreeRopeAt + 4 * 1024;
 constexpr int kTreeSteps = 18;            // of 16 dims a wave: 16 of its 256 latent dims, two of its 32 roped ones
-// A row's largest weight of its first tile is one, later ones may grow to 2^15 (65 504 is the largest of 16 bits, 2^-14 the least with all of its bits).
+// A row's largest weight of its first tile is 2^lift, later ones may grow to 2^15 (65 504 is the largest of 16 bits, 2^-14 the least with all of its bits).
 constexpr uint16_t kTreeGrown = 0x7800;  // 2^15; a number with a sign bit counts as more (negative softmax scales)
+constexpr int kTreeMostLift = 14;
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 constexpr uint32_t kTreeHole = 0x80000000u;  // the scale of a token that is not there: -0
 
@@ -193,6 +198,7 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
     const int last_row = min(kTreeRows * rb + kTreeRows, rows) - 1;
     const int len = a.masks ? s.ctx + s.nodes : s.ctx + last_row / a.H + 1;
     const int n_tiles = min(tile_hi, (len + kTreeTokens - 1) / kTreeTokens) - tile_lo;
+    const int lift = n_tiles < 64 ? 0 : min(26 - __builtin_clz((unsigned)n_tiles), kTreeMostLift);
 
     // ---- where a tile's rows are: eight lanes have rows 16 wave + 8 o + (lane >> 3) -----------------------------
     // Lookups and transfers have no branches, so that they go between the matrix instructions: tiles past the end are asked for too,
@@ -443,7 +449,7 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
             top = fmaxf(__uint_as_float(other[0]), __uint_as_float(other[1]));
             if (half == 0) sh->top[th][own] = top;
             lds_barrier();
-            top = fmaxf(sh->top[0][own], sh->top[1][own]);
+            top = fmaxf(sh->top[0][own], sh->top[1][own]) - (float)lift;
             const bool grow = top > m_ref;
             const float corr = grow ? __builtin_amdgcn_exp2f(m_ref - top) : 1.0f;  // 2^-inf = 0 at first
             if (grow) m_ref = top;
