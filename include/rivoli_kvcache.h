@@ -512,7 +512,7 @@ int rivoli_kv_compress_decode(float* kv_state, float* score_state, const rivoli_
  * for contexts longer than trained: every f_j / factor when orig_ctx is 0 (factor 1: none), else by parts - pairs that turn
  * more than beta_fast times within orig_ctx positions keep f_j, those that turn less than beta_slow times have f_j /
  * factor, a linear ramp over the pairs between (its ends floored and ceiled, within [0, rd - 1]). Angles
- * are taken in 64 bits. Guards: 1001 null / non-positive sizes, negative first, base <= 1, factor <= 0, anything not finite, with
+ * and products are taken in 64 bits, rounded once. Guards: 1001 null / non-positive sizes, negative first, base <= 1, factor <= 0, anything not finite, with
  * orig_ctx betas not beta_fast > beta_slow > 0; 1002 rd > 1024 or positions past int; 1004 odd rd or table not 8-byte aligned. */
 int rivoli_rope_table(float* table, int first, int n_positions, int rd, float base, float factor, int orig_ctx,
                       float beta_fast, float beta_slow, float mscale, void* stream);

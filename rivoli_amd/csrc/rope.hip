@@ -20,7 +20,7 @@ struct RopeTableArgs {
     float* table;
     int first, n, pairs;
     double log2_base, factor, low, high;  // ramp over pairs low .. high; high < 0: every pair is stretched
-    float mscale;
+    double mscale;
 };
 constexpr int kTableRun = 16;
 
@@ -47,7 +47,7 @@ __global__ __launch_bounds__(256) void rope_table_kernel(const RopeTableArgs a) 
     for (int i = 0; i < kTableRun; ++i) {
         const unsigned p = run + (unsigned)i * runs;
         if (p >= (unsigned)a.n) return;
-        reinterpret_cast<f32x2*>(a.table)[(size_t)p * a.pairs + j] = f32x2{(float)c * a.mscale, (float)s * a.mscale};
+        reinterpret_cast<f32x2*>(a.table)[(size_t)p * a.pairs + j] = f32x2{(float)(c * a.mscale), (float)(s * a.mscale)};
         const double was = c;
         c = c * dc - s * ds, s = was * ds + s * dc;
     }
