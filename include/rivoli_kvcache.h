@@ -579,8 +579,8 @@ int rivoli_draft_verify(const void* target_probs, const void* draft_probs, const
 /* The kept rows where the next step expects them, in place: row ctx_lens[s] + path[s][k] (codes and scale, as they are) becomes row
  * ctx_lens[s] + k for k < n_path[s] (path as rivoli_draft_verify writes it, [n_seqs][max_path]), in n_layers pools of the same layout
  * that start layer_bytes apart (not read for one layer), as if all rows moved at once. new_lens[s] (nullable, not ctx_lens) = ctx_lens[s] +
- * n_path[s]. An entry below k, or either of whose rows has no page, is left out and counted once in *bad_rows when non-null.
- * Drafted rows must not share pages between sequences. Guards: 1001 null / non-positive, new_lens == ctx_lens; 1002 width > 1024,
+ * n_path[s]. An entry below k, or either of whose rows has no page, is left out and counted once in *bad_rows when non-null (an
+ * entry of k too, which moves nothing). Drafted rows must not share pages between sequences. Guards: 1001 null / non-positive, new_lens == ctx_lens; 1002 width > 1024,
  * n_seqs > 65535, layer_bytes less than a pool; 1004 width % 16, page_tokens % 4, layer_bytes % 16, pool not 16-byte aligned.
  * rivoli_index_commit_paged: the same for the paged index keys ([n_pages * page_tokens][hd] bf16, pools layer_keys keys apart);
  * 1002 hd > 512, 1004 hd % 8. */

@@ -45,9 +45,11 @@ __global__ __launch_bounds__(64) void kv_commit_kernel(const CommitArgs a) {
         bool moves = false;
         if (k < n) {
             const int node = path[k];
-            if (node != k) {
-                unsigned long long page_at;
-                unsigned int off;
+            unsigned long long page_at;
+            unsigned int off;
+            if (node == k) {  // stays; looked up for the count alone
+                if (a.bad && layer == 0 && lane < kCommitRows && !find((long long)ctx + k, page_at, off)) atomicAdd(a.bad, 1u);
+            } else {
                 bool ok = node > k && find((long long)ctx + node, page_at, off);
                 src = page_at + (unsigned long long)off * (unsigned)a.row_bytes;
                 src_scale = page_at + (unsigned long long)a.page_tokens * (unsigned)a.row_bytes + 4ull * off;
