@@ -513,7 +513,7 @@ int rivoli_kv_compress_decode(float* kv_state, float* score_state, const rivoli_
  * more than beta_fast times within orig_ctx positions keep f_j, those that turn less than beta_slow times have f_j /
  * factor, a linear ramp over the pairs between (its ends floored and ceiled, within [0, rd - 1]). Angles
  * and products are taken in 64 bits, rounded once. Guards: 1001 null / non-positive sizes, negative first, base <= 1, factor <= 0, anything not finite, with
- * orig_ctx betas not beta_fast > beta_slow > 0; 1002 rd > 1024 or positions past int; 1004 odd rd or table not 8-byte aligned. */
+ * orig_ctx betas not beta_fast > beta_slow > 0; 1002 rd > 1024, positions past int or more than a launch has (2^36 / (rd / 2)); 1004 odd rd or table not 8-byte aligned. */
 int rivoli_rope_table(float* table, int first, int n_positions, int rd, float base, float factor, int orig_ctx,
                       float beta_fast, float beta_slow, float mscale, void* stream);
 
@@ -546,7 +546,7 @@ int rivoli_rope_rows(const void* x, void* out, const float* table, const int* po
  * two calls in flight need one each. The plan depends on the sizes and the device-side lengths alone: equal calls give equal bits.
  * Rows of 512 + 64 run on the matrix cores, other widths (kvl a multiple of 128 up to 512, rope a multiple of 8 up to 64) a slower kernel.
  * Guards: 1001 null / non-positive (max_ctx may be 0), a null `partial` where one is needed; 1002 n_seqs > 65535, max_nodes > 4096, max_ctx >
- * 2^31 - 8193, n_nodes * H > 2^30, H > 262140, page_tokens > 2^22; 1004 widths as above, page_tokens % 4, qabs / qrope / pool / clat / partial not 16-byte aligned. */
+ * 2^31 - 8193, n_nodes * H > 2^30, H > 262140, page_tokens > 2^22, 2^24 blocks of 64 rows, or nodes where the rows are of other widths, or more; 1004 widths as above, page_tokens % 4, qabs / qrope / pool / clat / partial not 16-byte aligned. */
 size_t rivoli_mla_attend_tree_paged_scratch_floats(int n_seqs, int H, int n_nodes, int max_nodes, int max_ctx);
 int rivoli_mla_attend_tree_paged(const unsigned short* qabs, const unsigned short* qrope, const unsigned char* pool,
                                  const int* block_table, const int* ctx_lens, const int* cu_nodes,
@@ -567,8 +567,8 @@ int rivoli_mla_attend_tree_paged(const unsigned short* qabs, const unsigned shor
  * path[s][max_nodes] = 0 and the accepted nodes in order, then -1; n_path[s] their number (0 and next_token -1 for a sequence
  * without nodes). A node whose parent or token is out of range is nobody's child and counted in *bad_nodes when non-null.
  * `workspace`: rivoli_draft_verify_workspace_bytes(n_seqs, max_nodes, vocab) bytes, 16-byte aligned, nothing to be cleared, null when
- * that is 0; two calls in flight need one each. Guards: 1001 null / non-positive, a null workspace where one is needed; 1002 max_nodes > 1024, vocab > 2^21
- * or above a stride; 1004 rows not on an element, workspace not 16-byte aligned. */
+ * that is 0; two calls in flight need one each. Guards: 1001 null / non-positive, a null workspace where one is needed; 1002 n_seqs >= 2^22, max_nodes > 1024,
+ * vocab > 2^21 or above a stride; 1004 rows not on an element, workspace not 16-byte aligned. */
 size_t rivoli_draft_verify_workspace_bytes(int n_seqs, int max_nodes, int vocab);
 int rivoli_draft_verify(const void* target_probs, const void* draft_probs, const int* tokens, const int* parents,
                         const int* cu_nodes, const float* uniforms, const float* final_uniforms, int n_seqs,
@@ -581,7 +581,7 @@ int rivoli_draft_verify(const void* target_probs, const void* draft_probs, const
  * that start layer_bytes apart (not read for one layer), as if all rows moved at once. new_lens[s] (nullable, not ctx_lens) = ctx_lens[s] +
  * n_path[s]. An entry below k, or either of whose rows has no page, is left out and counted once in *bad_rows when non-null (an
  * entry of k too, which moves nothing). Drafted rows must not share pages between sequences. Guards: 1001 null / non-positive, new_lens == ctx_lens; 1002 width > 1024,
- * n_seqs > 65535, layer_bytes less than a pool; 1004 width % 16, page_tokens % 4, layer_bytes % 16, pool not 16-byte aligned.
+ * n_seqs or n_layers > 65535, layer_bytes less than a pool; 1004 width % 16, page_tokens % 4, layer_bytes % 16, pool not 16-byte aligned.
  * rivoli_index_commit_paged: the same for the paged index keys ([n_pages * page_tokens][hd] bf16, pools layer_keys keys apart);
  * 1002 hd > 512, 1004 hd % 8. */
 int rivoli_kv_commit_paged(unsigned char* pool, const int* block_table, const int* ctx_lens, const int* path,

@@ -212,6 +212,9 @@ __device__ __forceinline__ unsigned long long wave_xor(unsigned long long v) {
 // buffer that is not 16-byte aligned rather than let the kernel fault on it.
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// Threads along a dimension of a launch: 32 bits of them, whole workgroups.
+constexpr unsigned long long kLaunchThreads = 0xffffff00ull;
+
 // kernel<<<grid, block, lds, stream>>>(args...) without the configuration that the launch syntax
 // pushes for the kernel's stub and the stub pops again: 2.29 us of host time a launch, 2.44 with
 // it. The arguments are converted to the kernel's own parameter types first.

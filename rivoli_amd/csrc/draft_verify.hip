@@ -483,7 +483,7 @@ extern "C" int rivoli_draft_verify(const void* target_probs, const void* draft_p
     if (!target_probs || !tokens || !parents || !cu_nodes || !uniforms || !final_uniforms || !path || !n_path ||
         !next_token || n_seqs <= 0 || n_nodes <= 0 || max_nodes <= 0 || vocab <= 0)
         return 1001;
-    if (max_nodes > rk::kVerifyNodes || vocab > rk::kVerifyBlocks * rk::kVerifyBlock || target_stride < vocab ||
+    if (n_seqs > (int)(rk::kLaunchThreads / rk::kVerifyThreads) || max_nodes > rk::kVerifyNodes || vocab > rk::kVerifyBlocks * rk::kVerifyBlock || target_stride < vocab ||
         (draft_probs && draft_stride < vocab))
         return 1002;
     const rk::VerifySplit split = rk::verify_split(n_seqs, max_nodes, vocab);

@@ -96,7 +96,7 @@ extern "C" int rivoli_kv_commit_paged(unsigned char* pool, const int* block_tabl
         max_blocks_per_seq <= 0 || width <= 0 || page_tokens <= 0 || n_pages <= 0 || n_layers <= 0)
         return 1001;
     if (new_lens == ctx_lens) return 1001;  // layers read it while the first one writes
-    if (width > 1024 || n_seqs > 65535) return 1002;
+    if (width > 1024 || n_seqs > 65535 || n_layers > 65535) return 1002;
     if (width % 16 != 0 || page_tokens % 4 != 0 || !rk::aligned16(pool) || (n_layers > 1 && layer_bytes % 16 != 0)) return 1004;
     const unsigned long long page_bytes = (unsigned long long)page_tokens * (unsigned)(width + 4);
     if (n_layers > 1 && layer_bytes < (long long)(page_bytes * (unsigned)n_pages)) return 1002;
@@ -113,7 +113,7 @@ extern "C" int rivoli_index_commit_paged(unsigned short* kpool, const int* block
         max_blocks_per_seq <= 0 || hd <= 0 || page_tokens <= 0 || n_pages <= 0 || n_layers <= 0)
         return 1001;
     if (new_lens == ctx_lens) return 1001;
-    if (hd > 512 || n_seqs > 65535) return 1002;
+    if (hd > 512 || n_seqs > 65535 || n_layers > 65535) return 1002;
     if (hd % 8 != 0 || !rk::aligned16(kpool)) return 1004;
     if (n_layers > 1 && layer_keys < (long long)page_tokens * n_pages) return 1002;
     const rk::CommitArgs a{reinterpret_cast<unsigned char*>(kpool), block_table, ctx_lens, path, n_path, max_path, max_blocks_per_seq,

@@ -169,6 +169,8 @@ extern "C" int rivoli_mla_attend_tree_paged(const unsigned short* qabs, const un
     const bool plain = kvl != 512 || rope != 64;
     const rk::TreePlan plan = rk::tree_plan(n_seqs, H, n_nodes, max_nodes, max_ctx);
     if (!plain && plan.groups && !partial) return 1001;
+    const long long grid = plain ? n_nodes : plan.groups ? plan.groups : plan.blocks;
+    if (grid * rk::kTreeThreads > (long long)rk::kLaunchThreads) return 1002;
     float qscale = scale * rk::kLog2e;
     if (std::fabs(qscale) < 1e-20f) qscale = std::copysign(1e-20f, qscale);  // as good as nothing to any softmax
     const rk::TreeArgs a{qabs, qrope, pool, block_table, ctx_lens, cu_nodes, masks, n_seqs, H, n_nodes, max_nodes, (max_nodes + 31) / 32,
@@ -177,11 +179,11 @@ extern "C" int rivoli_mla_attend_tree_paged(const unsigned short* qabs, const un
     const hipStream_t st = (hipStream_t)stream;
     (void)hipGetLastError();
     if (plain) {
-        rk::launch_kernel(rk::mla_attend_tree_rowwise_kernel, dim3((unsigned)n_nodes, (unsigned)((H + rk::kTreeRowWaves - 1) / rk::kTreeRowWaves)),
+        rk::launch_kernel(rk::mla_attend_tree_rowwise_kernel, dim3((unsigned)grid, (unsigned)((H + rk::kTreeRowWaves - 1) / rk::kTreeRowWaves)),
                           dim3(rk::kTreeRowWaves * rk::kWave), 0, st, a);
         return rk::launch_status();
     }
-    rk::launch_kernel(page_tokens % 16 == 0 ? rk::mla_attend_tree_kernel<true> : rk::mla_attend_tree_kernel<false>, dim3((unsigned)(plan.groups ? plan.groups : plan.blocks)), dim3(rk::kTreeThreads), 0, st, a);
+    rk::launch_kernel(page_tokens % 16 == 0 ? rk::mla_attend_tree_kernel<true> : rk::mla_attend_tree_kernel<false>, dim3((unsigned)grid), dim3(rk::kTreeThreads), 0, st, a);
     const int rc = rk::launch_status();
     if (rc != 0 || plan.groups < 2) return rc;
     if (plan.blocks < plan.groups) rk::launch_kernel(rk::mla_attend_tree_merge_kernel<false>, dim3((unsigned)plan.blocks, 32), dim3(256), 0, st, a);

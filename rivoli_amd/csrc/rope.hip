@@ -144,8 +144,8 @@ static int rope_rows(RopeArgs& a, bool wide, hipStream_t st) {
     const bool many = a.n_heads >= kRopeHeads;
     a.groups = many ? (a.n_heads + kRopeHeads - 1) / kRopeHeads : a.n_heads;
     // (pieces and groups are 512 and 2^29 at most)
-    const unsigned long long per_token = (unsigned long long)a.groups * a.pieces, most = 0xffffff00ull;
-    if (per_token > most || (unsigned long long)a.n_tokens > most / per_token) return 1002;
+    const unsigned long long per_token = (unsigned long long)a.groups * a.pieces;
+    if (per_token > kLaunchThreads || (unsigned long long)a.n_tokens > kLaunchThreads / per_token) return 1002;
     const unsigned long long blocks = (a.n_tokens * per_token + 255) / 256;
     (void)hipGetLastError();
     const dim3 grid((unsigned)blocks), block(256);
@@ -177,7 +177,8 @@ extern "C" int rivoli_rope_table(float* table, int first, int n_positions, int r
         if (a.high <= a.low) a.high = a.low + 0.001;
     }
     const long long runs = ((long long)n_positions + rk::kTableRun - 1) / rk::kTableRun;
-    const long long blocks = (runs * a.pairs + 255) / 256;  // <= 2^27 runs of <= 512 pairs: fits a launch
+    if ((unsigned long long)(runs * a.pairs) > rk::kLaunchThreads) return 1002;
+    const long long blocks = (runs * a.pairs + 255) / 256;
     (void)hipGetLastError();
     rk::launch_kernel(rk::rope_table_kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a);
     return rk::launch_status();
