@@ -99,7 +99,7 @@ extern "C" int rivoli_kv_commit_paged(unsigned char* pool, const int* block_tabl
     if (width > 1024 || n_seqs > 65535 || n_layers > 65535) return 1002;
     if (width % 16 != 0 || page_tokens % 4 != 0 || !rk::aligned16(pool) || (n_layers > 1 && layer_bytes % 16 != 0)) return 1004;
     const unsigned long long page_bytes = (unsigned long long)page_tokens * (unsigned)(width + 4);
-    if (n_layers > 1 && layer_bytes < (long long)(page_bytes * (unsigned)n_pages)) return 1002;
+    if (n_layers > 1 && (layer_bytes < 0 || (unsigned long long)layer_bytes / page_bytes < (unsigned)n_pages)) return 1002;
     const rk::CommitArgs a{pool, block_table, ctx_lens, path, n_path, max_path, max_blocks_per_seq, page_tokens, n_pages, width, 1,
                            page_bytes, layer_bytes, new_lens, bad_rows};
     return rk::kv_commit(a, n_seqs, n_layers, (hipStream_t)stream);
@@ -118,6 +118,6 @@ extern "C" int rivoli_index_commit_paged(unsigned short* kpool, const int* block
     if (n_layers > 1 && layer_keys < (long long)page_tokens * n_pages) return 1002;
     const rk::CommitArgs a{reinterpret_cast<unsigned char*>(kpool), block_table, ctx_lens, path, n_path, max_path, max_blocks_per_seq,
                            page_tokens, n_pages, 2 * hd, 0, (unsigned long long)page_tokens * (unsigned)(2 * hd),
-                           layer_keys * 2 * hd, new_lens, bad_rows};
+                           n_layers > 1 ? layer_keys * 2 * hd : 0, new_lens, bad_rows};
     return rk::kv_commit(a, n_seqs, n_layers, (hipStream_t)stream);
 }

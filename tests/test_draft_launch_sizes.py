@@ -31,3 +31,10 @@ def test_commits_past_a_launch():
     good = dict(block_table=B, ctx_lens=B, path=B, n_path=B, n_seqs=1, max_path=4, max_blocks_per_seq=2, page_tokens=64, n_pages=2, n_layers=65536)
     refused(hip.launch_kv_commit_paged, dict(good, pool=B, width=576, layer_bytes=2 * 37120), [(dict(), 1002), (dict(n_layers=2 ** 31 - 1), 1002)])
     refused(hip.launch_index_commit_paged, dict(good, kpool=B, hd=128, layer_keys=128), [(dict(), 1002), (dict(n_layers=2 ** 31 - 1), 1002)])
+
+
+def test_pools_whose_bytes_pass_64_bits():
+    """2^30 tokens of 1 028 bytes in 2^23 pages are past 2^63: no distance between layers holds them."""
+    good = dict(pool=B, block_table=B, ctx_lens=B, path=B, n_path=B, n_seqs=1, max_path=4, max_blocks_per_seq=2, width=1024, page_tokens=2 ** 30, n_pages=2 ** 23,
+                n_layers=2, layer_bytes=2 ** 62)
+    refused(hip.launch_kv_commit_paged, good, [(dict(), 1002), (dict(n_pages=2 ** 24), 1002), (dict(layer_bytes=-16), 1002)])
