@@ -57,6 +57,40 @@ def check_resources(k: str, report: str) -> None:
             raise RuntimeError(f"{k}: no kernel matching {part}...{suffix} in the resource report")
 
 
+# Kernels whose register copies the compiler has put in front of a join's exec restore, where a wave that took the branch with no lane
+# enabled skips them: their listing is searched for such work, and the build refuses to produce one that has it.
+JOINS = ["mla_attend_tree.hip"]
+
+
+def early_vector_work(listing: str) -> list[tuple[str, str]]:
+    """(label, instruction) of vector instructions between a label that s_cbranch_execz goes to and the exec restore of its block."""
+    targets = set(re.findall(r"s_cbranch_execz\s+(\.LBB\w+)", listing))
+    found = []
+    for block in re.split(r"\n(?=\.LBB\w+:)", listing):
+        label = block.split(":", 1)[0].strip()
+        early: list[str] = []
+        for line in block.split("\n")[1:] if label in targets else []:
+            line = line.split(";", 1)[0].strip()
+            if not line or line.startswith("."):
+                continue
+            if re.match(r"s_(or|mov|xor|andn2|and)_b64 exec, |s_or_saveexec_b64 ", line):
+                found += [(label, x) for x in early]
+                break
+            if re.match(r"s_(cbranch|branch|endpgm|setpc)", line):
+                break
+            # (scalar instructions and moves of one lane's register work whatever the lanes)
+            if not re.match(r"s_|v_(readlane|writelane|readfirstlane)_b32", line):
+                early.append(line)
+    return found
+
+
+def check_joins(k: str, listing: str) -> None:
+    """Raises when the listing of a file of JOINS has vector work in front of a join's exec restore."""
+    early = early_vector_work(listing) if k in JOINS else []
+    if early:
+        raise RuntimeError(f"{k}: vector work in front of an exec restore: {early[:3]}")
+
+
 def hipcc() -> str:
     return os.environ.get("HIPCC", "hipcc")
 
@@ -94,6 +128,12 @@ def build_kernels(verbose: bool = False) -> str:
             raise RuntimeError("hipcc failed compiling " + k)
         try:
             check_resources(k, res.stderr)
+            if k in JOINS:
+                res = subprocess.run(compile_command(k) + ["--offload-device-only", "-S", os.path.join(CSRC, k), "-o", "-"],
+                                     capture_output=True, text=True)
+                if res.returncode != 0:
+                    raise RuntimeError("hipcc failed listing " + k)
+                check_joins(k, res.stdout)
         except RuntimeError:
             os.remove(obj)  # never link it
             raise
