@@ -20,7 +20,7 @@ namespace rk {
 // What bounds it. The walk is a chain of short steps in LDS by one wave, some 7 us with the launch and the nodes' scattered loads; a row's sum reads it once,
 // and a rejected draft whose sibling is still to be judged reads target and draft rows once more, by the sequence's own workgroup: 131 072 tokens
 // of f32 and a draft are 1 MB, some 16 us for a compute unit, as much its conversions and sums in 64 bits as its loads. 256 sequences of 8 drawn nodes
-// of that size take 94 us where one read of two rows each is 54, the rest being second and third siblings; 32 of 16 picked nodes 11 us; one of 4 over 32 001 tokens 8.4.
+// of that size take 98 us where one read of two rows each is 54, the rest being second and third siblings; 32 of 16 picked nodes 11 us; one of 4 over 32 001 tokens 8.2.
 // A wave's loads of a block are all on their way before the first is used, and picked tokens that were rejected are looked for once a block:
 // testing each weight against each of them took 28 us where one launch now takes 16.
 constexpr int kVerifyThreads = 1024, kVerifyWaves = kVerifyThreads / kWave;
@@ -32,7 +32,9 @@ constexpr int kVerifyBlocks = 2048;            // block sums in LDS: up to 2^21 
 // Calls of few sequences and long rows have the last pass over a row, the only one that most have, by many workgroups, and the draw in a launch of its
 // own. Picked drafts' walk takes no sums, so that every workgroup makes it for itself: two launches. In us, in one launch and in two: 1 sequence of 131 072
 // bf16 tokens 15.6 and 9.3, 32 of them 16.0 and 9.9, 64 16.3 and 14.6, 128 16.9 and 21.3; 64 of 65 536 11.4 and 10.1, 32 of 32 768 9.3 and 9.5. Drawn drafts have the
-// walk in front in a launch of its own, three launches: 32 of 131 072 f32 tokens 45 and 39, 64 of them 40 and 45.
+// walk in front in a launch of its own, three launches, of f32 tokens: 1 sequence of 49 152 8.1 and 9.6, of 65 536 9.0 and 9.5, of 98 304 11.1 and 10.0, of 131 072 12.7 and 10.0; 16 of
+// 49 152 37.1 and 37.6, of 65 536 20.6 and 18.5, of 98 304 40.4 and 33.8; 32 of 131 072 50.8 and 42.4; 48 of 98 304 41.2 and 37.3, 64 of 49 152 24.7 and 24.7, of 131 072 43.9 and 47.6 (what
+// is judged on the way, the same in both, makes most of these times).
 constexpr int kVerifySplitSeqs = 32, kVerifySplitVocab = 98304;
 constexpr int kPickedSplitSeqs = 64, kPickedSplitVocab = 49152;
 constexpr int kVerifySumThreads = 256, kVerifySumBlocks = 4;  // a workgroup of the split form: a block a wave

@@ -23,12 +23,12 @@
 // Against 64 bits results are off by 1.6e-3 of the norm, their own rounding to bf16 (by bf16 weights 2.4e-3). The sum of the weights, and so lse, is of the unrounded ones, in f32.
 // One wave a SIMD issues an instruction in four cycles at best and a matrix instruction of 32 cycles in sixteen, which leaves room for four
 // others under each. So what counts beside the matrix instructions is how many others there are and what waits: fragments are asked for steps
-// ahead of their use, control flow and a run's address are scalar, rare work sits behind flags. An iteration is 68 matrix instructions and some 430 others a
-// wave, 4 100 cycles (2 176 of matrix instructions; 70 more others took 4 680).
-// Measured: 32 sequences of 32 768 tokens, 8 nodes of 64 heads 1 020 us, 1.14 PFLOP/s; 131 072 tokens, 64 nodes of 128 heads 1 930 us, 1.21 PFLOP/s, where
-// a large bf16 product reaches 1.36. The clock follows the power: 2.33 GHz at 4 680 cycles a tile, 2.08 at 4 100, 1.8 in a loop of nothing but these
+// ahead of their use, control flow and a run's address are scalar, rare work sits behind flags. An iteration is 68 matrix instructions, 315 other vector and 55 LDS instructions a
+// wave, 4 270 cycles (counted over 32 sequences of 32 768 tokens; 2 176 are of matrix instructions; with 70 more others 4 580).
+// Measured: 32 sequences of 32 768 tokens, 8 nodes of 64 heads 1 030 to 1 040 us, 1.13 PFLOP/s; 131 072 tokens, 64 nodes of 128 heads 1 955 to 1 975, 1.19 PFLOP/s, where
+// a large bf16 product reaches 1.36. The clock follows the power: some 2.1 GHz here, 1.8 in a loop of nothing but these
 // matrix instructions (1.86 PFLOP/s), so that an instruction saved gives about a quarter of its cycles. Short calls are bound by
-// what a block costs to begin with and end (kTreeBeginTiles): 4 nodes of 16 heads over 200 tokens 13.5 us, 10 of them here (of some 20 000 cycles, 6 500 until the first tile and q are there, 2 000 until q is
+// what a block costs to begin with and end (kTreeBeginTiles): 4 nodes of 16 heads over 200 tokens 13.4 us, 10 of them here (of some 20 000 cycles, 6 500 until the first tile and q are there, 2 000 until q is
 // in its registers, 3 000 for the record).
 #pragma once
 
@@ -707,7 +707,8 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
     lds_barrier();
 }
 
-// RUNS: pages are whole runs of 16 rows.
+// RUNS: pages are whole runs of 16 rows, whose addresses are scalar. 32 sequences of 8 192 tokens, 8 nodes of 64 heads, in pages of 48 and 64 rows 269 us, of 4 and 60
+// rows, by the form for any, 275; 64 nodes of 128 heads over 32 768 524 and 535.
 template <bool RUNS>
 __global__ __launch_bounds__(kTreeThreads, 1) void mla_attend_tree_kernel(const TreeArgs a) {
     __shared__ __attribute__((aligned(1024))) TreeShared shared;
