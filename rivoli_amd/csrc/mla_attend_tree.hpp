@@ -434,16 +434,17 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
             }
             return __builtin_amdgcn_ballot_w64(nan) != 0;
         };
-        // New references for the rows of a tile (the workgroup's decision), and a factor for what came before. (The exponent of a scale is held to 2^-90, so
-        // that a sum of exponentials alone stays a number.)
+        // New references for the rows of a tile (the workgroup's decision), and a factor for what came before. (A scale counts as 2^(lift - 90) at least, so
+        // that an exponential is 2^90 at most and the sum of 2^31 of them a number.)
         auto refer = [&](int buf) -> float {
             float top = -INFINITY;
+            const float least = (float)(lift - 90);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const f32x4 s4 = scales_of(buf, i);
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                    top = fmaxf(top, bit_of(4 * i + k) ? __builtin_fmaf(sc[4 * i + k], s4[k], fmaxf(__builtin_amdgcn_logf(fabsf(s4[k])), -90.0f)) : -INFINITY);
+                    top = fmaxf(top, bit_of(4 * i + k) ? __builtin_fmaf(sc[4 * i + k], s4[k], fmaxf(__builtin_amdgcn_logf(fabsf(s4[k])), least)) : -INFINITY);
             }
             const auto other = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
             top = fmaxf(__uint_as_float(other[0]), __uint_as_float(other[1]));
