@@ -546,7 +546,8 @@ int rivoli_rope_rows(const void* x, void* out, const float* table, const int* po
  * two calls in flight need one each. The plan depends on the sizes and the device-side lengths alone: equal calls give equal bits.
  * Rows of 512 + 64 run on the matrix cores, other widths (kvl a multiple of 128 up to 512, rope a multiple of 8 up to 64) a slower kernel.
  * Guards: 1001 null / non-positive (max_ctx may be 0), a null `partial` where one is needed; 1002 n_seqs > 65535, max_nodes > 4096, max_ctx >
- * 2^31 - 8193, n_nodes * H > 2^30, H > 262140, page_tokens > 2^22, 2^24 blocks of 64 rows, or nodes where the rows are of other widths, or more; 1004 widths as above, page_tokens % 4, qabs / qrope / pool / clat / partial not 16-byte aligned. */
+ * 2^31 - 8193, n_nodes * H > 2^30, H > 262140, page_tokens > 2^22,
+ * more workgroups than a launch has (2^24 blocks of 64 rows that are not cut, or nodes where rows are of other widths); 1004 widths as above, page_tokens % 4, qabs / qrope / pool / clat / partial not 16-byte aligned. */
 size_t rivoli_mla_attend_tree_paged_scratch_floats(int n_seqs, int H, int n_nodes, int max_nodes, int max_ctx);
 int rivoli_mla_attend_tree_paged(const unsigned short* qabs, const unsigned short* qrope, const unsigned char* pool,
                                  const int* block_table, const int* ctx_lens, const int* cu_nodes,
