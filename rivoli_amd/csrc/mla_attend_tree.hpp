@@ -25,7 +25,7 @@
 // others under each. So what counts beside the matrix instructions is how many others there are and what waits: fragments are asked for steps
 // ahead of their use, control flow and a run's address are scalar, rare work sits behind flags. An iteration is 68 matrix instructions, 315 other vector and 55 LDS instructions a
 // wave, 4 270 cycles (counted over 32 sequences of 32 768 tokens; 2 176 are of matrix instructions; with 70 more others 4 580).
-// Measured: 32 sequences of 32 768 tokens, 8 nodes of 64 heads 1 030 to 1 040 us, 1.13 PFLOP/s; 131 072 tokens, 64 nodes of 128 heads 1 955 to 1 975, 1.19 PFLOP/s, where
+// Measured: 32 sequences of 32 768 tokens, 8 nodes of 64 heads 1 030 to 1 085 us by the card, 1.13 to 1.08 PFLOP/s; 131 072 tokens, 64 nodes of 128 heads 1 955 to 2 040, 1.19 to 1.15, where
 // a large bf16 product reaches 1.36. The clock follows the power: some 2.1 GHz here, 1.8 in a loop of nothing but these
 // matrix instructions (1.86 PFLOP/s), so that an instruction saved gives about a quarter of its cycles. Short calls are bound by
 // what a block costs to begin with and end (kTreeBeginTiles): 4 nodes of 16 heads over 200 tokens 13.4 us, 10 of them here (of some 20 000 cycles, 6 500 until the first tile and q are there, 2 000 until q is
