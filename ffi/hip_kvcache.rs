@@ -562,6 +562,61 @@ launchers! {
         stream: *mut c_void,
     );
 
+    /// Norm and rotation of every head's row in one pass, to rows or to the paged index keys.
+    /// See `include/rivoli_kvcache.h` for the full contract.
+    launch_norm_rope_rows -> rivoli_norm_rope_rows, "norm_rope_rows" (
+        x: *const c_void,
+        out: *mut c_void,
+        weight: *const f32,
+        bias: *const f32,
+        table: *const f32,
+        positions: *const i32,
+        slots: *const i32,
+        n_tokens: usize as i32,
+        n_heads: usize as i32,
+        width: usize as i32,
+        norm_n: usize as i32,
+        rope_at: usize as i32,
+        rd: usize as i32,
+        n_positions: usize as i32,
+        n_slots: usize as i32,
+        x_token_stride: i64,
+        x_head_stride: i64,
+        out_token_stride: i64,
+        out_head_stride: i64,
+        weight_head_stride: i64,
+        eps: f32,
+        center: i32,
+        half: i32,
+        x_bf16: i32,
+        out_bf16: i32,
+        bad_tokens: *mut u32,
+        stream: *mut c_void,
+    );
+
+    /// Quantize-and-append of latent rows that are normed and rotated on the way.
+    /// See `include/rivoli_kvcache.h` for the full contract.
+    launch_kv_norm_append_paged -> rivoli_kv_norm_append_paged, "kv_norm_append_paged" (
+        x: *const c_void,
+        slot_mapping: *const i32,
+        weight: *const f32,
+        table: *const f32,
+        positions: *const i32,
+        pool: *mut u8,
+        n_tokens: usize as i32,
+        x_stride: i64,
+        kvl: usize as i32,
+        rope: usize as i32,
+        n_positions: usize as i32,
+        page_tokens: usize as i32,
+        n_pages: usize as i32,
+        eps: f32,
+        half: i32,
+        bf16: i32,
+        bad_tokens: *mut u32,
+        stream: *mut c_void,
+    );
+
     /// Element codecs as launchers (what formats.hpp:42-57,99-106 and fwd.hip:20-45 are to the
     /// reference's kernels), for census tests of the device codecs on arbitrary inputs:
     /// e4m3_encode: out[i] = f32_to_e4m3(x[i]) (rule of crates/core/src/num.rs:128-152)

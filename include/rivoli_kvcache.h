@@ -594,6 +594,37 @@ int rivoli_index_commit_paged(unsigned short* kpool, const int* block_table, con
                               int page_tokens, int n_pages, int n_layers, long long layer_keys, int* new_lens,
                               unsigned int* bad_rows, void* stream);
 
+/* ---- a token's rows before they are cached or attended with: norm and rotation in one pass. Neither call has a counterpart in the
+ * reference, whose norms are kernels of the engine. ---- */
+
+/* Every head of every token: its first norm_n values become (x - c) / sqrt(mean of (x - c)^2 + eps) * weight + bias, c their mean with
+ * center != 0, else 0 (weight and bias f32, weight_head_stride values apart from head to head, 0: the same for all; null: one, zero); then the rd values from rope_at on
+ * turn by the table's row of the token's position as rivoli_rope_rows turns them (rd 0: none, and table and positions are not read); the other
+ * values of `width` are copied. f32 throughout, rounded once. Token t's head h is at x + t * x_token_stride + h * x_head_stride and goes to
+ * out + r * out_token_stride + h * out_head_stride (strides in elements), r = t, or slots[t] where slots is not null: the paged index keys
+ * (out = kpool, out_token_stride = hd) with n_slots = n_pages * page_tokens. x_bf16, out_bf16 != 0: bf16 values, else f32. In place: out == x with the
+ * same strides and types, no slots; other overlaps, and a slot twice, are outside the contract. A token whose slot is negative is left out (padding); one whose slot is
+ * n_slots or more, or whose position is not in [0, n_positions), is left out and counted once in *bad_tokens when non-null.
+ * Rows of whole 16-byte pieces (addresses, strides; width, norm_n, rope_at and rd multiples of 8, half: rd of 16) go 16 bytes a lane, others by ones.
+ * Guards: 1001 null / non-positive (rope_at, rd, weight_head_stride: negative; eps negative or not finite); 1002 width > 1024, norm_n or rope_at + rd > width, more rows
+ * than a launch has; 1004 odd rd, table not 8-byte aligned, rows, weight or bias not on an element. */
+int rivoli_norm_rope_rows(const void* x, void* out, const float* weight, const float* bias, const float* table,
+                          const int* positions, const int* slots, int n_tokens, int n_heads, int width, int norm_n,
+                          int rope_at, int rd, int n_positions, int n_slots, long long x_token_stride,
+                          long long x_head_stride, long long out_token_stride, long long out_head_stride,
+                          long long weight_head_stride, float eps, int center, int half, int x_bf16, int out_bf16,
+                          unsigned int* bad_tokens, void* stream);
+
+/* rivoli_kv_append_paged of rows that are normed and rotated on the way: of each of the rows x + t * x_stride (kvl + rope values, bf16 != 0: bf16, else
+ * f32) the first kvl are normed (as above, without mean and bias), the other `rope` turned by the table's row of positions[t]; scale = amax / 448 (1 where amax is 0) and codes by
+ * the append's rule, of the f32 values, to slot_mapping[t]. Slots and positions count as above; two tokens of one slot are outside the contract. Guards: 1001 null (weight
+ * may be) / non-positive; 1002 kvl + rope > 1024, n_tokens > 2^28; 1004 kvl + rope not a multiple of 16, kvl of 8, rope of 8 (half: 16), page_tokens of 4,
+ * x, x_stride or pool not on 16 bytes, table not on 8, weight not on 4. */
+int rivoli_kv_norm_append_paged(const void* x, const int* slot_mapping, const float* weight, const float* table,
+                                const int* positions, unsigned char* pool, int n_tokens, long long x_stride, int kvl,
+                                int rope, int n_positions, int page_tokens, int n_pages, float eps, int half, int bf16,
+                                unsigned int* bad_tokens, void* stream);
+
 /* Element codecs as launchers (what formats.hpp:42-57,99-106 and fwd.hip:20-45 are to the
  * reference's kernels), for census tests of the device codecs on arbitrary inputs:
  *   e4m3_encode: out[i] = f32_to_e4m3(x[i])            (rule of crates/core/src/num.rs:128-152)

@@ -75,6 +75,8 @@ RIVOLI_LAUNCHER(launch_attend_tree_paged, rivoli_mla_attend_tree_paged, "mla_att
 RIVOLI_LAUNCHER(launch_draft_verify, rivoli_draft_verify, "draft_verify")
 RIVOLI_LAUNCHER(launch_kv_commit_paged, rivoli_kv_commit_paged, "kv_commit_paged")
 RIVOLI_LAUNCHER(launch_index_commit_paged, rivoli_index_commit_paged, "index_commit_paged")
+RIVOLI_LAUNCHER(launch_norm_rope_rows, rivoli_norm_rope_rows, "norm_rope_rows")
+RIVOLI_LAUNCHER(launch_kv_norm_append_paged, rivoli_kv_norm_append_paged, "kv_norm_append_paged")
 RIVOLI_LAUNCHER(launch_codec_e4m3_encode, rivoli_codec_e4m3_encode, "codec_e4m3_encode")
 RIVOLI_LAUNCHER(launch_codec_e4m3_dequant_bf16, rivoli_codec_e4m3_dequant_bf16, "codec_e4m3_dequant_bf16")
 RIVOLI_LAUNCHER(launch_codec_bf16_encode, rivoli_codec_bf16_encode, "codec_bf16_encode")

@@ -1,0 +1,430 @@
+// Norm and rotation of a token's rows in one pass: of query and key heads into rows or into the paged index keys, and
+// of the latent row into its page as codes. Launch-only.
+//
+// A row's first norm_n values become (x - c) * r * w + b, r = 1 / sqrt(mean of (x - c)^2 + eps), c their mean (or zero); then
+// the pairs of its rd values from rope_at on turn by the table's row of the token's position, (x, y) -> (x c - y s, x s + y c);
+// the others are copied. Sums, statistics and values are f32 from the load to the one rounding at the store: in two
+// calls the normed values were rounded, written and read again in between.
+#include <cfloat>
+#include <cmath>
+
+#include "codec.hpp"
+
+namespace rk {
+
+struct NormRopeArgs {
+    const void* x;
+    void* out;
+    const float *weight, *bias, *table;
+    const int *positions, *slots;
+    int n_tokens, n_heads, groups;  // of heads: head g, g + groups, ...
+    int width, norm_n, rope_at, rd, n_positions;
+    long long n_slots;
+    long long x_token, x_head, out_token, out_head, weight_head;  // in elements
+    float eps;
+    int center, half;
+    int lanes_log2;                 // of a row
+    unsigned int* bad;
+};
+
+typedef float f32x4n __attribute__((ext_vector_type(4)));
+
+// Eight values of a row that starts on 16 bytes, or of f32 numbers that start anywhere.
+__device__ __forceinline__ void load8(const __bf16* src, float (&v)[8]) {
+    const u32x4 w = *reinterpret_cast<const u32x4*>(src);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[2 * i] = bf16_lo_to_f32(w[i]), v[2 * i + 1] = bf16_hi_to_f32(w[i]);
+}
+__device__ __forceinline__ void load8(const float* src, float (&v)[8]) {
+    typedef f32x4n any __attribute__((aligned(4)));
+    const f32x4n a = *reinterpret_cast<const any*>(src), b = *reinterpret_cast<const any*>(src + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
+}
+__device__ __forceinline__ void store8(__bf16* dst, const float (&v)[8]) {
+    *reinterpret_cast<u32x4*>(dst) = u32x4{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
+}
+__device__ __forceinline__ void store8(float* dst, const float (&v)[8]) {
+    *reinterpret_cast<f32x4n*>(dst) = f32x4n{v[0], v[1], v[2], v[3]};
+    *reinterpret_cast<f32x4n*>(dst + 4) = f32x4n{v[4], v[5], v[6], v[7]};
+}
+
+// A row's values, eight a lane and step: unit u = lane + 64 s of the row's (a row of up to 512 values has 2^lanes_log2 lanes and one step).
+// What is summed over a row stays within its lanes.
+__device__ __forceinline__ float row_sum(float x, int lanes_log2) {
+    for (int k = 0; k < lanes_log2; ++k) x += __shfl_xor(x, 1 << k, kWave);
+    return x;
+}
+
+struct NormRopeRow {
+    int norm_n, rope_at, rd, center, half, lanes_log2;
+    float eps;
+};
+
+template <int S>
+__device__ __forceinline__ void norm_row(const NormRopeRow& p, int lane, float (&v)[S][8], const float (&w)[S][8], const float (&b)[S][8]) {
+    const float n = (float)p.norm_n;
+    float c = 0.0f;
+    if (p.center) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+            if (8 * (lane + kWave * s) < p.norm_n) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sum += v[s][i];
+            }
+        c = row_sum(sum, p.lanes_log2) / n;
+    }
+    float sum = 0.0f;
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+        if (8 * (lane + kWave * s) < p.norm_n) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[s][i] -= c, sum = __builtin_fmaf(v[s][i], v[s][i], sum);
+        }
+    const float r = 1.0f / sqrtf(row_sum(sum, p.lanes_log2) / n + p.eps);
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+        if (8 * (lane + kWave * s) < p.norm_n) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[s][i] = __builtin_fmaf(v[s][i] * r, w[s][i], b[s][i]);
+        }
+}
+
+// Every lane of the row must be here: halves that belong together are in other lanes.
+template <int S>
+__device__ __forceinline__ void rotate_row(const NormRopeRow& p, int lane, float (&v)[S][8], const float (&turn)[S][16]) {
+    if (!p.half) {
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            const int o = 8 * (lane + kWave * s) - p.rope_at;
+            if (o >= 0 && o < p.rd) {
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) {
+                    const float x = v[s][i], y = v[s][i + 1], c = turn[s][i], n = turn[s][i + 1];
+                    v[s][i] = x * c - y * n, v[s][i + 1] = x * n + y * c;
+                }
+            }
+        }
+        return;
+    }
+    const int apart = p.rd / 16;  // units
+    float other[S][8];
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+        const int unit = lane + kWave * s, o = 8 * unit - p.rope_at;
+        const int from = 2 * o < p.rd ? unit + apart : unit - apart;  // (of no matter where nothing is rotated)
+        const int at = (int)(threadIdx.x & 63) - lane + (from & (S == 1 ? (1 << p.lanes_log2) - 1 : kWave - 1));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            other[s][i] = __shfl(v[0][i], at, kWave);
+            if constexpr (S > 1) {
+                const float more = __shfl(v[1][i], at, kWave);
+                if (from >= kWave) other[s][i] = more;
+            }
+        }
+    }
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+        const int o = 8 * (lane + kWave * s) - p.rope_at;
+        if (o >= 0 && o < p.rd) {
+            const bool first = 2 * o < p.rd;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float c = turn[s][2 * i], n = turn[s][2 * i + 1];
+                v[s][i] = first ? v[s][i] * c - other[s][i] * n : other[s][i] * n + v[s][i] * c;
+            }
+        }
+    }
+}
+
+// The lane's part of the table's row: four pairs, or the eight of a half.
+template <int S>
+__device__ __forceinline__ void turns_of(const NormRopeRow& p, const float* row, int lane, float (&turn)[S][16]) {
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+        const int o = 8 * (lane + kWave * s) - p.rope_at;
+        if (o < 0 || o >= p.rd) continue;
+        float a[8];
+        if (p.half) {
+            const float* const from = row + 2 * (2 * o < p.rd ? o : o - p.rd / 2);
+            float b[8];
+            load8(from, a), load8(from + 8, b);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) turn[s][i] = a[i], turn[s][8 + i] = b[i];
+        } else {
+            load8(row + o, a);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) turn[s][i] = a[i];
+        }
+    }
+}
+
+template <int S>
+__device__ __forceinline__ void weights_of(const NormRopeRow& p, const float* from, float otherwise, int lane, float (&w)[S][8]) {
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+        const int at = 8 * (lane + kWave * s);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[s][i] = otherwise;
+        if (from && at < p.norm_n) load8(from + at, w[s]);
+    }
+}
+
+// Rows of whole 16-byte pieces. A row's lanes have it in S steps; HEADS of them go through at once, so that their loads are on their way
+// together and the weights and the table's row serve them all.
+template <class TX, class TO, int S, int HEADS>
+__global__ __launch_bounds__(256) void norm_rope_rows_kernel(const NormRopeArgs a) {
+    const unsigned long long at = blockIdx.x * 256ull + threadIdx.x;
+    const unsigned item = (unsigned)(at >> a.lanes_log2);
+    const int lane = (int)(at & ((1u << a.lanes_log2) - 1));
+    const unsigned token_of = item / (unsigned)a.groups;
+    const int h0 = (int)(item - token_of * (unsigned)a.groups);
+    const bool past = token_of >= (unsigned)a.n_tokens;  // (a wave's rows stay together)
+    const int token = past ? 0 : (int)token_of;
+    const NormRopeRow p{a.norm_n, a.rope_at, a.rd, a.center, a.half, a.lanes_log2, a.eps};
+    const TX* const x = static_cast<const TX*>(a.x) + (long long)token * a.x_token;
+    float v[HEADS][S][8];
+#pragma unroll
+    for (int k = 0; k < HEADS; ++k)
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            const int unit = 8 * (lane + kWave * s);
+            // (a head past the last re-reads the last)
+            if (unit < a.width) load8(x + (long long)min(h0 + k * a.groups, a.n_heads - 1) * a.x_head + unit, v[k][s]);
+            else
+                for (int i = 0; i < 8; ++i) v[k][s][i] = 0.0f;
+        }
+    const int pos = a.rd ? a.positions[token] : 0;
+    const int slot = a.slots ? a.slots[token] : token;
+    const bool bad = (a.rd && (unsigned)pos >= (unsigned)a.n_positions) || (a.slots && slot >= a.n_slots);
+    const bool skip = past || bad || slot < 0;
+    if (!past && bad && slot >= 0 && a.bad && lane == 0 && h0 == 0) atomicAdd(a.bad, 1u);
+    float turn[S][16], w[S][8], b[S][8];
+    if (a.rd) turns_of<S>(p, a.table + (size_t)(skip ? 0 : pos) * a.rd, lane, turn);
+    if (a.weight_head == 0) weights_of<S>(p, a.weight, 1.0f, lane, w), weights_of<S>(p, a.bias, 0.0f, lane, b);
+    TO* const out = static_cast<TO*>(a.out) + (long long)slot * a.out_token;
+#pragma unroll
+    for (int k = 0; k < HEADS; ++k) {
+        const int h = h0 + k * a.groups;
+        if (a.weight_head != 0) {
+            const long long of = (long long)min(h, a.n_heads - 1) * a.weight_head;
+            weights_of<S>(p, a.weight ? a.weight + of : nullptr, 1.0f, lane, w);
+            weights_of<S>(p, a.bias ? a.bias + of : nullptr, 0.0f, lane, b);
+        }
+        norm_row<S>(p, lane, v[k], w, b);
+        if (a.rd) rotate_row<S>(p, lane, v[k], turn);
+        if (skip || h >= a.n_heads) continue;
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            const int unit = 8 * (lane + kWave * s);
+            if (unit < a.width) store8(out + (long long)h * a.out_head + unit, v[k][s]);
+        }
+    }
+}
+
+// Rows that start or end off the 16 bytes: a wave a row, its values by ones through LDS.
+constexpr int kNormWidth = 1024;
+template <class TX, class TO>
+__global__ __launch_bounds__(kWave) void norm_rope_any_kernel(const NormRopeArgs a) {
+    __shared__ float row[kNormWidth];
+    const int lane = threadIdx.x;
+    const unsigned token = blockIdx.x / (unsigned)a.n_heads;
+    const int h = (int)(blockIdx.x - token * (unsigned)a.n_heads);
+    const int pos = a.rd ? a.positions[token] : 0;
+    const long long slot = a.slots ? a.slots[token] : (int)token;
+    const bool bad = (a.rd && (unsigned)pos >= (unsigned)a.n_positions) || (a.slots && slot >= a.n_slots);
+    if (bad || slot < 0) {
+        if (bad && slot >= 0 && a.bad && lane == 0 && h == 0) atomicAdd(a.bad, 1u);
+        return;
+    }
+    const TX* const x = static_cast<const TX*>(a.x) + (long long)token * a.x_token + (long long)h * a.x_head;
+    TO* const out = static_cast<TO*>(a.out) + slot * a.out_token + (long long)h * a.out_head;
+    const float n = (float)a.norm_n;
+    float sum = 0.0f, squares = 0.0f;
+    for (int i = lane; i < a.width; i += kWave) {
+        const float v = (float)x[i];
+        row[i] = v;
+        sum += i < a.norm_n ? v : 0.0f;
+    }
+    const float c = a.center ? row_sum(sum, 6) / n : 0.0f;
+    for (int i = lane; i < a.norm_n; i += kWave) {
+        const float v = row[i] - c;
+        squares = __builtin_fmaf(v, v, squares);
+    }
+    const float r = 1.0f / sqrtf(row_sum(squares, 6) / n + a.eps);
+    const long long of = (long long)h * a.weight_head;
+    for (int i = lane; i < a.norm_n; i += kWave)
+        row[i] = __builtin_fmaf((row[i] - c) * r, a.weight ? a.weight[of + i] : 1.0f, a.bias ? a.bias[of + i] : 0.0f);
+    __syncthreads();
+    for (int i = lane; i < a.width; i += kWave) {
+        const int o = i - a.rope_at, apart = a.rd / 2;
+        float v = row[i];
+        if (o >= 0 && o < a.rd) {
+            const bool first = a.half ? o < apart : o % 2 == 0;
+            const float y = row[first ? i + (a.half ? apart : 1) : i - (a.half ? apart : 1)];
+            const f32x2 turn = reinterpret_cast<const f32x2*>(a.table)[(size_t)pos * apart + (a.half ? (first ? o : o - apart) : o / 2)];
+            v = first ? v * turn.x - y * turn.y : y * turn.y + v * turn.x;
+        }
+        out[i] = (TO)v;
+    }
+}
+
+template <class TX, class TO>
+static int norm_rope_rows(NormRopeArgs& a, bool wide, hipStream_t st) {
+    (void)hipGetLastError();
+    if (!wide) {
+        const unsigned long long rows = (unsigned long long)a.n_tokens * a.n_heads;
+        if (rows > kLaunchThreads / kWave) return 1002;
+        launch_kernel(norm_rope_any_kernel<TX, TO>, dim3((unsigned)rows), dim3(kWave), 0, st, a);
+        return launch_status();
+    }
+    const int units = a.width / 8, steps = units > kWave ? 2 : 1;
+    a.lanes_log2 = 0;
+    while (a.lanes_log2 < 6 && 1 << a.lanes_log2 < units) ++a.lanes_log2;
+    const bool many = steps == 1 && a.n_heads >= 4;
+    a.groups = many ? (a.n_heads + 3) / 4 : a.n_heads;
+    const unsigned long long per_token = (unsigned long long)a.groups << a.lanes_log2;
+    if (per_token > kLaunchThreads || (unsigned long long)a.n_tokens > kLaunchThreads / per_token) return 1002;
+    const dim3 grid((unsigned)((a.n_tokens * per_token + 255) / 256)), block(256);
+    if (steps == 2) launch_kernel(norm_rope_rows_kernel<TX, TO, 2, 1>, grid, block, 0, st, a);
+    else if (many) launch_kernel(norm_rope_rows_kernel<TX, TO, 1, 4>, grid, block, 0, st, a);
+    else launch_kernel(norm_rope_rows_kernel<TX, TO, 1, 1>, grid, block, 0, st, a);
+    return launch_status();
+}
+
+// ---- the latent row into its page -----------------------------------------------------------------------------
+// A wave a token: the row is normed over its latent values and rotated over the others as above, its largest value makes the scale, and the codes
+// are of the f32 values (rivoli_kv_append_paged's rule, whose rows come rounded to bf16 once more).
+struct NormAppendArgs {
+    const void* x;
+    const int* slots;
+    const float *weight, *table;
+    const int* positions;
+    uint8_t* pool;
+    int n_tokens, width, page_tokens, n_positions;
+    long long x_stride, n_slots;
+    size_t page_bytes;
+    NormRopeRow row;
+    unsigned int* bad;
+};
+
+// Eight codes of values under a scale. The quotient is a product by the reciprocal, corrected by its residual; the hardware's conversion has the
+// rule's result but below 2^-6, where the rule rounds halves away.
+__device__ __forceinline__ u32x2 codes8(const float (&v)[8], float scl, float rinv) {
+    float q[8];
+    bool plain = row_scale_is_fast(scl);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float q0 = v[i] * rinv;
+        q[i] = __builtin_fmaf(-__builtin_fmaf(q0, scl, -v[i]), rinv, q0);
+        plain &= e4m3_hw_exact_domain(q[i]);
+    }
+    if (plain) return u32x2{e4m3x4_hw(q[0], q[1], q[2], q[3]), e4m3x4_hw(q[4], q[5], q[6], q[7])};
+    uint32_t lo = 0, hi = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        lo |= f32_to_e4m3_sw(v[i] / scl) << (8 * i);
+        hi |= f32_to_e4m3_sw(v[4 + i] / scl) << (8 * i);
+    }
+    return u32x2{lo, hi};
+}
+
+template <class TX, int S>
+__global__ __launch_bounds__(256) void kv_norm_append_kernel(const NormAppendArgs a) {
+    const int lane = threadIdx.x & 63;
+    const unsigned token = blockIdx.x * 4u + (threadIdx.x >> 6);
+    if (token >= (unsigned)a.n_tokens) return;
+    const TX* const x = static_cast<const TX*>(a.x) + (long long)token * a.x_stride;
+    float v[S][8], w[S][8], b[S][8], turn[S][16];
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+        const int unit = 8 * (lane + kWave * s);
+        if (unit < a.width) load8(x + unit, v[s]);
+        else
+            for (int i = 0; i < 8; ++i) v[s][i] = 0.0f;
+    }
+    weights_of<S>(a.row, a.weight, 1.0f, lane, w), weights_of<S>(a.row, nullptr, 0.0f, lane, b);
+    const int slot = a.slots[token], pos = a.positions[token];
+    if (slot < 0) return;
+    if (slot >= a.n_slots || (unsigned)pos >= (unsigned)a.n_positions) {
+        if (a.bad && lane == 0) atomicAdd(a.bad, 1u);
+        return;
+    }
+    turns_of<S>(a.row, a.table + (size_t)pos * a.row.rd, lane, turn);
+    norm_row<S>(a.row, lane, v, w, b);
+    rotate_row<S>(a.row, lane, v, turn);
+    float top = 0.0f;
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[s][i]));
+    top = wave_max(top);
+    const float scl = top > 0.0f ? top / 448.0f : 1.0f, rinv = 1.0f / scl;
+    const int page = slot / a.page_tokens, off = slot - page * a.page_tokens;
+    uint8_t* const pg = a.pool + (size_t)page * a.page_bytes;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+        const int unit = 8 * (lane + kWave * s);
+        if (unit < a.width) *reinterpret_cast<u32x2*>(pg + (size_t)off * a.width + unit) = codes8(v[s], scl, rinv);
+    }
+    if (lane == 0) *reinterpret_cast<float*>(pg + (size_t)a.page_tokens * a.width + 4 * (size_t)off) = scl;
+}
+
+}  // namespace rk
+
+extern "C" int rivoli_norm_rope_rows(const void* x, void* out, const float* weight, const float* bias, const float* table,
+                                     const int* positions, const int* slots, int n_tokens, int n_heads, int width, int norm_n,
+                                     int rope_at, int rd, int n_positions, int n_slots, long long x_token_stride,
+                                     long long x_head_stride, long long out_token_stride, long long out_head_stride,
+                                     long long weight_head_stride, float eps, int center, int half, int x_bf16, int out_bf16,
+                                     unsigned int* bad_tokens, void* stream) {
+    if (!x || !out || n_tokens <= 0 || n_heads <= 0 || width <= 0 || norm_n <= 0 || rope_at < 0 || rd < 0 || weight_head_stride < 0) return 1001;
+    if (rd > 0 && (!table || !positions || n_positions <= 0)) return 1001;
+    if (slots && n_slots <= 0) return 1001;
+    if (!(eps >= 0.0f && eps <= FLT_MAX)) return 1001;
+    if (width > rk::kNormWidth || norm_n > width || (long long)rope_at + rd > width) return 1002;
+    const uintptr_t x_size = x_bf16 ? 2 : 4, out_size = out_bf16 ? 2 : 4;
+    if (rd % 2 != 0 || (rd > 0 && (uintptr_t)table % 8 != 0) || (uintptr_t)x % x_size != 0 || (uintptr_t)out % out_size != 0 ||
+        (uintptr_t)weight % 4 != 0 || (uintptr_t)bias % 4 != 0)
+        return 1004;
+    // whole 16-byte pieces from 16-byte boundaries, in every row, and no pair, and no border, inside of a lane's eight values
+    const long long xu = 16 / (long long)x_size, ou = 16 / (long long)out_size;
+    const bool wide = rk::aligned16(x) && rk::aligned16(out) && x_token_stride % xu == 0 && x_head_stride % xu == 0 && out_token_stride % ou == 0 &&
+                      out_head_stride % ou == 0 && width % 8 == 0 && norm_n % 8 == 0 && rope_at % 8 == 0 && rd % (half ? 16 : 8) == 0;
+    rk::NormRopeArgs a{x, out, weight, bias, table, positions, slots, n_tokens, n_heads, 0, width, norm_n, rope_at, rd, n_positions, n_slots,
+                       x_token_stride, x_head_stride, out_token_stride, out_head_stride, weight || bias ? weight_head_stride : 0, eps, center, half, 0,
+                       bad_tokens};
+    const hipStream_t st = (hipStream_t)stream;
+    if (x_bf16) return out_bf16 ? rk::norm_rope_rows<__bf16, __bf16>(a, wide, st) : rk::norm_rope_rows<__bf16, float>(a, wide, st);
+    return out_bf16 ? rk::norm_rope_rows<float, __bf16>(a, wide, st) : rk::norm_rope_rows<float, float>(a, wide, st);
+}
+
+extern "C" int rivoli_kv_norm_append_paged(const void* x, const int* slot_mapping, const float* weight, const float* table,
+                                           const int* positions, unsigned char* pool, int n_tokens, long long x_stride, int kvl,
+                                           int rope, int n_positions, int page_tokens, int n_pages, float eps, int half, int bf16,
+                                           unsigned int* bad_tokens, void* stream) {
+    if (!x || !slot_mapping || !table || !positions || !pool || n_tokens <= 0 || kvl <= 0 || rope <= 0 || n_positions <= 0 || page_tokens <= 0 ||
+        n_pages <= 0 || !(eps >= 0.0f && eps <= FLT_MAX))
+        return 1001;
+    if ((long long)kvl + rope > rk::kNormWidth || n_tokens > 1 << 28) return 1002;
+    const int width = kvl + rope;
+    const long long unit = bf16 ? 8 : 4;
+    if (width % 16 != 0 || kvl % 8 != 0 || rope % (half ? 16 : 8) != 0 || page_tokens % 4 != 0 || x_stride % unit != 0 || !rk::aligned16(x) ||
+        !rk::aligned16(pool) || (uintptr_t)table % 8 != 0 || (uintptr_t)weight % 4 != 0)
+        return 1004;
+    const rk::NormAppendArgs a{x, slot_mapping, weight, table, positions, pool, n_tokens, width, page_tokens, n_positions, x_stride,
+                               (long long)n_pages * page_tokens, (size_t)page_tokens * (size_t)(width + 4),
+                               rk::NormRopeRow{kvl, kvl, rope, 0, half, 6, eps}, bad_tokens};
+    const dim3 grid((unsigned)((n_tokens + 3) / 4)), block(256);
+    const hipStream_t st = (hipStream_t)stream;
+    (void)hipGetLastError();
+    if (width > 512) {
+        if (bf16) rk::launch_kernel(rk::kv_norm_append_kernel<__bf16, 2>, grid, block, 0, st, a);
+        else rk::launch_kernel(rk::kv_norm_append_kernel<float, 2>, grid, block, 0, st, a);
+    } else {
+        if (bf16) rk::launch_kernel(rk::kv_norm_append_kernel<__bf16, 1>, grid, block, 0, st, a);
+        else rk::launch_kernel(rk::kv_norm_append_kernel<float, 1>, grid, block, 0, st, a);
+    }
+    return rk::launch_status();
+}

@@ -102,6 +102,8 @@ PyMethodDef kEntries[] = {
     ENTRY(rivoli_kv_compress_deposit), ENTRY(rivoli_kv_compress_prefill), ENTRY(rivoli_kv_compress_decode),
     ENTRY(rivoli_rope_table), ENTRY(rivoli_rope_rows), ENTRY(rivoli_mla_attend_tree_paged), ENTRY(rivoli_draft_verify),
     ENTRY(rivoli_kv_commit_paged), ENTRY(rivoli_index_commit_paged),
+    ENTRY(rivoli_norm_rope_rows),
+    ENTRY(rivoli_kv_norm_append_paged),
     ENTRY(rivoli_codec_e4m3_encode), ENTRY(rivoli_codec_e4m3_dequant_bf16), ENTRY(rivoli_codec_bf16_encode),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "pylaunch", nullptr, -1, kEntries, nullptr, nullptr, nullptr, nullptr};

@@ -82,6 +82,8 @@ _SIGNATURES = {
     "rivoli_draft_verify": [_VP] * 7 + [_I] * 4 + [_LL, _LL, _I] + [_VP] * 6,
     "rivoli_kv_commit_paged": [_VP] * 5 + [_I] * 7 + [_LL] + [_VP] * 3,
     "rivoli_index_commit_paged": [_VP] * 5 + [_I] * 7 + [_LL] + [_VP] * 3,
+    "rivoli_norm_rope_rows": [_VP] * 7 + [_I] * 8 + [_LL] * 5 + [_F] + [_I] * 4 + [_VP] * 2,
+    "rivoli_kv_norm_append_paged": [_VP] * 6 + [_I] + [_LL] + [_I] * 5 + [_F] + [_I] * 2 + [_VP] * 2,
     "rivoli_codec_e4m3_encode": [_VP, _VP, _LL, _VP],
     "rivoli_codec_e4m3_dequant_bf16": [_VP, _F, _VP, _LL, _VP],
     "rivoli_codec_bf16_encode": [_VP, _VP, _LL, _VP],
@@ -563,6 +565,28 @@ def launch_index_commit_paged(kpool, block_table, ctx_lens, path, n_path, n_seqs
     ensure_hip_status(entry.rivoli_index_commit_paged(
         kpool, block_table, ctx_lens, path, n_path, n_seqs, max_path, max_blocks_per_seq, hd, page_tokens, n_pages,
         n_layers, layer_keys, new_lens, bad_rows, stream), "index_commit_paged")
+
+
+# ---- a token's rows before they are cached or attended with -----------------------------------
+
+def launch_norm_rope_rows(x, out, weight, bias, table, positions, slots, n_tokens, n_heads, width, norm_n, rope_at, rd, n_positions,
+                          n_slots, x_token_stride, x_head_stride, out_token_stride, out_head_stride, weight_head_stride, eps, center,
+                          half, x_bf16, out_bf16, bad_tokens=None, stream=NULL_STREAM) -> None:
+    """Norms the first norm_n values of every head (center: around their mean), rotates rd of them from rope_at on by
+    the table's row of the token's position, and writes the row to its place or, with slots, to the
+    paged index keys."""
+    ensure_hip_status(entry.rivoli_norm_rope_rows(
+        x, out, weight, bias, table, positions, slots, n_tokens, n_heads, width, norm_n, rope_at, rd, n_positions, n_slots,
+        x_token_stride, x_head_stride, out_token_stride, out_head_stride, weight_head_stride, eps, 1 if center else 0,
+        1 if half else 0, 1 if x_bf16 else 0, 1 if out_bf16 else 0, bad_tokens, stream), "norm_rope_rows")
+
+
+def launch_kv_norm_append_paged(x, slot_mapping, weight, table, positions, pool, n_tokens, x_stride, kvl, rope, n_positions,
+                                page_tokens, n_pages, eps, half, bf16, bad_tokens=None, stream=NULL_STREAM) -> None:
+    """launch_kv_append_paged of rows whose latent part is normed and whose roped part is rotated on the way."""
+    ensure_hip_status(entry.rivoli_kv_norm_append_paged(
+        x, slot_mapping, weight, table, positions, pool, n_tokens, x_stride, kvl, rope, n_positions, page_tokens, n_pages, eps,
+        1 if half else 0, 1 if bf16 else 0, bad_tokens, stream), "kv_norm_append_paged")
 
 
 # ---- element codecs -----------------------------------------------------------------------
