@@ -617,6 +617,28 @@ launchers! {
         stream: *mut c_void,
     );
 
+    /// Tokens drawn from logits after temperature, top-k, top-p and min-p, by given random numbers.
+    /// See `include/rivoli_kvcache.h` for the full contract.
+    launch_sample_rows -> rivoli_sample_rows, "sample_rows" (
+        logits: *const c_void,
+        temperatures: *const f32,
+        top_ks: *const i32,
+        top_ps: *const f32,
+        min_ps: *const f32,
+        uniforms: *const f32,
+        n_rows: usize as i32,
+        vocab: usize as i32,
+        stride: i64,
+        bf16: i32,
+        tokens: *mut i32,
+        n_kept: *mut i32,
+        logprobs: *mut f32,
+        probs: *mut f32,
+        probs_stride: i64,
+        workspace: *mut c_void,
+        stream: *mut c_void,
+    );
+
     /// Element codecs as launchers (what formats.hpp:42-57,99-106 and fwd.hip:20-45 are to the
     /// reference's kernels), for census tests of the device codecs on arbitrary inputs:
     /// e4m3_encode: out[i] = f32_to_e4m3(x[i]) (rule of crates/core/src/num.rs:128-152)
@@ -668,6 +690,7 @@ unsafe extern "C" {
     fn rivoli_gather_attn_scratch_floats(m: i32, h: i32, d: i32, topk: i32) -> usize;
     fn rivoli_mla_attend_tree_paged_scratch_floats(n_seqs: i32, h: i32, n_nodes: i32, max_nodes: i32, max_ctx: i32) -> usize;
     fn rivoli_draft_verify_workspace_bytes(n_seqs: i32, max_nodes: i32, vocab: i32) -> usize;
+    fn rivoli_sample_rows_workspace_bytes(n_rows: i32, vocab: i32) -> usize;
 }
 
 /// Bytes of one page: `page_tokens * width` codes followed by `page_tokens` f32 scales.
@@ -706,6 +729,12 @@ pub fn attend_tree_paged_scratch_floats(n_seqs: usize, h: usize, n_nodes: usize,
 pub fn draft_verify_workspace_bytes(n_seqs: usize, max_nodes: usize, vocab: usize) -> usize {
     // SAFETY: pure host function, no pointers.
     unsafe { rivoli_draft_verify_workspace_bytes(n_seqs as i32, max_nodes as i32, vocab as i32) }
+}
+
+/// Bytes of the workspace `launch_sample_rows` wants for this shape (nothing to be cleared).
+pub fn sample_rows_workspace_bytes(n_rows: usize, vocab: usize) -> usize {
+    // SAFETY: pure host function, no pointers.
+    unsafe { rivoli_sample_rows_workspace_bytes(n_rows as i32, vocab as i32) }
 }
 
 /// Rows and columns of a selection rectangle, or the guard code `Sel::shape` would refuse with.

@@ -625,6 +625,22 @@ int rivoli_kv_norm_append_paged(const void* x, const int* slot_mapping, const fl
                                 int rope, int n_positions, int page_tokens, int n_pages, float eps, int half, int bf16,
                                 unsigned int* bad_tokens, void* stream);
 
+/* Tokens from logits by given random numbers in [0, 1), and the distributions that they were drawn from. Row r is logits + r * stride ([vocab], f32 or with bf16 != 0
+ * bf16; stride 0: all rows draw from one). Its tokens in order of their logits, the lower index first of equal ones; w_v = exp((x_v - max) / temperatures[r]). Kept are the first
+ * top_ks[r] of them (all when not positive); of those the shortest beginning whose weight reaches top_ps[r] of theirs (all when not below 1, one token when not positive); of those the ones
+ * whose w_v is min_ps[r] or more (the first always). The four arrays may each be null: temperature 1, all kept. tokens[r] = the first v, by index, whose running sum
+ * of kept weights exceeds uniforms[r] times their whole (the last kept one when none does). A temperature that is not positive takes the first in the order, whatever is kept of it. Logits that are NaN or -inf
+ * are never drawn nor kept, +inf counts as FLT_MAX; a row without any other gets token -1. n_kept[r] (nullable) = how many are kept, logprobs[r] (nullable) = the logarithm
+ * of the token's share of their weight (-inf without a token), probs (nullable) + r * probs_stride = every token's share, zero for those not kept: what rivoli_draft_verify takes. Weights and sums have 42 bits below
+ * the largest weight or more; what is kept and drawn does not depend on any order of sums: equal calls give equal results.
+ * `workspace`: rivoli_sample_rows_workspace_bytes(n_rows, vocab) bytes, 16-byte aligned, nothing to be cleared; two calls in flight need one each. Guards: 1001 null / non-positive; 1002 n_rows >= 2^22,
+ * vocab > 2^21 or above a stride, more rows than a launch has; 1004 rows not on an element, workspace not 16-byte aligned. */
+size_t rivoli_sample_rows_workspace_bytes(int n_rows, int vocab);
+int rivoli_sample_rows(const void* logits, const float* temperatures, const int* top_ks, const float* top_ps,
+                       const float* min_ps, const float* uniforms, int n_rows, int vocab, long long stride, int bf16,
+                       int* tokens, int* n_kept, float* logprobs, float* probs, long long probs_stride, void* workspace,
+                       void* stream);
+
 /* Element codecs as launchers (what formats.hpp:42-57,99-106 and fwd.hip:20-45 are to the
  * reference's kernels), for census tests of the device codecs on arbitrary inputs:
  *   e4m3_encode: out[i] = f32_to_e4m3(x[i])            (rule of crates/core/src/num.rs:128-152)

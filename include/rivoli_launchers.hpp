@@ -77,6 +77,7 @@ RIVOLI_LAUNCHER(launch_kv_commit_paged, rivoli_kv_commit_paged, "kv_commit_paged
 RIVOLI_LAUNCHER(launch_index_commit_paged, rivoli_index_commit_paged, "index_commit_paged")
 RIVOLI_LAUNCHER(launch_norm_rope_rows, rivoli_norm_rope_rows, "norm_rope_rows")
 RIVOLI_LAUNCHER(launch_kv_norm_append_paged, rivoli_kv_norm_append_paged, "kv_norm_append_paged")
+RIVOLI_LAUNCHER(launch_sample_rows, rivoli_sample_rows, "sample_rows")
 RIVOLI_LAUNCHER(launch_codec_e4m3_encode, rivoli_codec_e4m3_encode, "codec_e4m3_encode")
 RIVOLI_LAUNCHER(launch_codec_e4m3_dequant_bf16, rivoli_codec_e4m3_dequant_bf16, "codec_e4m3_dequant_bf16")
 RIVOLI_LAUNCHER(launch_codec_bf16_encode, rivoli_codec_bf16_encode, "codec_bf16_encode")
@@ -112,6 +113,7 @@ inline size_t attend_tree_paged_scratch_floats(int n_seqs, int H, int n_nodes, i
 inline size_t draft_verify_workspace_bytes(int n_seqs, int max_nodes, int vocab) {
     return rivoli_draft_verify_workspace_bytes(n_seqs, max_nodes, vocab);
 }
+inline size_t sample_rows_workspace_bytes(int n_rows, int vocab) { return rivoli_sample_rows_workspace_bytes(n_rows, vocab); }
 
 }  // namespace rivoli
 

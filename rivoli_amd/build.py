@@ -19,7 +19,7 @@ LAUNCH_PATH = os.path.join(CSRC, "pylaunch.so")
 KERNELS = ["kv_append.hip", "kv_gather.hip", "index_topk.hip", "index_score.hip", "mla_attend.hip",
            "act_quant.hip", "kv_compress.hip", "kv_ring.hip", "gather_attn.hip", "hash_rows.hip",
            "block_index.hip", "rope.hip", "mla_attend_tree.hip", "draft_verify.hip", "kv_commit.hip",
-           "norm_rope.hip"]
+           "norm_rope.hip", "sample.hip"]
 # Matrix-instruction results in ordinary registers: the 8-bit attention kernel keeps its 128
 # accumulators there and its q terms in the accumulation registers (mla_attend_f8.hpp); the bf16
 # kernels of the same file time the same either way.

@@ -84,6 +84,7 @@ _SIGNATURES = {
     "rivoli_index_commit_paged": [_VP] * 5 + [_I] * 7 + [_LL] + [_VP] * 3,
     "rivoli_norm_rope_rows": [_VP] * 7 + [_I] * 8 + [_LL] * 5 + [_F] + [_I] * 4 + [_VP] * 2,
     "rivoli_kv_norm_append_paged": [_VP] * 6 + [_I] + [_LL] + [_I] * 5 + [_F] + [_I] * 2 + [_VP] * 2,
+    "rivoli_sample_rows": [_VP] * 6 + [_I] * 2 + [_LL] + [_I] + [_VP] * 4 + [_LL] + [_VP] * 2,
     "rivoli_codec_e4m3_encode": [_VP, _VP, _LL, _VP],
     "rivoli_codec_e4m3_dequant_bf16": [_VP, _F, _VP, _LL, _VP],
     "rivoli_codec_bf16_encode": [_VP, _VP, _LL, _VP],
@@ -99,6 +100,7 @@ _SIZE_SIGNATURES = {
     "rivoli_gather_attn_scratch_floats": [_I, _I, _I, _I],
     "rivoli_mla_attend_tree_paged_scratch_floats": [_I] * 5,
     "rivoli_draft_verify_workspace_bytes": [_I] * 3,
+    "rivoli_sample_rows_workspace_bytes": [_I] * 2,
 }
 
 
@@ -587,6 +589,21 @@ def launch_kv_norm_append_paged(x, slot_mapping, weight, table, positions, pool,
     ensure_hip_status(entry.rivoli_kv_norm_append_paged(
         x, slot_mapping, weight, table, positions, pool, n_tokens, x_stride, kvl, rope, n_positions, page_tokens, n_pages, eps,
         1 if half else 0, 1 if bf16 else 0, bad_tokens, stream), "kv_norm_append_paged")
+
+
+# ---- from logits to tokens ----------------------------------------------------------------------
+
+def sample_rows_workspace_bytes(n_rows: int, vocab: int) -> int:
+    return int(lib().rivoli_sample_rows_workspace_bytes(n_rows, vocab))
+
+
+def launch_sample_rows(logits, temperatures, top_ks, top_ps, min_ps, uniforms, n_rows, vocab, stride, bf16, tokens, n_kept=None,
+                       logprobs=None, probs=None, probs_stride=0, workspace=None, stream=NULL_STREAM) -> None:
+    """Draws a token of every row by its given random number, after temperature, top-k, top-p and min-p (arrays
+    by row, each may be None); probs: the rows that launch_draft_verify takes."""
+    ensure_hip_status(entry.rivoli_sample_rows(
+        logits, temperatures, top_ks, top_ps, min_ps, uniforms, n_rows, vocab, stride, 1 if bf16 else 0, tokens, n_kept, logprobs,
+        probs, probs_stride, workspace, stream), "sample_rows")
 
 
 # ---- element codecs -----------------------------------------------------------------------

@@ -34,3 +34,17 @@ def test_norm_append_refusals():
                 (dict(x_stride=578, bf16=False), 1004), (dict(x=B.data_ptr() + 8), 1004), (dict(pool=B.data_ptr() + 8), 1004),
                 (dict(table=B.data_ptr() + 4), 1004), (dict(weight=B.data_ptr() + 2), 1004)]
     refused(hip.launch_kv_norm_append_paged, good, changes)
+
+
+def test_sample_refusals():
+    good = dict(logits=B, temperatures=None, top_ks=None, top_ps=None, min_ps=None, uniforms=B, n_rows=1, vocab=32, stride=32, bf16=False, tokens=B,
+                n_kept=None, logprobs=None, probs=B, probs_stride=32, workspace=B)
+    changes = [(dict([(name, None)]), 1001) for name in ("logits", "uniforms", "tokens", "workspace")]
+    changes += [(dict([(name, 0)]), 1001) for name in ("n_rows", "vocab")]
+    changes += [(dict(n_rows=2 ** 22), 1002), (dict(vocab=2 ** 21 + 1, stride=2 ** 22, probs_stride=2 ** 22), 1002), (dict(stride=31), 1002),
+                (dict(stride=-32), 1002), (dict(probs_stride=31), 1002), (dict(n_rows=2 ** 22 - 1, vocab=2 ** 21, stride=2 ** 21, probs_stride=2 ** 21), 1002),
+                (dict(logits=B.data_ptr() + 2), 1004), (dict(logits=B.data_ptr() + 1, bf16=True), 1004), (dict(probs=B.data_ptr() + 2), 1004),
+                (dict(workspace=B.data_ptr() + 8), 1004)]
+    refused(hip.launch_sample_rows, good, changes)
+    assert hip.sample_rows_workspace_bytes(0, 32) == hip.sample_rows_workspace_bytes(4, 0) == hip.sample_rows_workspace_bytes(4, 2 ** 21 + 1) == 0
+    assert hip.sample_rows_workspace_bytes(4, 32) >= 4 * hip.sample_rows_workspace_bytes(1, 1) > 0
