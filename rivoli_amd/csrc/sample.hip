@@ -6,41 +6,49 @@
 // what is kept is known by its last token, the cut. The token drawn is the first, by index, whose running weight exceeds u times the whole of what is kept.
 //
 // Which tokens are kept and which one is drawn are decided by sums of up to 2^21 weights next to a border, so that weights and sums have more than 32 bits: over 131 072 tokens
-// sums in f32 would move a draw in some hundred. A weight is made in 64 bits to 10^-14 and summed as a whole number of 2^-42 of the largest (in a histogram 2^-36 of
+// sums in f32 would move a draw in some hundred. A weight is made in 64 bits and summed as a whole number of 2^-42 of the largest (in a histogram 2^-36 of
 // its bin's least), so that no sum depends on its order and equal calls give equal tokens.
 #include <cfloat>
+#include <climits>
 
 #include "codec.hpp"
 
 namespace rk {
 
-// Bins of a logit: of a power of two's width h, 16 to 32 of them to T, numbered on one grid for all of a row: x / h and the place in a bin are exact. Below a
-// chunk's largest logit's bin are kSampleBins of them in its histogram; what lies lower (e^-16 of it and less) is a tail, counted as a whole.
-constexpr int kSampleBins = 512;
+typedef unsigned long long u64;
+
+// Logits are binned on one grid for all of a row: bins of a power of two's width h, 16 to 32 of them to T, so that x / h, its bin and its place in the bin are exact in f32
+// (logits beyond 2^25 T count as that: bins have 31 bits). A histogram has some 250 bins from its top on (kFine; 8 T and more), then 256 of eight bins each, another 64 T; what lies
+// deeper weighs less than 2^-92 of the top and is a tail that is only counted. Eights begin at multiples of eight, in every histogram of a row, so that histograms
+// of unlike tops add up exactly: the finer ones' bins are parts of the coarser ones'.
+constexpr int kFine = 256, kSampleBins = 512;
 constexpr int kSampleThreads = 256, kSampleItems = 32;
 constexpr int kSampleChunk = kSampleThreads * kSampleItems;  // tokens a workgroup of the first launch
 constexpr int kSampleMaxVocab = 1 << 21, kSampleMaxChunks = kSampleMaxVocab / kSampleChunk;
-constexpr int kPickThreads = 1024, kPickWaves = kPickThreads / kWave;
+constexpr int kSampleList = 256;           // of a chunk's largest logits that are listed
+constexpr int kPickThreads = 512, kPickWaves = kPickThreads / kWave;
 constexpr int kPickList = 8192;            // tokens in LDS
 constexpr int kPickSubs = 2048, kPickFew = 256;
+constexpr int kCountedK = 2048;            // up to this k a row's histogram has counts alone
+constexpr float kLeastTemperature = 1.0f / 65536;  // up to it the largest logit is taken
 constexpr double kMassOne = 4398046511104.0;       // 2^42
 constexpr double kBinOne = 68719476736.0;          // 2^36
 constexpr double kWhole = 4503599627370496.0;      // 2^52: a number below it added to it is a whole number in its low bits
-constexpr unsigned long long kWholeBits = 0x4330000000000000ull;
-constexpr int kCountShift = 50;            // of a histogram's word: tokens above, their weight below (2^13 tokens of 2^36.1 at most)
-
-typedef unsigned long long u64;
+constexpr u64 kWholeBits = 0x4330000000000000ull;
+constexpr int kCountShift = 50;            // of a histogram's word: tokens above, their weight below (2^13 tokens of 2^36.8 at most)
+constexpr u64 kMassBits = (1ull << kCountShift) - 1;
 
 struct SampleChunk {
-    double top;                  // its largest logit's bin
-    u64 mass;                    // of all of its tokens, or, where there is a histogram, of the tail, in 2^-42 of the weight at that bin's beginning
+    u64 mass;                    // of a row without filters: all of its tokens', in 2^-42 of what its top bin's beginning weighs
+    int top, cover;              // its largest logit's bin; its tokens of bins from `cover` on are listed
     float most;                  // its largest logit
-    int first;                   // that one's token
-    unsigned count, tail;        // tokens that may be drawn, and of the tail
+    int first;                   // that one's token, in a row that takes the largest
+    unsigned count, listed;      // tokens that may be drawn; that are listed
 };
 struct SampleEnd {               // what the third launch writes a row's probabilities by
-    double top, inv;             // the row's top bin, 1 / the whole of what is kept
+    double inv;                  // 1 / the whole of what is kept
     u64 cut;                     // the last kept token's place in the order
+    int top;                     // the row's top bin
     int token, kind;             // kind: 0 nothing may be drawn, 1 one token, 2 by weight
 };
 struct SampleArgs {
@@ -52,60 +60,73 @@ struct SampleArgs {
     int *tokens, *n_kept;
     float *logprobs, *probs;
     SampleChunk* chunk;
-    u64* hist;                   // [rows][chunks][kSampleBins]
+    u64 *hist, *list;            // [rows][chunks][kSampleBins] (of counts alone: of 32 bits), [kSampleList] places
     SampleEnd* end;
 };
 
 struct SampleRow {
     bool greedy, k_on, p_on, m_on;
     int k;
-    double inv_h, a, p, m;       // a = h / T
+    float inv_h, most;           // 1 / h; logits count as at most this, and at least minus it
+    double a, p, m;              // a = h / T
     __device__ __forceinline__ bool filtered() const { return k_on || p_on || m_on; }
+    __device__ __forceinline__ bool weighed() const { return !k_on || k > kCountedK; }  // the histogram has weights
 };
 __device__ __forceinline__ SampleRow sample_row(const SampleArgs& a, int row) {
     SampleRow r;
     const float t = a.temperatures ? a.temperatures[row] : 1.0f;
-    r.greedy = !(t > 0.0f);
-    const double td = r.greedy ? 1.0 : (double)fminf(t, FLT_MAX);
-    const int e = ilogb(td) - 4;
-    r.inv_h = ldexp(1.0, -e), r.a = ldexp(1.0, e) / td;
+    r.greedy = !(t > kLeastTemperature);
+    const float tf = r.greedy ? 1.0f : fminf(t, FLT_MAX);
+    const int e = (int)((__float_as_uint(tf) >> 23) & 0xff) - 127 - 4;  // (tf is a normal number)
+    r.inv_h = __uint_as_float((uint32_t)(127 - e) << 23), r.most = fminf(tf * 33554432.0f, FLT_MAX);
+    r.a = 1.0 / ((double)tf * (double)r.inv_h);
     r.k = a.top_ks ? a.top_ks[row] : 0;
     r.p = a.top_ps ? (double)a.top_ps[row] : 1.0;
-    r.m = a.min_ps ? fmin((double)a.min_ps[row], 1.0) : 0.0;
-    if (r.p <= 0.0 || (a.min_ps && a.min_ps[row] > 1.0f)) r.k = 1;  // (the first token alone)
+    r.m = a.min_ps ? (double)a.min_ps[row] : 0.0;
+    if (r.p <= 0.0 || r.m > 1.0) r.k = 1;  // (the first token alone)
     r.k_on = r.k > 0 && r.k < a.vocab;
     r.p_on = r.p > 0.0 && r.p < 1.0;
-    r.m_on = r.m > 0.0;
+    r.m_on = r.m > 0.0 && r.m <= 1.0;
     return r;
 }
+// A logit as it counts: what is no number as -inf, which is never drawn; one zero.
+__device__ __forceinline__ float logit(const SampleRow& r, float x) { return x > -INFINITY ? __builtin_amdgcn_fmed3f(x, -r.most, r.most) + 0.0f : -INFINITY; }
 
-// A logit as it counts: what is no number as -inf, which is never drawn; infinity as the largest number; one zero.
-__device__ __forceinline__ float logit(float x) { return x != x ? -INFINITY : fminf(x, FLT_MAX) + 0.0f; }
-
-// The bin, and the weight over that of the bin's beginning: exp(y), 0 <= y < 1/16, to 6e-15 by its series.
-__device__ __forceinline__ double bin_of(const SampleRow& r, float x, double& weight) {
-    const double t = (double)x * r.inv_h, b = floor(t), y = (t - b) * r.a;
+// The least logit of a bin's, or of one between it and the next that there is.
+__device__ __forceinline__ float least_of(const SampleRow& r, int b) {
+    float t = (float)b;
+    if ((double)t < (double)b) t = __uint_as_float(__float_as_uint(t) + (t < 0.0f ? -1 : 1));
+    return t / r.inv_h;
+}
+__device__ __forceinline__ int bin_of(const SampleRow& r, float x) { return (int)floorf(x * r.inv_h); }
+// exp(place in the bin * a), or of a place in eight bins: arguments up to 1/16 to 2^-47, up to 1/2 to 2^-23.
+__device__ __forceinline__ double weight_in(const SampleRow& r, float place) {
+    const double y = (double)place * r.a;
     double s = 1.0 / 5040;
     s = __builtin_fma(s, y, 1.0 / 720), s = __builtin_fma(s, y, 1.0 / 120), s = __builtin_fma(s, y, 1.0 / 24);
     s = __builtin_fma(s, y, 1.0 / 6), s = __builtin_fma(s, y, 0.5), s = __builtin_fma(s, y, 1.0);
-    weight = __builtin_fma(s, y, 1.0);
-    return b;
+    return __builtin_fma(s, y, 1.0);
 }
+// A histogram by its top bin.
+struct SampleGrid {
+    int top, fine8;              // the least bin that is its own, an eighth of it
+    __device__ __forceinline__ explicit SampleGrid(int t) : top(t), fine8((t - 248) >> 3) {}
+    __device__ __forceinline__ int of(int b) const { return b >= 8 * fine8 ? top - b : min(kFine + fine8 - 1 - (b >> 3), kSampleBins); }
+    __device__ __forceinline__ int least(int i) const { return i < kFine ? max(top - i, 8 * fine8) : 8 * (fine8 - 1 - (i - kFine)); }  // of number i's bins (of some at the change, none)
+};
 // What a bin's beginning weighs, `down` bins below the top: exp(-a down) by two tables of 64.
 struct SampleTable {
     double fine[64], coarse[64];
-    __device__ __forceinline__ double of(double down) const {
-        const int g = (int)fmin(down, 4096.0);
-        return g >= 4096 ? 0.0 : fine[g & 63] * coarse[g >> 6];
-    }
+    __device__ __forceinline__ double of(int down) const { return (unsigned)down >= 4096u ? 0.0 : fine[down & 63] * coarse[down >> 6]; }
 };
 __device__ __forceinline__ void make_table(SampleTable& t, const SampleRow& r) {
-    if (threadIdx.x < 64) t.fine[threadIdx.x] = exp(-r.a * (double)threadIdx.x);
-    else if (threadIdx.x < 128) t.coarse[threadIdx.x - 64] = exp(-r.a * 64.0 * (double)(threadIdx.x - 64));
+    if (threadIdx.x < 128) {
+        const double v = exp(-r.a * (double)(threadIdx.x < 64 ? threadIdx.x : 64 * (threadIdx.x - 64)));
+        (threadIdx.x < 64 ? t.fine : t.coarse)[threadIdx.x & 63] = v;
+    }
 }
-__device__ __forceinline__ u64 whole(double x) { return __builtin_bit_cast(u64, x + kWhole) - kWholeBits; }  // x < 2^51
-__device__ __forceinline__ u64 mass_of(double weight) { return whole(weight * kMassOne); }
-// The same of a sum's product with a weight: up to 2^63.
+__device__ __forceinline__ u64 mass_of(double weight) { return __builtin_bit_cast(u64, __builtin_fma(weight, kMassOne, kWhole)) - kWholeBits; }
+// A sum of such numbers times a weight: up to 2^63.
 __device__ __forceinline__ u64 scaled(u64 mass, double by) { return (u64)((double)mass * by + 0.5); }
 
 // A token's place in the order, larger first: its logit's bits in order, then the lower index.
@@ -115,6 +136,10 @@ __device__ __forceinline__ u64 place_of(float x, unsigned index) {
     return ((u64)key << 21) | (kSampleMaxVocab - 1 - index);
 }
 __device__ __forceinline__ unsigned index_of(u64 place) { return kSampleMaxVocab - 1 - (unsigned)(place & (kSampleMaxVocab - 1)); }
+__device__ __forceinline__ float logit_of(u64 place) {
+    const uint32_t key = (uint32_t)(place >> 21);
+    return __uint_as_float(key ^ (key >> 31 ? 0x80000000u : 0xffffffffu));
+}
 
 // N tokens of a row from `at` on (bf16: eight, f32: four), those at `end` and past it as -inf. A row starts on an element.
 template <bool BF16>
@@ -137,7 +162,7 @@ struct Logits<true> {
             }
         }
     }
-    __device__ __forceinline__ float operator[](int i) const { return logit(i & 1 ? bf16_hi_to_f32(v[i >> 1]) : bf16_lo_to_f32(v[i >> 1])); }
+    __device__ __forceinline__ float operator[](int i) const { return i & 1 ? bf16_hi_to_f32(v[i >> 1]) : bf16_lo_to_f32(v[i >> 1]); }
 };
 template <>
 struct Logits<false> {
@@ -158,18 +183,30 @@ struct Logits<false> {
             }
         }
     }
-    __device__ __forceinline__ float operator[](int i) const { return logit(v[i]); }
+    __device__ __forceinline__ float operator[](int i) const { return v[i]; }
 };
 
-__device__ __forceinline__ u64 wave_sum(u64 x) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, kWave);
-    return x;
+// Sums and maxima over a wave, in every lane, by rotations within sixteen lanes and swaps of those rows: no trip through LDS, which a shuffle is.
+template <int CTRL>
+__device__ __forceinline__ u64 rotated64(u64 v) {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)v, CTRL, 0xf, 0xf, true), hi = (uint32_t)__builtin_amdgcn_mov_dpp((int)(v >> 32), CTRL, 0xf, 0xf, true);
+    return ((u64)hi << 32) | lo;
 }
-__device__ __forceinline__ u64 wave_most(u64 x) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) x = max(x, (u64)__shfl_xor(x, off, kWave));
-    return x;
+template <class F>
+__device__ __forceinline__ u64 wave_all(u64 x, F f) {
+    x = f(x, rotated64<0x128>(x)), x = f(x, rotated64<0x124>(x)), x = f(x, rotated64<0x122>(x)), x = f(x, rotated64<0x121>(x));
+    auto l = __builtin_amdgcn_permlane16_swap((uint32_t)x, (uint32_t)x, false, false);
+    auto h = __builtin_amdgcn_permlane16_swap((uint32_t)(x >> 32), (uint32_t)(x >> 32), false, false);
+    x = f(((u64)h[0] << 32) | l[0], ((u64)h[1] << 32) | l[1]);
+    l = __builtin_amdgcn_permlane32_swap((uint32_t)x, (uint32_t)x, false, false);
+    h = __builtin_amdgcn_permlane32_swap((uint32_t)(x >> 32), (uint32_t)(x >> 32), false, false);
+    return f(((u64)h[0] << 32) | l[0], ((u64)h[1] << 32) | l[1]);
+}
+__device__ __forceinline__ u64 wave_sum64(u64 x) {
+    return wave_all(x, [](u64 a, u64 b) { return a + b; });
+}
+__device__ __forceinline__ u64 wave_most64(u64 x) {
+    return wave_all(x, [](u64 a, u64 b) { return a > b ? a : b; });
 }
 __device__ __forceinline__ u64 wave_upto(u64 x) {  // the lane's and those before
 #pragma unroll
@@ -182,10 +219,10 @@ __device__ __forceinline__ u64 wave_upto(u64 x) {  // the lane's and those befor
 // Of a whole workgroup, in every thread.
 template <int WAVES>
 __device__ __forceinline__ u64 all_sum(u64 x, u64* room) {
-    x = wave_sum(x);
-    __syncthreads();
+    x = wave_sum64(x);
+    lds_barrier();
     if ((threadIdx.x & 63) == 0) room[threadIdx.x >> 6] = x;
-    __syncthreads();
+    lds_barrier();
     x = 0;
 #pragma unroll
     for (int i = 0; i < WAVES; ++i) x += room[i];
@@ -193,10 +230,10 @@ __device__ __forceinline__ u64 all_sum(u64 x, u64* room) {
 }
 template <int WAVES>
 __device__ __forceinline__ u64 all_most(u64 x, u64* room) {
-    x = wave_most(x);
-    __syncthreads();
+    x = wave_most64(x);
+    lds_barrier();
     if ((threadIdx.x & 63) == 0) room[threadIdx.x >> 6] = x;
-    __syncthreads();
+    lds_barrier();
     x = 0;
 #pragma unroll
     for (int i = 0; i < WAVES; ++i) x = max(x, room[i]);
@@ -204,141 +241,231 @@ __device__ __forceinline__ u64 all_most(u64 x, u64* room) {
 }
 
 // ---- the first launch: a chunk of a row -----------------------------------------------------------------------
+// Its largest logit, its histogram, and a list of its largest logits, bin by bin as many as there is room for.
 template <bool BF16>
 __global__ __launch_bounds__(kSampleThreads) void sample_chunk_kernel(const SampleArgs a) {
     __shared__ u64 hist[kSampleBins];
     __shared__ SampleTable table;
     __shared__ u64 room[kSampleThreads / kWave];
-    constexpr int N = Logits<BF16>::N, kLoads = kSampleItems / N;
+    __shared__ unsigned upto[kSampleThreads / kWave], n_listed;
+    __shared__ int last_bin;
+    constexpr int N = Logits<BF16>::N, kLoads = kSampleItems / N, kWaves = kSampleThreads / kWave;
     const int row = blockIdx.x / a.chunks, c = blockIdx.x - row * a.chunks, tid = threadIdx.x;
-    const int first = c * kSampleChunk;
-    Logits<BF16> v[kLoads];
+    const int first = c * kSampleChunk + N * tid;
+    Logits<BF16> raw[kLoads];
 #pragma unroll
-    for (int j = 0; j < kLoads; ++j) v[j].load(a.logits, (long long)row * a.stride, first + N * (tid + j * kSampleThreads), a.vocab);
+    for (int j = 0; j < kLoads; ++j) raw[j].load(a.logits, (long long)row * a.stride, first + N * j * kSampleThreads, a.vocab);
     const SampleRow r = sample_row(a, row);
     for (int b = tid; b < kSampleBins; b += kSampleThreads) hist[b] = 0;
-    make_table(table, r);
-    float most = -INFINITY;
+    if (tid == 0) n_listed = 0, last_bin = -1;
+    float v[kSampleItems], most = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < kLoads; ++j)
-#pragma unroll
-        for (int i = 0; i < N; ++i) most = fmaxf(most, v[j][i]);
-    // the largest and the first token that has it
-    unsigned at = 0;
-#pragma unroll
-    for (int j = kLoads - 1; j >= 0; --j)
-#pragma unroll
-        for (int i = N - 1; i >= 0; --i)
-            if (v[j][i] == most) at = first + N * (tid + j * kSampleThreads) + i;
-    const u64 best = all_most<kSampleThreads / kWave>(place_of(most, at), room);
-    at = index_of(best);
-    const uint32_t key = (uint32_t)(best >> 21);
-    most = __uint_as_float(key ^ (key >> 31 ? 0x80000000u : 0xffffffffu));
+    for (int i = 0; i < kSampleItems; ++i) v[i] = logit(r, raw[i / N][i % N]), most = fmaxf(most, v[i]);
+    const auto index = [&](int i) { return (unsigned)(first + (i / N) * N * kSampleThreads + i % N); };
     SampleChunk* const out = a.chunk + (size_t)row * a.chunks + c;
-    if (most == -INFINITY) {
-        if (tid == 0) *out = SampleChunk{-INFINITY, 0, most, 0, 0, 0};
+    if (r.greedy) {
+        unsigned at = 0;
+#pragma unroll
+        for (int i = kSampleItems - 1; i >= 0; --i)
+            if (v[i] == most) at = index(i);
+        const u64 best = all_most<kWaves>(place_of(most, at), room);
+        if (tid == 0) *out = SampleChunk{0, 0, 0, logit_of(best), (int)index_of(best), logit_of(best) > -INFINITY ? 1u : 0u, 0};
         return;
     }
-    double weight;
-    const double top = bin_of(r, most, weight);
-    const bool filtered = r.filtered() && !r.greedy;
-    unsigned count = 0, tail = 0;
-    u64 mass = 0;
-    if (!r.greedy) {
+    most = wave_max(most);
+    if ((tid & 63) == 0) room[tid >> 6] = __float_as_uint(most);
+    __syncthreads();
 #pragma unroll
-        for (int j = 0; j < kLoads; ++j)
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const float x = v[j][i];
-                if (x == -INFINITY) continue;
-                ++count;
-                const double down = top - bin_of(r, x, weight);
-                if (filtered && down < kSampleBins) {
-                    atomicAdd(&hist[(int)down], whole(weight * kBinOne) + (1ull << kCountShift));
-                } else {
-                    ++tail;
-                    mass += mass_of(weight * table.of(down));
-                }
-            }
+    for (int i = 0; i < kWaves; ++i) most = fmaxf(most, __uint_as_float((uint32_t)room[i]));
+    if (most == -INFINITY) {
+        if (tid == 0) *out = SampleChunk{0, 0, 0, most, 0, 0, 0};
+        return;
     }
-    mass = all_sum<kSampleThreads / kWave>(mass, room);
-    const u64 counts = all_sum<kSampleThreads / kWave>((u64)count << 32 | tail, room);
-    if (filtered)
-        for (int b = tid; b < kSampleBins; b += kSampleThreads) a.hist[((size_t)row * a.chunks + c) * kSampleBins + b] = hist[b];
-    if (tid == 0) *out = SampleChunk{top, mass, most, (int)at, r.greedy ? 1u : (unsigned)(counts >> 32), (unsigned)counts};
+    const SampleGrid grid(bin_of(r, most));
+    unsigned* const counts = reinterpret_cast<unsigned*>(hist);
+    unsigned count = 0;
+    if (r.weighed()) {
+#pragma unroll
+        for (int i = 0; i < kSampleItems; ++i) {
+            const float t = v[i] * r.inv_h, floor_t = floorf(t);
+            const int b = (int)floor_t, at = grid.of(b);
+            const float place = t - floor_t + (at < kFine ? 0.0f : (float)(b & 7));
+            count += v[i] != -INFINITY;
+            if (v[i] != -INFINITY && at < kSampleBins)
+                atomicAdd(&hist[at], __builtin_bit_cast(u64, __builtin_fma(weight_in(r, place), kBinOne, kWhole)) - kWholeBits + (1ull << kCountShift));
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < kSampleItems; ++i) {
+            const int at = grid.of(bin_of(r, v[i]));
+            count += v[i] != -INFINITY;
+            if (v[i] != -INFINITY && at < kSampleBins) atomicAdd(&counts[at], 1u);
+        }
+    }
+    u64 mass = 0;
+    if (!r.filtered()) {
+        make_table(table, r);
+        __syncthreads();
+        for (int i = tid; i < kSampleBins; i += kSampleThreads)
+            if (hist[i]) mass += scaled(hist[i] & kMassBits, table.of(grid.top - grid.least(i)) * (kMassOne / kBinOne));
+        mass = all_sum<kWaves>(mass, room);
+    } else {
+        __syncthreads();
+        // the histogram goes out, and the bins down to which there is room in the list
+        const u64 two[2] = {hist[2 * tid], hist[2 * tid + 1]};
+        unsigned n[2] = {(unsigned)(two[0] >> kCountShift), (unsigned)(two[1] >> kCountShift)};
+        u64* const to = a.hist + ((size_t)row * a.chunks + c) * kSampleBins;
+        if (r.weighed()) {
+            to[2 * tid] = two[0], to[2 * tid + 1] = two[1];
+        } else {
+            n[0] = counts[2 * tid], n[1] = counts[2 * tid + 1];
+            reinterpret_cast<unsigned*>(to)[2 * tid] = n[0], reinterpret_cast<unsigned*>(to)[2 * tid + 1] = n[1];
+        }
+        unsigned sum = wave_inclusive_sum(n[0] + n[1]);
+        if ((tid & 63) == 63) upto[tid >> 6] = sum;
+        __syncthreads();
+        for (int w = 0; w < tid >> 6; ++w) sum += upto[w];
+        if (sum <= kSampleList) atomicMax(&last_bin, 2 * tid + 1);
+        else if (sum - n[1] <= kSampleList) atomicMax(&last_bin, 2 * tid);
+        __syncthreads();
+        const int last = last_bin, cover = last < 0 ? grid.top + 1 : grid.least(last);
+        const float least = least_of(r, cover);
+        u64* const list = a.list + ((size_t)row * a.chunks + c) * kSampleList;
+#pragma unroll
+        for (int i = 0; i < kSampleItems; ++i)
+            if (v[i] >= least && v[i] != -INFINITY) {
+                const unsigned at = atomicAdd(&n_listed, 1u);
+                if (at < kSampleList) list[at] = place_of(v[i], index(i));
+            }
+        __syncthreads();
+        if (tid == 0) out->cover = cover, out->listed = min(n_listed, (unsigned)kSampleList);
+    }
+    count = (unsigned)all_sum<kWaves>(count, room);
+    if (tid == 0) out->mass = mass, out->top = grid.top, out->most = most, out->first = 0, out->count = count;
 }
 
 // ---- the second: a row -------------------------------------------------------------------------------------------
+// The chunks' histograms added up say down to which bin there are tokens that may be kept. Mostly they are few: those of the chunks' lists, which are compared each with each (pick_few).
+// Else the bins of the cuts are sorted out by themselves, 2 048 places at a time, from lists of their tokens or, where even a bin has more than the list has room for, from the row.
 struct PickShared {
     SampleTable table;
+    double eighth[8];                      // what a bin weighs more than the first of its eight
     u64 room[kPickWaves];
     u64 chunk_mass[kSampleMaxChunks];
-    int shift[kSampleMaxChunks];           // of a chunk's top bin below the row's
-    unsigned count[kSampleBins + 1];       // of the bins, then of all up to them; the last is the tail
-    u64 mass[kSampleBins + 1];
+    int top[kSampleMaxChunks], cover[kSampleMaxChunks];
+    unsigned listed[kSampleMaxChunks];     // + 1; 0: a chunk without tokens
+    unsigned count[kSampleBins];           // of the bins, then of all up to them
+    u64 mass[kSampleBins];
     unsigned sub_count[kPickSubs];
     u64 sub_mass[kPickSubs];
     u64 few[kPickFew], few_mass[kPickFew];
-    float list_x[kPickList];
-    unsigned list_at[kPickList];
+    u64 list[kPickList];                   // places
     unsigned n, found;
     u64 lo, hi, cut, before;
     unsigned rank;
+    int k_bin, p_bin, m_bin;
 };
 
-// A row as its kept tokens are asked for.
 template <bool BF16>
 struct Pick {
     const SampleArgs& a;
     const SampleRow r;
     PickShared& sh;
     const int row;
-    double top, least;                     // the top bin; the least weight that min-p keeps
+    const SampleGrid grid;
+    double least;                          // weight that min-p keeps
+    static constexpr int N = Logits<BF16>::N;
     // The weight of a logit, that of the top bin's beginning being one.
     __device__ __forceinline__ double weight_of(float x) const {
-        double w;
-        const double b = bin_of(r, x, w);
-        return w * sh.table.of(top - b);
-    }
-    __device__ __forceinline__ int bin(float x) const { return (int)fmin(top - floor((double)x * r.inv_h), (double)kSampleBins); }
-    // f(x, index) of the tokens in a bin, the tail being bin kSampleBins: those in the list, or all of the row's.
-    template <class F>
-    __device__ __forceinline__ void each(bool listed, int of, F f) const {
-        if (listed) {
-            for (unsigned i = threadIdx.x; i < sh.n; i += kPickThreads)
-                if (bin(sh.list_x[i]) == of) f(sh.list_x[i], sh.list_at[i]);
-        } else {
-            row_each([&](float x, unsigned i) {
-                if (x != -INFINITY && bin(x) == of) f(x, i);
-            }, [](int) {});
-        }
+        const float t = x * r.inv_h, floor_t = floorf(t);
+        return weight_in(r, t - floor_t) * sh.table.of(grid.top - (int)floor_t);
     }
     // f(x, index) of all of a row's; then done(first token) after every piece that the workgroup's threads have together: of one chunk.
     template <class F, class D>
     __device__ __forceinline__ void row_each(F f, D done) const {
-        constexpr int N = Logits<BF16>::N, kLoads = 4;
+        constexpr int kLoads = 4;
         for (int from = 0; from < a.vocab; from += kLoads * N * kPickThreads) {
             Logits<BF16> v[kLoads];
 #pragma unroll
             for (int j = 0; j < kLoads; ++j) v[j].load(a.logits, (long long)row * a.stride, from + N * ((int)threadIdx.x + j * kPickThreads), a.vocab);
-#pragma unroll
+#pragma unroll 1
             for (int j = 0; j < kLoads; ++j) {
+                Logits<BF16> one = v[0];
 #pragma unroll
-                for (int i = 0; i < N; ++i) f(v[j][i], (unsigned)(from + N * ((int)threadIdx.x + j * kPickThreads) + i));
+                for (int k = 1; k < kLoads; ++k)
+                    if (j == k) one = v[k];
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const float x = logit(r, one[i]);
+                    if (x != -INFINITY) f(x, (unsigned)(from + N * ((int)threadIdx.x + j * kPickThreads) + i));
+                }
                 done(from + N * j * kPickThreads);
             }
         }
     }
-    // The cut inside of a bin: the place of its rank-th token, or (by mass) of the last whose tokens before it weigh less than `left`; and what the bin's
-    // tokens up to it weigh. Places are sorted out 2 048 at a time until few are left, which are compared with each other.
-    __device__ void resolve(bool listed, int of, bool by_mass, unsigned rank, u64 left, u64& cut, u64& upto) const {
+    // The places of the tokens of bins lo .. hi into the list, in no order: from the chunks' lists, or from the chunks that have more of them.
+    __device__ void gather(int lo, int hi) const {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        lds_barrier();
+        if (threadIdx.x == 0) sh.n = 0;
+        lds_barrier();
+        const auto put = [&](u64 place) {
+            const unsigned at = atomicAdd(&sh.n, 1u);
+            if (at < kPickList) sh.list[at] = place;
+        };
+        for (int c = wave; c < a.chunks; c += kPickWaves) {
+            if (sh.listed[c] == 0 || sh.top[c] < lo) continue;
+            if (sh.cover[c] <= lo) {
+                const u64* const from = a.list + ((size_t)row * a.chunks + c) * kSampleList;
+                constexpr int kEach = kSampleList / kWave;
+                u64 p[kEach];
+#pragma unroll
+                for (int i = 0; i < kEach; ++i) p[i] = (unsigned)(lane + kWave * i) < sh.listed[c] - 1 ? from[lane + kWave * i] : 0;
+#pragma unroll
+                for (int i = 0; i < kEach; ++i) {
+                    const int b = bin_of(r, logit_of(p[i]));
+                    if (p[i] && b >= lo && b <= hi) put(p[i]);
+                }
+            } else {
+#pragma unroll 1
+                for (int from = c * kSampleChunk + N * lane; from < (c + 1) * kSampleChunk; from += 4 * N * kWave) {
+                    Logits<BF16> v[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[j].load(a.logits, (long long)row * a.stride, from + j * N * kWave, a.vocab);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int i = 0; i < N; ++i) {
+                            const float x = logit(r, v[j][i]);
+                            const int b = bin_of(r, x);
+                            if (b >= lo && b <= hi && x != -INFINITY) put(place_of(x, (unsigned)(from + j * N * kWave + i)));
+                        }
+                }
+            }
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) sh.n = min(sh.n, (unsigned)kPickList);
+        lds_barrier();
+    }
+    // f(place) of the tokens of bins lo .. hi: those in the list, or all of the row's.
+    template <class F>
+    __device__ __forceinline__ void each(bool listed, int lo, int hi, F f) const {
+        if (listed) {
+            for (unsigned i = threadIdx.x; i < sh.n; i += kPickThreads) {
+                const int b = bin_of(r, logit_of(sh.list[i]));
+                if (b >= lo && b <= hi) f(sh.list[i]);
+            }
+        } else {
+            row_each([&](float x, unsigned i) { f(place_of(x, i)); }, [](int) {});
+        }
+    }
+    // The cut among those: the place of the rank-th, or (by mass) of the last whose tokens before it weigh less than `left`; and what they weigh up to
+    // it. Places are sorted out 2 048 at a time until few are left, which are compared with each other.
+    __device__ __forceinline__ void resolve(bool listed, int b_lo, int b_hi, bool by_mass, unsigned rank, u64 left, u64& cut, u64& upto) const {
         const int tid = threadIdx.x;
         u64 most = 0, least_place = 0;  // (the second inverted)
         unsigned n = 0;
-        each(listed, of, [&](float x, unsigned i) {
-            const u64 p = place_of(x, i);
-            most = max(most, p), least_place = max(least_place, ~p), ++n;
-        });
+        each(listed, b_lo, b_hi, [&](u64 p) { most = max(most, p), least_place = max(least_place, ~p), ++n; });
         u64 hi = all_most<kPickWaves>(most, sh.room), lo = ~all_most<kPickWaves>(least_place, sh.room);
         n = (unsigned)all_sum<kPickWaves>(n, sh.room);
         u64 before = 0;
@@ -346,15 +473,14 @@ struct Pick {
         while (n > kPickFew) {
             const u64 span = hi - lo;
             const int bits = 64 - __builtin_clzll(span | 1), shift = bits > 11 ? bits - 11 : 0;
-            __syncthreads();
+            lds_barrier();
             for (int i = tid; i < kPickSubs; i += kPickThreads) sh.sub_count[i] = 0, sh.sub_mass[i] = 0;
-            __syncthreads();
-            each(listed, of, [&](float x, unsigned i) {
-                const u64 p = place_of(x, i);
+            lds_barrier();
+            each(listed, b_lo, b_hi, [&](u64 p) {
                 if (p < lo || p > hi) return;
                 const int s = (int)((hi - p) >> shift);
                 atomicAdd(&sh.sub_count[s], 1u);
-                atomicAdd(&sh.sub_mass[s], mass_of(weight_of(x)));
+                atomicAdd(&sh.sub_mass[s], mass_of(weight_of(logit_of(p))));
             });
             __syncthreads();
             if (tid < kWave) {  // a lane has 32 of them
@@ -363,7 +489,7 @@ struct Pick {
                 unsigned k = 0;
                 for (int i = 0; i < kEach; ++i) m += sh.sub_mass[kEach * tid + i], k += sh.sub_count[kEach * tid + i];
                 u64 m_at = wave_upto(m) - m;
-                unsigned k_at = (unsigned)(wave_upto(k) - k);
+                unsigned k_at = wave_inclusive_sum(k) - k;
                 // the sub-bin of the cut: the first up to which there is enough; the last that has a token where there never is
                 int last = -1, hit = -1;
                 u64 hit_m = 0, last_m = 0;
@@ -382,8 +508,8 @@ struct Pick {
                 const int lane = hits ? __builtin_ctzll(hits) : 63 - __builtin_clzll(lasts);
                 if (tid == lane) {
                     const int s = hits ? hit : last;
-                    sh.hi = hi - ((u64)s << shift);
                     const u64 size = (1ull << shift) - 1;
+                    sh.hi = hi - ((u64)s << shift);
                     sh.lo = sh.hi - lo > size ? sh.hi - size : lo;
                     sh.before = hits ? hit_m : last_m;
                     sh.rank = hits ? hit_k : last_k;
@@ -396,11 +522,10 @@ struct Pick {
         __syncthreads();
         if (tid == 0) sh.found = 0, sh.cut = ~0ull;
         __syncthreads();
-        each(listed, of, [&](float x, unsigned i) {
-            const u64 p = place_of(x, i);
+        each(listed, b_lo, b_hi, [&](u64 p) {
             if (p < lo || p > hi) return;
             const unsigned k = atomicAdd(&sh.found, 1u);
-            if (k < kPickFew) sh.few[k] = p, sh.few_mass[k] = mass_of(weight_of(x));
+            if (k < kPickFew) sh.few[k] = p, sh.few_mass[k] = mass_of(weight_of(logit_of(p)));
         });
         __syncthreads();
         if (tid < (int)n) {
@@ -409,10 +534,8 @@ struct Pick {
             unsigned k = ahead;
             for (unsigned j = 0; j < n; ++j)
                 if (sh.few[j] > p) m += sh.few_mass[j], ++k;
-            // (the first is kept whatever it takes: it is in the bin of the cut)
-            if (by_mass ? m < left || k == ahead : k < rank) {
-                atomicMin(&sh.cut, p);
-            }
+            // (the first is kept whatever it takes: it is where the cut is)
+            if (by_mass ? m < left || k == ahead : k < rank) atomicMin(&sh.cut, p);
         }
         __syncthreads();
         cut = sh.cut;
@@ -427,11 +550,18 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
     __shared__ PickShared sh;
     const int row = blockIdx.x, tid = threadIdx.x;
     const SampleChunk* const chunks = a.chunk + (size_t)row * a.chunks;
-    SampleChunk mine{-INFINITY, 0, -INFINITY, 0, 0, 0};
+    SampleChunk mine{0, 0, 0, -INFINITY, 0, 0, 0};
     if (tid < a.chunks) mine = chunks[tid];
     const SampleRow r = sample_row(a, row);
     const float u = a.uniforms[row];
     make_table(sh.table, r);
+    if (tid >= 128 && tid < 136) sh.eighth[tid - 128] = exp(r.a * (double)(tid - 128));
+    sh.count[tid] = 0, sh.mass[tid] = 0;
+    if (tid < kSampleMaxChunks) {
+        sh.chunk_mass[tid] = 0;
+        sh.top[tid] = mine.top, sh.cover[tid] = mine.cover, sh.listed[tid] = mine.count ? mine.listed + 1 : 0;
+    }
+    if (tid == 0) sh.n = 0, sh.k_bin = sh.p_bin = sh.m_bin = kSampleBins;
     const u64 best = all_most<kPickWaves>(mine.count ? place_of(mine.most, (unsigned)mine.first) : 0, sh.room);
     const unsigned candidates = (unsigned)all_sum<kPickWaves>(mine.count, sh.room);
     const auto finish = [&](int token, unsigned kept, float logprob, const SampleEnd& end) {
@@ -444,197 +574,225 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
         if (tid == 0) finish(-1, 0, -INFINITY, SampleEnd{0, 0, 0, -1, 0});
         return;
     }
-    const int greedy = (int)index_of(best);
     if (r.greedy) {
-        if (tid == 0) finish(greedy, 1, 0.0f, SampleEnd{0, 0, 0, greedy, 1});
+        if (tid == 0) finish((int)index_of(best), 1, 0.0f, SampleEnd{0, 0, 0, (int)index_of(best), 1});
         return;
     }
-    const uint32_t key = (uint32_t)(best >> 21);
-    const float most = __uint_as_float(key ^ (key >> 31 ? 0x80000000u : 0xffffffffu));
-    double most_weight;
-    const double top = bin_of(r, most, most_weight);
-    Pick<BF16> pick{a, r, sh, row, top, r.m_on ? r.m * most_weight : 0.0};
+    const float most = logit_of(best);
+    Pick<BF16> pick{a, r, sh, row, SampleGrid(bin_of(r, most)), 0.0};
+    const SampleGrid& grid = pick.grid;
+    if (r.m_on) pick.least = r.m * pick.weight_of(most);
     u64 cut = 0;
     unsigned kept = candidates;
-    bool listed = false;
-    if (tid < kSampleMaxChunks) sh.chunk_mass[tid] = 0;
-    if (tid < a.chunks) {
-        sh.shift[tid] = mine.count ? (int)fmin(top - mine.top, 4096.0) : 4096;
-        if (!r.filtered() && mine.count) sh.chunk_mass[tid] = scaled(mine.mass, sh.table.of(top - mine.top));
-    }
-    if (r.filtered()) {
+    if (!r.filtered()) {
+        if (mine.count) sh.chunk_mass[tid] = scaled(mine.mass, sh.table.of(grid.top - mine.top));
+        lds_barrier();
+    } else {
         // ---- the row's histogram
-        if (tid <= kSampleBins) sh.count[tid] = 0, sh.mass[tid] = 0;
-        __syncthreads();
+        const bool weighed = r.weighed();
         {
-            const int b = tid & (kSampleBins - 1);
             constexpr int kAtOnce = 8;
-            for (int c0 = tid / kSampleBins; c0 < a.chunks; c0 += 2 * kAtOnce) {
+            for (int c0 = 0; c0 < a.chunks; c0 += kAtOnce) {
                 u64 v[kAtOnce];
 #pragma unroll
                 for (int j = 0; j < kAtOnce; ++j) {
-                    const int c = c0 + 2 * j;
-                    v[j] = c < a.chunks && sh.shift[c] < 4096 ? a.hist[((size_t)row * a.chunks + c) * kSampleBins + b] : 0;
+                    const int c = c0 + j;
+                    const u64* const from = a.hist + ((size_t)row * a.chunks + c) * kSampleBins;
+                    v[j] = 0;
+                    if (c < a.chunks && sh.listed[c]) v[j] = weighed ? from[tid] : (u64)reinterpret_cast<const unsigned*>(from)[tid] << kCountShift;
                 }
 #pragma unroll
                 for (int j = 0; j < kAtOnce; ++j) {
                     if (v[j] == 0) continue;
-                    const int g = b + sh.shift[c0 + 2 * j];
-                    const u64 m = v[j] & ((1ull << kCountShift) - 1);
-                    // (the tail's weights are rounded one by one)
-                    atomicAdd(&sh.count[min(g, kSampleBins)], (unsigned)(v[j] >> kCountShift));
-                    atomicAdd(&sh.mass[min(g, kSampleBins)], g < kSampleBins ? m : scaled(m, sh.table.of(g) * (kMassOne / kBinOne)));
+                    const int b = SampleGrid(sh.top[c0 + j]).least(tid), to = grid.of(b);
+                    if (to >= kSampleBins) continue;
+                    u64 m = v[j] & kMassBits;
+                    if (tid < kFine && to >= kFine) m = scaled(m, sh.eighth[b & 7]);
+                    atomicAdd(&sh.count[to], (unsigned)(v[j] >> kCountShift));
+                    if (weighed) atomicAdd(&sh.mass[to], m);
                 }
             }
-            if (mine.count) {
-                // a chunk far below the top has no histogram that is looked at: its tokens belong to the tail, and weigh nothing
-                atomicAdd(&sh.count[kSampleBins], sh.shift[tid] < 4096 ? mine.tail : mine.count);
-                atomicAdd(&sh.mass[kSampleBins], scaled(mine.mass, sh.table.of(top - mine.top)));
-            }
         }
-        __syncthreads();
-        if (tid < kSampleBins) sh.mass[tid] = scaled(sh.mass[tid], sh.table.of(tid) * (kMassOne / kBinOne));
-        __syncthreads();
-        if (tid < kWave) {  // sums up to each bin: a lane has eight
-            constexpr int kEach = kSampleBins / kWave;
-            u64 m = 0;
-            unsigned k = 0;
-            for (int i = 0; i < kEach; ++i) m += sh.mass[kEach * tid + i], k += sh.count[kEach * tid + i];
-            u64 m_at = wave_upto(m) - m;
-            unsigned k_at = (unsigned)(wave_upto(k) - k);
-            for (int i = 0; i < kEach; ++i) {
-                sh.mass[kEach * tid + i] = m_at += sh.mass[kEach * tid + i];
-                sh.count[kEach * tid + i] = k_at += sh.count[kEach * tid + i];
-            }
-            if (tid == kWave - 1) sh.mass[kSampleBins] += m_at, sh.count[kSampleBins] += k_at;
+        lds_barrier();
+        // sums up to each bin
+        unsigned count = sh.count[tid];
+        const unsigned count_of = count;
+        u64 mass = weighed ? scaled(sh.mass[tid], sh.table.of(grid.top - grid.least(tid)) * (kMassOne / kBinOne)) : 0;
+        const u64 mass_of_bin = mass;
+        count = wave_inclusive_sum(count);
+        if (weighed) mass = wave_upto(mass);
+        if ((tid & 63) == 63) sh.few[tid >> 6] = count, sh.few_mass[tid >> 6] = mass;
+        lds_barrier();
+        u64 total = 0;
+#pragma unroll
+        for (int w = 0; w < kPickWaves; ++w) {
+            if (w < tid >> 6) count += (unsigned)sh.few[w], mass += sh.few_mass[w];
+            total += sh.few_mass[w];
         }
-        __syncthreads();
-        // the first bin up to which there is enough, the tail if never: in every thread, by a search
-        const auto bin_by_count = [&](unsigned want) {
-            int lo = 0, hi = kSampleBins;
-            while (lo < hi) {
-                const int mid = (lo + hi) >> 1;
-                if (sh.count[mid] >= want) hi = mid;
-                else lo = mid + 1;
-            }
-            return lo;
-        };
-        const auto bin_by_mass = [&](u64 want) {
-            int lo = 0, hi = kSampleBins;
-            while (lo < hi) {
-                const int mid = (lo + hi) >> 1;
-                if (sh.mass[mid] >= want) hi = mid;
-                else lo = mid + 1;
-            }
-            return lo;
-        };
+        sh.count[tid] = count, sh.mass[tid] = mass;
+        // the first bins up to which there is enough, none being the tail; the first whose beginning is too light for min-p
         const bool by_k = r.k_on && (unsigned)r.k < candidates;
-        const auto share = [&](u64 mass) -> u64 { return max((u64)ceil(r.p * (double)mass), 1ull); };
-        int last = kSampleBins;            // the lowest bin that may have a kept token
-        const int k_bin = by_k ? bin_by_count((unsigned)r.k) : kSampleBins;
-        if (by_k) last = k_bin;
-        else if (r.p_on) last = bin_by_mass(share(sh.mass[kSampleBins]));
-        if (r.m_on) {  // the first whose beginning is too light: bins past it hold nothing that is kept
-            int lo = 0, hi = kSampleBins;
-            while (lo < hi) {
-                const int mid = (lo + hi) >> 1;
-                if (sh.table.of(mid) < pick.least) hi = mid;
-                else lo = mid + 1;
-            }
-            last = min(last, lo);
-        }
-        // ---- the tokens down to there (what the first k weigh is asked for by top-p, wherever min-p ends), where they are no more than the list has room for
-        const int depth = by_k && r.p_on ? k_bin : last;
-        listed = depth < kSampleBins && sh.count[depth] <= kPickList;
-        if (tid == 0) sh.n = 0;
+        const auto share = [&](u64 of) -> u64 { return max((u64)ceil(r.p * (double)of), 1ull); };
+        if (by_k && count - count_of < (unsigned)r.k && count >= (unsigned)r.k) sh.k_bin = tid;
+        if (!by_k && r.p_on && mass - mass_of_bin < share(total) && mass >= share(total)) sh.p_bin = tid;
+        const auto light = [&](int i) { return sh.table.of(grid.top - grid.least(i)) < pick.least; };
+        if (r.m_on && light(tid) && (tid == 0 || !light(tid - 1))) sh.m_bin = tid;
         __syncthreads();
-        if (listed) {
-            const double edge = (top - depth) / r.inv_h;  // exact: a whole number times a power of two
-            pick.row_each([&](float x, unsigned i) {
-                if (x != -INFINITY && (double)x >= edge) {
-                    const unsigned at = atomicAdd(&sh.n, 1u);
-                    if (at < kPickList) sh.list_x[at] = x, sh.list_at[at] = i;
-                }
-            }, [](int) {});
+        const int k_bin = sh.k_bin, m_bin = sh.m_bin;
+        int p_bin = sh.p_bin;
+        // the lowest that may have a kept token, or one whose weight is asked for: what the first k weigh is, by top-p, wherever min-p ends
+        const int depth = by_k ? (r.p_on ? k_bin : min(k_bin, m_bin)) : min(p_bin, m_bin);
+        const unsigned deep = depth < kSampleBins ? sh.count[depth] : ~0u;
+        const auto count_in = [&](int b) { return b >= kSampleBins ? ~0u : sh.count[b] - (b ? sh.count[b - 1] : 0u); };
+        if (deep <= kPickList) pick.gather(grid.least(depth), INT_MAX);
+        if (deep <= kPickFew) {
+            // ---- few: each compared with each, by two threads
+            const int n = (int)sh.n, i = tid >> 1, part = tid & 1;
+            const u64 p = i < n ? sh.list[i] : 0;
+            const double w = i < n ? pick.weight_of(logit_of(p)) : 0.0;
+            const u64 m = mass_of(w);
+            if (part == 0 && i < n) sh.few_mass[i] = m;
             __syncthreads();
-            if (tid == 0) sh.n = min(sh.n, (unsigned)kPickList);
+            unsigned rank = 0;
+            u64 before = 0;
+            for (int j = part; j < n; j += 2)
+                if (sh.list[j] > p) ++rank, before += sh.few_mass[j];
+            rank += __shfl_xor(rank, 1, kWave), before += __shfl_xor(before, 1, kWave);
+            const bool in_k = i < n && (!by_k || rank < (unsigned)r.k);
+            if (by_k && r.p_on) total = all_sum<kPickWaves>(in_k && part == 0 ? m : 0, sh.room);
+            const bool stays = in_k && (rank == 0 || ((!r.p_on || before < share(total)) && w >= pick.least));
+            const u64 both = all_sum<kPickWaves>(stays && part == 0 ? m + (1ull << 54) : 0, sh.room);
+            const u64 all = both & ((1ull << 54) - 1);
+            kept = (unsigned)(both >> 54);
+            if (stays && rank == kept - 1) sh.cut = p;
+            if (part == 0 && i < n) sh.few_mass[i] = stays ? m : 0;
             __syncthreads();
+            const unsigned index = index_of(p);
+            u64 run = 0;
+            for (int j = part; j < n; j += 2)
+                if (index_of(sh.list[j]) < index) run += sh.few_mass[j];
+            run += __shfl_xor(run, 1, kWave);
+            const double target = (double)u * (double)all;
+            // the first whose sum is past the target; where none's is the last
+            if (stays && part == 0 && m != 0 && ((double)(run + m) > target ? !((double)run > target) : run + m == all)) {
+                const double whole_weight = (double)all / kMassOne;
+                finish((int)index, kept, (float)log(w / whole_weight), SampleEnd{1.0 / whole_weight, sh.cut, grid.top, (int)index, 2});
+            }
+            return;
         }
-        // ---- the cut
-        u64 whole_mass = sh.mass[kSampleBins];
-        const auto count_before = [&](int b) { return b ? sh.count[b - 1] : 0u; };
+        // ---- many: the cuts by themselves. From lists of all down to there, or of the cuts' bins alone, or from the row
+        const bool whole_list = deep <= kPickList;
         const auto mass_before = [&](int b) { return b ? sh.mass[b - 1] : 0ull; };
-        if (by_k && (r.p_on || k_bin <= last)) {
-            u64 upto;
-            pick.resolve(listed, k_bin, false, (unsigned)r.k - count_before(k_bin), 0, cut, upto);
-            whole_mass = mass_before(k_bin) + upto;
-        }
-        if (r.p_on) {
-            const u64 want = share(whole_mass);
-            const int p_bin = min(bin_by_mass(want), by_k ? k_bin : kSampleBins);
-            if (p_bin <= last) {
-                u64 upto, p_cut;
-                const u64 ahead = mass_before(p_bin);
-                pick.resolve(listed, p_bin, true, 0, want > ahead ? want - ahead : 1, p_cut, upto);
-                cut = max(cut, p_cut);
+        bool by_bins = !whole_list && weighed && depth < kSampleBins && (!by_k || count_in(k_bin) <= kPickList);
+        int end_bin = min(by_k ? k_bin : p_bin, m_bin);  // of the cut
+#pragma unroll 1
+        for (int step = 0; step < 2; ++step) {
+            const bool by_mass = step == 1;
+            // (a cut below what min-p keeps is none)
+            if (by_mass ? !r.p_on || (!by_k && m_bin < p_bin) : !by_k || (!r.p_on && m_bin < k_bin)) continue;
+            const u64 want = by_mass ? share(total) : 0;
+            if (by_mass && by_k && weighed) {  // (the first bin up to which there is enough)
+                __syncthreads();
+                if (tid == 0) sh.p_bin = k_bin;
+                __syncthreads();
+                if (tid < k_bin && sh.mass[tid] >= want && (tid == 0 || sh.mass[tid - 1] < want)) sh.p_bin = tid;
+                __syncthreads();
+                p_bin = sh.p_bin;
             }
+            const int bin = by_mass ? p_bin : k_bin;
+            // (a list of all without weights in its histogram: the row's order from its first token on)
+            const bool from_bin = weighed && (whole_list || by_bins);
+            if (from_bin && by_bins && count_in(bin) > kPickList) by_bins = false;
+            const bool binned = from_bin && (whole_list || by_bins);
+            if (binned && by_bins) pick.gather(grid.least(bin), bin < kFine ? grid.least(bin) : grid.least(bin) + 7);
+            const int lo = binned ? grid.least(bin) : INT_MIN, hi = binned ? (bin < kFine ? lo : lo + 7) : INT_MAX;
+            const u64 ahead = binned ? mass_before(bin) : 0;
+            const unsigned k_ahead = binned && bin ? sh.count[bin - 1] : 0;
+            u64 upto, its_cut;
+            pick.resolve(whole_list || binned, lo, hi, by_mass, (unsigned)r.k - k_ahead, by_mass ? (want > ahead ? want - ahead : 1) : 0, its_cut, upto);
+            cut = max(cut, its_cut);
+            if (!by_mass) total = ahead + upto;
+            end_bin = min(end_bin, by_mass ? p_bin : k_bin);
         }
         __syncthreads();
+        if (by_bins && (end_bin >= kSampleBins || count_in(end_bin) > kPickList)) by_bins = false;
         // ---- what is kept, by chunk
         unsigned n = 0;
         u64 end = 0;                       // (inverted: the last kept token's place)
-        const auto keep = [&](float x, unsigned i) -> u64 {
-            const u64 p = place_of(x, i);
+        const auto keep = [&](u64 p) -> u64 {
             if (p < cut) return 0;
-            const double w = pick.weight_of(x);
+            const double w = pick.weight_of(logit_of(p));
             if (w < pick.least) return 0;
             ++n, end = max(end, ~p);
             return mass_of(w);
         };
-        if (listed) {
+        if (by_bins) {
+            // bins in front of the cut's out of the histograms; its own tokens one by one
+            pick.gather(grid.least(end_bin), end_bin < kFine ? grid.least(end_bin) : grid.least(end_bin) + 7);
+            for (int c = tid >> 6; c < a.chunks; c += kPickWaves) {
+                if (sh.listed[c] == 0) continue;
+                const SampleGrid of(sh.top[c]);
+                u64 sum = 0;
+                for (int i = tid & 63; i < kSampleBins; i += kWave) {
+                    const u64 v = a.hist[((size_t)row * a.chunks + c) * kSampleBins + i];
+                    if (v && grid.of(of.least(i)) < end_bin) sum += scaled(v & kMassBits, sh.table.of(grid.top - of.least(i)) * (kMassOne / kBinOne));
+                }
+                sum = wave_sum64(sum);
+                if ((tid & 63) == 0 && sum) atomicAdd(&sh.chunk_mass[c], sum);
+            }
+        }
+        if (whole_list || by_bins) {
             for (unsigned i = tid; i < sh.n; i += kPickThreads) {
-                const u64 m = keep(sh.list_x[i], sh.list_at[i]);
-                if (m) atomicAdd(&sh.chunk_mass[sh.list_at[i] / kSampleChunk], m);
+                const u64 m = keep(sh.list[i]);
+                if (m) atomicAdd(&sh.chunk_mass[index_of(sh.list[i]) / kSampleChunk], m);
             }
         } else {
             u64 piece = 0;
-            pick.row_each([&](float x, unsigned i) {
-                if (x != -INFINITY) piece += keep(x, i);
-            }, [&](int from) {
-                piece = wave_sum(piece);
+            pick.row_each([&](float x, unsigned i) { piece += keep(place_of(x, i)); }, [&](int from) {
+                piece = wave_sum64(piece);
                 if (piece && (tid & 63) == 0) atomicAdd(&sh.chunk_mass[from / kSampleChunk], piece);
                 piece = 0;
             });
         }
-        kept = (unsigned)all_sum<kPickWaves>(n, sh.room);
-        cut = ~all_most<kPickWaves>(end, sh.room);
+        kept = (unsigned)all_sum<kPickWaves>(n, sh.room) + (by_bins && end_bin ? sh.count[end_bin - 1] : 0u);
+        const u64 last = all_most<kPickWaves>(end, sh.room);
+        // (none of the cut's bin kept, by min-p: whatever is in the bins in front of it is)
+        cut = last ? ~last : place_of(least_of(r, grid.least(end_bin - 1)), kSampleMaxVocab - 1);
     }
-    // ---- the chunk that the draw falls into, and the token
-    __syncthreads();
-    u64 all = 0;
-    int c = -1, last_c = 0;
-    for (int i = 0; i < a.chunks; ++i) all += sh.chunk_mass[i];
+    // ---- the chunk that the draw falls into, in every wave: a lane has four
+    u64 mass[4], sum = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) mass[i] = sh.chunk_mass[4 * (tid & 63) + i], sum += mass[i];
+    u64 run = wave_upto(sum);
+    const u64 all = ((u64)(uint32_t)__builtin_amdgcn_readlane((int)(run >> 32), 63) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)run, 63);
+    run -= sum;
     const double target = (double)u * (double)all;
-    u64 run = 0, run_c = 0, run_last = 0;
-    for (int i = 0; i < a.chunks; ++i) {
-        const u64 m = sh.chunk_mass[i];
-        if (m) {
-            if (c < 0 && (double)(run + m) > target) c = i, run_c = run;
-            last_c = i, run_last = run;
+    int c = -1, last_c = -1;
+    u64 run_c = 0, run_last = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (mass[i]) {
+            if (c < 0 && (double)(run + mass[i]) > target) c = 4 * (tid & 63) + i, run_c = run;
+            last_c = 4 * (tid & 63) + i, run_last = run;
         }
-        run += m;
+        run += mass[i];
     }
-    if (c < 0) c = last_c, run_c = run_last;
-    constexpr int kEach = kSampleChunk / kPickThreads;
+    const u64 hits = __builtin_amdgcn_ballot_w64(c >= 0), lasts = __builtin_amdgcn_ballot_w64(last_c >= 0);
+    const int lane = hits ? __builtin_ctzll(hits) : 63 - __builtin_clzll(lasts);
+    c = __shfl(hits ? c : last_c, lane, kWave);
+    run_c = __shfl(hits ? run_c : run_last, lane, kWave);
+    // ---- the token
+    constexpr int kEach = kSampleChunk / kPickThreads, N = Logits<BF16>::N;
     float x[kEach];
-    u64 m[kEach], sum = 0;
+    u64 m[kEach];
+    sum = 0;
     const int from = c * kSampleChunk + kEach * tid;
 #pragma unroll
-    for (int i = 0; i < kEach; i += Logits<BF16>::N) {
+    for (int i = 0; i < kEach; i += N) {
         Logits<BF16> v;
-        v.load(a.logits, (long long)row * a.stride, min(from + i, a.vocab), a.vocab);
+        v.load(a.logits, (long long)row * a.stride, from + i, a.vocab);
 #pragma unroll
-        for (int j = 0; j < Logits<BF16>::N; ++j) x[i + j] = v[j];
+        for (int j = 0; j < N; ++j) x[i + j] = logit(r, v[j]);
     }
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
@@ -667,7 +825,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
 #pragma unroll
         for (int i = 1; i < kEach; ++i) of = token - from == i ? x[i] : of;
         const double whole_weight = (double)all / kMassOne;
-        finish(token, kept, (float)log(pick.weight_of(of) / whole_weight), SampleEnd{top, 1.0 / whole_weight, cut, token, 2});
+        finish(token, kept, (float)log(pick.weight_of(of) / whole_weight), SampleEnd{1.0 / whole_weight, cut, grid.top, token, 2});
     }
 }
 
@@ -679,12 +837,13 @@ __global__ __launch_bounds__(kSampleThreads) void sample_probs_kernel(const Samp
     const int row = blockIdx.x / a.chunks, c = blockIdx.x - row * a.chunks, tid = threadIdx.x;
     Logits<BF16> v[kLoads];
 #pragma unroll
-    for (int j = 0; j < kLoads; ++j) v[j].load(a.logits, (long long)row * a.stride, min(c * kSampleChunk + N * (tid + j * kSampleThreads), a.vocab), a.vocab);
+    for (int j = 0; j < kLoads; ++j) v[j].load(a.logits, (long long)row * a.stride, c * kSampleChunk + N * (tid + j * kSampleThreads), a.vocab);
     const SampleRow r = sample_row(a, row);
     const SampleEnd end = a.end[row];
     make_table(table, r);
     __syncthreads();
     float* const out = a.probs + (long long)row * a.probs_stride;
+    const float least = end.cut ? logit_of(end.cut) : -FLT_MAX;
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
         const int at = c * kSampleChunk + N * (tid + j * kSampleThreads);
@@ -692,11 +851,11 @@ __global__ __launch_bounds__(kSampleThreads) void sample_probs_kernel(const Samp
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             p[i] = 0.0f;
+            const float x = logit(r, v[j][i]);
             if (end.kind == 1) p[i] = at + i == end.token ? 1.0f : 0.0f;
-            if (end.kind == 2 && v[j][i] != -INFINITY && place_of(v[j][i], (unsigned)(at + i)) >= end.cut) {
-                double w;
-                const double b = bin_of(r, v[j][i], w);
-                p[i] = (float)(w * table.of(end.top - b) * end.inv);
+            if (end.kind == 2 && x >= least && place_of(x, (unsigned)(at + i)) >= end.cut) {
+                const float t = x * r.inv_h, floor_t = floorf(t);
+                p[i] = (float)(weight_in(r, t - floor_t) * table.of(end.top - (int)floor_t) * end.inv);
             }
         }
         typedef float f32x4v __attribute__((ext_vector_type(4)));
@@ -716,7 +875,7 @@ static size_t sample_chunks(int vocab) { return ((size_t)vocab + kSampleChunk - 
 static size_t sample_bytes(int n_rows, int vocab) {
     if (n_rows <= 0 || vocab <= 0 || vocab > kSampleMaxVocab) return 0;
     const size_t chunks = (size_t)n_rows * sample_chunks(vocab);
-    return chunks * (kSampleBins * sizeof(u64) + sizeof(SampleChunk)) + (size_t)n_rows * sizeof(SampleEnd);
+    return chunks * ((kSampleBins + kSampleList) * sizeof(u64) + sizeof(SampleChunk)) + (size_t)n_rows * sizeof(SampleEnd);
 }
 
 template <bool BF16>
@@ -748,9 +907,10 @@ extern "C" int rivoli_sample_rows(const void* logits, const float* temperatures,
     const size_t chunks = rk::sample_chunks(vocab), all = (size_t)n_rows * chunks;
     if (all * rk::kSampleThreads > rk::kLaunchThreads || (size_t)n_rows * rk::kPickThreads > rk::kLaunchThreads) return 1002;
     rk::u64* const hist = static_cast<rk::u64*>(workspace);
-    rk::SampleChunk* const chunk = reinterpret_cast<rk::SampleChunk*>(hist + all * rk::kSampleBins);
+    rk::u64* const list = hist + all * rk::kSampleBins;
+    rk::SampleChunk* const chunk = reinterpret_cast<rk::SampleChunk*>(list + all * rk::kSampleList);
     rk::SampleEnd* const end = reinterpret_cast<rk::SampleEnd*>(chunk + all);
     const rk::SampleArgs a{logits, temperatures, top_ps, min_ps, uniforms, top_ks, n_rows, vocab, (int)chunks, stride, probs_stride, tokens, n_kept,
-                           logprobs, probs, chunk, hist, end};
+                           logprobs, probs, chunk, hist, list, end};
     return bf16 ? rk::sample_rows<true>(a, (hipStream_t)stream) : rk::sample_rows<false>(a, (hipStream_t)stream);
 }

@@ -8,7 +8,12 @@ FLT_MAX = np.finfo(np.float32).max
 
 def sample_row(x, t, k, p, m, u):
     """(token, kept, share of every token) of one row of f32 logits, by the definition."""
-    x = np.where(np.isnan(x), -np.inf, np.minimum(x.astype(np.float64), FLT_MAX))
+    t = np.float32(t)
+    if t > 0 and t > 2.0 ** -16:
+        most = min(float(t) * 2.0 ** 25, float(FLT_MAX))
+        x = np.where(x > -np.inf, np.clip(x.astype(np.float64), -most, most), -np.inf)
+    else:
+        t, x = np.float32(0), np.where(x > -np.inf, x.astype(np.float64), -np.inf)
     order = np.lexsort((np.arange(len(x)), -x))
     order = order[x[order] > -np.inf]
     share = np.zeros(len(x))
