@@ -18,17 +18,17 @@ namespace rk {
 typedef unsigned long long u64;
 
 // Logits are binned on one grid for all of a row: bins of a power of two's width h, 16 to 32 of them to T, so that x / h, its bin and its place in the bin are exact in f32
-// (logits beyond 2^25 T count as that: bins have 31 bits). A histogram has some 250 bins from its top on (kFine; 8 T and more), then 256 of eight bins each, another 64 T; what lies
+// (logits above 2^25 T count as that, those not above -2^25 T are never drawn: bins have 31 bits). A histogram has some 250 bins from its top on (kFine; 8 T and more), then 256 of eight bins each, another 64 T; what lies
 // deeper weighs less than 2^-92 of the top and is a tail that is only counted. Eights begin at multiples of eight, in every histogram of a row, so that histograms
 // of unlike tops add up exactly: the finer ones' bins are parts of the coarser ones'.
 constexpr int kFine = 256, kSampleBins = 512;
 constexpr int kSampleThreads = 256, kSampleItems = 32;
 constexpr int kSampleChunk = kSampleThreads * kSampleItems;  // tokens a workgroup of the first launch
 constexpr int kSampleMaxVocab = 1 << 21, kSampleMaxChunks = kSampleMaxVocab / kSampleChunk;
-constexpr int kSampleList = 256;           // of a chunk's largest logits that are listed
+constexpr int kSampleList = 128;           // of a chunk's largest logits that are listed
 constexpr int kPickThreads = 512, kPickWaves = kPickThreads / kWave;
 constexpr int kPickList = 8192;            // tokens in LDS
-constexpr int kPickSubs = 2048, kPickFew = 256;
+constexpr int kPickSubs = kPickThreads, kPickFew = 256;
 constexpr int kCountedK = 2048;            // up to this k a row's histogram has counts alone
 constexpr float kLeastTemperature = 1.0f / 65536;  // up to it the largest logit is taken
 constexpr double kMassOne = 4398046511104.0;       // 2^42
@@ -60,14 +60,15 @@ struct SampleArgs {
     int *tokens, *n_kept;
     float *logprobs, *probs;
     SampleChunk* chunk;
-    u64 *hist, *list;            // [rows][chunks][kSampleBins] (of counts alone: of 32 bits), [kSampleList] places
+    u64 *masses, *list;          // [rows][chunks][kSampleBins], where the histogram has weights; [kSampleList] places
+    unsigned* counts;            // [kSampleBins]
     SampleEnd* end;
 };
 
 struct SampleRow {
     bool greedy, k_on, p_on, m_on;
     int k;
-    float inv_h, most;           // 1 / h; logits count as at most this, and at least minus it
+    float inv_h, most;           // 1 / h; logits count as this at most, and not at all up to minus it
     double a, p, m;              // a = h / T
     __device__ __forceinline__ bool filtered() const { return k_on || p_on || m_on; }
     __device__ __forceinline__ bool weighed() const { return !k_on || k > kCountedK; }  // the histogram has weights
@@ -89,8 +90,8 @@ __device__ __forceinline__ SampleRow sample_row(const SampleArgs& a, int row) {
     r.m_on = r.m > 0.0 && r.m <= 1.0;
     return r;
 }
-// A logit as it counts: what is no number as -inf, which is never drawn; one zero.
-__device__ __forceinline__ float logit(const SampleRow& r, float x) { return x > -INFINITY ? __builtin_amdgcn_fmed3f(x, -r.most, r.most) + 0.0f : -INFINITY; }
+// A logit as it counts: what is no number, or further down than all that counts, as -inf, which is never drawn.
+__device__ __forceinline__ float logit(const SampleRow& r, float x) { return x > -r.most ? fminf(x, r.most) : -INFINITY; }
 
 // The least logit of a bin's, or of one between it and the next that there is.
 __device__ __forceinline__ float least_of(const SampleRow& r, int b) {
@@ -111,7 +112,7 @@ __device__ __forceinline__ double weight_in(const SampleRow& r, float place) {
 struct SampleGrid {
     int top, fine8;              // the least bin that is its own, an eighth of it
     __device__ __forceinline__ explicit SampleGrid(int t) : top(t), fine8((t - 248) >> 3) {}
-    __device__ __forceinline__ int of(int b) const { return b >= 8 * fine8 ? top - b : min(kFine + fine8 - 1 - (b >> 3), kSampleBins); }
+    __device__ __forceinline__ int of(int b) const { return b >= 8 * fine8 ? top - b : kFine + fine8 - 1 - (b >> 3); }  // (kSampleBins and more: the tail; bin -2^31: what is never drawn)
     __device__ __forceinline__ int least(int i) const { return i < kFine ? max(top - i, 8 * fine8) : 8 * (fine8 - 1 - (i - kFine)); }  // of number i's bins (of some at the change, none)
 };
 // What a bin's beginning weighs, `down` bins below the top: exp(-a down) by two tables of 64.
@@ -131,7 +132,7 @@ __device__ __forceinline__ u64 scaled(u64 mass, double by) { return (u64)((doubl
 
 // A token's place in the order, larger first: its logit's bits in order, then the lower index.
 __device__ __forceinline__ u64 place_of(float x, unsigned index) {
-    const uint32_t b = __float_as_uint(x);
+    const uint32_t b = __float_as_uint(x + 0.0f);  // (one zero)
     const uint32_t key = b ^ ((uint32_t)((int)b >> 31) | 0x80000000u);
     return ((u64)key << 21) | (kSampleMaxVocab - 1 - index);
 }
@@ -208,6 +209,17 @@ __device__ __forceinline__ u64 wave_sum64(u64 x) {
 __device__ __forceinline__ u64 wave_most64(u64 x) {
     return wave_all(x, [](u64 a, u64 b) { return a > b ? a : b; });
 }
+template <int CTRL>
+__device__ __forceinline__ float rotated32(float x) {
+    return __uint_as_float((uint32_t)__builtin_amdgcn_mov_dpp((int)__float_as_uint(x), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float wave_top(float x) {
+    x = fmaxf(x, rotated32<0x128>(x)), x = fmaxf(x, rotated32<0x124>(x)), x = fmaxf(x, rotated32<0x122>(x)), x = fmaxf(x, rotated32<0x121>(x));
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
 __device__ __forceinline__ u64 wave_upto(u64 x) {  // the lane's and those before
 #pragma unroll
     for (int off = 1; off < kWave; off <<= 1) {
@@ -244,10 +256,10 @@ __device__ __forceinline__ u64 all_most(u64 x, u64* room) {
 // Its largest logit, its histogram, and a list of its largest logits, bin by bin as many as there is room for.
 template <bool BF16>
 __global__ __launch_bounds__(kSampleThreads) void sample_chunk_kernel(const SampleArgs a) {
-    __shared__ u64 hist[kSampleBins];
+    __shared__ u64 hist[kSampleBins + kWave];
     __shared__ SampleTable table;
     __shared__ u64 room[kSampleThreads / kWave];
-    __shared__ unsigned upto[kSampleThreads / kWave], n_listed;
+    __shared__ unsigned upto[kSampleThreads / kWave], n_listed, all_count;
     __shared__ int last_bin;
     constexpr int N = Logits<BF16>::N, kLoads = kSampleItems / N, kWaves = kSampleThreads / kWave;
     const int row = blockIdx.x / a.chunks, c = blockIdx.x - row * a.chunks, tid = threadIdx.x;
@@ -257,7 +269,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_chunk_kernel(const Samp
     for (int j = 0; j < kLoads; ++j) raw[j].load(a.logits, (long long)row * a.stride, first + N * j * kSampleThreads, a.vocab);
     const SampleRow r = sample_row(a, row);
     for (int b = tid; b < kSampleBins; b += kSampleThreads) hist[b] = 0;
-    if (tid == 0) n_listed = 0, last_bin = -1;
+    if (tid == 0) n_listed = all_count = 0, last_bin = -1;
     float v[kSampleItems], most = -INFINITY;
 #pragma unroll
     for (int i = 0; i < kSampleItems; ++i) v[i] = logit(r, raw[i / N][i % N]), most = fmaxf(most, v[i]);
@@ -272,9 +284,9 @@ __global__ __launch_bounds__(kSampleThreads) void sample_chunk_kernel(const Samp
         if (tid == 0) *out = SampleChunk{0, 0, 0, logit_of(best), (int)index_of(best), logit_of(best) > -INFINITY ? 1u : 0u, 0};
         return;
     }
-    most = wave_max(most);
+    most = wave_top(most);
     if ((tid & 63) == 0) room[tid >> 6] = __float_as_uint(most);
-    __syncthreads();
+    lds_barrier();
 #pragma unroll
     for (int i = 0; i < kWaves; ++i) most = fmaxf(most, __uint_as_float((uint32_t)room[i]));
     if (most == -INFINITY) {
@@ -283,70 +295,79 @@ __global__ __launch_bounds__(kSampleThreads) void sample_chunk_kernel(const Samp
     }
     const SampleGrid grid(bin_of(r, most));
     unsigned* const counts = reinterpret_cast<unsigned*>(hist);
-    unsigned count = 0;
+    // No branches: tokens without a bin go to spare ones, a lane's own, so that the elements' chains of dependent instructions run beside each other.
+    const int spare = kSampleBins + (tid & 63);
+    unsigned count = 0;                    // of the wave
     if (r.weighed()) {
 #pragma unroll
         for (int i = 0; i < kSampleItems; ++i) {
             const float t = v[i] * r.inv_h, floor_t = floorf(t);
             const int b = (int)floor_t, at = grid.of(b);
             const float place = t - floor_t + (at < kFine ? 0.0f : (float)(b & 7));
-            count += v[i] != -INFINITY;
-            if (v[i] != -INFINITY && at < kSampleBins)
-                atomicAdd(&hist[at], __builtin_bit_cast(u64, __builtin_fma(weight_in(r, place), kBinOne, kWhole)) - kWholeBits + (1ull << kCountShift));
+            count += (unsigned)__builtin_popcountll(__builtin_amdgcn_ballot_w64(v[i] > -INFINITY));
+            atomicAdd(&hist[at < kSampleBins ? at : spare],
+                      __builtin_bit_cast(u64, __builtin_fma(weight_in(r, place), kBinOne, kWhole)) + ((1ull << kCountShift) - kWholeBits));
         }
     } else {
 #pragma unroll
         for (int i = 0; i < kSampleItems; ++i) {
             const int at = grid.of(bin_of(r, v[i]));
-            count += v[i] != -INFINITY;
-            if (v[i] != -INFINITY && at < kSampleBins) atomicAdd(&counts[at], 1u);
+            count += (unsigned)__builtin_popcountll(__builtin_amdgcn_ballot_w64(v[i] > -INFINITY));
+            atomicAdd(&counts[at < kSampleBins ? at : spare], 1u);
         }
     }
+    if ((tid & 63) == 0) atomicAdd(&all_count, count);
     u64 mass = 0;
     if (!r.filtered()) {
         make_table(table, r);
-        __syncthreads();
+        lds_barrier();
         for (int i = tid; i < kSampleBins; i += kSampleThreads)
             if (hist[i]) mass += scaled(hist[i] & kMassBits, table.of(grid.top - grid.least(i)) * (kMassOne / kBinOne));
         mass = all_sum<kWaves>(mass, room);
     } else {
-        __syncthreads();
+        lds_barrier();
         // the histogram goes out, and the bins down to which there is room in the list
-        const u64 two[2] = {hist[2 * tid], hist[2 * tid + 1]};
-        unsigned n[2] = {(unsigned)(two[0] >> kCountShift), (unsigned)(two[1] >> kCountShift)};
-        u64* const to = a.hist + ((size_t)row * a.chunks + c) * kSampleBins;
+        unsigned n[2] = {counts[2 * tid], counts[2 * tid + 1]};
+        const size_t to = ((size_t)row * a.chunks + c) * kSampleBins + 2 * tid;
         if (r.weighed()) {
-            to[2 * tid] = two[0], to[2 * tid + 1] = two[1];
-        } else {
-            n[0] = counts[2 * tid], n[1] = counts[2 * tid + 1];
-            reinterpret_cast<unsigned*>(to)[2 * tid] = n[0], reinterpret_cast<unsigned*>(to)[2 * tid + 1] = n[1];
+            const u64 two[2] = {hist[2 * tid], hist[2 * tid + 1]};
+            n[0] = (unsigned)(two[0] >> kCountShift), n[1] = (unsigned)(two[1] >> kCountShift);
+            a.masses[to] = two[0] & kMassBits, a.masses[to + 1] = two[1] & kMassBits;
         }
+        a.counts[to] = n[0], a.counts[to + 1] = n[1];
         unsigned sum = wave_inclusive_sum(n[0] + n[1]);
         if ((tid & 63) == 63) upto[tid >> 6] = sum;
-        __syncthreads();
+        lds_barrier();
         for (int w = 0; w < tid >> 6; ++w) sum += upto[w];
-        if (sum <= kSampleList) atomicMax(&last_bin, 2 * tid + 1);
-        else if (sum - n[1] <= kSampleList) atomicMax(&last_bin, 2 * tid);
-        __syncthreads();
+        // (lanes before one that has room have it too)
+        const u64 one = __builtin_amdgcn_ballot_w64(sum - n[1] <= kSampleList), both = __builtin_amdgcn_ballot_w64(sum <= kSampleList);
+        const int wave_last = 63 - __builtin_clzll(one | 1);
+        if ((tid & 63) == 0 && one) atomicMax(&last_bin, 2 * (tid + wave_last) + (int)(both >> wave_last & 1));
+        lds_barrier();
         const int last = last_bin, cover = last < 0 ? grid.top + 1 : grid.least(last);
-        const float least = least_of(r, cover);
+        const float least = fmaxf(least_of(r, cover), -FLT_MAX);
         u64* const list = a.list + ((size_t)row * a.chunks + c) * kSampleList;
+        unsigned here = 0;
 #pragma unroll
-        for (int i = 0; i < kSampleItems; ++i)
-            if (v[i] >= least && v[i] != -INFINITY) {
-                const unsigned at = atomicAdd(&n_listed, 1u);
-                if (at < kSampleList) list[at] = place_of(v[i], index(i));
-            }
-        __syncthreads();
+        for (int i = 0; i < kSampleItems; ++i) here += v[i] >= least;
+        const unsigned before = wave_inclusive_sum(here);
+        unsigned base = 0;
+        if ((tid & 63) == 63) base = atomicAdd(&n_listed, before);
+        unsigned at = (unsigned)__builtin_amdgcn_readlane((int)base, 63) + before - here;
+        if (__builtin_amdgcn_readlane((int)before, 63) != 0) {
+#pragma unroll
+            for (int i = 0; i < kSampleItems; ++i)
+                if (v[i] >= least) list[min(at++, kSampleList - 1u)] = place_of(v[i], index(i));
+        }
+        lds_barrier();
         if (tid == 0) out->cover = cover, out->listed = min(n_listed, (unsigned)kSampleList);
     }
-    count = (unsigned)all_sum<kWaves>(count, room);
-    if (tid == 0) out->mass = mass, out->top = grid.top, out->most = most, out->first = 0, out->count = count;
+    if (tid == 0) out->mass = mass, out->top = grid.top, out->most = most, out->first = 0, out->count = all_count;
 }
 
 // ---- the second: a row -------------------------------------------------------------------------------------------
 // The chunks' histograms added up say down to which bin there are tokens that may be kept. Mostly they are few: those of the chunks' lists, which are compared each with each (pick_few).
-// Else the bins of the cuts are sorted out by themselves, 2 048 places at a time, from lists of their tokens or, where even a bin has more than the list has room for, from the row.
+// Else the bins of the cuts are sorted out by themselves, by 512 ranges of places at a time, from lists of their tokens or, where even a bin has more than the list has room for, from the row.
 struct PickShared {
     SampleTable table;
     double eighth[8];                      // what a bin weighs more than the first of its eight
@@ -354,15 +375,16 @@ struct PickShared {
     u64 chunk_mass[kSampleMaxChunks];
     int top[kSampleMaxChunks], cover[kSampleMaxChunks];
     unsigned listed[kSampleMaxChunks];     // + 1; 0: a chunk without tokens
-    unsigned count[kSampleBins];           // of the bins, then of all up to them
-    u64 mass[kSampleBins];
+    unsigned count[kSampleBins + kWave];   // of the bins, then of all up to them
+    u64 mass[kSampleBins + kWave];
     unsigned sub_count[kPickSubs];
     u64 sub_mass[kPickSubs];
-    u64 few[kPickFew], few_mass[kPickFew];
+    u64 few[kPickFew], few_mass[kPickFew], few_upto[kPickFew], by_index[kPickFew], index_upto[kPickFew];
+    unsigned rank_of[kPickFew];
     u64 list[kPickList];                   // places
     unsigned n, found;
     u64 lo, hi, cut, before;
-    unsigned rank;
+    unsigned rank, n_ahead;
     int k_bin, p_bin, m_bin;
 };
 
@@ -403,8 +425,18 @@ struct Pick {
             }
         }
     }
+    // A wave's chunks' lists: of the first two of its chunks, asked for when the kernel begins.
+    static constexpr int kEarly = 2, kListed = kSampleList / kWave;
+    struct Lists {
+        u64 p[kEarly][kListed];
+    };
+    __device__ __forceinline__ void list_of(int c, u64 (&p)[kListed]) const {
+        const u64* const from = a.list + ((size_t)row * a.chunks + min(c, a.chunks - 1)) * kSampleList;
+#pragma unroll
+        for (int i = 0; i < kListed; ++i) p[i] = from[(threadIdx.x & 63) + kWave * i];
+    }
     // The places of the tokens of bins lo .. hi into the list, in no order: from the chunks' lists, or from the chunks that have more of them.
-    __device__ void gather(int lo, int hi) const {
+    __device__ __forceinline__ void gather(int lo, int hi, const Lists& early) const {
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
         lds_barrier();
         if (threadIdx.x == 0) sh.n = 0;
@@ -413,37 +445,45 @@ struct Pick {
             const unsigned at = atomicAdd(&sh.n, 1u);
             if (at < kPickList) sh.list[at] = place;
         };
-        for (int c = wave; c < a.chunks; c += kPickWaves) {
-            if (sh.listed[c] == 0 || sh.top[c] < lo) continue;
-            if (sh.cover[c] <= lo) {
-                const u64* const from = a.list + ((size_t)row * a.chunks + c) * kSampleList;
-                constexpr int kEach = kSampleList / kWave;
-                u64 p[kEach];
+        const auto use = [&](int c, const u64 (&p)[kListed]) {
 #pragma unroll
-                for (int i = 0; i < kEach; ++i) p[i] = (unsigned)(lane + kWave * i) < sh.listed[c] - 1 ? from[lane + kWave * i] : 0;
-#pragma unroll
-                for (int i = 0; i < kEach; ++i) {
-                    const int b = bin_of(r, logit_of(p[i]));
-                    if (p[i] && b >= lo && b <= hi) put(p[i]);
-                }
-            } else {
+            for (int i = 0; i < kListed; ++i) {
+                const int b = bin_of(r, logit_of(p[i]));
+                if ((unsigned)(lane + kWave * i) < sh.listed[c] - 1 && b >= lo && b <= hi) put(p[i]);
+            }
+        };
+        const auto read = [&](int c) {
 #pragma unroll 1
-                for (int from = c * kSampleChunk + N * lane; from < (c + 1) * kSampleChunk; from += 4 * N * kWave) {
-                    Logits<BF16> v[4];
+            for (int from = c * kSampleChunk + N * lane; from < (c + 1) * kSampleChunk; from += 4 * N * kWave) {
+                Logits<BF16> v[4];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) v[j].load(a.logits, (long long)row * a.stride, from + j * N * kWave, a.vocab);
+                for (int j = 0; j < 4; ++j) v[j].load(a.logits, (long long)row * a.stride, from + j * N * kWave, a.vocab);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
+                for (int j = 0; j < 4; ++j)
 #pragma unroll
-                        for (int i = 0; i < N; ++i) {
-                            const float x = logit(r, v[j][i]);
-                            const int b = bin_of(r, x);
-                            if (b >= lo && b <= hi && x != -INFINITY) put(place_of(x, (unsigned)(from + j * N * kWave + i)));
-                        }
-                }
+                    for (int i = 0; i < N; ++i) {
+                        const float x = logit(r, v[j][i]);
+                        const int b = bin_of(r, x);
+                        if (b >= lo && b <= hi && x != -INFINITY) put(place_of(x, (unsigned)(from + j * N * kWave + i)));
+                    }
+            }
+        };
+        const auto has = [&](int c) { return c < a.chunks && sh.listed[c] != 0 && sh.top[c] >= lo; };
+#pragma unroll
+        for (int k = 0; k < kEarly; ++k)
+            if (has(wave + k * kPickWaves) && sh.cover[wave + k * kPickWaves] <= lo) use(wave + k * kPickWaves, early.p[k]);
+#pragma unroll 1
+        for (int c = wave; c < a.chunks; c += kPickWaves) {
+            if (!has(c)) continue;
+            if (sh.cover[c] > lo) {
+                read(c);
+            } else if (c >= kEarly * kPickWaves) {
+                u64 p[kListed];
+                list_of(c, p);
+                use(c, p);
             }
         }
-        __syncthreads();
+        lds_barrier();
         if (threadIdx.x == 0) sh.n = min(sh.n, (unsigned)kPickList);
         lds_barrier();
     }
@@ -459,8 +499,45 @@ struct Pick {
             row_each([&](float x, unsigned i) { f(place_of(x, i)); }, [](int) {});
         }
     }
+    // Up to kPickFew unlike keys, the largest first, with the masses of theirs (a thread has its own key's) and the sums of those up to each. A key's number is
+    // that of the keys above it: a thread compares two of them with a quarter of all.
+    __device__ __forceinline__ void order(int n, u64* keys, u64 mass, u64* sorted, u64* sorted_mass, u64* upto) const {
+        const int tid = threadIdx.x, part = __builtin_amdgcn_readfirstlane(tid >> 7), first = tid & 127;
+        static_assert(kPickThreads == 512 && kPickFew == 256, "two keys a thread, four parts");
+        const int rounds = (n + 31) / 32;
+        if (tid >= n && tid < 32 * rounds) keys[tid] = 0;  // above none
+        if (tid < kPickFew) rank_of(tid) = 0;
+        lds_barrier();
+        const u64 own = tid < n ? keys[tid] : 0, one = keys[min(first, 32 * rounds - 1)], two = keys[min(first + 128, 32 * rounds - 1)];
+        unsigned above_one = 0, above_two = 0;
+        for (int j = 0; j < rounds; ++j) {
+            u64 k[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) k[i] = keys[32 * j + 8 * part + i];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) above_one += k[i] > one, above_two += k[i] > two;
+        }
+        if (first < n) atomicAdd(&sh.rank_of[first], above_one);
+        if (first + 128 < n) atomicAdd(&sh.rank_of[first + 128], above_two);
+        lds_barrier();
+        if (tid < n) {
+            const unsigned at = sh.rank_of[tid];
+            sorted[at] = own, sorted_mass[at] = mass;
+        }
+        lds_barrier();
+        if (tid < kWave) {
+            u64 m[4], sum = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) m[i] = 4 * tid + i < n ? sorted_mass[4 * tid + i] : 0, sum += m[i];
+            u64 run = wave_upto(sum) - sum;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) upto[4 * tid + i] = run += m[i];
+        }
+        lds_barrier();
+    }
+    __device__ __forceinline__ unsigned& rank_of(int i) const { return sh.rank_of[i]; }
     // The cut among those: the place of the rank-th, or (by mass) of the last whose tokens before it weigh less than `left`; and what they weigh up to
-    // it. Places are sorted out 2 048 at a time until few are left, which are compared with each other.
+    // it. Places are sorted out by 512 ranges at a time until few are left, which are compared with each other.
     __device__ __forceinline__ void resolve(bool listed, int b_lo, int b_hi, bool by_mass, unsigned rank, u64 left, u64& cut, u64& upto) const {
         const int tid = threadIdx.x;
         u64 most = 0, least_place = 0;  // (the second inverted)
@@ -472,9 +549,11 @@ struct Pick {
         unsigned ahead = 0;
         while (n > kPickFew) {
             const u64 span = hi - lo;
-            const int bits = 64 - __builtin_clzll(span | 1), shift = bits > 11 ? bits - 11 : 0;
+            const int bits = 64 - __builtin_clzll(span | 1), shift = bits > 9 ? bits - 9 : 0;
+            static_assert(kPickSubs == 1 << 9 && kPickSubs == kPickThreads, "a thread's each");
             lds_barrier();
-            for (int i = tid; i < kPickSubs; i += kPickThreads) sh.sub_count[i] = 0, sh.sub_mass[i] = 0;
+            sh.sub_count[tid] = 0, sh.sub_mass[tid] = 0;
+            if (tid == 0) sh.rank = ~0u;
             lds_barrier();
             each(listed, b_lo, b_hi, [&](u64 p) {
                 if (p < lo || p > hi) return;
@@ -482,52 +561,44 @@ struct Pick {
                 atomicAdd(&sh.sub_count[s], 1u);
                 atomicAdd(&sh.sub_mass[s], mass_of(weight_of(logit_of(p))));
             });
-            __syncthreads();
-            if (tid < kWave) {  // a lane has 32 of them
-                constexpr int kEach = kPickSubs / kWave;
-                u64 m = 0;
-                unsigned k = 0;
-                for (int i = 0; i < kEach; ++i) m += sh.sub_mass[kEach * tid + i], k += sh.sub_count[kEach * tid + i];
-                u64 m_at = wave_upto(m) - m;
-                unsigned k_at = wave_inclusive_sum(k) - k;
-                // the sub-bin of the cut: the first up to which there is enough; the last that has a token where there never is
-                int last = -1, hit = -1;
-                u64 hit_m = 0, last_m = 0;
-                unsigned hit_k = 0, last_k = 0;
-                for (int i = 0; i < kEach; ++i) {
-                    const int s = kEach * tid + i;
-                    const u64 dm = sh.sub_mass[s];
-                    const unsigned dk = sh.sub_count[s];
-                    if (dk) {
-                        last = s, last_m = m_at, last_k = k_at;
-                        if (hit < 0 && (by_mass ? before + m_at + dm >= left : ahead + k_at + dk >= rank)) hit = s, hit_m = m_at, hit_k = k_at;
-                    }
-                    m_at += dm, k_at += dk;
-                }
-                const u64 hits = __builtin_amdgcn_ballot_w64(hit >= 0), lasts = __builtin_amdgcn_ballot_w64(last >= 0);
-                const int lane = hits ? __builtin_ctzll(hits) : 63 - __builtin_clzll(lasts);
-                if (tid == lane) {
-                    const int s = hits ? hit : last;
-                    const u64 size = (1ull << shift) - 1;
-                    sh.hi = hi - ((u64)s << shift);
-                    sh.lo = sh.hi - lo > size ? sh.hi - size : lo;
-                    sh.before = hits ? hit_m : last_m;
-                    sh.rank = hits ? hit_k : last_k;
-                    sh.found = sh.sub_count[s];
-                }
+            lds_barrier();
+            const unsigned dk = sh.sub_count[tid];
+            const u64 dm = sh.sub_mass[tid];
+            unsigned k_at = wave_inclusive_sum(dk);
+            u64 m_at = wave_upto(dm);
+            if ((tid & 63) == 63) sh.few[tid >> 6] = k_at, sh.few_mass[tid >> 6] = m_at;
+            lds_barrier();
+            unsigned k_all = 0;
+            u64 m_all = 0;
+#pragma unroll
+            for (int w = 0; w < kPickWaves; ++w) {
+                if (w < tid >> 6) k_at += (unsigned)sh.few[w], m_at += sh.few_mass[w];
+                k_all += (unsigned)sh.few[w], m_all += sh.few_mass[w];
             }
-            __syncthreads();
-            hi = sh.hi, lo = sh.lo, before += sh.before, ahead += sh.rank, n = sh.found;
+            // the sub-bin of the cut: the first up to which there is enough; the last that has a token where there never is
+            const bool never = by_mass && before + m_all < left;
+            const bool hit = never ? dk && k_at == k_all
+                                   : by_mass ? dk && before + m_at >= left && (before + m_at - dm < left || k_at == dk) : k_at - dk + ahead < rank && k_at + ahead >= rank;
+            if (hit) atomicMin(&sh.rank, (unsigned)tid);
+            lds_barrier();
+            if ((unsigned)tid == sh.rank) {
+                const u64 size = (1ull << shift) - 1;
+                sh.hi = hi - ((u64)tid << shift);
+                sh.lo = sh.hi - lo > size ? sh.hi - size : lo;
+                sh.before = m_at - dm, sh.found = dk, sh.n_ahead = k_at - dk;
+            }
+            lds_barrier();
+            hi = sh.hi, lo = sh.lo, before += sh.before, ahead += sh.n_ahead, n = sh.found;
         }
-        __syncthreads();
+        lds_barrier();
         if (tid == 0) sh.found = 0, sh.cut = ~0ull;
-        __syncthreads();
+        lds_barrier();
         each(listed, b_lo, b_hi, [&](u64 p) {
             if (p < lo || p > hi) return;
             const unsigned k = atomicAdd(&sh.found, 1u);
             if (k < kPickFew) sh.few[k] = p, sh.few_mass[k] = mass_of(weight_of(logit_of(p)));
         });
-        __syncthreads();
+        lds_barrier();
         if (tid < (int)n) {
             const u64 p = sh.few[tid];
             u64 m = before;
@@ -537,7 +608,7 @@ struct Pick {
             // (the first is kept whatever it takes: it is where the cut is)
             if (by_mass ? m < left || k == ahead : k < rank) atomicMin(&sh.cut, p);
         }
-        __syncthreads();
+        lds_barrier();
         cut = sh.cut;
         u64 m = 0;
         if (tid < (int)n && sh.few[tid] >= cut) m = sh.few_mass[tid];
@@ -554,6 +625,26 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
     if (tid < a.chunks) mine = chunks[tid];
     const SampleRow r = sample_row(a, row);
     const float u = a.uniforms[row];
+    // What the chunks have left, all on its way before anything is waited for: their histograms' words of the thread's bin, sixteen chunks at once, and their lists.
+    constexpr int kAtOnce = 16;
+    const bool weighed = r.weighed(), asks = r.filtered() && !r.greedy;
+    u64 masses[kAtOnce];
+    unsigned counts[kAtOnce];
+    const auto words_of = [&](int c0) {
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j) counts[j] = a.counts[((size_t)row * a.chunks + min(c0 + j, a.chunks - 1)) * kSampleBins + tid];
+        if (weighed) {
+#pragma unroll
+            for (int j = 0; j < kAtOnce; ++j) masses[j] = a.masses[((size_t)row * a.chunks + min(c0 + j, a.chunks - 1)) * kSampleBins + tid];
+        }
+    };
+    typename Pick<BF16>::Lists lists;
+    if (asks) {
+        words_of(0);
+        const Pick<BF16> early{a, r, sh, row, SampleGrid(0), 0.0};
+#pragma unroll
+        for (int k = 0; k < Pick<BF16>::kEarly; ++k) early.list_of((tid >> 6) + k * kPickWaves, lists.p[k]);
+    }
     make_table(sh.table, r);
     if (tid >= 128 && tid < 136) sh.eighth[tid - 128] = exp(r.a * (double)(tid - 128));
     sh.count[tid] = 0, sh.mass[tid] = 0;
@@ -562,8 +653,14 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
         sh.top[tid] = mine.top, sh.cover[tid] = mine.cover, sh.listed[tid] = mine.count ? mine.listed + 1 : 0;
     }
     if (tid == 0) sh.n = 0, sh.k_bin = sh.p_bin = sh.m_bin = kSampleBins;
-    const u64 best = all_most<kPickWaves>(mine.count ? place_of(mine.most, (unsigned)mine.first) : 0, sh.room);
-    const unsigned candidates = (unsigned)all_sum<kPickWaves>(mine.count, sh.room);
+    u64 best = wave_most64(mine.count ? place_of(mine.most, (unsigned)mine.first) : 0);
+    unsigned candidates = (unsigned)wave_sum64(mine.count);
+    if ((tid & 63) == 0) sh.few[tid >> 6] = best, sh.room[tid >> 6] = candidates;
+    lds_barrier();
+    best = 0, candidates = 0;
+#pragma unroll
+    for (int w = 0; w < kPickWaves; ++w) best = max(best, sh.few[w]), candidates += (unsigned)sh.room[w];
+    lds_barrier();
     const auto finish = [&](int token, unsigned kept, float logprob, const SampleEnd& end) {
         a.tokens[row] = token;
         if (a.n_kept) a.n_kept[row] = (int)kept;
@@ -589,29 +686,27 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
         lds_barrier();
     } else {
         // ---- the row's histogram
-        const bool weighed = r.weighed();
-        {
-            constexpr int kAtOnce = 8;
-            for (int c0 = 0; c0 < a.chunks; c0 += kAtOnce) {
-                u64 v[kAtOnce];
+        // (no branches: what has no bin goes to spare ones, a lane's own)
+        for (int c0 = 0;;) {
+            int tops[kAtOnce];
+            unsigned there[kAtOnce];
 #pragma unroll
-                for (int j = 0; j < kAtOnce; ++j) {
-                    const int c = c0 + j;
-                    const u64* const from = a.hist + ((size_t)row * a.chunks + c) * kSampleBins;
-                    v[j] = 0;
-                    if (c < a.chunks && sh.listed[c]) v[j] = weighed ? from[tid] : (u64)reinterpret_cast<const unsigned*>(from)[tid] << kCountShift;
-                }
+            for (int j = 0; j < kAtOnce; ++j) tops[j] = sh.top[min(c0 + j, kSampleMaxChunks - 1)], there[j] = sh.listed[min(c0 + j, kSampleMaxChunks - 1)];
 #pragma unroll
-                for (int j = 0; j < kAtOnce; ++j) {
-                    if (v[j] == 0) continue;
-                    const int b = SampleGrid(sh.top[c0 + j]).least(tid), to = grid.of(b);
-                    if (to >= kSampleBins) continue;
-                    u64 m = v[j] & kMassBits;
-                    if (tid < kFine && to >= kFine) m = scaled(m, sh.eighth[b & 7]);
-                    atomicAdd(&sh.count[to], (unsigned)(v[j] >> kCountShift));
-                    if (weighed) atomicAdd(&sh.mass[to], m);
+            for (int j = 0; j < kAtOnce; ++j) {
+                const int b = SampleGrid(tops[j]).least(tid), number = grid.of(b);
+                const bool in = c0 + j < a.chunks && there[j] != 0 && counts[j] != 0 && number < kSampleBins;
+                const int to = in ? number : kSampleBins + (tid & 63);
+                atomicAdd(&sh.count[to], counts[j]);
+                if (weighed) {
+                    u64 m = masses[j];
+                    if (in && tid < kFine && number >= kFine) m = scaled(m, sh.eighth[b & 7]);
+                    atomicAdd(&sh.mass[to], m);
                 }
             }
+            c0 += kAtOnce;
+            if (c0 >= a.chunks) break;
+            words_of(c0);
         }
         lds_barrier();
         // sums up to each bin
@@ -637,46 +732,42 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
         if (!by_k && r.p_on && mass - mass_of_bin < share(total) && mass >= share(total)) sh.p_bin = tid;
         const auto light = [&](int i) { return sh.table.of(grid.top - grid.least(i)) < pick.least; };
         if (r.m_on && light(tid) && (tid == 0 || !light(tid - 1))) sh.m_bin = tid;
-        __syncthreads();
+        lds_barrier();
         const int k_bin = sh.k_bin, m_bin = sh.m_bin;
         int p_bin = sh.p_bin;
         // the lowest that may have a kept token, or one whose weight is asked for: what the first k weigh is, by top-p, wherever min-p ends
         const int depth = by_k ? (r.p_on ? k_bin : min(k_bin, m_bin)) : min(p_bin, m_bin);
         const unsigned deep = depth < kSampleBins ? sh.count[depth] : ~0u;
         const auto count_in = [&](int b) { return b >= kSampleBins ? ~0u : sh.count[b] - (b ? sh.count[b - 1] : 0u); };
-        if (deep <= kPickList) pick.gather(grid.least(depth), INT_MAX);
+        if (deep <= kPickList) pick.gather(grid.least(depth), INT_MAX, lists);
         if (deep <= kPickFew) {
-            // ---- few: each compared with each, by two threads
-            const int n = (int)sh.n, i = tid >> 1, part = tid & 1;
-            const u64 p = i < n ? sh.list[i] : 0;
-            const double w = i < n ? pick.weight_of(logit_of(p)) : 0.0;
-            const u64 m = mass_of(w);
-            if (part == 0 && i < n) sh.few_mass[i] = m;
-            __syncthreads();
-            unsigned rank = 0;
-            u64 before = 0;
-            for (int j = part; j < n; j += 2)
-                if (sh.list[j] > p) ++rank, before += sh.few_mass[j];
-            rank += __shfl_xor(rank, 1, kWave), before += __shfl_xor(before, 1, kWave);
-            const bool in_k = i < n && (!by_k || rank < (unsigned)r.k);
-            if (by_k && r.p_on) total = all_sum<kPickWaves>(in_k && part == 0 ? m : 0, sh.room);
-            const bool stays = in_k && (rank == 0 || ((!r.p_on || before < share(total)) && w >= pick.least));
-            const u64 both = all_sum<kPickWaves>(stays && part == 0 ? m + (1ull << 54) : 0, sh.room);
-            const u64 all = both & ((1ull << 54) - 1);
-            kept = (unsigned)(both >> 54);
-            if (stays && rank == kept - 1) sh.cut = p;
-            if (part == 0 && i < n) sh.few_mass[i] = stays ? m : 0;
-            __syncthreads();
-            const unsigned index = index_of(p);
-            u64 run = 0;
-            for (int j = part; j < n; j += 2)
-                if (index_of(sh.list[j]) < index) run += sh.few_mass[j];
-            run += __shfl_xor(run, 1, kWave);
-            const double target = (double)u * (double)all;
-            // the first whose sum is past the target; where none's is the last
-            if (stays && part == 0 && m != 0 && ((double)(run + m) > target ? !((double)run > target) : run + m == all)) {
-                const double whole_weight = (double)all / kMassOne;
-                finish((int)index, kept, (float)log(w / whole_weight), SampleEnd{1.0 / whole_weight, sh.cut, grid.top, (int)index, 2});
+            // ---- few: in order, with what they weigh up to each
+            const int n = (int)sh.n;
+            pick.order(n, sh.list, tid < n ? mass_of(pick.weight_of(logit_of(sh.list[tid]))) : 0, sh.few, sh.few_mass, sh.few_upto);
+            // thread t has the t-th
+            if (by_k && r.p_on) total = sh.few_upto[min(n, r.k) - 1];
+            const auto stays = [&](int t) {
+                if (t >= n || (by_k && t >= r.k)) return false;
+                if (t == 0) return true;
+                return (!r.p_on || sh.few_upto[t - 1] < share(total)) && (!r.m_on || pick.weight_of(logit_of(sh.few[t])) >= pick.least);
+            };
+            const bool mine_stays = tid < kPickFew && stays(tid);
+            if (mine_stays && !stays(tid + 1)) sh.rank = tid + 1, sh.cut = sh.few[tid], sh.before = sh.few_upto[tid];
+            // those by their indexes, with their numbers
+            if (mine_stays) sh.list[tid] = (u64)(kSampleMaxVocab - 1 - index_of(sh.few[tid])) << 8 | (u64)tid;
+            lds_barrier();
+            kept = sh.rank;
+            const u64 all = sh.before;
+            pick.order((int)kept, sh.list, mine_stays ? sh.few_mass[tid] : 0, sh.by_index, sh.sub_mass, sh.index_upto);
+            if (tid < (int)kept) {
+                const double target = (double)u * (double)all;
+                const u64 upto = sh.index_upto[tid], before = tid ? sh.index_upto[tid - 1] : 0;
+                // the first whose sum is past the target; where none's is the last
+                if ((double)upto > target ? tid == 0 || !((double)before > target) : upto == all && (tid == 0 || before != all) && !((double)all > target)) {
+                    const u64 p = sh.few[sh.by_index[tid] & 255];
+                    const double whole_weight = (double)all / kMassOne;
+                    finish((int)index_of(p), kept, (float)log(pick.weight_of(logit_of(p)) / whole_weight), SampleEnd{1.0 / whole_weight, sh.cut, grid.top, (int)index_of(p), 2});
+                }
             }
             return;
         }
@@ -692,11 +783,11 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
             if (by_mass ? !r.p_on || (!by_k && m_bin < p_bin) : !by_k || (!r.p_on && m_bin < k_bin)) continue;
             const u64 want = by_mass ? share(total) : 0;
             if (by_mass && by_k && weighed) {  // (the first bin up to which there is enough)
-                __syncthreads();
+                lds_barrier();
                 if (tid == 0) sh.p_bin = k_bin;
-                __syncthreads();
+                lds_barrier();
                 if (tid < k_bin && sh.mass[tid] >= want && (tid == 0 || sh.mass[tid - 1] < want)) sh.p_bin = tid;
-                __syncthreads();
+                lds_barrier();
                 p_bin = sh.p_bin;
             }
             const int bin = by_mass ? p_bin : k_bin;
@@ -704,7 +795,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
             const bool from_bin = weighed && (whole_list || by_bins);
             if (from_bin && by_bins && count_in(bin) > kPickList) by_bins = false;
             const bool binned = from_bin && (whole_list || by_bins);
-            if (binned && by_bins) pick.gather(grid.least(bin), bin < kFine ? grid.least(bin) : grid.least(bin) + 7);
+            if (binned && by_bins) pick.gather(grid.least(bin), bin < kFine ? grid.least(bin) : grid.least(bin) + 7, lists);
             const int lo = binned ? grid.least(bin) : INT_MIN, hi = binned ? (bin < kFine ? lo : lo + 7) : INT_MAX;
             const u64 ahead = binned ? mass_before(bin) : 0;
             const unsigned k_ahead = binned && bin ? sh.count[bin - 1] : 0;
@@ -714,7 +805,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
             if (!by_mass) total = ahead + upto;
             end_bin = min(end_bin, by_mass ? p_bin : k_bin);
         }
-        __syncthreads();
+        lds_barrier();
         if (by_bins && (end_bin >= kSampleBins || count_in(end_bin) > kPickList)) by_bins = false;
         // ---- what is kept, by chunk
         unsigned n = 0;
@@ -728,14 +819,14 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
         };
         if (by_bins) {
             // bins in front of the cut's out of the histograms; its own tokens one by one
-            pick.gather(grid.least(end_bin), end_bin < kFine ? grid.least(end_bin) : grid.least(end_bin) + 7);
+            pick.gather(grid.least(end_bin), end_bin < kFine ? grid.least(end_bin) : grid.least(end_bin) + 7, lists);
             for (int c = tid >> 6; c < a.chunks; c += kPickWaves) {
                 if (sh.listed[c] == 0) continue;
                 const SampleGrid of(sh.top[c]);
                 u64 sum = 0;
                 for (int i = tid & 63; i < kSampleBins; i += kWave) {
-                    const u64 v = a.hist[((size_t)row * a.chunks + c) * kSampleBins + i];
-                    if (v && grid.of(of.least(i)) < end_bin) sum += scaled(v & kMassBits, sh.table.of(grid.top - of.least(i)) * (kMassOne / kBinOne));
+                    const u64 v = a.masses[((size_t)row * a.chunks + c) * kSampleBins + i];
+                    if (v && grid.of(of.least(i)) < end_bin) sum += scaled(v, sh.table.of(grid.top - of.least(i)) * (kMassOne / kBinOne));
                 }
                 sum = wave_sum64(sum);
                 if ((tid & 63) == 0 && sum) atomicAdd(&sh.chunk_mass[c], sum);
@@ -801,10 +892,10 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
     }
     // the threads' sums in order
     const u64 upto = wave_upto(sum);
-    __syncthreads();
+    lds_barrier();
     if ((tid & 63) == 63) sh.room[tid >> 6] = upto;
     if (tid == 0) sh.lo = ~0ull, sh.hi = 0;
-    __syncthreads();
+    lds_barrier();
     u64 before = run_c + upto - sum;
     for (int w = 0; w < tid >> 6; ++w) before += sh.room[w];
     int hit = -1, last = -1;
@@ -818,7 +909,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
     }
     if (hit >= 0) atomicMin(&sh.lo, (u64)(from + hit));
     if (last >= 0) atomicMax(&sh.hi, (u64)(from + last));
-    __syncthreads();
+    lds_barrier();
     const int token = (int)(sh.lo != ~0ull ? sh.lo : sh.hi);
     if (token >= from && token < from + kEach) {
         float of = x[0];
@@ -841,7 +932,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_probs_kernel(const Samp
     const SampleRow r = sample_row(a, row);
     const SampleEnd end = a.end[row];
     make_table(table, r);
-    __syncthreads();
+    lds_barrier();
     float* const out = a.probs + (long long)row * a.probs_stride;
     const float least = end.cut ? logit_of(end.cut) : -FLT_MAX;
 #pragma unroll
@@ -875,7 +966,7 @@ static size_t sample_chunks(int vocab) { return ((size_t)vocab + kSampleChunk - 
 static size_t sample_bytes(int n_rows, int vocab) {
     if (n_rows <= 0 || vocab <= 0 || vocab > kSampleMaxVocab) return 0;
     const size_t chunks = (size_t)n_rows * sample_chunks(vocab);
-    return chunks * ((kSampleBins + kSampleList) * sizeof(u64) + sizeof(SampleChunk)) + (size_t)n_rows * sizeof(SampleEnd);
+    return chunks * ((kSampleBins + kSampleList) * sizeof(u64) + kSampleBins * sizeof(unsigned) + sizeof(SampleChunk)) + (size_t)n_rows * sizeof(SampleEnd);
 }
 
 template <bool BF16>
@@ -906,11 +997,12 @@ extern "C" int rivoli_sample_rows(const void* logits, const float* temperatures,
     if ((uintptr_t)logits % size != 0 || (uintptr_t)probs % 4 != 0 || !rk::aligned16(workspace)) return 1004;
     const size_t chunks = rk::sample_chunks(vocab), all = (size_t)n_rows * chunks;
     if (all * rk::kSampleThreads > rk::kLaunchThreads || (size_t)n_rows * rk::kPickThreads > rk::kLaunchThreads) return 1002;
-    rk::u64* const hist = static_cast<rk::u64*>(workspace);
-    rk::u64* const list = hist + all * rk::kSampleBins;
-    rk::SampleChunk* const chunk = reinterpret_cast<rk::SampleChunk*>(list + all * rk::kSampleList);
+    rk::u64* const masses = static_cast<rk::u64*>(workspace);
+    rk::u64* const list = masses + all * rk::kSampleBins;
+    unsigned* const counts = reinterpret_cast<unsigned*>(list + all * rk::kSampleList);
+    rk::SampleChunk* const chunk = reinterpret_cast<rk::SampleChunk*>(counts + all * rk::kSampleBins);
     rk::SampleEnd* const end = reinterpret_cast<rk::SampleEnd*>(chunk + all);
     const rk::SampleArgs a{logits, temperatures, top_ps, min_ps, uniforms, top_ks, n_rows, vocab, (int)chunks, stride, probs_stride, tokens, n_kept,
-                           logprobs, probs, chunk, hist, list, end};
+                           logprobs, probs, chunk, masses, list, counts, end};
     return bf16 ? rk::sample_rows<true>(a, (hipStream_t)stream) : rk::sample_rows<false>(a, (hipStream_t)stream);
 }

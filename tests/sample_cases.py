@@ -11,9 +11,9 @@ def sample_row(x, t, k, p, m, u):
     t = np.float32(t)
     if t > 0 and t > 2.0 ** -16:
         most = min(float(t) * 2.0 ** 25, float(FLT_MAX))
-        x = np.where(x > -np.inf, np.clip(x.astype(np.float64), -most, most), -np.inf)
+        x = np.where(x > -most, np.minimum(x.astype(np.float64), most), -np.inf)
     else:
-        t, x = np.float32(0), np.where(x > -np.inf, x.astype(np.float64), -np.inf)
+        t, x = np.float32(0), np.where(x > -2.0 ** 25, x.astype(np.float64), -np.inf)
     order = np.lexsort((np.arange(len(x)), -x))
     order = order[x[order] > -np.inf]
     share = np.zeros(len(x))
