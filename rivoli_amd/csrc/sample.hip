@@ -25,11 +25,13 @@ constexpr int kFine = 256, kSampleBins = 512;
 constexpr int kSampleThreads = 256, kSampleItems = 32;
 constexpr int kSampleChunk = kSampleThreads * kSampleItems;  // tokens a workgroup of the first launch
 constexpr int kSampleMaxVocab = 1 << 21, kSampleMaxChunks = kSampleMaxVocab / kSampleChunk;
-constexpr int kSampleList = 128;           // of a chunk's largest logits that are listed
+// Of a chunk's largest logits that are listed: the first part is asked for by every row's workgroup, the second by those that need more.
+constexpr int kSampleList = 128, kSampleMore = 512, kSampleListed = kSampleList + kSampleMore;
 constexpr int kPickThreads = 512, kPickWaves = kPickThreads / kWave;
 constexpr int kPickList = 8192;            // tokens in LDS
 constexpr int kPickSubs = kPickThreads, kPickFew = 256;
-constexpr int kCountedK = 2048;            // up to this k a row's histogram has counts alone
+constexpr int kCountedK = 2048;            // up to this k a row's histogram has counts alone, and by min-p alone from this m on
+constexpr double kCountedM = 1.0 / 1024;
 constexpr float kLeastTemperature = 1.0f / 65536;  // up to it the largest logit is taken
 constexpr double kMassOne = 4398046511104.0;       // 2^42
 constexpr double kBinOne = 68719476736.0;          // 2^36
@@ -40,10 +42,10 @@ constexpr u64 kMassBits = (1ull << kCountShift) - 1;
 
 struct SampleChunk {
     u64 mass;                    // of a row without filters: all of its tokens', in 2^-42 of what its top bin's beginning weighs
-    int top, cover;              // its largest logit's bin; its tokens of bins from `cover` on are listed
+    int top, cover[2];           // its largest logit's bin; its tokens of bins from cover on are listed, in the first part alone, in both
     float most;                  // its largest logit
     int first;                   // that one's token, in a row that takes the largest
-    unsigned count, listed;      // tokens that may be drawn; that are listed
+    unsigned count, listed[2];   // tokens that may be drawn; that are listed in either part
 };
 struct SampleEnd {               // what the third launch writes a row's probabilities by
     double inv;                  // 1 / the whole of what is kept
@@ -60,7 +62,7 @@ struct SampleArgs {
     int *tokens, *n_kept;
     float *logprobs, *probs;
     SampleChunk* chunk;
-    u64 *masses, *list;          // [rows][chunks][kSampleBins], where the histogram has weights; [kSampleList] places
+    u64 *masses, *list;          // [rows][chunks][kSampleBins], where the histogram has weights; [kSampleListed] places
     unsigned* counts;            // [kSampleBins]
     SampleEnd* end;
 };
@@ -71,7 +73,10 @@ struct SampleRow {
     float inv_h, most;           // 1 / h; logits count as this at most, and not at all up to minus it
     double a, p, m;              // a = h / T
     __device__ __forceinline__ bool filtered() const { return k_on || p_on || m_on; }
-    __device__ __forceinline__ bool weighed() const { return !k_on || k > kCountedK; }  // the histogram has weights
+    // Whether the histogram has weights: not where they are asked for of few tokens alone.
+    __device__ __forceinline__ bool weighed() const { return k_on ? k > kCountedK : p_on || !m_on || m < kCountedM; }
+    // Whether more tokens than the lists' first parts may be asked for.
+    __device__ __forceinline__ bool more() const { return !k_on || k > kSampleList; }
 };
 __device__ __forceinline__ SampleRow sample_row(const SampleArgs& a, int row) {
     SampleRow r;
@@ -259,8 +264,8 @@ __global__ __launch_bounds__(kSampleThreads) void sample_chunk_kernel(const Samp
     __shared__ u64 hist[kSampleBins + kWave];
     __shared__ SampleTable table;
     __shared__ u64 room[kSampleThreads / kWave];
-    __shared__ unsigned upto[kSampleThreads / kWave], n_listed, all_count;
-    __shared__ int last_bin;
+    __shared__ unsigned upto[kSampleThreads / kWave], n_listed[2], all_count;
+    __shared__ int last_bin[2];
     constexpr int N = Logits<BF16>::N, kLoads = kSampleItems / N, kWaves = kSampleThreads / kWave;
     const int row = blockIdx.x / a.chunks, c = blockIdx.x - row * a.chunks, tid = threadIdx.x;
     const int first = c * kSampleChunk + N * tid;
@@ -269,7 +274,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_chunk_kernel(const Samp
     for (int j = 0; j < kLoads; ++j) raw[j].load(a.logits, (long long)row * a.stride, first + N * j * kSampleThreads, a.vocab);
     const SampleRow r = sample_row(a, row);
     for (int b = tid; b < kSampleBins; b += kSampleThreads) hist[b] = 0;
-    if (tid == 0) n_listed = all_count = 0, last_bin = -1;
+    if (tid == 0) n_listed[0] = n_listed[1] = all_count = 0, last_bin[0] = last_bin[1] = -1;
     float v[kSampleItems], most = -INFINITY;
 #pragma unroll
     for (int i = 0; i < kSampleItems; ++i) v[i] = logit(r, raw[i / N][i % N]), most = fmaxf(most, v[i]);
@@ -281,7 +286,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_chunk_kernel(const Samp
         for (int i = kSampleItems - 1; i >= 0; --i)
             if (v[i] == most) at = index(i);
         const u64 best = all_most<kWaves>(place_of(most, at), room);
-        if (tid == 0) *out = SampleChunk{0, 0, 0, logit_of(best), (int)index_of(best), logit_of(best) > -INFINITY ? 1u : 0u, 0};
+        if (tid == 0) *out = SampleChunk{0, 0, {0, 0}, logit_of(best), (int)index_of(best), logit_of(best) > -INFINITY ? 1u : 0u, {0, 0}};
         return;
     }
     most = wave_top(most);
@@ -290,7 +295,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_chunk_kernel(const Samp
 #pragma unroll
     for (int i = 0; i < kWaves; ++i) most = fmaxf(most, __uint_as_float((uint32_t)room[i]));
     if (most == -INFINITY) {
-        if (tid == 0) *out = SampleChunk{0, 0, 0, most, 0, 0, 0};
+        if (tid == 0) *out = SampleChunk{0, 0, {0, 0}, most, 0, 0, {0, 0}};
         return;
     }
     const SampleGrid grid(bin_of(r, most));
@@ -339,28 +344,46 @@ __global__ __launch_bounds__(kSampleThreads) void sample_chunk_kernel(const Samp
         if ((tid & 63) == 63) upto[tid >> 6] = sum;
         lds_barrier();
         for (int w = 0; w < tid >> 6; ++w) sum += upto[w];
-        // (lanes before one that has room have it too)
-        const u64 one = __builtin_amdgcn_ballot_w64(sum - n[1] <= kSampleList), both = __builtin_amdgcn_ballot_w64(sum <= kSampleList);
-        const int wave_last = 63 - __builtin_clzll(one | 1);
-        if ((tid & 63) == 0 && one) atomicMax(&last_bin, 2 * (tid + wave_last) + (int)(both >> wave_last & 1));
-        lds_barrier();
-        const int last = last_bin, cover = last < 0 ? grid.top + 1 : grid.least(last);
-        const float least = fmaxf(least_of(r, cover), -FLT_MAX);
-        u64* const list = a.list + ((size_t)row * a.chunks + c) * kSampleList;
-        unsigned here = 0;
 #pragma unroll
-        for (int i = 0; i < kSampleItems; ++i) here += v[i] >= least;
-        const unsigned before = wave_inclusive_sum(here);
-        unsigned base = 0;
-        if ((tid & 63) == 63) base = atomicAdd(&n_listed, before);
-        unsigned at = (unsigned)__builtin_amdgcn_readlane((int)base, 63) + before - here;
-        if (__builtin_amdgcn_readlane((int)before, 63) != 0) {
-#pragma unroll
-            for (int i = 0; i < kSampleItems; ++i)
-                if (v[i] >= least) list[min(at++, kSampleList - 1u)] = place_of(v[i], index(i));
+        for (int part = 0; part < 2; ++part) {
+            const unsigned room_for = part && r.more() ? kSampleMore : kSampleList;
+            // (lanes before one that has room have it too)
+            const u64 one = __builtin_amdgcn_ballot_w64(sum - n[1] <= room_for), both = __builtin_amdgcn_ballot_w64(sum <= room_for);
+            const int wave_last = 63 - __builtin_clzll(one | 1);
+            if ((tid & 63) == 0 && one) atomicMax(&last_bin[part], 2 * (tid + wave_last) + (int)(both >> wave_last & 1));
         }
         lds_barrier();
-        if (tid == 0) out->cover = cover, out->listed = min(n_listed, (unsigned)kSampleList);
+        int cover[2];
+        float least[2];
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+            cover[part] = last_bin[part] < 0 ? grid.top + 1 : grid.least(last_bin[part]);
+            least[part] = fmaxf(least_of(r, cover[part]), -FLT_MAX);
+        }
+        u64* const list = a.list + ((size_t)row * a.chunks + c) * kSampleListed;
+        unsigned here[2] = {0, 0}, at[2];
+#pragma unroll
+        for (int i = 0; i < kSampleItems; ++i) here[0] += v[i] >= least[0], here[1] += v[i] >= least[1];
+        here[1] -= here[0];
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+            const unsigned before = wave_inclusive_sum(here[part]);
+            unsigned base = 0;
+            if ((tid & 63) == 63) base = atomicAdd(&n_listed[part], before);
+            at[part] = (part ? kSampleList : 0) + (unsigned)__builtin_amdgcn_readlane((int)base, 63) + before - here[part];
+        }
+#pragma unroll
+        for (int i = 0; i < kSampleItems; ++i)
+            if (v[i] >= least[1]) {
+                const bool top = v[i] >= least[0];
+                list[min(top ? at[0] : at[1], kSampleListed - 1u)] = place_of(v[i], index(i));
+                at[0] += top, at[1] += !top;
+            }
+        lds_barrier();
+        if (tid == 0) {
+            out->cover[0] = cover[0], out->cover[1] = cover[1];
+            out->listed[0] = min(n_listed[0], (unsigned)kSampleList), out->listed[1] = min(n_listed[1], (unsigned)kSampleMore);
+        }
     }
     if (tid == 0) out->mass = mass, out->top = grid.top, out->most = most, out->first = 0, out->count = all_count;
 }
@@ -373,8 +396,8 @@ struct PickShared {
     double eighth[8];                      // what a bin weighs more than the first of its eight
     u64 room[kPickWaves];
     u64 chunk_mass[kSampleMaxChunks];
-    int top[kSampleMaxChunks], cover[kSampleMaxChunks];
-    unsigned listed[kSampleMaxChunks];     // + 1; 0: a chunk without tokens
+    int top[kSampleMaxChunks], cover[2][kSampleMaxChunks];
+    unsigned listed[2][kSampleMaxChunks];  // the first + 1; 0: a chunk without tokens
     unsigned count[kSampleBins + kWave];   // of the bins, then of all up to them
     u64 mass[kSampleBins + kWave];
     unsigned sub_count[kPickSubs];
@@ -431,7 +454,7 @@ struct Pick {
         u64 p[kEarly][kListed];
     };
     __device__ __forceinline__ void list_of(int c, u64 (&p)[kListed]) const {
-        const u64* const from = a.list + ((size_t)row * a.chunks + min(c, a.chunks - 1)) * kSampleList;
+        const u64* const from = a.list + ((size_t)row * a.chunks + min(c, a.chunks - 1)) * kSampleListed;
 #pragma unroll
         for (int i = 0; i < kListed; ++i) p[i] = from[(threadIdx.x & 63) + kWave * i];
     }
@@ -445,42 +468,79 @@ struct Pick {
             const unsigned at = atomicAdd(&sh.n, 1u);
             if (at < kPickList) sh.list[at] = place;
         };
-        const auto use = [&](int c, const u64 (&p)[kListed]) {
-#pragma unroll
-            for (int i = 0; i < kListed; ++i) {
-                const int b = bin_of(r, logit_of(p[i]));
-                if ((unsigned)(lane + kWave * i) < sh.listed[c] - 1 && b >= lo && b <= hi) put(p[i]);
-            }
+        const auto use = [&](u64 p, bool is) {
+            const int b = bin_of(r, logit_of(p));
+            if (is && b >= lo && b <= hi) put(p);
         };
-        const auto read = [&](int c) {
-#pragma unroll 1
-            for (int from = c * kSampleChunk + N * lane; from < (c + 1) * kSampleChunk; from += 4 * N * kWave) {
-                Logits<BF16> v[4];
+        const auto has = [&](int c) { return c < a.chunks && sh.listed[0][c] != 0 && sh.top[c] >= lo && sh.cover[1][c] <= lo; };
 #pragma unroll
-                for (int j = 0; j < 4; ++j) v[j].load(a.logits, (long long)row * a.stride, from + j * N * kWave, a.vocab);
+        for (int k = 0; k < kEarly; ++k) {
+            const int c = wave + k * kPickWaves;
+            if (has(c))
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int i = 0; i < N; ++i) {
-                        const float x = logit(r, v[j][i]);
-                        const int b = bin_of(r, x);
-                        if (b >= lo && b <= hi && x != -INFINITY) put(place_of(x, (unsigned)(from + j * N * kWave + i)));
-                    }
-            }
-        };
-        const auto has = [&](int c) { return c < a.chunks && sh.listed[c] != 0 && sh.top[c] >= lo; };
-#pragma unroll
-        for (int k = 0; k < kEarly; ++k)
-            if (has(wave + k * kPickWaves) && sh.cover[wave + k * kPickWaves] <= lo) use(wave + k * kPickWaves, early.p[k]);
+                for (int i = 0; i < kListed; ++i) use(early.p[k][i], (unsigned)(lane + kWave * i) < sh.listed[0][c] - 1);
+        }
 #pragma unroll 1
         for (int c = wave; c < a.chunks; c += kPickWaves) {
             if (!has(c)) continue;
-            if (sh.cover[c] > lo) {
-                read(c);
-            } else if (c >= kEarly * kPickWaves) {
+            if (c >= kEarly * kPickWaves) {
                 u64 p[kListed];
                 list_of(c, p);
-                use(c, p);
+#pragma unroll
+                for (int i = 0; i < kListed; ++i) use(p[i], (unsigned)(lane + kWave * i) < sh.listed[0][c] - 1);
+            }
+            if (sh.cover[0][c] > lo) {
+                const u64* const from = a.list + ((size_t)row * a.chunks + c) * kSampleListed + kSampleList;
+                const unsigned n = sh.listed[1][c];
+                constexpr int kEach = 8;
+#pragma unroll 1
+                for (unsigned i0 = 0; i0 < n; i0 += kEach * kWave) {
+                    u64 p[kEach];
+#pragma unroll
+                    for (int i = 0; i < kEach; ++i) p[i] = from[i0 + kWave * i + lane];
+#pragma unroll
+                    for (int i = 0; i < kEach; ++i) use(p[i], i0 + kWave * i + lane < n);
+                }
+            }
+        }
+        // the chunks that have more, by all threads, two of them on their way at once
+        const float least_x = fmaxf(least_of(r, lo), -FLT_MAX), past_x = hi == INT_MAX ? INFINITY : least_of(r, hi + 1);
+        constexpr int kChunks = 2, kLoads = kSampleChunk / (N * kPickThreads);
+#pragma unroll 1
+        for (int c0 = 0; c0 < a.chunks; c0 += kChunks) {
+            Logits<BF16> v[kChunks][kLoads];
+            bool asked[kChunks];
+#pragma unroll
+            for (int k = 0; k < kChunks; ++k) {
+                const int c = min(c0 + k, a.chunks - 1);
+                asked[k] = c0 + k < a.chunks && sh.listed[0][c] != 0 && sh.top[c] >= lo && sh.cover[1][c] > lo;
+                if (asked[k])
+#pragma unroll
+                    for (int j = 0; j < kLoads; ++j)
+                        v[k][j].load(a.logits, (long long)row * a.stride, (c0 + k) * kSampleChunk + N * ((int)threadIdx.x + j * kPickThreads), a.vocab);
+            }
+#pragma unroll
+            for (int k = 0; k < kChunks; ++k) {
+                if (!asked[k]) continue;
+                const auto wanted = [&](int i) {
+                    const float x = logit(r, v[k][i / N][i % N]);
+                    return x >= least_x && x < past_x;
+                };
+                unsigned here = 0;
+#pragma unroll
+                for (int i = 0; i < kLoads * N; ++i) here += wanted(i);
+                const unsigned before = wave_inclusive_sum(here);
+                if (__builtin_amdgcn_readlane((int)before, 63) == 0) continue;
+                unsigned base = 0;
+                if (lane == 63) base = atomicAdd(&sh.n, before);
+                unsigned at = (unsigned)__builtin_amdgcn_readlane((int)base, 63) + before - here;
+#pragma unroll
+                for (int i = 0; i < kLoads * N; ++i)
+                    if (wanted(i)) {
+                        const unsigned index = (unsigned)((c0 + k) * kSampleChunk + N * ((int)threadIdx.x + i / N * kPickThreads) + i % N);
+                        if (at < kPickList) sh.list[at] = place_of(logit(r, v[k][i / N][i % N]), index);
+                        ++at;
+                    }
             }
         }
         lds_barrier();
@@ -591,7 +651,7 @@ struct Pick {
             hi = sh.hi, lo = sh.lo, before += sh.before, ahead += sh.n_ahead, n = sh.found;
         }
         lds_barrier();
-        if (tid == 0) sh.found = 0, sh.cut = ~0ull;
+        if (tid == 0) sh.found = 0;
         lds_barrier();
         each(listed, b_lo, b_hi, [&](u64 p) {
             if (p < lo || p > hi) return;
@@ -599,20 +659,13 @@ struct Pick {
             if (k < kPickFew) sh.few[k] = p, sh.few_mass[k] = mass_of(weight_of(logit_of(p)));
         });
         lds_barrier();
-        if (tid < (int)n) {
-            const u64 p = sh.few[tid];
-            u64 m = before;
-            unsigned k = ahead;
-            for (unsigned j = 0; j < n; ++j)
-                if (sh.few[j] > p) m += sh.few_mass[j], ++k;
-            // (the first is kept whatever it takes: it is where the cut is)
-            if (by_mass ? m < left || k == ahead : k < rank) atomicMin(&sh.cut, p);
-        }
+        order((int)n, sh.few, tid < (int)n ? sh.few_mass[tid] : 0, sh.by_index, sh.sub_mass, sh.few_upto);
+        // the last that stays (the first does whatever it takes: it is where the cut is)
+        const auto stays = [&](unsigned t) { return t < n && (t == 0 || (by_mass ? before + sh.few_upto[t - 1] < left : ahead + t < rank)); };
+        if (stays(tid) && !stays(tid + 1)) sh.cut = sh.by_index[tid], sh.before = sh.few_upto[tid];
         lds_barrier();
-        cut = sh.cut;
-        u64 m = 0;
-        if (tid < (int)n && sh.few[tid] >= cut) m = sh.few_mass[tid];
-        upto = before + all_sum<kPickWaves>(m, sh.room);
+        cut = sh.cut, upto = before + sh.before;
+        lds_barrier();
     }
 };
 
@@ -621,7 +674,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
     __shared__ PickShared sh;
     const int row = blockIdx.x, tid = threadIdx.x;
     const SampleChunk* const chunks = a.chunk + (size_t)row * a.chunks;
-    SampleChunk mine{0, 0, 0, -INFINITY, 0, 0, 0};
+    SampleChunk mine{0, 0, {0, 0}, -INFINITY, 0, 0, {0, 0}};
     if (tid < a.chunks) mine = chunks[tid];
     const SampleRow r = sample_row(a, row);
     const float u = a.uniforms[row];
@@ -650,7 +703,8 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
     sh.count[tid] = 0, sh.mass[tid] = 0;
     if (tid < kSampleMaxChunks) {
         sh.chunk_mass[tid] = 0;
-        sh.top[tid] = mine.top, sh.cover[tid] = mine.cover, sh.listed[tid] = mine.count ? mine.listed + 1 : 0;
+        sh.top[tid] = mine.top, sh.cover[0][tid] = mine.cover[0], sh.cover[1][tid] = mine.cover[1];
+        sh.listed[0][tid] = mine.count ? mine.listed[0] + 1 : 0, sh.listed[1][tid] = mine.listed[1];
     }
     if (tid == 0) sh.n = 0, sh.k_bin = sh.p_bin = sh.m_bin = kSampleBins;
     u64 best = wave_most64(mine.count ? place_of(mine.most, (unsigned)mine.first) : 0);
@@ -691,7 +745,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
             int tops[kAtOnce];
             unsigned there[kAtOnce];
 #pragma unroll
-            for (int j = 0; j < kAtOnce; ++j) tops[j] = sh.top[min(c0 + j, kSampleMaxChunks - 1)], there[j] = sh.listed[min(c0 + j, kSampleMaxChunks - 1)];
+            for (int j = 0; j < kAtOnce; ++j) tops[j] = sh.top[min(c0 + j, kSampleMaxChunks - 1)], there[j] = sh.listed[0][min(c0 + j, kSampleMaxChunks - 1)];
 #pragma unroll
             for (int j = 0; j < kAtOnce; ++j) {
                 const int b = SampleGrid(tops[j]).least(tid), number = grid.of(b);
@@ -821,7 +875,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
             // bins in front of the cut's out of the histograms; its own tokens one by one
             pick.gather(grid.least(end_bin), end_bin < kFine ? grid.least(end_bin) : grid.least(end_bin) + 7, lists);
             for (int c = tid >> 6; c < a.chunks; c += kPickWaves) {
-                if (sh.listed[c] == 0) continue;
+                if (sh.listed[0][c] == 0) continue;
                 const SampleGrid of(sh.top[c]);
                 u64 sum = 0;
                 for (int i = tid & 63; i < kSampleBins; i += kWave) {
@@ -894,7 +948,6 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
     const u64 upto = wave_upto(sum);
     lds_barrier();
     if ((tid & 63) == 63) sh.room[tid >> 6] = upto;
-    if (tid == 0) sh.lo = ~0ull, sh.hi = 0;
     lds_barrier();
     u64 before = run_c + upto - sum;
     for (int w = 0; w < tid >> 6; ++w) before += sh.room[w];
@@ -902,15 +955,25 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
         if (m[i]) {
-            if (hit < 0 && (double)(before + m[i]) > target) hit = i;
-            last = i;
+            if (hit < 0 && (double)(before + m[i]) > target) hit = from + i;
+            last = from + i;
         }
         before += m[i];
     }
-    if (hit >= 0) atomicMin(&sh.lo, (u64)(from + hit));
-    if (last >= 0) atomicMax(&sh.hi, (u64)(from + last));
+    // the first hit; where there is none, the last token that weighs
+    const u64 hit_lanes = __builtin_amdgcn_ballot_w64(hit >= 0), last_lanes = __builtin_amdgcn_ballot_w64(last >= 0);
+    const int wave_hit = hit_lanes ? __builtin_amdgcn_readlane(hit, __builtin_ctzll(hit_lanes)) : -1;
+    const int wave_last = last_lanes ? __builtin_amdgcn_readlane(last, 63 - __builtin_clzll(last_lanes)) : -1;
+    if ((tid & 63) == 0) sh.few[tid >> 6] = (u64)(uint32_t)wave_hit << 32 | (uint32_t)wave_last;
     lds_barrier();
-    const int token = (int)(sh.lo != ~0ull ? sh.lo : sh.hi);
+    int token = -1, last_token = 0;
+#pragma unroll
+    for (int w = 0; w < kPickWaves; ++w) {
+        const int h = (int)(sh.few[w] >> 32), l = (int)(uint32_t)sh.few[w];
+        if (token < 0) token = h;
+        if (l >= 0) last_token = l;
+    }
+    if (token < 0) token = last_token;
     if (token >= from && token < from + kEach) {
         float of = x[0];
 #pragma unroll
@@ -966,7 +1029,7 @@ static size_t sample_chunks(int vocab) { return ((size_t)vocab + kSampleChunk - 
 static size_t sample_bytes(int n_rows, int vocab) {
     if (n_rows <= 0 || vocab <= 0 || vocab > kSampleMaxVocab) return 0;
     const size_t chunks = (size_t)n_rows * sample_chunks(vocab);
-    return chunks * ((kSampleBins + kSampleList) * sizeof(u64) + kSampleBins * sizeof(unsigned) + sizeof(SampleChunk)) + (size_t)n_rows * sizeof(SampleEnd);
+    return chunks * ((kSampleBins + kSampleListed) * sizeof(u64) + kSampleBins * sizeof(unsigned) + sizeof(SampleChunk)) + (size_t)n_rows * sizeof(SampleEnd);
 }
 
 template <bool BF16>
@@ -999,7 +1062,7 @@ extern "C" int rivoli_sample_rows(const void* logits, const float* temperatures,
     if (all * rk::kSampleThreads > rk::kLaunchThreads || (size_t)n_rows * rk::kPickThreads > rk::kLaunchThreads) return 1002;
     rk::u64* const masses = static_cast<rk::u64*>(workspace);
     rk::u64* const list = masses + all * rk::kSampleBins;
-    unsigned* const counts = reinterpret_cast<unsigned*>(list + all * rk::kSampleList);
+    unsigned* const counts = reinterpret_cast<unsigned*>(list + all * rk::kSampleListed);
     rk::SampleChunk* const chunk = reinterpret_cast<rk::SampleChunk*>(counts + all * rk::kSampleBins);
     rk::SampleEnd* const end = reinterpret_cast<rk::SampleEnd*>(chunk + all);
     const rk::SampleArgs a{logits, temperatures, top_ps, min_ps, uniforms, top_ks, n_rows, vocab, (int)chunks, stride, probs_stride, tokens, n_kept,
