@@ -41,7 +41,7 @@ constexpr int kCountShift = 50;            // of a histogram's word: tokens abov
 constexpr u64 kMassBits = (1ull << kCountShift) - 1;
 
 struct SampleChunk {
-    u64 mass;                    // of a row without filters: all of its tokens', in 2^-42 of what its top bin's beginning weighs
+    double weight;               // of a row without filters: all of its tokens', that of its top bin's beginning being one
     int top, cover[2];           // its largest logit's bin; its tokens of bins from cover on are listed, in the first part alone, in both
     float most;                  // its largest logit
     int first;                   // that one's token, in a row that takes the largest
@@ -131,6 +131,8 @@ __device__ __forceinline__ void make_table(SampleTable& t, const SampleRow& r) {
         (threadIdx.x < 64 ? t.fine : t.coarse)[threadIdx.x & 63] = v;
     }
 }
+// The same rounded to 2^-36, as a histogram adds it up: every weight is one of these, so that sums of either kind agree.
+__device__ __forceinline__ double rounded_in(const SampleRow& r, float place) { return __builtin_fma(weight_in(r, place), kBinOne, kWhole) - kWhole; }
 __device__ __forceinline__ u64 mass_of(double weight) { return __builtin_bit_cast(u64, __builtin_fma(weight, kMassOne, kWhole)) - kWholeBits; }
 // A sum of such numbers times a weight: up to 2^63.
 __device__ __forceinline__ u64 scaled(u64 mass, double by) { return (u64)((double)mass * by + 0.5); }
@@ -210,6 +212,10 @@ __device__ __forceinline__ u64 wave_all(u64 x, F f) {
 }
 __device__ __forceinline__ u64 wave_sum64(u64 x) {
     return wave_all(x, [](u64 a, u64 b) { return a + b; });
+}
+__device__ __forceinline__ double wave_sum_f64(double x) {
+    const auto f = [](u64 a, u64 b) { return __builtin_bit_cast(u64, __builtin_bit_cast(double, a) + __builtin_bit_cast(double, b)); };
+    return __builtin_bit_cast(double, wave_all(__builtin_bit_cast(u64, x), f));
 }
 __device__ __forceinline__ u64 wave_most64(u64 x) {
     return wave_all(x, [](u64 a, u64 b) { return a > b ? a : b; });
@@ -322,13 +328,18 @@ __global__ __launch_bounds__(kSampleThreads) void sample_chunk_kernel(const Samp
         }
     }
     if ((tid & 63) == 0) atomicAdd(&all_count, count);
-    u64 mass = 0;
+    double weight = 0.0;
     if (!r.filtered()) {
         make_table(table, r);
         lds_barrier();
         for (int i = tid; i < kSampleBins; i += kSampleThreads)
-            if (hist[i]) mass += scaled(hist[i] & kMassBits, table.of(grid.top - grid.least(i)) * (kMassOne / kBinOne));
-        mass = all_sum<kWaves>(mass, room);
+            weight += (double)(hist[i] & kMassBits) * (table.of(grid.top - grid.least(i)) * (1 / kBinOne));
+        weight = wave_sum_f64(weight);
+        if ((tid & 63) == 0) room[tid >> 6] = __builtin_bit_cast(u64, weight);
+        lds_barrier();
+        weight = 0.0;
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) weight += __builtin_bit_cast(double, room[i]);
     } else {
         lds_barrier();
         // the histogram goes out, and the bins down to which there is room in the list
@@ -385,7 +396,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_chunk_kernel(const Samp
             out->listed[0] = min(n_listed[0], (unsigned)kSampleList), out->listed[1] = min(n_listed[1], (unsigned)kSampleMore);
         }
     }
-    if (tid == 0) out->mass = mass, out->top = grid.top, out->most = most, out->first = 0, out->count = all_count;
+    if (tid == 0) out->weight = weight, out->top = grid.top, out->most = most, out->first = 0, out->count = all_count;
 }
 
 // ---- the second: a row -------------------------------------------------------------------------------------------
@@ -423,7 +434,7 @@ struct Pick {
     // The weight of a logit, that of the top bin's beginning being one.
     __device__ __forceinline__ double weight_of(float x) const {
         const float t = x * r.inv_h, floor_t = floorf(t);
-        return weight_in(r, t - floor_t) * sh.table.of(grid.top - (int)floor_t);
+        return rounded_in(r, t - floor_t) * (sh.table.of(grid.top - (int)floor_t) * (1 / kBinOne));
     }
     // f(x, index) of all of a row's; then done(first token) after every piece that the workgroup's threads have together: of one chunk.
     template <class F, class D>
@@ -735,9 +746,15 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
     if (r.m_on) pick.least = r.m * pick.weight_of(most);
     u64 cut = 0;
     unsigned kept = candidates;
+    double whole_weight = 0.0;             // of what is kept, where it is had but as a whole number
     if (!r.filtered()) {
-        if (mine.count) sh.chunk_mass[tid] = scaled(mine.mass, sh.table.of(grid.top - mine.top));
+        const double weight = mine.count ? mine.weight * sh.table.of(grid.top - mine.top) : 0.0;
+        if (mine.count) sh.chunk_mass[tid] = (u64)(weight * kMassOne + 0.5);
+        const double of_wave = wave_sum_f64(weight);
+        if ((tid & 63) == 0) sh.few[tid >> 6] = __builtin_bit_cast(u64, of_wave);
         lds_barrier();
+#pragma unroll
+        for (int w = 0; w < kPickWaves; ++w) whole_weight += __builtin_bit_cast(double, sh.few[w]);
     } else {
         // ---- the row's histogram
         // (no branches: what has no bin goes to spare ones, a lane's own)
@@ -812,6 +829,8 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
             lds_barrier();
             kept = sh.rank;
             const u64 all = sh.before;
+            const double of_wave = wave_sum_f64(mine_stays ? pick.weight_of(logit_of(sh.few[tid])) : 0.0);
+            if ((tid & 63) == 0) sh.room[tid >> 6] = __builtin_bit_cast(u64, of_wave);
             pick.order((int)kept, sh.list, mine_stays ? sh.few_mass[tid] : 0, sh.by_index, sh.sub_mass, sh.index_upto);
             if (tid < (int)kept) {
                 const double target = (double)u * (double)all;
@@ -819,7 +838,8 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
                 // the first whose sum is past the target; where none's is the last
                 if ((double)upto > target ? tid == 0 || !((double)before > target) : upto == all && (tid == 0 || before != all) && !((double)all > target)) {
                     const u64 p = sh.few[sh.by_index[tid] & 255];
-                    const double whole_weight = (double)all / kMassOne;
+#pragma unroll
+                    for (int w = 0; w < kPickFew / kWave; ++w) whole_weight += __builtin_bit_cast(double, sh.room[w]);
                     finish((int)index_of(p), kept, (float)log(pick.weight_of(logit_of(p)) / whole_weight), SampleEnd{1.0 / whole_weight, sh.cut, grid.top, (int)index_of(p), 2});
                 }
             }
@@ -978,8 +998,13 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
         float of = x[0];
 #pragma unroll
         for (int i = 1; i < kEach; ++i) of = token - from == i ? x[i] : of;
-        const double whole_weight = (double)all / kMassOne;
-        finish(token, kept, (float)log(pick.weight_of(of) / whole_weight), SampleEnd{1.0 / whole_weight, cut, grid.top, token, 2});
+        // (a whole number's last bits are those of its tokens': where one is nearly all of it, as a whole number too)
+        double weight = pick.weight_of(of);
+        if (r.filtered()) {
+            whole_weight = (double)all / kMassOne;
+            if (weight > 0.25 * whole_weight) weight = (double)mass_of(weight) / kMassOne;
+        }
+        finish(token, kept, (float)log(weight / whole_weight), SampleEnd{1.0 / whole_weight, cut, grid.top, token, 2});
     }
 }
 
@@ -1009,7 +1034,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_probs_kernel(const Samp
             if (end.kind == 1) p[i] = at + i == end.token ? 1.0f : 0.0f;
             if (end.kind == 2 && x >= least && place_of(x, (unsigned)(at + i)) >= end.cut) {
                 const float t = x * r.inv_h, floor_t = floorf(t);
-                p[i] = (float)(weight_in(r, t - floor_t) * table.of(end.top - (int)floor_t) * end.inv);
+                p[i] = (float)(rounded_in(r, t - floor_t) * (table.of(end.top - (int)floor_t) * (1 / kBinOne)) * end.inv);
             }
         }
         typedef float f32x4v __attribute__((ext_vector_type(4)));
