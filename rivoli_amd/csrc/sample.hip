@@ -515,7 +515,8 @@ struct Pick {
             }
         }
         // the chunks that have more, by all threads, two of them on their way at once
-        const float least_x = fmaxf(least_of(r, lo), -FLT_MAX), past_x = hi == INT_MAX ? INFINITY : least_of(r, hi + 1);
+        // (as they are: a NaN is in no range, what counts as the most is in the top bin, past which nothing is: a NaN)
+        const float least_x = fmaxf(least_of(r, lo), __uint_as_float(__float_as_uint(-r.most) - 1)), past_x = hi >= grid.top ? __uint_as_float(0x7fc00000u) : least_of(r, hi + 1);
         constexpr int kChunks = 2, kLoads = kSampleChunk / (N * kPickThreads);
 #pragma unroll 1
         for (int c0 = 0; c0 < a.chunks; c0 += kChunks) {
@@ -534,8 +535,8 @@ struct Pick {
             for (int k = 0; k < kChunks; ++k) {
                 if (!asked[k]) continue;
                 const auto wanted = [&](int i) {
-                    const float x = logit(r, v[k][i / N][i % N]);
-                    return x >= least_x && x < past_x;
+                    const float x = v[k][i / N][i % N];
+                    return x >= least_x && !(x >= past_x);
                 };
                 unsigned here = 0;
 #pragma unroll
@@ -848,6 +849,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
         // ---- many: the cuts by themselves. From lists of all down to there, or of the cuts' bins alone, or from the row
         const bool whole_list = deep <= kPickList;
         const auto mass_before = [&](int b) { return b ? sh.mass[b - 1] : 0ull; };
+        int held = -1;                     // the bin that the list is of
         bool by_bins = !whole_list && weighed && depth < kSampleBins && (!by_k || count_in(k_bin) <= kPickList);
         int end_bin = min(by_k ? k_bin : p_bin, m_bin);  // of the cut
 #pragma unroll 1
@@ -869,7 +871,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
             const bool from_bin = weighed && (whole_list || by_bins);
             if (from_bin && by_bins && count_in(bin) > kPickList) by_bins = false;
             const bool binned = from_bin && (whole_list || by_bins);
-            if (binned && by_bins) pick.gather(grid.least(bin), bin < kFine ? grid.least(bin) : grid.least(bin) + 7, lists);
+            if (binned && by_bins && held != bin) pick.gather(grid.least(bin), bin < kFine ? grid.least(bin) : grid.least(bin) + 7, lists), held = bin;
             const int lo = binned ? grid.least(bin) : INT_MIN, hi = binned ? (bin < kFine ? lo : lo + 7) : INT_MAX;
             const u64 ahead = binned ? mass_before(bin) : 0;
             const unsigned k_ahead = binned && bin ? sh.count[bin - 1] : 0;
@@ -893,7 +895,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
         };
         if (by_bins) {
             // bins in front of the cut's out of the histograms; its own tokens one by one
-            pick.gather(grid.least(end_bin), end_bin < kFine ? grid.least(end_bin) : grid.least(end_bin) + 7, lists);
+            if (held != end_bin) pick.gather(grid.least(end_bin), end_bin < kFine ? grid.least(end_bin) : grid.least(end_bin) + 7, lists);
             for (int c = tid >> 6; c < a.chunks; c += kPickWaves) {
                 if (sh.listed[0][c] == 0) continue;
                 const SampleGrid of(sh.top[c]);
