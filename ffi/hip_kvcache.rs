@@ -639,6 +639,38 @@ launchers! {
         stream: *mut c_void,
     );
 
+    /// Tree attention for groups of sequences whose first pages are the same, attended once a group.
+    /// See `include/rivoli_kvcache.h` for the full contract.
+    launch_attend_tree_shared_paged -> rivoli_mla_attend_tree_shared_paged, "mla_attend_tree_shared_paged" (
+        qabs: *const u16,
+        qrope: *const u16,
+        pool: *const u8,
+        block_table: *const i32,
+        ctx_lens: *const i32,
+        cu_nodes: *const i32,
+        masks: *const u32,
+        cu_groups: *const i32,
+        prefix_lens: *const i32,
+        n_seqs: usize as i32,
+        n_groups: usize as i32,
+        h: usize as i32,
+        n_nodes: usize as i32,
+        max_nodes: usize as i32,
+        max_prefix: usize as i32,
+        max_ctx: usize as i32,
+        max_blocks_per_seq: usize as i32,
+        kvl: usize as i32,
+        rope: usize as i32,
+        page_tokens: usize as i32,
+        n_pages: usize as i32,
+        scale: f32,
+        clat: *mut u16,
+        lse: *mut f32,
+        partial: *mut f32,
+        bad_rows: *mut u32,
+        stream: *mut c_void,
+    );
+
     /// Element codecs as launchers (what formats.hpp:42-57,99-106 and fwd.hip:20-45 are to the
     /// reference's kernels), for census tests of the device codecs on arbitrary inputs:
     /// e4m3_encode: out[i] = f32_to_e4m3(x[i]) (rule of crates/core/src/num.rs:128-152)
@@ -689,6 +721,7 @@ unsafe extern "C" {
     fn rivoli_sel_shape(win: i32, ratio: i32, index_topk: i32, seqlen: i32, start_pos: i32, rows: *mut i32, cols: *mut i32) -> i32;
     fn rivoli_gather_attn_scratch_floats(m: i32, h: i32, d: i32, topk: i32) -> usize;
     fn rivoli_mla_attend_tree_paged_scratch_floats(n_seqs: i32, h: i32, n_nodes: i32, max_nodes: i32, max_ctx: i32) -> usize;
+    fn rivoli_mla_attend_tree_shared_paged_scratch_floats(n_seqs: i32, n_groups: i32, h: i32, n_nodes: i32, max_nodes: i32, max_prefix: i32, max_ctx: i32) -> usize;
     fn rivoli_draft_verify_workspace_bytes(n_seqs: i32, max_nodes: i32, vocab: i32) -> usize;
     fn rivoli_sample_rows_workspace_bytes(n_rows: i32, vocab: i32) -> usize;
 }
@@ -722,6 +755,16 @@ pub fn attend_tree_paged_scratch_floats(n_seqs: usize, h: usize, n_nodes: usize,
     // SAFETY: pure host function, no pointers.
     unsafe {
         rivoli_mla_attend_tree_paged_scratch_floats(n_seqs as i32, h as i32, n_nodes as i32, max_nodes as i32, max_ctx as i32)
+    }
+}
+
+/// f32 elements of the scratch `launch_attend_tree_shared_paged` wants for this shape.
+pub fn attend_tree_shared_paged_scratch_floats(n_seqs: usize, n_groups: usize, h: usize, n_nodes: usize, max_nodes: usize,
+                                               max_prefix: usize, max_ctx: usize) -> usize {
+    // SAFETY: pure host function, no pointers.
+    unsafe {
+        rivoli_mla_attend_tree_shared_paged_scratch_floats(n_seqs as i32, n_groups as i32, h as i32, n_nodes as i32,
+                                                           max_nodes as i32, max_prefix as i32, max_ctx as i32)
     }
 }
 

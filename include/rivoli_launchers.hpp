@@ -78,6 +78,7 @@ RIVOLI_LAUNCHER(launch_index_commit_paged, rivoli_index_commit_paged, "index_com
 RIVOLI_LAUNCHER(launch_norm_rope_rows, rivoli_norm_rope_rows, "norm_rope_rows")
 RIVOLI_LAUNCHER(launch_kv_norm_append_paged, rivoli_kv_norm_append_paged, "kv_norm_append_paged")
 RIVOLI_LAUNCHER(launch_sample_rows, rivoli_sample_rows, "sample_rows")
+RIVOLI_LAUNCHER(launch_attend_tree_shared_paged, rivoli_mla_attend_tree_shared_paged, "mla_attend_tree_shared_paged")
 RIVOLI_LAUNCHER(launch_codec_e4m3_encode, rivoli_codec_e4m3_encode, "codec_e4m3_encode")
 RIVOLI_LAUNCHER(launch_codec_e4m3_dequant_bf16, rivoli_codec_e4m3_dequant_bf16, "codec_e4m3_dequant_bf16")
 RIVOLI_LAUNCHER(launch_codec_bf16_encode, rivoli_codec_bf16_encode, "codec_bf16_encode")
@@ -109,6 +110,10 @@ inline size_t gather_attn_scratch_floats(int m, int h, int d, int topk) {
 
 inline size_t attend_tree_paged_scratch_floats(int n_seqs, int H, int n_nodes, int max_nodes, int max_ctx) {
     return rivoli_mla_attend_tree_paged_scratch_floats(n_seqs, H, n_nodes, max_nodes, max_ctx);
+}
+inline size_t attend_tree_shared_paged_scratch_floats(int n_seqs, int n_groups, int H, int n_nodes, int max_nodes, int max_prefix,
+                                                      int max_ctx) {
+    return rivoli_mla_attend_tree_shared_paged_scratch_floats(n_seqs, n_groups, H, n_nodes, max_nodes, max_prefix, max_ctx);
 }
 inline size_t draft_verify_workspace_bytes(int n_seqs, int max_nodes, int vocab) {
     return rivoli_draft_verify_workspace_bytes(n_seqs, max_nodes, vocab);

@@ -19,12 +19,13 @@ LAUNCH_PATH = os.path.join(CSRC, "pylaunch.so")
 KERNELS = ["kv_append.hip", "kv_gather.hip", "index_topk.hip", "index_score.hip", "mla_attend.hip",
            "act_quant.hip", "kv_compress.hip", "kv_ring.hip", "gather_attn.hip", "hash_rows.hip",
            "block_index.hip", "rope.hip", "mla_attend_tree.hip", "draft_verify.hip", "kv_commit.hip",
-           "norm_rope.hip", "sample.hip"]
+           "norm_rope.hip", "sample.hip", "mla_attend_shared.hip"]
 # Matrix-instruction results in ordinary registers: the 8-bit attention kernel keeps its 128
 # accumulators there and its q terms in the accumulation registers (mla_attend_f8.hpp); the bf16
 # kernels of the same file time the same either way.
 EXTRA_FLAGS = {"mla_attend.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
-               "mla_attend_tree.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+               "mla_attend_tree.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+               "mla_attend_shared.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 HOST_SOURCES = ["pagepool.cpp"]
 # Kernels whose design rests on "no scratch memory": source file -> (substring of the mangled
 # name, suffix of it) of each family. The 8-bit attention kernels and those of 16 and 32 heads a workgroup
@@ -36,7 +37,8 @@ NO_SCRATCH = {"mla_attend.hip": [("mla_attend_paged_kernel", "Lb1EEEvNS_10Attend
                                  ("mla_attend_heads16_kernel", "EEEvNS_10AttendArgsE"),
                                  ("mla_attend_few_kernel", "EEEvNS_10AttendArgsE"),
                                  ("mla_attend_wide_kernel", "EEEvNS_10AttendArgsE")],
-              "mla_attend_tree.hip": [("mla_attend_tree_kernel", "EEEvNS_8TreeArgsE")]}
+              "mla_attend_tree.hip": [("mla_attend_tree_kernel", "EEEvNS_8TreeArgsE")],
+              "mla_attend_shared.hip": [("mla_attend_shared_kernel", "EEEvNS_10SharedArgsE")]}
 
 
 def check_resources(k: str, report: str) -> None:
@@ -60,7 +62,7 @@ def check_resources(k: str, report: str) -> None:
 
 # Kernels whose register copies the compiler has put in front of a join's exec restore, where a wave that took the branch with no lane
 # enabled skips them: their listing is searched for such work, and the build refuses to produce one that has it.
-JOINS = ["mla_attend_tree.hip"]
+JOINS = ["mla_attend_tree.hip", "mla_attend_shared.hip"]
 
 
 def early_vector_work(listing: str) -> list[tuple[str, str]]:

@@ -1,4 +1,4 @@
-// Tree attention for rows of 512 + 64 codes on the matrix cores, included by mla_attend_tree.hip.
+// Tree attention for rows of 512 + 64 codes on the matrix cores, included by mla_attend_tree.hip and, for its tiles' work, mla_attend_shared.hip.
 //
 // What bounds it: of a tile of 64 tokens 64 rows of q need 64 * 64 * (576 + 512) multiply-adds, 2 176 cycles of a compute unit's four
 // matrix cores at 512 a cycle, while its LDS moves 128 bytes a cycle. So no operand may pass through LDS more often than
@@ -184,10 +184,11 @@ __device__ __forceinline__ uint32_t numbers_only(uint32_t c) {
 }
 
 // Tiles [tile_lo, tile_hi) of rows 64 rb .. of a sequence. `whole`: they are all it has, results go out; else its record.
-// `number`: a count of the tiles the workgroup has had, for the flag.
-template <bool RUNS>
+// `number`: a count of the tiles the workgroup has had, for the flag. PARTS: the rows of `s` are cached from row `first` of the sequence on, whole pages in front of
+// them; `cached`: they are those rows alone, and the nodes' own none of them.
+template <bool RUNS, bool PARTS = false>
 __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeShared> sh, const TreeSeq& s, int seq, int rb, bool last_block,
-                                          int tile_lo, int tile_hi, bool whole, float* rec, int& number) {
+                                          int tile_lo, int tile_hi, bool whole, float* rec, int& number, int first = 0, bool cached = false) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int half = lane >> 5, n32 = lane & 31;
     const int th = wave & 1, kh = wave >> 1;  // its 32 tokens and its half of the dims, in the scores
@@ -196,7 +197,7 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
     const int rows = s.nodes * a.H;           // of the sequence
     // what the block's last row may see: a chain's later nodes are nobody's business here
     const int last_row = min(kTreeRows * rb + kTreeRows, rows) - 1;
-    const int len = a.masks ? s.ctx + s.nodes : s.ctx + last_row / a.H + 1;
+    const int len = PARTS && cached ? s.ctx : a.masks ? s.ctx + s.nodes : s.ctx + last_row / a.H + 1;
     const int n_tiles = min(tile_hi, (len + kTreeTokens - 1) / kTreeTokens) - tile_lo;
     const int lift = n_tiles < 64 ? 0 : min(26 - __builtin_clz((unsigned)n_tiles), kTreeMostLift);
 
@@ -205,7 +206,8 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
     // and a row's page and its place in it move on by a tile's tokens without a division. RUNS: pages are whole runs of 16 rows, so that the
     // wave's rows have one page and one place, which are scalar.
     const int l8 = lane & 7, r8 = lane >> 3;
-    const int end_row = min(len, tile_hi * kTreeTokens);
+    const int at_row = PARTS ? first : 0;
+    const int end_row = at_row + min(len, tile_hi * kTreeTokens);
     const int* const table = a.block_table + (size_t)seq * a.max_blocks;
     const unsigned page_tokens = (unsigned)a.page_tokens, on_pages = kTreeTokens / page_tokens, on_rows = kTreeTokens % page_tokens;
     constexpr int kRuns = RUNS ? 1 : 2;
@@ -213,7 +215,7 @@ __device__ __forceinline__ void tree_part(const TreeArgs& a, const lds_ptr<TreeS
     unsigned block[kRuns], place[kRuns];      // of it; and of the next when that has been looked up
 #pragma unroll
     for (int o = 0; o < kRuns; ++o) {
-        token[o] = tile_lo * kTreeTokens + 16 * wave + (RUNS ? 0 : 8 * o + r8);
+        token[o] = at_row + tile_lo * kTreeTokens + 16 * wave + (RUNS ? 0 : 8 * o + r8);
         block[o] = (unsigned)token[o] / page_tokens, place[o] = (unsigned)token[o] - block[o] * page_tokens;
     }
     int no_lane = 0;                          // (a vector zero: the page is a load of every lane, not a scalar one, which LDS reads would wait for)

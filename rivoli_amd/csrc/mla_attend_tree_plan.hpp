@@ -42,6 +42,28 @@ static inline TreePlan tree_plan(int n_seqs, int H, int n_nodes, int max_nodes, 
     p.groups = (int)(groups < kTreeGroups ? groups : kTreeGroups);
     return p;
 }
+
+// The same of a call whose sequences share prefixes (mla_attend_shared.hip): `blocks` are the sequences' own. All of it is cut, by the most tiles that there may be; a block's
+// record has a place of its own behind those of the work items. `groups` 0: more than 31 bits count, the call goes as one that shares nothing.
+struct SharedPlan {
+    long long blocks, records;
+    int groups;
+};
+static inline SharedPlan shared_plan(int n_seqs, int n_groups, int H, int n_nodes, int max_nodes, int max_prefix, int max_ctx) {
+    SharedPlan p{0, 0, 0};
+    if (n_seqs <= 0 || n_groups <= 0 || H <= 0 || n_nodes <= 0 || max_nodes <= 0 || max_prefix < 0 || max_ctx < 0) return p;
+    const long long by_seq = ((long long)max_nodes * H + kTreeRows - 1) / kTreeRows * n_seqs;
+    const long long by_node = (long long)n_nodes * H / kTreeRows + (n_seqs < n_nodes ? n_seqs : n_nodes);
+    p.blocks = by_seq < by_node ? by_seq : by_node;
+    const long long shared = (long long)n_nodes * H / kTreeRows + (n_groups < n_nodes ? n_groups : n_nodes);
+    const long long tiles = ((long long)max_ctx + max_nodes + kTreeTokens - 1) / kTreeTokens, shared_tiles = ((long long)max_prefix + kTreeTokens - 1) / kTreeTokens;
+    const long long most = p.blocks * tiles + shared * shared_tiles;
+    if (most + kTreeBeginTiles * (p.blocks + shared) >= 1ll << 31) return p;
+    const long long groups = most <= kTreeFewTiles ? most : most / kTreeMinTiles > kTreeFewTiles ? most / kTreeMinTiles : kTreeFewTiles;
+    p.groups = (int)(groups < kTreeGroups ? groups : kTreeGroups);
+    p.records = 2 * p.groups + p.blocks + shared;
+    return p;
+}
 static inline size_t tree_scratch_floats(const TreePlan& p) { return (size_t)p.groups * 2 * kTreeRecordFloats; }
 
 }  // namespace rk

@@ -105,6 +105,7 @@ PyMethodDef kEntries[] = {
     ENTRY(rivoli_norm_rope_rows),
     ENTRY(rivoli_kv_norm_append_paged),
     ENTRY(rivoli_sample_rows),
+    ENTRY(rivoli_mla_attend_tree_shared_paged),
     ENTRY(rivoli_codec_e4m3_encode), ENTRY(rivoli_codec_e4m3_dequant_bf16), ENTRY(rivoli_codec_bf16_encode),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "pylaunch", nullptr, -1, kEntries, nullptr, nullptr, nullptr, nullptr};

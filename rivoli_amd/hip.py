@@ -85,6 +85,7 @@ _SIGNATURES = {
     "rivoli_norm_rope_rows": [_VP] * 7 + [_I] * 8 + [_LL] * 5 + [_F] + [_I] * 4 + [_VP] * 2,
     "rivoli_kv_norm_append_paged": [_VP] * 6 + [_I] + [_LL] + [_I] * 5 + [_F] + [_I] * 2 + [_VP] * 2,
     "rivoli_sample_rows": [_VP] * 6 + [_I] * 2 + [_LL] + [_I] + [_VP] * 4 + [_LL] + [_VP] * 2,
+    "rivoli_mla_attend_tree_shared_paged": [_VP] * 9 + [_I] * 12 + [_F] + [_VP] * 5,
     "rivoli_codec_e4m3_encode": [_VP, _VP, _LL, _VP],
     "rivoli_codec_e4m3_dequant_bf16": [_VP, _F, _VP, _LL, _VP],
     "rivoli_codec_bf16_encode": [_VP, _VP, _LL, _VP],
@@ -99,6 +100,7 @@ _SIZE_SIGNATURES = {
     "rivoli_mla_attend_scratch_floats": [_I, _I],
     "rivoli_gather_attn_scratch_floats": [_I, _I, _I, _I],
     "rivoli_mla_attend_tree_paged_scratch_floats": [_I] * 5,
+    "rivoli_mla_attend_tree_shared_paged_scratch_floats": [_I] * 7,
     "rivoli_draft_verify_workspace_bytes": [_I] * 3,
     "rivoli_sample_rows_workspace_bytes": [_I] * 2,
 }
@@ -534,6 +536,22 @@ def launch_mla_attend_tree_paged(qabs, qrope, pool, block_table, ctx_lens, cu_no
         qabs, qrope, pool, block_table, ctx_lens, cu_nodes, masks, n_seqs, H, n_nodes, max_nodes, max_ctx,
         max_blocks_per_seq, kvl, rope, page_tokens, n_pages, scale, clat, lse, partial, bad_rows, stream),
         "mla_attend_tree_paged")
+
+
+def mla_attend_tree_shared_paged_scratch_floats(n_seqs: int, n_groups: int, H: int, n_nodes: int, max_nodes: int, max_prefix: int,
+                                                max_ctx: int) -> int:
+    return int(lib().rivoli_mla_attend_tree_shared_paged_scratch_floats(n_seqs, n_groups, H, n_nodes, max_nodes, max_prefix, max_ctx))
+
+
+def launch_mla_attend_tree_shared_paged(qabs, qrope, pool, block_table, ctx_lens, cu_nodes, masks, cu_groups, prefix_lens, n_seqs,
+                                        n_groups, H, n_nodes, max_nodes, max_prefix, max_ctx, max_blocks_per_seq, kvl, rope,
+                                        page_tokens, n_pages, scale, clat, lse, partial, bad_rows=None, stream=NULL_STREAM) -> None:
+    """launch_mla_attend_tree_paged for groups of sequences (cu_groups) whose first pages, of prefix_lens rows, are the
+    same: those are attended once for all of a group's rows."""
+    ensure_hip_status(entry.rivoli_mla_attend_tree_shared_paged(
+        qabs, qrope, pool, block_table, ctx_lens, cu_nodes, masks, cu_groups, prefix_lens, n_seqs, n_groups, H, n_nodes, max_nodes,
+        max_prefix, max_ctx, max_blocks_per_seq, kvl, rope, page_tokens, n_pages, scale, clat, lse, partial, bad_rows, stream),
+        "mla_attend_tree_shared_paged")
 
 
 def draft_verify_workspace_bytes(n_seqs: int, max_nodes: int, vocab: int) -> int:

@@ -48,3 +48,25 @@ def test_sample_refusals():
     refused(hip.launch_sample_rows, good, changes)
     assert hip.sample_rows_workspace_bytes(0, 32) == hip.sample_rows_workspace_bytes(4, 0) == hip.sample_rows_workspace_bytes(4, 2 ** 21 + 1) == 0
     assert hip.sample_rows_workspace_bytes(4, 32) >= 4 * hip.sample_rows_workspace_bytes(1, 1) > 0
+
+
+def test_shared_attention_refusals():
+    good = dict(qabs=B, qrope=B, pool=B, block_table=B, ctx_lens=B, cu_nodes=B, masks=None, cu_groups=B, prefix_lens=B, n_seqs=1, n_groups=1, H=16,
+                n_nodes=4, max_nodes=4, max_prefix=64, max_ctx=128, max_blocks_per_seq=3, kvl=512, rope=64, page_tokens=64, n_pages=3, scale=1.0, clat=B,
+                lse=None, partial=B)
+    changes = [(dict([(name, None)]), 1001) for name in ("qabs", "qrope", "pool", "block_table", "ctx_lens", "cu_nodes", "cu_groups", "prefix_lens", "clat",
+                                                        "partial")]
+    changes += [(dict([(name, 0)]), 1001) for name in ("n_seqs", "n_groups", "H", "n_nodes", "max_nodes", "max_blocks_per_seq", "kvl", "rope",
+                                                      "page_tokens", "n_pages")]
+    changes += [(dict(max_ctx=-1), 1001), (dict(max_prefix=-1), 1001), (dict(n_groups=65536), 1002), (dict(n_seqs=65536), 1002), (dict(max_nodes=4097), 1002),
+                (dict(max_ctx=2 ** 31 - 8192), 1002), (dict(n_nodes=2 ** 27), 1002), (dict(page_tokens=2 ** 22 + 4), 1002), (dict(kvl=640), 1004),
+                (dict(kvl=192), 1004), (dict(rope=12), 1004), (dict(page_tokens=6), 1004)]
+    changes += [(dict([(name, B.data_ptr() + 8)]), 1004) for name in ("qabs", "qrope", "pool", "clat", "partial")]
+    refused(hip.launch_mla_attend_tree_shared_paged, good, changes)
+    sizes = hip.mla_attend_tree_shared_paged_scratch_floats
+    record = 64 * (512 + 2)
+    assert sizes(0, 1, 16, 4, 4, 64, 128) == sizes(1, 0, 16, 4, 4, 64, 128) == 0
+    # two records a workgroup, one a block: one of the sequence's own, two that the group's rows may fill
+    assert sizes(1, 1, 16, 4, 4, 64, 125) == (2 * 5 + 1 + 2) * record
+    # past 31 bits of tiles: what the call without groups asks for
+    assert sizes(65535, 1, 128, 2 ** 23, 128, 0, 2 ** 31 - 8193) == hip.mla_attend_tree_paged_scratch_floats(65535, 128, 2 ** 23, 128, 2 ** 31 - 8193)
