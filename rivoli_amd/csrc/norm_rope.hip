@@ -29,145 +29,145 @@ struct NormRopeArgs {
 
 typedef float f32x4n __attribute__((ext_vector_type(4)));
 
-// Eight values of a row that starts on 16 bytes, or of f32 numbers that start anywhere.
-__device__ __forceinline__ void load8(const __bf16* src, float (&v)[8]) {
-    const u32x4 w = *reinterpret_cast<const u32x4*>(src);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[2 * i] = bf16_lo_to_f32(w[i]), v[2 * i + 1] = bf16_hi_to_f32(w[i]);
-}
-__device__ __forceinline__ void load8(const float* src, float (&v)[8]) {
-    typedef f32x4n any __attribute__((aligned(4)));
-    const f32x4n a = *reinterpret_cast<const any*>(src), b = *reinterpret_cast<const any*>(src + 4);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
-}
-__device__ __forceinline__ void store8(__bf16* dst, const float (&v)[8]) {
-    *reinterpret_cast<u32x4*>(dst) = u32x4{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
-}
-__device__ __forceinline__ void store8(float* dst, const float (&v)[8]) {
-    *reinterpret_cast<f32x4n*>(dst) = f32x4n{v[0], v[1], v[2], v[3]};
-    *reinterpret_cast<f32x4n*>(dst + 4) = f32x4n{v[4], v[5], v[6], v[7]};
-}
-
-// A row's values, eight a lane and step: unit u = lane + 64 s of the row's (a row of up to 512 values has 2^lanes_log2 lanes and one step).
-// What is summed over a row stays within its lanes.
-__device__ __forceinline__ float row_sum(float x, int lanes_log2) {
-    for (int k = 0; k < lanes_log2; ++k) x += __shfl_xor(x, 1 << k, kWave);
-    return x;
-}
-
 struct NormRopeRow {
     int norm_n, rope_at, rd, center, half, lanes_log2;
     float eps;
 };
 
+// A lane's eight values of a row: of unit u = lane + 64 s (a row of up to 512 values has 2^lanes_log2 lanes and one step) they are 8 u ..; where pairs are
+// halves apart, units of the part that is turned have four values of either half instead, so that pairs meet in a lane.
+struct Piece {
+    int lo, hi;                  // where its first and its last four begin
+    int pairs;                   // of them the first in the table's row, as numbers; negative: nothing is turned
+    bool apart;
+};
+__device__ __forceinline__ Piece piece_of(const NormRopeRow& p, int unit) {
+    const int o = 8 * unit - p.rope_at;
+    const bool turned = o >= 0 && o < p.rd, apart = turned && p.half;
+    Piece r;
+    r.lo = apart ? p.rope_at + o / 2 : 8 * unit;
+    r.hi = apart ? r.lo + p.rd / 2 : r.lo + 4;
+    r.pairs = turned ? o : -1, r.apart = apart;
+    return r;
+}
+__device__ __forceinline__ void load8(const __bf16* row, const Piece& at, float (&v)[8]) {
+    u32x4 w;
+    if (at.apart) {
+        const u32x2 a = *reinterpret_cast<const u32x2*>(row + at.lo), b = *reinterpret_cast<const u32x2*>(row + at.hi);
+        w = u32x4{a.x, a.y, b.x, b.y};
+    } else {
+        w = *reinterpret_cast<const u32x4*>(row + at.lo);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[2 * i] = bf16_lo_to_f32(w[i]), v[2 * i + 1] = bf16_hi_to_f32(w[i]);
+}
+__device__ __forceinline__ void load8(const float* row, const Piece& at, float (&v)[8]) {
+    typedef f32x4n any __attribute__((aligned(4)));
+    const f32x4n a = *reinterpret_cast<const any*>(row + at.lo), b = *reinterpret_cast<const any*>(row + at.hi);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
+}
+__device__ __forceinline__ void store8(__bf16* row, const Piece& at, const float (&v)[8]) {
+    const u32x4 w = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
+    if (at.apart) {
+        *reinterpret_cast<u32x2*>(row + at.lo) = u32x2{w.x, w.y};
+        *reinterpret_cast<u32x2*>(row + at.hi) = u32x2{w.z, w.w};
+    } else {
+        *reinterpret_cast<u32x4*>(row + at.lo) = w;
+    }
+}
+__device__ __forceinline__ void store8(float* row, const Piece& at, const float (&v)[8]) {
+    *reinterpret_cast<f32x4n*>(row + at.lo) = f32x4n{v[0], v[1], v[2], v[3]};
+    *reinterpret_cast<f32x4n*>(row + at.hi) = f32x4n{v[4], v[5], v[6], v[7]};
+}
+
+// A sum over a row's lanes, in each of them: neighbours, pairs, quads and eights by instruction operands, sixteens and halves of the wave by swaps.
+template <int CTRL>
+__device__ __forceinline__ float lane_of(float x) {
+    return __uint_as_float((uint32_t)__builtin_amdgcn_mov_dpp((int)__float_as_uint(x), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float row_sum(float x, int lanes_log2) {
+    if (lanes_log2 > 0) x += lane_of<0xb1>(x);   // quad_perm [1, 0, 3, 2]
+    if (lanes_log2 > 1) x += lane_of<0x4e>(x);   // quad_perm [2, 3, 0, 1]
+    if (lanes_log2 > 2) x += lane_of<0x141>(x);  // row_half_mirror
+    if (lanes_log2 > 3) x += lane_of<0x140>(x);  // row_mirror
+    if (lanes_log2 > 4) {
+        const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    }
+    if (lanes_log2 > 5) {
+        const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    }
+    return x;
+}
+
 template <int S>
-__device__ __forceinline__ void norm_row(const NormRopeRow& p, int lane, float (&v)[S][8], const float (&w)[S][8], const float (&b)[S][8]) {
+__device__ __forceinline__ void norm_row(const NormRopeRow& p, const Piece (&at)[S], float (&v)[S][8], const float (&w)[S][8], const float (&b)[S][8]) {
     const float n = (float)p.norm_n;
+    const auto in = [&](int s, int i) { return (i < 4 ? at[s].lo : at[s].hi) < p.norm_n; };  // (borders are eights': four values are in or out)
     float c = 0.0f;
     if (p.center) {
         float sum = 0.0f;
 #pragma unroll
         for (int s = 0; s < S; ++s)
-            if (8 * (lane + kWave * s) < p.norm_n) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) sum += v[s][i];
-            }
+            for (int i = 0; i < 8; ++i) sum += in(s, i) ? v[s][i] : 0.0f;
         c = row_sum(sum, p.lanes_log2) / n;
     }
     float sum = 0.0f;
 #pragma unroll
     for (int s = 0; s < S; ++s)
-        if (8 * (lane + kWave * s) < p.norm_n) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[s][i] -= c, sum = __builtin_fmaf(v[s][i], v[s][i], sum);
+        for (int i = 0; i < 8; ++i) {
+            const float d = in(s, i) ? v[s][i] - c : 0.0f;
+            sum = __builtin_fmaf(d, d, sum);
         }
     const float r = 1.0f / sqrtf(row_sum(sum, p.lanes_log2) / n + p.eps);
 #pragma unroll
     for (int s = 0; s < S; ++s)
-        if (8 * (lane + kWave * s) < p.norm_n) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[s][i] = __builtin_fmaf(v[s][i] * r, w[s][i], b[s][i]);
-        }
+        for (int i = 0; i < 8; ++i) v[s][i] = in(s, i) ? __builtin_fmaf((v[s][i] - c) * r, w[s][i], b[s][i]) : v[s][i];
 }
 
-// Every lane of the row must be here: halves that belong together are in other lanes.
 template <int S>
-__device__ __forceinline__ void rotate_row(const NormRopeRow& p, int lane, float (&v)[S][8], const float (&turn)[S][16]) {
-    if (!p.half) {
+__device__ __forceinline__ void rotate_row(const NormRopeRow& p, const Piece (&at)[S], float (&v)[S][8], const float (&turn)[S][8]) {
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
-            const int o = 8 * (lane + kWave * s) - p.rope_at;
-            if (o >= 0 && o < p.rd) {
+    for (int s = 0; s < S; ++s)
+        if (at[s].pairs >= 0) {
 #pragma unroll
-                for (int i = 0; i < 8; i += 2) {
-                    const float x = v[s][i], y = v[s][i + 1], c = turn[s][i], n = turn[s][i + 1];
-                    v[s][i] = x * c - y * n, v[s][i + 1] = x * n + y * c;
+            for (int i = 0; i < 4; ++i) {
+                const float c = turn[s][2 * i], n = turn[s][2 * i + 1];
+                if (p.half) {
+                    const float x = v[s][i], y = v[s][i + 4];
+                    v[s][i] = x * c - y * n, v[s][i + 4] = x * n + y * c;
+                } else {
+                    const float x = v[s][2 * i], y = v[s][2 * i + 1];
+                    v[s][2 * i] = x * c - y * n, v[s][2 * i + 1] = x * n + y * c;
                 }
             }
         }
-        return;
-    }
-    const int apart = p.rd / 16;  // units
-    float other[S][8];
-#pragma unroll
-    for (int s = 0; s < S; ++s) {
-        const int unit = lane + kWave * s, o = 8 * unit - p.rope_at;
-        const int from = 2 * o < p.rd ? unit + apart : unit - apart;  // (of no matter where nothing is rotated)
-        const int at = (int)(threadIdx.x & 63) - lane + (from & (S == 1 ? (1 << p.lanes_log2) - 1 : kWave - 1));
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            other[s][i] = __shfl(v[0][i], at, kWave);
-            if constexpr (S > 1) {
-                const float more = __shfl(v[1][i], at, kWave);
-                if (from >= kWave) other[s][i] = more;
-            }
-        }
-    }
-#pragma unroll
-    for (int s = 0; s < S; ++s) {
-        const int o = 8 * (lane + kWave * s) - p.rope_at;
-        if (o >= 0 && o < p.rd) {
-            const bool first = 2 * o < p.rd;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float c = turn[s][2 * i], n = turn[s][2 * i + 1];
-                v[s][i] = first ? v[s][i] * c - other[s][i] * n : other[s][i] * n + v[s][i] * c;
-            }
-        }
-    }
 }
 
-// The lane's part of the table's row: four pairs, or the eight of a half.
+// The lane's four pairs of the table's row.
 template <int S>
-__device__ __forceinline__ void turns_of(const NormRopeRow& p, const float* row, int lane, float (&turn)[S][16]) {
+__device__ __forceinline__ void turns_of(const Piece (&at)[S], const float* row, float (&turn)[S][8]) {
 #pragma unroll
-    for (int s = 0; s < S; ++s) {
-        const int o = 8 * (lane + kWave * s) - p.rope_at;
-        if (o < 0 || o >= p.rd) continue;
-        float a[8];
-        if (p.half) {
-            const float* const from = row + 2 * (2 * o < p.rd ? o : o - p.rd / 2);
-            float b[8];
-            load8(from, a), load8(from + 8, b);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) turn[s][i] = a[i], turn[s][8 + i] = b[i];
-        } else {
-            load8(row + o, a);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) turn[s][i] = a[i];
-        }
-    }
+    for (int s = 0; s < S; ++s)
+        if (at[s].pairs >= 0) load8(row, Piece{at[s].pairs, at[s].pairs + 4, 0, false}, turn[s]);
 }
 
+// The lane's weights or biases: eight numbers, or four and four, of those that there are.
 template <int S>
-__device__ __forceinline__ void weights_of(const NormRopeRow& p, const float* from, float otherwise, int lane, float (&w)[S][8]) {
+__device__ __forceinline__ void weights_of(const NormRopeRow& p, const Piece (&at)[S], const float* from, float otherwise, float (&w)[S][8]) {
+    typedef f32x4n any __attribute__((aligned(4)));
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-        const int at = 8 * (lane + kWave * s);
+        f32x4n a = {otherwise, otherwise, otherwise, otherwise}, b = a;
+        if (from && at[s].lo < p.norm_n) a = *reinterpret_cast<const any*>(from + at[s].lo);
+        if (from && at[s].hi < p.norm_n) b = *reinterpret_cast<const any*>(from + at[s].hi);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w[s][i] = otherwise;
-        if (from && at < p.norm_n) load8(from + at, w[s]);
+        for (int i = 0; i < 4; ++i) w[s][i] = a[i], w[s][4 + i] = b[i];
     }
 }
 
@@ -184,14 +184,17 @@ __global__ __launch_bounds__(256) void norm_rope_rows_kernel(const NormRopeArgs 
     const int token = past ? 0 : (int)token_of;
     const NormRopeRow p{a.norm_n, a.rope_at, a.rd, a.center, a.half, a.lanes_log2, a.eps};
     const TX* const x = static_cast<const TX*>(a.x) + (long long)token * a.x_token;
+    Piece part[S];
+    bool there[S];
+#pragma unroll
+    for (int s = 0; s < S; ++s) part[s] = piece_of(p, lane + kWave * s), there[s] = 8 * (lane + kWave * s) < a.width;
     float v[HEADS][S][8];
 #pragma unroll
     for (int k = 0; k < HEADS; ++k)
 #pragma unroll
         for (int s = 0; s < S; ++s) {
-            const int unit = 8 * (lane + kWave * s);
             // (a head past the last re-reads the last)
-            if (unit < a.width) load8(x + (long long)min(h0 + k * a.groups, a.n_heads - 1) * a.x_head + unit, v[k][s]);
+            if (there[s]) load8(x + (long long)min(h0 + k * a.groups, a.n_heads - 1) * a.x_head, part[s], v[k][s]);
             else
                 for (int i = 0; i < 8; ++i) v[k][s][i] = 0.0f;
         }
@@ -200,26 +203,24 @@ __global__ __launch_bounds__(256) void norm_rope_rows_kernel(const NormRopeArgs 
     const bool bad = (a.rd && (unsigned)pos >= (unsigned)a.n_positions) || (a.slots && slot >= a.n_slots);
     const bool skip = past || bad || slot < 0;
     if (!past && bad && slot >= 0 && a.bad && lane == 0 && h0 == 0) atomicAdd(a.bad, 1u);
-    float turn[S][16], w[S][8], b[S][8];
-    if (a.rd) turns_of<S>(p, a.table + (size_t)(skip ? 0 : pos) * a.rd, lane, turn);
-    if (a.weight_head == 0) weights_of<S>(p, a.weight, 1.0f, lane, w), weights_of<S>(p, a.bias, 0.0f, lane, b);
+    float turn[S][8], w[S][8], b[S][8];
+    if (a.rd) turns_of<S>(part, a.table + (size_t)(skip ? 0 : pos) * a.rd, turn);
+    if (a.weight_head == 0) weights_of<S>(p, part, a.weight, 1.0f, w), weights_of<S>(p, part, a.bias, 0.0f, b);
     TO* const out = static_cast<TO*>(a.out) + (long long)slot * a.out_token;
 #pragma unroll
     for (int k = 0; k < HEADS; ++k) {
         const int h = h0 + k * a.groups;
         if (a.weight_head != 0) {
             const long long of = (long long)min(h, a.n_heads - 1) * a.weight_head;
-            weights_of<S>(p, a.weight ? a.weight + of : nullptr, 1.0f, lane, w);
-            weights_of<S>(p, a.bias ? a.bias + of : nullptr, 0.0f, lane, b);
+            weights_of<S>(p, part, a.weight ? a.weight + of : nullptr, 1.0f, w);
+            weights_of<S>(p, part, a.bias ? a.bias + of : nullptr, 0.0f, b);
         }
-        norm_row<S>(p, lane, v[k], w, b);
-        if (a.rd) rotate_row<S>(p, lane, v[k], turn);
+        norm_row<S>(p, part, v[k], w, b);
+        if (a.rd) rotate_row<S>(p, part, v[k], turn);
         if (skip || h >= a.n_heads) continue;
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
-            const int unit = 8 * (lane + kWave * s);
-            if (unit < a.width) store8(out + (long long)h * a.out_head + unit, v[k][s]);
-        }
+        for (int s = 0; s < S; ++s)
+            if (there[s]) store8(out + (long long)h * a.out_head, part[s], v[k][s]);
     }
 }
 
@@ -336,24 +337,25 @@ __global__ __launch_bounds__(256) void kv_norm_append_kernel(const NormAppendArg
     const unsigned token = blockIdx.x * 4u + (threadIdx.x >> 6);
     if (token >= (unsigned)a.n_tokens) return;
     const TX* const x = static_cast<const TX*>(a.x) + (long long)token * a.x_stride;
-    float v[S][8], w[S][8], b[S][8], turn[S][16];
+    Piece part[S];
+    float v[S][8], w[S][8], b[S][8], turn[S][8];
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-        const int unit = 8 * (lane + kWave * s);
-        if (unit < a.width) load8(x + unit, v[s]);
+        part[s] = piece_of(a.row, lane + kWave * s);
+        if (8 * (lane + kWave * s) < a.width) load8(x, part[s], v[s]);
         else
             for (int i = 0; i < 8; ++i) v[s][i] = 0.0f;
     }
-    weights_of<S>(a.row, a.weight, 1.0f, lane, w), weights_of<S>(a.row, nullptr, 0.0f, lane, b);
+    weights_of<S>(a.row, part, a.weight, 1.0f, w), weights_of<S>(a.row, part, nullptr, 0.0f, b);
     const int slot = a.slots[token], pos = a.positions[token];
     if (slot < 0) return;
     if (slot >= a.n_slots || (unsigned)pos >= (unsigned)a.n_positions) {
         if (a.bad && lane == 0) atomicAdd(a.bad, 1u);
         return;
     }
-    turns_of<S>(a.row, a.table + (size_t)pos * a.row.rd, lane, turn);
-    norm_row<S>(a.row, lane, v, w, b);
-    rotate_row<S>(a.row, lane, v, turn);
+    turns_of<S>(part, a.table + (size_t)pos * a.row.rd, turn);
+    norm_row<S>(a.row, part, v, w, b);
+    rotate_row<S>(a.row, part, v, turn);
     float top = 0.0f;
 #pragma unroll
     for (int s = 0; s < S; ++s)
@@ -365,8 +367,11 @@ __global__ __launch_bounds__(256) void kv_norm_append_kernel(const NormAppendArg
     uint8_t* const pg = a.pool + (size_t)page * a.page_bytes;
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-        const int unit = 8 * (lane + kWave * s);
-        if (unit < a.width) *reinterpret_cast<u32x2*>(pg + (size_t)off * a.width + unit) = codes8(v[s], scl, rinv);
+        if (8 * (lane + kWave * s) >= a.width) continue;
+        uint8_t* const to = pg + (size_t)off * a.width;
+        const u32x2 codes = codes8(v[s], scl, rinv);
+        if (part[s].apart) *reinterpret_cast<uint32_t*>(to + part[s].lo) = codes.x, *reinterpret_cast<uint32_t*>(to + part[s].hi) = codes.y;
+        else *reinterpret_cast<u32x2*>(to + part[s].lo) = codes;
     }
     if (lane == 0) *reinterpret_cast<float*>(pg + (size_t)a.page_tokens * a.width + 4 * (size_t)off) = scl;
 }
