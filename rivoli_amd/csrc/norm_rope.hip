@@ -130,6 +130,10 @@ __device__ __forceinline__ void norm_row(const NormRopeRow& p, const Piece (&at)
         for (int i = 0; i < 8; ++i) v[s][i] = in(s, i) ? __builtin_fmaf((v[s][i] - c) * r, w[s][i], b[s][i]) : v[s][i];
 }
 
+// (Written out: every kernel rounds the same products.)
+__device__ __forceinline__ void turn_pair(float x, float y, float c, float n, float& re, float& im) {
+    re = __builtin_fmaf(x, c, -(y * n)), im = __builtin_fmaf(x, n, y * c);
+}
 template <int S>
 __device__ __forceinline__ void rotate_row(const NormRopeRow& p, const Piece (&at)[S], float (&v)[S][8], const float (&turn)[S][8]) {
 #pragma unroll
@@ -140,10 +144,10 @@ __device__ __forceinline__ void rotate_row(const NormRopeRow& p, const Piece (&a
                 const float c = turn[s][2 * i], n = turn[s][2 * i + 1];
                 if (p.half) {
                     const float x = v[s][i], y = v[s][i + 4];
-                    v[s][i] = x * c - y * n, v[s][i + 4] = x * n + y * c;
+                    turn_pair(x, y, c, n, v[s][i], v[s][i + 4]);
                 } else {
                     const float x = v[s][2 * i], y = v[s][2 * i + 1];
-                    v[s][2 * i] = x * c - y * n, v[s][2 * i + 1] = x * n + y * c;
+                    turn_pair(x, y, c, n, v[s][2 * i], v[s][2 * i + 1]);
                 }
             }
         }
@@ -267,7 +271,9 @@ __global__ __launch_bounds__(kWave) void norm_rope_any_kernel(const NormRopeArgs
             const bool first = a.half ? o < apart : o % 2 == 0;
             const float y = row[first ? i + (a.half ? apart : 1) : i - (a.half ? apart : 1)];
             const f32x2 turn = reinterpret_cast<const f32x2*>(a.table)[(size_t)pos * apart + (a.half ? (first ? o : o - apart) : o / 2)];
-            v = first ? v * turn.x - y * turn.y : y * turn.y + v * turn.x;
+            float other;
+            if (first) turn_pair(v, y, turn.x, turn.y, v, other);
+            else turn_pair(y, v, turn.x, turn.y, other, v);
         }
         out[i] = (TO)v;
     }
@@ -313,17 +319,20 @@ struct NormAppendArgs {
 };
 
 // Eight codes of values under a scale. The quotient is a product by the reciprocal, corrected by its residual; the hardware's conversion has the
-// rule's result but below 2^-6, where the rule rounds halves away.
+// rule's result but below 2^-6, where the rule rounds halves away, and for what is no number. Both show in the quotients' bits: without their sign and less one, so that a
+// zero is the largest (a zero goes the long way, to the same code).
 __device__ __forceinline__ u32x2 codes8(const float (&v)[8], float scl, float rinv) {
     float q[8];
-    bool plain = row_scale_is_fast(scl);
+    uint32_t low = 0xffffffffu, high = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const float q0 = v[i] * rinv;
         q[i] = __builtin_fmaf(-__builtin_fmaf(q0, scl, -v[i]), rinv, q0);
-        plain &= e4m3_hw_exact_domain(q[i]);
+        const uint32_t size = (__float_as_uint(q[i]) << 1) - 1u;
+        low = min(low, size), high = max(high, size);
     }
-    if (plain) return u32x2{e4m3x4_hw(q[0], q[1], q[2], q[3]), e4m3x4_hw(q[4], q[5], q[6], q[7])};
+    constexpr uint32_t kLeast = (0x3c800000u << 1) - 1u, kInfinite = 0xff000000u;  // of 2^-6
+    if (low >= kLeast && high < kInfinite && row_scale_is_fast(scl)) return u32x2{e4m3x4_hw(q[0], q[1], q[2], q[3]), e4m3x4_hw(q[4], q[5], q[6], q[7])};
     uint32_t lo = 0, hi = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -378,6 +387,81 @@ __global__ __launch_bounds__(256) void kv_norm_append_kernel(const NormAppendArg
     if (lane == 0) *reinterpret_cast<float*>(pg + (size_t)a.page_tokens * a.width + 4 * (size_t)off) = scl;
 }
 
+// The same for many rows of 512 + 64: sixteen lanes a token, which have four latent pieces each and half of them one of the others (a wave a token has its 72 pieces in two
+// steps of 64). A lane's latent pieces lie in pairs, whose codes are 16 bytes.
+// 8 192 rows of bf16 8.3 us, 2.0 TB/s, a wave a token 11.5 (eight lanes a token 9.2); 16 000 11.7, 17.0 (12.4); 4 096 5.9, 6.8; but 2 048 5.4, 5.1, and 1 024 5.4, 4.9: the empty launch and a
+// chain of loads, sums, quotients and stores are some 4 us of each. Half of the rest is the quotients' and codes' instructions.
+constexpr int kManyTokens = 16;            // a workgroup's
+constexpr int kWaveTokens = 2048;          // up to so many a call, a wave has each
+template <class TX>
+__global__ __launch_bounds__(256) void kv_norm_append_many_kernel(const NormAppendArgs a) {
+    const int lane = threadIdx.x & 15;
+    const unsigned token = blockIdx.x * (unsigned)kManyTokens + (threadIdx.x >> 4);
+    const bool past = token >= (unsigned)a.n_tokens, has_roped = lane < 8;
+    const TX* const x = static_cast<const TX*>(a.x) + (past ? 0ll : (long long)token * a.x_stride);
+    const auto begin_of = [&](int s) { return 256 * (s >> 1) + 16 * lane + 8 * (s & 1); };
+    Piece roped;
+    roped.lo = 512 + (a.row.half ? 4 : 8) * (lane & 7), roped.hi = roped.lo + (a.row.half ? 32 : 4), roped.pairs = 8 * (lane & 7), roped.apart = a.row.half != 0;
+    float v[5][8], w[4][8], turn[8];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) load8(x, Piece{begin_of(s), begin_of(s) + 4, -1, false}, v[s]);
+    if (has_roped) load8(x, roped, v[4]);
+    const int slot = past ? -1 : a.slots[token], pos = past ? 0 : a.positions[token];
+    const bool bad = slot >= a.n_slots || (unsigned)pos >= (unsigned)a.n_positions, skip = slot < 0 || bad;
+    if (slot >= 0 && bad && a.bad && lane == 0) atomicAdd(a.bad, 1u);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+        if (a.weight) load8(a.weight, Piece{begin_of(s), begin_of(s) + 4, 0, false}, w[s]);
+        else
+            for (int i = 0; i < 8; ++i) w[s][i] = 1.0f;
+    }
+    if (has_roped) load8(a.table + (size_t)(skip ? 0 : pos) * 64, Piece{roped.pairs, roped.pairs + 4, 0, false}, turn);
+    // (pieces' sums in the order in which a wave adds them up: a token's row is the same by either kernel)
+    float of[2];
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+        float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum[0] = __builtin_fmaf(v[2 * g][i], v[2 * g][i], sum[0]), sum[1] = __builtin_fmaf(v[2 * g + 1][i], v[2 * g + 1][i], sum[1]);
+        of[g] = row_sum(sum[0] + sum[1], 4);
+    }
+    const float r = 1.0f / sqrtf((of[0] + of[1]) / 512.0f + a.row.eps);
+    float top = 0.0f;
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            v[s][i] = __builtin_fmaf(v[s][i] * r, w[s][i], 0.0f);
+            top = fmaxf(top, fabsf(v[s][i]));
+        }
+    if (has_roped) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float& p = a.row.half ? v[4][i] : v[4][2 * i];
+            float& q = a.row.half ? v[4][i + 4] : v[4][2 * i + 1];
+            turn_pair(p, q, turn[2 * i], turn[2 * i + 1], p, q);
+            top = fmaxf(top, fmaxf(fabsf(p), fabsf(q)));
+        }
+    }
+    top = fmaxf(top, lane_of<0xb1>(top)), top = fmaxf(top, lane_of<0x4e>(top)), top = fmaxf(top, lane_of<0x141>(top)), top = fmaxf(top, lane_of<0x140>(top));
+    if (skip) return;
+    const float scl = top > 0.0f ? top / 448.0f : 1.0f, rinv = 1.0f / scl;
+    const int page = slot / a.page_tokens, off = slot - page * a.page_tokens;
+    uint8_t* const pg = a.pool + (size_t)page * a.page_bytes;
+    uint8_t* const to = pg + (size_t)off * 576;
+#pragma unroll
+    for (int s = 0; s < 4; s += 2) {
+        const u32x2 one = codes8(v[s], scl, rinv), two = codes8(v[s + 1], scl, rinv);
+        *reinterpret_cast<u32x4*>(to + begin_of(s)) = u32x4{one.x, one.y, two.x, two.y};
+    }
+    if (has_roped) {
+        const u32x2 codes = codes8(v[4], scl, rinv);
+        if (roped.apart) *reinterpret_cast<uint32_t*>(to + roped.lo) = codes.x, *reinterpret_cast<uint32_t*>(to + roped.hi) = codes.y;
+        else *reinterpret_cast<u32x2*>(to + roped.lo) = codes;
+    }
+    if (lane == 8) *reinterpret_cast<float*>(pg + (size_t)a.page_tokens * 576 + 4 * (size_t)off) = scl;
+}
+
 }  // namespace rk
 
 extern "C" int rivoli_norm_rope_rows(const void* x, void* out, const float* weight, const float* bias, const float* table,
@@ -426,7 +510,11 @@ extern "C" int rivoli_kv_norm_append_paged(const void* x, const int* slot_mappin
     const dim3 grid((unsigned)((n_tokens + 3) / 4)), block(256);
     const hipStream_t st = (hipStream_t)stream;
     (void)hipGetLastError();
-    if (width > 512) {
+    if (kvl == 512 && rope == 64 && n_tokens > rk::kWaveTokens) {
+        const dim3 many((unsigned)((n_tokens + rk::kManyTokens - 1) / rk::kManyTokens));
+        if (bf16) rk::launch_kernel(rk::kv_norm_append_many_kernel<__bf16>, many, block, 0, st, a);
+        else rk::launch_kernel(rk::kv_norm_append_many_kernel<float>, many, block, 0, st, a);
+    } else if (width > 512) {
         if (bf16) rk::launch_kernel(rk::kv_norm_append_kernel<__bf16, 2>, grid, block, 0, st, a);
         else rk::launch_kernel(rk::kv_norm_append_kernel<float, 2>, grid, block, 0, st, a);
     } else {

@@ -200,6 +200,35 @@ def test_append_against_the_formula_and_the_rule(oracle, tokens, kvl, rope, page
     assert (got == expect).all()
 
 
+@pytest.mark.parametrize("bf16", [True, False])
+@pytest.mark.parametrize("half", [True, False])
+def test_a_prompts_rows_are_those_of_its_parts(half, bf16):
+    """Many tokens take another kernel: every token's row is the same to the bit, whatever the call it comes in."""
+    tokens, page = 2500, 48
+    x, weight, _, table, positions = inputs(11, tokens, 1, 576, 512, 64, bf16)
+    x[7], x[8, 0, :512], x[9, 0, 100], x[10, 0, 540], x[11] = 0.0, 0.0, np.inf, np.nan, x[11] * 1e-30
+    rng = np.random.default_rng(12)
+    n_pages = -(-tokens // page) + 2
+    slots = rng.permutation(n_pages * page)[:tokens].astype(np.int32)
+    slots[4], slots[2100], positions[9], slots[2499], positions[2300] = -1, n_pages * page, 97, -5, -1
+    held = rng.integers(0, 256, n_pages * page * 580, dtype=np.uint8)
+    xs, w, tb = dev(bits(x, bf16)), dev(weight), dev(table)
+    pos, at = dev(positions), dev(slots)
+    size = 576 * (2 if bf16 else 4)
+
+    def append(pool, bad, lo, hi, weight):
+        hip.launch_kv_norm_append_paged(xs.data_ptr() + lo * size, at.data_ptr() + 4 * lo, weight, tb, pos.data_ptr() + 4 * lo, pool, hi - lo, 576, 512, 64,
+                                        97, page, n_pages, EPS, half, bf16, bad)
+
+    for weights in (w, None):
+        whole, parts, bad, bad_parts = dev(held), dev(held), dzeros(4), dzeros(4)
+        append(whole, bad, 0, tokens, weights)
+        for lo, hi in ((0, 1), (1, 40), (40, 2048), (2048, tokens)):
+            append(parts, bad_parts, lo, hi, weights)
+        assert (back(whole) == back(parts)).all()
+        assert back(bad, np.uint32)[0] == back(bad_parts, np.uint32)[0] == 3
+
+
 def test_a_captured_step_replays():
     torch = torch_cuda()
     x, weight, _, table, positions = inputs(5, 32, 1, 576, 512, 64, True)
