@@ -64,6 +64,11 @@ static inline SharedPlan shared_plan(int n_seqs, int n_groups, int H, int n_node
     p.records = 2 * p.groups + p.blocks + shared;
     return p;
 }
+// Records, then what the merge goes by: a head, and a note of each group and block, of 8 numbers each.
+constexpr int kSharedNoteFloats = 8;
+static inline size_t shared_scratch_floats(const SharedPlan& p, int n_groups) {
+    return (size_t)p.records * kTreeRecordFloats + (size_t)kSharedNoteFloats * (size_t)(1 + n_groups + p.records - 2 * p.groups);
+}
 static inline size_t tree_scratch_floats(const TreePlan& p) { return (size_t)p.groups * 2 * kTreeRecordFloats; }
 
 }  // namespace rk

@@ -66,7 +66,7 @@ def test_shared_attention_refusals():
     sizes = hip.mla_attend_tree_shared_paged_scratch_floats
     record = 64 * (512 + 2)
     assert sizes(0, 1, 16, 4, 4, 64, 128) == sizes(1, 0, 16, 4, 4, 64, 128) == 0
-    # two records a workgroup, one a block: one of the sequence's own, two that the group's rows may fill
-    assert sizes(1, 1, 16, 4, 4, 64, 125) == (2 * 5 + 1 + 2) * record
+    # two records a workgroup, one a block (one of the sequence's own, two that the group's rows may fill), eight numbers for each of these, the group and the call
+    assert sizes(1, 1, 16, 4, 4, 64, 125) == (2 * 5 + 1 + 2) * record + 8 * (1 + 2 + 1 + 1)
     # past 31 bits of tiles: what the call without groups asks for
     assert sizes(65535, 1, 128, 2 ** 23, 128, 0, 2 ** 31 - 8193) == hip.mla_attend_tree_paged_scratch_floats(65535, 128, 2 ** 23, 128, 2 ** 31 - 8193)
