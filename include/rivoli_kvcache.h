@@ -558,10 +558,11 @@ int rivoli_mla_attend_tree_paged(const unsigned short* qabs, const unsigned shor
 
 /* rivoli_mla_attend_tree_paged for sequences of which whole groups have the same first pages (a common prompt): group g's sequences are cu_groups[g] .. cu_groups[g+1] (ascending,
  * n_groups + 1 entries; sequences in front of the first and behind the last share nothing), whose block tables name the same pages for the whole pages among their first prefix_lens[g]
- * cached rows (which of them is read is not said). Those are attended once for all rows of the group, the rest by sequence; results as without groups but for the order of sums. A decode step
- * is one node a sequence (max_nodes 1, masks null), ctx_lens the rows in front of its own. A sequence whose ctx_lens is less than those pages' rows is by itself. prefix_lens[g] <=
- * max_prefix: what is past it is not shared. Tokens of shared pages that are not there are counted once a group. Few heads gain most: their sequences' rows share blocks of 64. Equal calls
- * give equal bits. `partial`: as there, of rivoli_mla_attend_tree_shared_paged_scratch_floats(same sizes) floats, never null for rows of 512 + 64; other widths, and calls of 2^31 tiles and more, go
+ * cached rows (which of them is read is not said). Where those fill enough fewer blocks of 64 rows (node, head) together than sequence by sequence - few heads, many sequences, long
+ * prefixes; a rule on the device-side lengths - they are attended once for all rows of the group; results as without groups but for the order of sums. A decode step is one node a sequence (max_nodes 1,
+ * masks null), ctx_lens the rows in front of its own. A sequence whose ctx_lens is less than those pages' rows is by itself. prefix_lens[g] <= max_prefix: what is past it is not
+ * shared. Tokens of shared pages that are not there are counted once a group, or once a sequence where those are attended by sequence. Equal calls give equal bits.
+ * `partial`: as there, of rivoli_mla_attend_tree_shared_paged_scratch_floats(same sizes) floats, never null for rows of 512 + 64; other widths, and calls of 2^31 tiles and more, go
  * through rivoli_mla_attend_tree_paged. Guards: as there; 1001 also cu_groups or prefix_lens null, n_groups <= 0, max_prefix < 0; 1002 n_groups > 65535. */
 size_t rivoli_mla_attend_tree_shared_paged_scratch_floats(int n_seqs, int n_groups, int H, int n_nodes, int max_nodes,
                                                           int max_prefix, int max_ctx);

@@ -37,17 +37,32 @@ __device__ __forceinline__ SharedGroup shared_group(const SharedArgs& a, int g) 
     r.lo = min(max(a.cu_groups[g], 0), a.n_seqs), r.hi = min(max(a.cu_groups[g + 1], r.lo), a.n_seqs);
     return r;
 }
-// The cached rows that it shares: whole pages, and none that is a sequence alone.
-__device__ __forceinline__ int shared_rows(const SharedArgs& a, int g, const SharedGroup& of) {
-    const int held = min(max(a.prefix_lens[g], 0), a.max_prefix);
-    return of.hi - of.lo < 2 ? 0 : held - held % a.page_tokens;
+// Its nodes, all of its sequences'.
+__device__ __forceinline__ int2 shared_nodes(const SharedArgs& a, const SharedGroup& of) {
+    const int node0 = min(max(a.cu_nodes[of.lo], 0), a.n_nodes);
+    return int2{node0, min(max(a.cu_nodes[of.hi], node0), a.n_nodes) - node0};
+}
+// What is to be gained before a group's pages are attended apart, in tiles of a block: of each block of the group's rows, whose sums are written and read once more, and of a
+// group. In us, shared and by sequence: 64 sequences of 16 heads behind 4 096 rows 48 and 60 (3 072 tiles saved, 16 blocks), 64 of 32 heads 55 and 62 (2 048; 32), 32 of 48
+// heads in two groups behind 8 192 56 and 59 (512; 12 each), 64 of 16 heads behind 256 33 and 29 (192; 16), 2 behind 4 096 30 and 24 (64; 1), 32 of 64 heads behind 1 024 35
+// and 31, 256 of 64 heads in 16 groups behind 512 106 and 56 (none saved).
+constexpr long long kSharedBlockGain = 24, kSharedGroupGain = 256;
+// The cached rows that a group shares: whole pages, where its rows fill enough fewer blocks together than sequence by sequence (as if its nodes were theirs evenly).
+__device__ __forceinline__ int shared_rows(const SharedArgs& a, int g, const SharedGroup& of, int nodes) {
+    int held = min(max(a.prefix_lens[g], 0), a.max_prefix);
+    held -= held % a.page_tokens;
+    const unsigned seqs = (unsigned)(of.hi - of.lo), rows = (unsigned)nodes * (unsigned)a.H;
+    if (seqs < 2) return 0;
+    const long long together = (rows + kTreeRows - 1) / kTreeRows, apart = (long long)seqs * (((rows + seqs - 1) / seqs + kTreeRows - 1) / kTreeRows);
+    const long long tiles = ((long long)held + kTreeTokens - 1) / kTreeTokens;
+    return (apart - together) * tiles > kSharedBlockGain * together + kSharedGroupGain ? held : 0;
 }
 __device__ __forceinline__ SharedPart shared_of_group(const SharedArgs& a, int g) {
     const SharedGroup of = shared_group(a, g);
+    const int2 nodes = shared_nodes(a, of);
     SharedPart p;
-    p.s.ctx = shared_rows(a, g, of);
-    p.s.node0 = min(max(a.cu_nodes[of.lo], 0), a.n_nodes);
-    p.s.nodes = min(max(a.cu_nodes[of.hi], p.s.node0), a.n_nodes) - p.s.node0;
+    p.s.ctx = shared_rows(a, g, of, nodes.y);
+    p.s.node0 = nodes.x, p.s.nodes = nodes.y;
     p.seq = min(of.lo, a.n_seqs - 1), p.first = 0, p.group = g;
     return p;
 }
@@ -59,7 +74,7 @@ struct SharedGroups {
     __device__ __forceinline__ explicit SharedGroups(const SharedArgs& a) {
         if (!FEW) return;
         const int g = min((int)(threadIdx.x & 63), a.n_groups - 1);
-        of = shared_group(a, g), rows = shared_rows(a, g, of);
+        of = shared_group(a, g), rows = shared_rows(a, g, of, shared_nodes(a, of).y);
     }
     // The group that a sequence is of and what it shares there (nothing: of none): the number of those that end in front of it.
     __device__ __forceinline__ int find(const SharedArgs& a, int seq, int& shared) const {
@@ -77,7 +92,10 @@ struct SharedGroups {
                 else hi = mid;
             }
             shared = 0;
-            if (g < a.n_groups && a.cu_groups[g] <= seq) shared = shared_rows(a, g, shared_group(a, g));
+            if (g < a.n_groups && a.cu_groups[g] <= seq) {
+                const SharedGroup in = shared_group(a, g);
+                shared = shared_rows(a, g, in, shared_nodes(a, in).y);
+            }
             return g;
         }
     }

@@ -86,6 +86,97 @@ def test_more_groups_than_lanes(n_groups):
            masks="chain").check()
 
 
+def many(n, prefix, step=3, at=0, nodes=lambda i: 1):
+    """A group large enough for its pages to be attended apart from its sequences' own: (cached rows, nodes) of each."""
+    return [prefix + at + step * i for i in range(n)], [nodes(i) for i in range(n)]
+
+
+@pytest.mark.parametrize("masks", ["chain", "tree", "empty"])
+def test_groups_that_pay(masks):
+    """Rows of many sequences in shared blocks: some that end within the prefix, begin, or have no nodes; one beside a small group; sequences of no group."""
+    ctx, nodes = many(32, 1000)
+    Shared(60, [0, 32], [1000], ctx, nodes, 8, masks=masks).check()
+    ctx, nodes = many(40, 1024, nodes=lambda i: i % 3)
+    ctx[5], ctx[6], ctx[7], nodes[5] = 1023, 100, 0, 2
+    more, more_nodes = many(30, 900, at=10, nodes=lambda i: 1 + i % 2)
+    Shared(61, [2, 42, 44, 74], [1024, 64, 900], [300, 7] + ctx + [100, 70] + more + [500], [1, 3] + nodes + [1, 1] + more_nodes + [2], 8, masks=masks).check()
+
+
+@pytest.mark.parametrize("page", [4, 16, 48, 60, 128, 256])
+def test_groups_that_pay_in_pages_of_any_size(page):
+    ctx, nodes = many(32, 1290, nodes=lambda i: 1 + i % 2)
+    Shared(page + 1, [0, 32], [1290], ctx, nodes, 8, page=page).check()
+
+
+def test_groups_that_pay_among_more_than_lanes():
+    rng = np.random.default_rng(62)
+    sizes = rng.integers(0, 3, 90)
+    sizes[3], sizes[80] = 32, 40
+    prefixes = rng.integers(0, 200, 90)
+    prefixes[3], prefixes[80] = 1000, 900
+    of = np.repeat(np.arange(90), sizes)
+    ctx = prefixes[of] + rng.integers(0, 100, len(of))
+    Shared(62, [int(x) for x in np.concatenate([[0], np.cumsum(sizes)])], [int(x) for x in prefixes], [int(x) for x in ctx], [1] * len(of), 8, masks="chain").check()
+
+
+def test_groups_that_pay_whatever_their_scores():
+    ctx, nodes = many(32, 1000)
+    case = Shared(63, [0, 32], [1000], ctx, nodes, 8, q_scale=1.0)
+    scales = case.pool[:, 64 * 576:].view(np.float32)
+    for page in range(case.n_pages):
+        scales[page] *= np.float32((1.0 if page % 3 else 2.0 ** -12) * (1.0 + page % 7))
+    case.qabs[::2] ^= 0x8000
+    case.check()
+    for scale in (0.0, -0.07, 3.0):
+        case = Shared(64, [0, 32], [1000], ctx, nodes, 8)
+        case.scale = scale
+        case.check()
+
+
+def test_groups_that_pay_with_rows_that_are_not_there():
+    """A shared page outside of the pool is counted once for the group, codes that are no number and scales that are none reach nobody."""
+    ctx, nodes = many(32, 1024)
+    case = Shared(65, [0, 32], [1024], ctx, nodes, 8)
+    case.tables[:, 3] = case.n_pages
+    case.tables[2, 16] = -1                              # the rest of the third's rows, 6 and its node
+    case.check(bad=64 + 7)
+    case = Shared(66, [0, 32], [1024], ctx, nodes, 8)
+    for t, bad in ((0, 0.0), (63, np.nan), (64, -0.0), (127, -np.inf)):
+        case.pool[case.tables[0][t // 64]][64 * 576:].view(np.float32)[t % 64] = bad
+    case.pool[case.tables[0][1]][0:576:5] = 0x7F         # under a scale of none
+    case.pool[case.tables[3][16]][1 * 576:2 * 576:5] = 0x7F  # a row of the fourth's own: its answer alone is none
+    out, _ = case.check()
+
+
+def test_groups_that_pay_from_a_graph_beside_another_stream():
+    torch = torch_cuda()
+    ctx, nodes = many(32, 1024)
+    one, two = (Shared(67 + i, [0, 32, 32], [1024, 0], ctx, nodes, 16, masks="chain") for i in range(2))
+    for c in (one, two):
+        c.buffers()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        one.launch(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        one.launch(torch.cuda.current_stream())
+    for lens, groups, prefixes in ((ctx, [0, 32, 32], [1024, 0]), ([c + 5 for c in ctx], [0, 16, 32], [1024, 1000]), ([1024] * 31 + [3], [1, 31, 32], [1000, 64])):
+        lens = [min(x, max(ctx)) for x in lens]
+        for c in (one, two):
+            c.ctx, c.groups, c.prefixes = (np.array(x, np.int32) for x in (lens, groups, prefixes))
+            for at, x in ((4, c.ctx), (7, c.groups), (8, c.prefixes)):
+                c.dev[at].copy_(dev(x))
+            c.out.fill_(0xEE)
+            c.lse.fill_(0xEE)
+        torch.cuda.synchronize()
+        graph.replay()
+        two.launch(side)
+        torch.cuda.synchronize()
+        one.check(one.results())
+        two.check(two.results())
+
+
 def test_other_widths_go_sequence_by_sequence():
     Shared(3, [0, 2], [64], [90, 140], [4, 2], 6, kvl=256, rope=32).check()
 
@@ -111,11 +202,12 @@ def test_softmax_scales(scale):
     case.check()
 
 
-def test_pages_outside_the_pool_are_left_out_and_counted_once_a_group():
+def test_pages_outside_the_pool_are_left_out_and_counted():
+    """A small group's rows are attended sequence by sequence, and so counted."""
     case = Shared(8, [0, 3], [192], [200, 250, 300], [1, 1, 1], 40)
     case.tables[:, 1] = case.n_pages
     case.tables[2, 4] = -1
-    case.check(bad=64 + 45)
+    case.check(bad=3 * 64 + 45)
 
 
 def test_rows_without_a_scale_and_codes_that_are_no_number():
