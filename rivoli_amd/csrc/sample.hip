@@ -231,13 +231,19 @@ __device__ __forceinline__ float wave_top(float x) {
     const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
-__device__ __forceinline__ u64 wave_upto(u64 x) {  // the lane's and those before
-#pragma unroll
-    for (int off = 1; off < kWave; off <<= 1) {
-        const u64 y = __shfl_up(x, off, kWave);
-        if ((int)(threadIdx.x & 63) >= off) x += y;
-    }
-    return x;
+// The lane's and those before, as wave_inclusive_sum.
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ u64 before64(u64 v) {
+    return ((u64)dpp_or_zero<CTRL, ROW_MASK>((uint32_t)(v >> 32)) << 32) | dpp_or_zero<CTRL, ROW_MASK>((uint32_t)v);
+}
+__device__ __forceinline__ u64 wave_upto(u64 v) {
+    v += before64<0x111, 0xf>(v);
+    v += before64<0x112, 0xf>(v);
+    v += before64<0x114, 0xf>(v);
+    v += before64<0x118, 0xf>(v);
+    v += before64<0x142, 0xa>(v);
+    v += before64<0x143, 0xc>(v);
+    return v;
 }
 // Of a whole workgroup, in every thread.
 template <int WAVES>
@@ -267,7 +273,8 @@ __device__ __forceinline__ u64 all_most(u64 x, u64* room) {
 // Its largest logit, its histogram, and a list of its largest logits, bin by bin as many as there is room for.
 template <bool BF16>
 __global__ __launch_bounds__(kSampleThreads) void sample_chunk_kernel(const SampleArgs a) {
-    __shared__ u64 hist[kSampleBins + kWave];
+    __shared__ u64 hist[kSampleListed + kWave];    // its bins or the list, and a lane's spare place
+    static_assert(kSampleBins <= kSampleListed, "room for either");
     __shared__ SampleTable table;
     __shared__ u64 room[kSampleThreads / kWave];
     __shared__ unsigned upto[kSampleThreads / kWave], n_listed[2], all_count;
@@ -385,16 +392,17 @@ __global__ __launch_bounds__(kSampleThreads) void sample_chunk_kernel(const Samp
         }
 #pragma unroll
         for (int i = 0; i < kSampleItems; ++i)
-            if (v[i] >= least[1]) {
-                const bool top = v[i] >= least[0];
-                list[min(top ? at[0] : at[1], kSampleListed - 1u)] = place_of(v[i], index(i));
-                at[0] += top, at[1] += !top;
-            }
-        lds_barrier();
-        if (tid == 0) {
-            out->cover[0] = cover[0], out->cover[1] = cover[1];
-            out->listed[0] = min(n_listed[0], (unsigned)kSampleList), out->listed[1] = min(n_listed[1], (unsigned)kSampleMore);
+        {   // (without a branch: a lane that has none writes to a spare place of its own)
+            const bool top = v[i] >= least[0], any = v[i] >= least[1];
+            const unsigned to = min(top ? at[0] : at[1], kSampleListed - 1u);
+            hist[any ? to : kSampleListed + (tid & 63)] = (u64)__float_as_uint(v[i]) << 32 | index(i);
+            at[0] += top, at[1] += any & !top;
         }
+        lds_barrier();
+        const unsigned n_first = min(n_listed[0], (unsigned)kSampleList), n_more = min(n_listed[1], (unsigned)kSampleMore);
+        for (unsigned i = tid; i < kSampleList + n_more; i += kSampleThreads)
+            if (i < n_first || i >= kSampleList) list[i] = place_of(__uint_as_float((uint32_t)(hist[i] >> 32)), (unsigned)hist[i]);
+        if (tid == 0) out->cover[0] = cover[0], out->cover[1] = cover[1], out->listed[0] = n_first, out->listed[1] = n_more;
     }
     if (tid == 0) out->weight = weight, out->top = grid.top, out->most = most, out->first = 0, out->count = all_count;
 }
@@ -483,49 +491,65 @@ struct Pick {
             const int b = bin_of(r, logit_of(p));
             if (is && b >= lo && b <= hi) put(p);
         };
-        const auto has = [&](int c) { return c < a.chunks && sh.listed[0][c] != 0 && sh.top[c] >= lo && sh.cover[1][c] <= lo; };
+        // which chunks have such tokens, and where: a lane has one
+        u64 raw[kSampleMaxChunks / kWave] = {};
 #pragma unroll
-        for (int k = 0; k < kEarly; ++k) {
-            const int c = wave + k * kPickWaves;
-            if (has(c))
+        for (int base = 0; base < kSampleMaxChunks; base += kWave) {
+            if (base >= a.chunks) continue;
+            const int c = base + lane;
+            const unsigned listed = sh.listed[0][c], more = sh.listed[1][c];
+            const bool has = c < a.chunks && listed != 0 && sh.top[c] >= lo, both = sh.cover[1][c] <= lo, first = sh.cover[0][c] <= lo;
+            raw[base / kWave] = __builtin_amdgcn_ballot_w64(has && !both);
+            // the wave's own of those that are listed: every eighth
+            const u64 mine = 0x0101010101010101ull << wave;
+            const u64 lists = __builtin_amdgcn_ballot_w64(has && both) & mine, seconds = __builtin_amdgcn_ballot_w64(has && both && !first) & mine;
+            static_assert(kPickWaves == 8, "every eighth chunk is a wave's");
+            if (base == 0) {
 #pragma unroll
-                for (int i = 0; i < kListed; ++i) use(early.p[k][i], (unsigned)(lane + kWave * i) < sh.listed[0][c] - 1);
-        }
-#pragma unroll 1
-        for (int c = wave; c < a.chunks; c += kPickWaves) {
-            if (!has(c)) continue;
-            if (c >= kEarly * kPickWaves) {
-                u64 p[kListed];
-                list_of(c, p);
+                for (int k = 0; k < kEarly; ++k) {
+                    const int at = wave + k * kPickWaves;
+                    if (lists >> at & 1) {
+                        const unsigned n = (unsigned)__builtin_amdgcn_readlane((int)listed, at) - 1;
 #pragma unroll
-                for (int i = 0; i < kListed; ++i) use(p[i], (unsigned)(lane + kWave * i) < sh.listed[0][c] - 1);
-            }
-            if (sh.cover[0][c] > lo) {
-                const u64* const from = a.list + ((size_t)row * a.chunks + c) * kSampleListed + kSampleList;
-                const unsigned n = sh.listed[1][c];
-                constexpr int kEach = 8;
-#pragma unroll 1
-                for (unsigned i0 = 0; i0 < n; i0 += kEach * kWave) {
-                    u64 p[kEach];
-#pragma unroll
-                    for (int i = 0; i < kEach; ++i) p[i] = from[i0 + kWave * i + lane];
-#pragma unroll
-                    for (int i = 0; i < kEach; ++i) use(p[i], i0 + kWave * i + lane < n);
+                        for (int i = 0; i < kListed; ++i) use(early.p[k][i], (unsigned)(lane + kWave * i) < n);
+                    }
                 }
             }
+            for (u64 left = base == 0 ? lists >> (kEarly * kPickWaves) << (kEarly * kPickWaves) : lists; left; left &= left - 1) {
+                const int at = __builtin_ctzll(left);
+                const unsigned n = (unsigned)__builtin_amdgcn_readlane((int)listed, at) - 1;
+                u64 p[kListed];
+                list_of(base + at, p);
+#pragma unroll
+                for (int i = 0; i < kListed; ++i) use(p[i], (unsigned)(lane + kWave * i) < n);
+            }
+            for (u64 left = seconds; left; left &= left - 1) {
+                const int at = __builtin_ctzll(left);
+                const unsigned n = (unsigned)__builtin_amdgcn_readlane((int)more, at);
+                const u64* const from = a.list + ((size_t)row * a.chunks + base + at) * kSampleListed + kSampleList;
+                constexpr int kEach = kSampleMore / kWave;
+                u64 p[kEach];
+#pragma unroll
+                for (int i = 0; i < kEach; ++i) p[i] = from[kWave * i + lane];
+#pragma unroll
+                for (int i = 0; i < kEach; ++i) use(p[i], (unsigned)(kWave * i + lane) < n);
+            }
         }
-        // the chunks that have more, by all threads, two of them on their way at once
+        // the chunks that have more than is listed, by all threads, two of them on their way at once
         // (as they are: a NaN is in no range, what counts as the most is in the top bin, past which nothing is: a NaN)
         const float least_x = fmaxf(least_of(r, lo), __uint_as_float(__float_as_uint(-r.most) - 1)), past_x = hi >= grid.top ? __uint_as_float(0x7fc00000u) : least_of(r, hi + 1);
         constexpr int kChunks = 2, kLoads = kSampleChunk / (N * kPickThreads);
 #pragma unroll 1
         for (int c0 = 0; c0 < a.chunks; c0 += kChunks) {
+            u64 of = raw[0];
+#pragma unroll
+            for (int w = 1; w < kSampleMaxChunks / kWave; ++w) of = c0 / kWave == w ? raw[w] : of;
+            if ((of >> (c0 % kWave) & ((1 << kChunks) - 1)) == 0) continue;
             Logits<BF16> v[kChunks][kLoads];
             bool asked[kChunks];
 #pragma unroll
             for (int k = 0; k < kChunks; ++k) {
-                const int c = min(c0 + k, a.chunks - 1);
-                asked[k] = c0 + k < a.chunks && sh.listed[0][c] != 0 && sh.top[c] >= lo && sh.cover[1][c] > lo;
+                asked[k] = of >> ((c0 + k) % kWave) & 1;
                 if (asked[k])
 #pragma unroll
                     for (int j = 0; j < kLoads; ++j)
@@ -760,14 +784,15 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
         // ---- the row's histogram
         // (no branches: what has no bin goes to spare ones, a lane's own)
         for (int c0 = 0;;) {
-            int tops[kAtOnce];
-            unsigned there[kAtOnce];
-#pragma unroll
-            for (int j = 0; j < kAtOnce; ++j) tops[j] = sh.top[min(c0 + j, kSampleMaxChunks - 1)], there[j] = sh.listed[0][min(c0 + j, kSampleMaxChunks - 1)];
+            // (a chunk's top is a scalar)
+            const int top_of = sh.top[min(c0 + (tid & (kAtOnce - 1)), kSampleMaxChunks - 1)];
+            const unsigned there_of = sh.listed[0][min(c0 + (tid & (kAtOnce - 1)), kSampleMaxChunks - 1)];
 #pragma unroll
             for (int j = 0; j < kAtOnce; ++j) {
-                const int b = SampleGrid(tops[j]).least(tid), number = grid.of(b);
-                const bool in = c0 + j < a.chunks && there[j] != 0 && counts[j] != 0 && number < kSampleBins;
+                const SampleGrid of(__builtin_amdgcn_readlane(top_of, j));
+                const bool there = c0 + j < a.chunks && __builtin_amdgcn_readlane((int)there_of, j) != 0;
+                const int b = of.least(tid), number = grid.of(b);
+                const bool in = there && counts[j] != 0 && number < kSampleBins;
                 const int to = in ? number : kSampleBins + (tid & 63);
                 atomicAdd(&sh.count[to], counts[j]);
                 if (weighed) {
@@ -1011,36 +1036,28 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
 }
 
 // ---- the third, where probabilities are asked for -------------------------------------------------------------------
+// A chunk whose list has all of its tokens that are kept is not read again: zeros, and those of the list over them.
+// 256 rows of 131 072 fp32 logits, most of them cut to a few tokens: 31 us, 4.3 TB/s written (all chunks read again: 42).
 template <bool BF16>
 __global__ __launch_bounds__(kSampleThreads) void sample_probs_kernel(const SampleArgs a) {
     __shared__ SampleTable table;
     constexpr int N = Logits<BF16>::N, kLoads = kSampleItems / N;
     const int row = blockIdx.x / a.chunks, c = blockIdx.x - row * a.chunks, tid = threadIdx.x;
-    Logits<BF16> v[kLoads];
-#pragma unroll
-    for (int j = 0; j < kLoads; ++j) v[j].load(a.logits, (long long)row * a.stride, c * kSampleChunk + N * (tid + j * kSampleThreads), a.vocab);
-    const SampleRow r = sample_row(a, row);
     const SampleEnd end = a.end[row];
-    make_table(table, r);
-    lds_barrier();
+    const SampleChunk of = a.chunk[blockIdx.x];
+    const SampleRow r = sample_row(a, row);
     float* const out = a.probs + (long long)row * a.probs_stride;
     const float least = end.cut ? logit_of(end.cut) : -FLT_MAX;
-#pragma unroll
-    for (int j = 0; j < kLoads; ++j) {
-        const int at = c * kSampleChunk + N * (tid + j * kSampleThreads);
-        float p[N];
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            p[i] = 0.0f;
-            const float x = logit(r, v[j][i]);
-            if (end.kind == 1) p[i] = at + i == end.token ? 1.0f : 0.0f;
-            if (end.kind == 2 && x >= least && place_of(x, (unsigned)(at + i)) >= end.cut) {
-                const float t = x * r.inv_h, floor_t = floorf(t);
-                p[i] = (float)(rounded_in(r, t - floor_t) * (table.of(end.top - (int)floor_t) * (1 / kBinOne)) * end.inv);
-            }
-        }
-        typedef float f32x4v __attribute__((ext_vector_type(4)));
-        typedef f32x4v words __attribute__((aligned(4)));
+    const int cut_bin = bin_of(r, least);
+    const bool none = end.kind != 2 || of.count == 0 || (end.cut && of.top < cut_bin);
+    const bool listed = none || (end.cut && of.cover[1] <= cut_bin);
+    typedef float f32x4v __attribute__((ext_vector_type(4)));
+    typedef f32x4v words __attribute__((aligned(4)));
+    const auto probability = [&](float x) {
+        const float t = x * r.inv_h, floor_t = floorf(t);
+        return (float)(rounded_in(r, t - floor_t) * (table.of(end.top - (int)floor_t) * (1 / kBinOne)) * end.inv);
+    };
+    const auto store = [&](int at, const float* p) {
         if (at + N <= a.vocab) {
 #pragma unroll
             for (int i = 0; i < N; i += 4) *reinterpret_cast<words*>(out + at + i) = f32x4v{p[i], p[i + 1], p[i + 2], p[i + 3]};
@@ -1049,6 +1066,45 @@ __global__ __launch_bounds__(kSampleThreads) void sample_probs_kernel(const Samp
             for (int i = 0; i < N; ++i)
                 if (at + i < a.vocab) out[at + i] = p[i];
         }
+    };
+    if (listed) {
+        constexpr int kEach = (kSampleListed + kSampleThreads - 1) / kSampleThreads;
+        u64 p[kEach];
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+            const int i = tid + k * kSampleThreads;
+            const bool is = !none && (i < kSampleList ? i < (int)of.listed[0] : i - kSampleList < (int)of.listed[1]);
+            p[k] = is ? a.list[(size_t)blockIdx.x * kSampleListed + i] : 0;
+        }
+        if (!none) make_table(table, r);
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+            const float zeros[N] = {};
+            store(c * kSampleChunk + N * (tid + j * kSampleThreads), zeros);
+        }
+        __syncthreads();                   // the zeros are there before what comes over them
+        if (end.kind == 1 && tid == 0 && end.token / kSampleChunk == c) out[end.token] = 1.0f;
+        if (none) return;
+#pragma unroll
+        for (int k = 0; k < kEach; ++k)
+            if (p[k] && p[k] >= end.cut) out[index_of(p[k])] = probability(logit_of(p[k]));
+        return;
+    }
+    Logits<BF16> v[kLoads];
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) v[j].load(a.logits, (long long)row * a.stride, c * kSampleChunk + N * (tid + j * kSampleThreads), a.vocab);
+    make_table(table, r);
+    lds_barrier();
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+        const int at = c * kSampleChunk + N * (tid + j * kSampleThreads);
+        float p[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float x = logit(r, v[j][i]);
+            p[i] = x >= least && place_of(x, (unsigned)(at + i)) >= end.cut ? probability(x) : 0.0f;
+        }
+        store(at, p);
     }
 }
 
