@@ -498,7 +498,7 @@ extern "C" int rivoli_kv_norm_append_paged(const void* x, const int* slot_mappin
     if (!x || !slot_mapping || !table || !positions || !pool || n_tokens <= 0 || kvl <= 0 || rope <= 0 || n_positions <= 0 || page_tokens <= 0 ||
         n_pages <= 0 || !(eps >= 0.0f && eps <= FLT_MAX))
         return 1001;
-    if ((long long)kvl + rope > rk::kNormWidth || n_tokens > 1 << 28) return 1002;
+    if ((long long)kvl + rope > rk::kNormWidth || (unsigned)n_tokens > rk::kLaunchThreads / rk::kWave) return 1002;
     const int width = kvl + rope;
     const long long unit = bf16 ? 8 : 4;
     if (width % 16 != 0 || kvl % 8 != 0 || rope % (half ? 16 : 8) != 0 || page_tokens % 4 != 0 || x_stride % unit != 0 || !rk::aligned16(x) ||
