@@ -560,7 +560,7 @@ int rivoli_mla_attend_tree_paged(const unsigned short* qabs, const unsigned shor
  * n_groups + 1 entries; sequences in front of the first and behind the last share nothing), whose block tables name the same pages for the whole pages among their first prefix_lens[g]
  * cached rows (which of them is read is not said). Where those fill enough fewer blocks of 64 rows (node, head) together than sequence by sequence - few heads, many sequences, long
  * prefixes; a rule on the device-side lengths - they are attended once for all rows of the group; results as without groups but for the order of sums. A decode step is one node a sequence (max_nodes 1,
- * masks null), ctx_lens the rows in front of its own. A sequence whose ctx_lens is less than those pages' rows is by itself. prefix_lens[g] <= max_prefix: what is past it is not
+ * masks null), ctx_lens the rows in front of its own. A sequence whose ctx_lens is less than those pages' rows is by itself, and its table is not asked for them. prefix_lens[g] <= max_prefix: what is past it is not
  * shared. Tokens of shared pages that are not there are counted once a group, or once a sequence where those are attended by sequence. Equal calls give equal bits.
  * `partial`: as there, of rivoli_mla_attend_tree_shared_paged_scratch_floats(same sizes) floats, never null for rows of 512 + 64; other widths, and calls of 2^31 tiles and more, go
  * through rivoli_mla_attend_tree_paged. Guards: as there; 1001 also cu_groups or prefix_lens null, n_groups <= 0, max_prefix < 0; 1002 n_groups > 65535. */
@@ -636,7 +636,7 @@ int rivoli_norm_rope_rows(const void* x, void* out, const float* weight, const f
 /* rivoli_kv_append_paged of rows that are normed and rotated on the way: of each of the rows x + t * x_stride (kvl + rope values, bf16 != 0: bf16, else
  * f32) the first kvl are normed (as above, without mean and bias), the other `rope` turned by the table's row of positions[t]; scale = amax / 448 (1 where amax is 0) and codes by
  * the append's rule, of the f32 values, to slot_mapping[t]. Slots and positions count as above; two tokens of one slot are outside the contract. Guards: 1001 null (weight
- * may be) / non-positive; 1002 kvl + rope > 1024, n_tokens > 2^28; 1004 kvl + rope not a multiple of 16, kvl of 8, rope of 8 (half: 16), page_tokens of 4,
+ * may be) / non-positive; 1002 kvl + rope > 1024, more tokens than a launch has waves (2^26 - 4); 1004 kvl + rope not a multiple of 16, kvl of 8, rope of 8 (half: 16), page_tokens of 4,
  * x, x_stride or pool not on 16 bytes, table not on 8, weight not on 4. */
 int rivoli_kv_norm_append_paged(const void* x, const int* slot_mapping, const float* weight, const float* table,
                                 const int* positions, unsigned char* pool, int n_tokens, long long x_stride, int kvl,
@@ -649,8 +649,8 @@ int rivoli_kv_norm_append_paged(const void* x, const int* slot_mapping, const fl
  * whose w_v is min_ps[r] or more (the first always). The four arrays may each be null: temperature 1, all kept. tokens[r] = the first v, by index, whose running sum
  * of kept weights exceeds uniforms[r] times their whole (the last kept one when none does). A temperature that is not above 2^-16 takes the first in the order. Logits that are NaN or not
  * above -2^25 temperatures (the type's lowest value, -inf) are never drawn nor kept, those above 2^25 temperatures count as that; a row without any other gets token -1. n_kept[r] (nullable) = how many are kept, logprobs[r] (nullable) = the logarithm
- * of the token's share of their weight (-inf without a token), probs (nullable) + r * probs_stride = every token's share, zero for those not kept: what rivoli_draft_verify takes. Weights and sums have 42 bits below
- * the largest weight or more; what is kept and drawn does not depend on any order of sums: equal calls give equal results.
+ * of the token's share of their weight (-inf without a token), probs (nullable) + r * probs_stride = every token's share, zero for those not kept: what rivoli_draft_verify takes; not over the logits. Weights are rounded
+ * to 2^-36 of themselves, sums to 2^-42 of the largest weight a token; what is kept and drawn does not depend on any order of sums: equal calls give equal results.
  * `workspace`: rivoli_sample_rows_workspace_bytes(n_rows, vocab) bytes, 16-byte aligned, nothing to be cleared; two calls in flight need one each. Guards: 1001 null / non-positive; 1002 n_rows >= 2^22,
  * vocab > 2^21 or above a stride, more rows than a launch has; 1004 rows not on an element, workspace not 16-byte aligned. */
 size_t rivoli_sample_rows_workspace_bytes(int n_rows, int vocab);

@@ -64,6 +64,11 @@ __device__ __forceinline__ SharedPart shared_of_group(const SharedArgs& a, int g
     p.s.ctx = shared_rows(a, g, of, nodes.y);
     p.s.node0 = nodes.x, p.s.nodes = nodes.y;
     p.seq = min(of.lo, a.n_seqs - 1), p.first = 0, p.group = g;
+    // the pages of the first that has so many rows: one that has not (an empty place in a batch) need not name them
+    if (p.s.ctx > 0) {
+        while (p.seq + 1 < of.hi && a.ctx_lens[p.seq] < p.s.ctx) ++p.seq;
+        if (min(a.ctx_lens[p.seq], a.max_ctx) < p.s.ctx) p.s.ctx = 0;
+    }
     return p;
 }
 // The groups. Up to 64 (FEW), a lane has one, which sequences and how many rows they share, so that no lookup waits for another.
@@ -361,6 +366,7 @@ extern "C" int rivoli_mla_attend_tree_shared_paged(const unsigned short* qabs, c
                             max_ctx, max_blocks_per_seq, kvl, rope, kvl + rope, page_tokens, n_pages,
                             (size_t)page_tokens * (size_t)(kvl + rope + 4), qscale, clat, lse, plan.groups, partial, bad_rows},
                            cu_groups, prefix_lens, n_groups, max_prefix, plan.records};
+    if (plan.blocks > (long long)(rk::kLaunchThreads / 256)) return 1002;
     const hipStream_t st = (hipStream_t)stream;
     (void)hipGetLastError();
     const bool runs = page_tokens % 16 == 0, few = n_groups <= rk::kWave;

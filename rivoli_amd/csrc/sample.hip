@@ -408,7 +408,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_chunk_kernel(const Samp
 }
 
 // ---- the second: a row -------------------------------------------------------------------------------------------
-// The chunks' histograms added up say down to which bin there are tokens that may be kept. Mostly they are few: those of the chunks' lists, which are compared each with each (pick_few).
+// The chunks' histograms added up say down to which bin there are tokens that may be kept. Mostly they are few: those of the chunks' lists, which are put in order by counting (few).
 // Else the bins of the cuts are sorted out by themselves, by 512 ranges of places at a time, from lists of their tokens or, where even a bin has more than the list has room for, from the row.
 struct PickShared {
     SampleTable table;

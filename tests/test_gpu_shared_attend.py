@@ -148,6 +148,22 @@ def test_groups_that_pay_with_rows_that_are_not_there():
     out, _ = case.check()
 
 
+def test_groups_that_pay_with_places_that_are_empty():
+    """Sequences that are not there (no rows, no nodes, tables of nothing) or are not as far yet, in front of the group's others and among them; a group of such alone."""
+    ctx, nodes = many(40, 1024)
+    for empty in (0, 1, 7, 39):
+        ctx[empty] = nodes[empty] = 0
+    ctx[2] = 1023
+    case = Shared(80, [0, 40, 42], [1024, 1024], ctx + [0, 1000], nodes + [0, 1], 16)
+    for empty in (0, 1, 7, 39, 40):
+        case.tables[empty] = -1
+    case.tables[2, :3] = case.tables[2, 3:6]             # its own pages in another order
+    case.check(bad=0)
+    ctx, nodes = many(40, 1024)
+    case = Shared(81, [0, 40], [1024], [1000] * 40, nodes, 16)  # as far as nobody is
+    case.check(bad=0)
+
+
 def test_groups_that_pay_from_a_graph_beside_another_stream():
     torch = torch_cuda()
     ctx, nodes = many(32, 1024)

@@ -29,7 +29,7 @@ def test_norm_append_refusals():
                 n_pages=1, eps=1e-6, half=False, bf16=True)
     changes = [(dict([(name, None)]), 1001) for name in ("x", "slot_mapping", "table", "positions", "pool")]
     changes += [(dict([(name, 0)]), 1001) for name in ("n_tokens", "kvl", "rope", "n_positions", "page_tokens", "n_pages")]
-    changes += [(dict(eps=NAN), 1001), (dict(kvl=1024), 1002), (dict(kvl=2 ** 31 - 16), 1002), (dict(n_tokens=2 ** 28 + 1), 1002), (dict(kvl=520), 1004),
+    changes += [(dict(eps=NAN), 1001), (dict(kvl=1024), 1002), (dict(kvl=2 ** 31 - 16), 1002), (dict(n_tokens=2 ** 26), 1002), (dict(kvl=520), 1004),
                 (dict(kvl=508, rope=68), 1004), (dict(kvl=520, rope=56, half=True), 1004), (dict(page_tokens=6), 1004), (dict(x_stride=580), 1004),
                 (dict(x_stride=578, bf16=False), 1004), (dict(x=B.data_ptr() + 8), 1004), (dict(pool=B.data_ptr() + 8), 1004),
                 (dict(table=B.data_ptr() + 4), 1004), (dict(weight=B.data_ptr() + 2), 1004)]
@@ -59,7 +59,7 @@ def test_shared_attention_refusals():
     changes += [(dict([(name, 0)]), 1001) for name in ("n_seqs", "n_groups", "H", "n_nodes", "max_nodes", "max_blocks_per_seq", "kvl", "rope",
                                                       "page_tokens", "n_pages")]
     changes += [(dict(max_ctx=-1), 1001), (dict(max_prefix=-1), 1001), (dict(n_groups=65536), 1002), (dict(n_seqs=65536), 1002), (dict(max_nodes=4097), 1002),
-                (dict(max_ctx=2 ** 31 - 8192), 1002), (dict(n_nodes=2 ** 27), 1002), (dict(page_tokens=2 ** 22 + 4), 1002), (dict(kvl=640), 1004),
+                (dict(max_ctx=2 ** 31 - 8192), 1002), (dict(n_nodes=2 ** 27), 1002), (dict(n_nodes=2 ** 26, max_ctx=0, max_prefix=0, max_nodes=4096, n_seqs=65535), 1002), (dict(page_tokens=2 ** 22 + 4), 1002), (dict(kvl=640), 1004),
                 (dict(kvl=192), 1004), (dict(rope=12), 1004), (dict(page_tokens=6), 1004)]
     changes += [(dict([(name, B.data_ptr() + 8)]), 1004) for name in ("qabs", "qrope", "pool", "clat", "partial")]
     refused(hip.launch_mla_attend_tree_shared_paged, good, changes)
