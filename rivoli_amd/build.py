@@ -131,19 +131,27 @@ def build_kernels(verbose: bool = False) -> str:
             raise RuntimeError("hipcc failed compiling " + k)
         try:
             check_resources(k, res.stderr)
-            if k in JOINS:
-                res = subprocess.run(compile_command(k) + ["--offload-device-only", "-S", os.path.join(CSRC, k), "-o", "-"],
-                                     capture_output=True, text=True)
-                if res.returncode != 0:
-                    raise RuntimeError("hipcc failed listing " + k)
-                check_joins(k, res.stdout)
         except RuntimeError:
             os.remove(obj)  # never link it
             raise
         return obj
 
+    def list_one(k: str, obj: str) -> None:
+        res = subprocess.run(compile_command(k) + ["--offload-device-only", "-S", os.path.join(CSRC, k), "-o", "-"],
+                             capture_output=True, text=True)
+        try:
+            if res.returncode != 0:
+                raise RuntimeError("hipcc failed listing " + k)
+            check_joins(k, res.stdout)
+        except RuntimeError:
+            os.remove(obj)
+            raise
+
     with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as pool:
-        objs = list(pool.map(compile_one, KERNELS))
+        compiled = {k: pool.submit(compile_one, k) for k in KERNELS}
+        for k in JOINS:  # (one after the other, while others compile: the first that fails is the one that is named)
+            list_one(k, compiled[k].result())
+        objs = [compiled[k].result() for k in KERNELS]
     res = subprocess.run([hipcc(), f"--offload-arch={offload_arch()}", "-shared", "-fPIC", "-o", LIB_PATH] + objs,
                          capture_output=True, text=True)
     if verbose or res.returncode != 0:
