@@ -635,7 +635,7 @@ int rivoli_norm_rope_rows(const void* x, void* out, const float* weight, const f
 
 /* rivoli_kv_append_paged of rows that are normed and rotated on the way: of each of the rows x + t * x_stride (kvl + rope values, bf16 != 0: bf16, else
  * f32) the first kvl are normed (as above, without mean and bias), the other `rope` turned by the table's row of positions[t]; scale = amax / 448 (1 where amax is 0) and codes by
- * the append's rule, of the f32 values, to slot_mapping[t]. Slots and positions count as above; two tokens of one slot are outside the contract. Guards: 1001 null (weight
+ * the append's rule to slot_mapping[t], all of it in 64 bits up to these two roundings. Slots and positions count as above; two tokens of one slot are outside the contract. Guards: 1001 null (weight
  * may be) / non-positive; 1002 kvl + rope > 1024, more tokens than a launch has waves (2^26 - 4); 1004 kvl + rope not a multiple of 16, kvl of 8, rope of 8 (half: 16), page_tokens of 4,
  * x, x_stride or pool not on 16 bytes, table not on 8, weight not on 4. */
 int rivoli_kv_norm_append_paged(const void* x, const int* slot_mapping, const float* weight, const float* table,

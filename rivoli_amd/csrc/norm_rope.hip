@@ -303,8 +303,9 @@ static int norm_rope_rows(NormRopeArgs& a, bool wide, hipStream_t st) {
 }
 
 // ---- the latent row into its page -----------------------------------------------------------------------------
-// A wave a token: the row is normed over its latent values and rotated over the others as above, its largest value makes the scale, and the codes
-// are of the f32 values (rivoli_kv_append_paged's rule, whose rows come rounded to bf16 once more).
+// A wave a token: the row is normed over its latent values and rotated over the others as above, and its largest value makes the scale, 448 of which it is; codes are those of the
+// quotients. All of it is in 64 bits up to the scale's rounding and the codes': a row is quantized once, and which of two codes a quotient next to their middle gets is decided by the last
+// bits of f32 and by the order of sums there, some one in a million values. 8 192 rows 9.2 us, in f32 8.3; 32 rows 4.6.
 struct NormAppendArgs {
     const void* x;
     const int* slots;
@@ -318,28 +319,91 @@ struct NormAppendArgs {
     unsigned int* bad;
 };
 
-// Eight codes of values under a scale. The quotient is a product by the reciprocal, corrected by its residual; the hardware's conversion has the
-// rule's result but below 2^-6, where the rule rounds halves away, and for what is no number. Both show in the quotients' bits: without their sign and less one, so that a
-// zero is the largest (a zero goes the long way, to the same code).
-__device__ __forceinline__ u32x2 codes8(const float (&v)[8], float scl, float rinv) {
-    float q[8];
-    uint32_t low = 0xffffffffu, high = 0;
+// Over a row's lanes, in each of them (row_sum's order).
+template <int CTRL>
+__device__ __forceinline__ double lane_of64(double x) {
+    const unsigned long long v = __builtin_bit_cast(unsigned long long, x);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)v, CTRL, 0xf, 0xf, true), hi = (uint32_t)__builtin_amdgcn_mov_dpp((int)(v >> 32), CTRL, 0xf, 0xf, true);
+    return __builtin_bit_cast(double, ((unsigned long long)hi << 32) | lo);
+}
+template <int LANES, class F>
+__device__ __forceinline__ double row_all64(double x, F f) {
+    static_assert(LANES == 16 || LANES == 64, "a row of lanes or the wave");
+    x = f(x, lane_of64<0xb1>(x)), x = f(x, lane_of64<0x4e>(x)), x = f(x, lane_of64<0x141>(x)), x = f(x, lane_of64<0x140>(x));
+    if constexpr (LANES == 64) {
+        const auto halves = [&](auto swap) {
+            const unsigned long long v = __builtin_bit_cast(unsigned long long, x);
+            const auto l = swap((uint32_t)v), h = swap((uint32_t)(v >> 32));
+            x = f(__builtin_bit_cast(double, ((unsigned long long)h[0] << 32) | l[0]), __builtin_bit_cast(double, ((unsigned long long)h[1] << 32) | l[1]));
+        };
+        halves([](uint32_t u) { return __builtin_amdgcn_permlane16_swap(u, u, false, false); });
+        halves([](uint32_t u) { return __builtin_amdgcn_permlane32_swap(u, u, false, false); });
+    }
+    return x;
+}
+template <int LANES>
+__device__ __forceinline__ double row_sum64(double x) {
+    return row_all64<LANES>(x, [](double a, double b) { return a + b; });
+}
+template <int LANES>
+__device__ __forceinline__ double row_top64(double x) {
+    return row_all64<LANES>(x, [](double a, double b) { return fmax(a, b); });
+}
+
+// A latent piece by its weights, before the norm: y = x w; the squares of x.
+__device__ __forceinline__ void weigh_piece(const float (&x)[8], const float (&w)[8], double (&y)[8], double& squares, double& top) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const float q0 = v[i] * rinv;
-        q[i] = __builtin_fmaf(-__builtin_fmaf(q0, scl, -v[i]), rinv, q0);
-        const uint32_t size = (__float_as_uint(q[i]) << 1) - 1u;
-        low = min(low, size), high = max(high, size);
+        const double d = x[i];
+        squares = __builtin_fma(d, d, squares);
+        y[i] = __builtin_fma(d, (double)w[i], 0.0);
+        top = fmax(top, fabs(y[i]));
     }
-    constexpr uint32_t kLeast = (0x3c800000u << 1) - 1u, kInfinite = 0xff000000u;  // of 2^-6
-    if (low >= kLeast && high < kInfinite && row_scale_is_fast(scl)) return u32x2{e4m3x4_hw(q[0], q[1], q[2], q[3]), e4m3x4_hw(q[4], q[5], q[6], q[7])};
-    uint32_t lo = 0, hi = 0;
+}
+__device__ __forceinline__ void turn_piece(const float (&x)[8], const float (&turn)[8], int half, double (&y)[8], double& top) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        lo |= f32_to_e4m3_sw(v[i] / scl) << (8 * i);
-        hi |= f32_to_e4m3_sw(v[4 + i] / scl) << (8 * i);
+        const double one = half ? x[i] : x[2 * i], two = half ? x[i + 4] : x[2 * i + 1], c = turn[2 * i], n = turn[2 * i + 1];
+        const double re = __builtin_fma(one, c, -(two * n)), im = __builtin_fma(one, n, two * c);
+        (half ? y[i] : y[2 * i]) = re, (half ? y[i + 4] : y[2 * i + 1]) = im;
+        top = fmax(top, fmax(fabs(re), fabs(im)));
     }
-    return u32x2{lo, hi};
+}
+// What a row's values are times for their quotients: normed ones and turned ones; and its scale.
+struct RowScale {
+    double normed, turned;
+    float scale;
+    __device__ __forceinline__ RowScale(double squares, double top_normed, double top_turned, int n, float eps) {
+        const double r = 1.0 / sqrt(squares / n + (double)eps), top = fmax(top_normed * r, top_turned);
+        turned = top > 0.0 ? 448.0 / top : 1.0, normed = r * turned;
+        scale = top > 0.0 ? (float)(top / 448.0) : 1.0f;
+    }
+};
+
+// Eight codes of y * by. The hardware's conversion from f32 has the rule's result but below 2^-6, where the rule rounds halves away, and for what is no number; and f32 has the middle
+// of two codes for quotients next to it. These show in the f32 quotients' bits (sizes: without their sign and less one, so that a zero is the largest; it goes the long way, to the same code).
+__device__ __forceinline__ u32x2 codes8(const double (&y)[8], double by) {
+    float q[8];
+    uint32_t low = 0xffffffffu, high = 0, middle = 0xffffffffu;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        q[i] = (float)(y[i] * by);
+        const uint32_t bits = __float_as_uint(q[i]), size = (bits << 1) - 1u;
+        low = min(low, size), high = max(high, size), middle = min(middle, (bits << 12) ^ 0x80000000u);
+    }
+    constexpr uint32_t kLeast = (0x3c800000u << 1) - 1u, kInfinite = 0xff000000u;  // of 2^-6
+    if (low >= kLeast && high < kInfinite && middle != 0) return u32x2{e4m3x4_hw(q[0], q[1], q[2], q[3]), e4m3x4_hw(q[4], q[5], q[6], q[7])};
+    u32x2 codes = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        // in f32 towards zero, the last bit set where that is not all of it: a middle only where it is one
+        const double d = y[i] * by;
+        uint32_t bits = __float_as_uint(q[i]);
+        if (fabs((double)q[i]) > fabs(d)) --bits;
+        if ((double)__uint_as_float(bits) != d) bits |= 1u;
+        codes[i / 4] |= f32_to_e4m3_sw(__uint_as_float(bits)) << (8 * (i & 3));
+    }
+    return codes;
 }
 
 template <class TX, int S>
@@ -349,7 +413,7 @@ __global__ __launch_bounds__(256) void kv_norm_append_kernel(const NormAppendArg
     if (token >= (unsigned)a.n_tokens) return;
     const TX* const x = static_cast<const TX*>(a.x) + (long long)token * a.x_stride;
     Piece part[S];
-    float v[S][8], w[S][8], b[S][8], turn[S][8];
+    float v[S][8], w[S][8], turn[S][8];
 #pragma unroll
     for (int s = 0; s < S; ++s) {
         part[s] = piece_of(a.row, lane + kWave * s);
@@ -357,7 +421,7 @@ __global__ __launch_bounds__(256) void kv_norm_append_kernel(const NormAppendArg
         else
             for (int i = 0; i < 8; ++i) v[s][i] = 0.0f;
     }
-    weights_of<S>(a.row, part, a.weight, 1.0f, w), weights_of<S>(a.row, part, nullptr, 0.0f, b);
+    weights_of<S>(a.row, part, a.weight, 1.0f, w);
     const int slot = a.slots[token], pos = a.positions[token];
     if (slot < 0) return;
     if (slot >= a.n_slots || (unsigned)pos >= (unsigned)a.n_positions) {
@@ -365,31 +429,29 @@ __global__ __launch_bounds__(256) void kv_norm_append_kernel(const NormAppendArg
         return;
     }
     turns_of<S>(part, a.table + (size_t)pos * a.row.rd, turn);
-    norm_row<S>(a.row, part, v, w, b);
-    rotate_row<S>(a.row, part, v, turn);
-    float top = 0.0f;
+    double y[S][8], squares = 0.0, top_normed = 0.0, top_turned = 0.0;
 #pragma unroll
-    for (int s = 0; s < S; ++s)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[s][i]));
-    top = wave_max(top);
-    const float scl = top > 0.0f ? top / 448.0f : 1.0f, rinv = 1.0f / scl;
+    for (int s = 0; s < S; ++s) {
+        if (part[s].pairs >= 0) turn_piece(v[s], turn[s], a.row.half, y[s], top_turned);
+        else weigh_piece(v[s], w[s], y[s], squares, top_normed);
+    }
+    const RowScale by(row_sum64<kWave>(squares), row_top64<kWave>(top_normed), row_top64<kWave>(top_turned), a.row.norm_n, a.row.eps);
     const int page = slot / a.page_tokens, off = slot - page * a.page_tokens;
     uint8_t* const pg = a.pool + (size_t)page * a.page_bytes;
+    uint8_t* const to = pg + (size_t)off * a.width;
 #pragma unroll
     for (int s = 0; s < S; ++s) {
         if (8 * (lane + kWave * s) >= a.width) continue;
-        uint8_t* const to = pg + (size_t)off * a.width;
-        const u32x2 codes = codes8(v[s], scl, rinv);
+        const u32x2 codes = codes8(y[s], part[s].pairs >= 0 ? by.turned : by.normed);
         if (part[s].apart) *reinterpret_cast<uint32_t*>(to + part[s].lo) = codes.x, *reinterpret_cast<uint32_t*>(to + part[s].hi) = codes.y;
         else *reinterpret_cast<u32x2*>(to + part[s].lo) = codes;
     }
-    if (lane == 0) *reinterpret_cast<float*>(pg + (size_t)a.page_tokens * a.width + 4 * (size_t)off) = scl;
+    if (lane == 0) *reinterpret_cast<float*>(pg + (size_t)a.page_tokens * a.width + 4 * (size_t)off) = by.scale;
 }
 
 // The same for many rows of 512 + 64: sixteen lanes a token, which have four latent pieces each and half of them one of the others (a wave a token has its 72 pieces in two
 // steps of 64). A lane's latent pieces lie in pairs, whose codes are 16 bytes.
-// 8 192 rows of bf16 8.3 us, 2.0 TB/s, a wave a token 11.5 (eight lanes a token 9.2); 16 000 11.7, 17.0 (12.4); 4 096 5.9, 6.8; but 2 048 5.4, 5.1, and 1 024 5.4, 4.9: the empty launch and a
+// 8 192 rows of bf16 9.2 us, 1.5 TB/s, a wave a token 14.4; 16 000 14.6 and 22.6; 4 096 6.1 and 8.0; but 2 048 5.5 either way, 1 024 5.4 and 4.7, f32 rows alike: the empty launch and a
 // chain of loads, sums, quotients and stores are some 4 us of each. Half of the rest is the quotients' and codes' instructions.
 constexpr int kManyTokens = 16;            // a workgroup's
 constexpr int kWaveTokens = 2048;          // up to so many a call, a wave has each
@@ -417,49 +479,31 @@ __global__ __launch_bounds__(256) void kv_norm_append_many_kernel(const NormAppe
     }
     if (has_roped) load8(a.table + (size_t)(skip ? 0 : pos) * 64, Piece{roped.pairs, roped.pairs + 4, 0, false}, turn);
     // (pieces' sums in the order in which a wave adds them up: a token's row is the same by either kernel)
-    float of[2];
+    double y[5][8], of[2], top_normed = 0.0, top_turned = 0.0;
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
-        float sum[2] = {0.0f, 0.0f};
-#pragma unroll
-        for (int i = 0; i < 8; ++i) sum[0] = __builtin_fmaf(v[2 * g][i], v[2 * g][i], sum[0]), sum[1] = __builtin_fmaf(v[2 * g + 1][i], v[2 * g + 1][i], sum[1]);
-        of[g] = row_sum(sum[0] + sum[1], 4);
+        double squares[2] = {0.0, 0.0};
+        weigh_piece(v[2 * g], w[2 * g], y[2 * g], squares[0], top_normed);
+        weigh_piece(v[2 * g + 1], w[2 * g + 1], y[2 * g + 1], squares[1], top_normed);
+        of[g] = row_sum64<16>(squares[0] + squares[1]);
     }
-    const float r = 1.0f / sqrtf((of[0] + of[1]) / 512.0f + a.row.eps);
-    float top = 0.0f;
-#pragma unroll
-    for (int s = 0; s < 4; ++s)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            v[s][i] = __builtin_fmaf(v[s][i] * r, w[s][i], 0.0f);
-            top = fmaxf(top, fabsf(v[s][i]));
-        }
-    if (has_roped) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float& p = a.row.half ? v[4][i] : v[4][2 * i];
-            float& q = a.row.half ? v[4][i + 4] : v[4][2 * i + 1];
-            turn_pair(p, q, turn[2 * i], turn[2 * i + 1], p, q);
-            top = fmaxf(top, fmaxf(fabsf(p), fabsf(q)));
-        }
-    }
-    top = fmaxf(top, lane_of<0xb1>(top)), top = fmaxf(top, lane_of<0x4e>(top)), top = fmaxf(top, lane_of<0x141>(top)), top = fmaxf(top, lane_of<0x140>(top));
+    if (has_roped) turn_piece(v[4], turn, a.row.half, y[4], top_turned);
+    const RowScale by(of[0] + of[1], row_top64<16>(top_normed), row_top64<16>(top_turned), 512, a.row.eps);
     if (skip) return;
-    const float scl = top > 0.0f ? top / 448.0f : 1.0f, rinv = 1.0f / scl;
     const int page = slot / a.page_tokens, off = slot - page * a.page_tokens;
     uint8_t* const pg = a.pool + (size_t)page * a.page_bytes;
     uint8_t* const to = pg + (size_t)off * 576;
 #pragma unroll
     for (int s = 0; s < 4; s += 2) {
-        const u32x2 one = codes8(v[s], scl, rinv), two = codes8(v[s + 1], scl, rinv);
+        const u32x2 one = codes8(y[s], by.normed), two = codes8(y[s + 1], by.normed);
         *reinterpret_cast<u32x4*>(to + begin_of(s)) = u32x4{one.x, one.y, two.x, two.y};
     }
     if (has_roped) {
-        const u32x2 codes = codes8(v[4], scl, rinv);
+        const u32x2 codes = codes8(y[4], by.turned);
         if (roped.apart) *reinterpret_cast<uint32_t*>(to + roped.lo) = codes.x, *reinterpret_cast<uint32_t*>(to + roped.hi) = codes.y;
         else *reinterpret_cast<u32x2*>(to + roped.lo) = codes;
     }
-    if (lane == 8) *reinterpret_cast<float*>(pg + (size_t)a.page_tokens * 576 + 4 * (size_t)off) = scl;
+    if (lane == 8) *reinterpret_cast<float*>(pg + (size_t)a.page_tokens * 576 + 4 * (size_t)off) = by.scale;
 }
 
 }  // namespace rk

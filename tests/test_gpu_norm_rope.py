@@ -150,13 +150,39 @@ def test_rows_of_zeros_infinities_and_nans_stay_with_themselves():
         assert np.isnan(got[4, 0]).all() and np.isnan(got[3, 1]).any()
 
 
+def nearest_codes(v):
+    """The 8-bit codes nearest to a row's values under its scale, in 64 bits: the even one of two, below 2^-6 the larger."""
+    top = np.abs(v).max()
+    q = np.abs(v) * (448 / top) if top > 0 else np.abs(v)
+    values = e4m3_values()[:127].astype(np.float64)
+    middles = (values[1:] + values[:-1]) / 2
+    low, high = np.searchsorted(middles, q), np.searchsorted(middles, q, side="right")  # (they differ at a middle alone)
+    code = np.where((low % 2 == 0) & (q >= 2.0 ** -6), low, high)
+    return np.where(np.signbit(v), code + 128, code).astype(np.uint8)
+
+
+@pytest.mark.parametrize("tokens,half,bf16", [(6000, True, True), (6000, False, False), (2000, False, True), (1900, True, False)])
+def test_codes_next_to_a_middle(tokens, half, bf16):
+    """A few of a million quotients lie where sums in 32 bits decide: the codes are those of 64."""
+    x, weight, _, table, positions = inputs(40 + tokens, tokens, 1, 576, 512, 64, bf16)
+    x[5, 0, 512:576], x[6] = np.where(np.arange(64) % 2, 1.0, 1 + 2.0 ** -6), np.float32(2.0 ** 66) * (1 + np.arange(576) % 3)  # products that cancel; squares past 32 bits
+    slots, n_pages = np.arange(tokens, dtype=np.int32), -(-tokens // 64)
+    pool = dev(np.zeros((n_pages, 64 * 580), np.uint8))
+    hip.launch_kv_norm_append_paged(dev(bits(x, bf16)), dev(slots), dev(weight), dev(table), dev(positions), pool, tokens, 576, 512, 64, 97, 64, n_pages, EPS,
+                                    half, bf16, None)
+    got = back(pool).reshape(n_pages, -1)[:, :64 * 576].reshape(-1, 576)[:tokens]
+    want, _ = normed(x, weight, None, table, positions, 512, 512, 64, False, half)
+    off = [t for t in range(tokens) if not (got[t] == nearest_codes(want[t, 0])).all()]
+    assert off == []
+
+
 @pytest.mark.parametrize("bf16", [True, False])
 @pytest.mark.parametrize("tokens,kvl,rope,page,half,weighted", [
     (1, 512, 64, 64, False, True), (32, 512, 64, 64, True, True), (777, 512, 64, 48, False, True), (5, 512, 64, 16, False, False),
     (9, 384, 64, 64, True, True), (9, 8, 8, 4, False, True), (6, 960, 64, 64, True, True), (6, 240, 272, 32, True, True),
 ])
-def test_append_against_the_formula_and_the_rule(oracle, tokens, kvl, rope, page, half, weighted, bf16):
-    """Scales and codes within what 32 bits may be off; and exactly the append's rule on the f32 rows of rivoli_norm_rope_rows."""
+def test_append_against_the_formula_and_the_rule(tokens, kvl, rope, page, half, weighted, bf16):
+    """Scales to their rounding, codes the nearest of the quotients, as in 64 bits."""
     width, n_pages = kvl + rope, -(-tokens // page) + 2
     x, weight, _, table, positions = inputs(tokens, tokens, 1, width, kvl, rope, bf16)
     if tokens > 5:
@@ -168,35 +194,24 @@ def test_append_against_the_formula_and_the_rule(oracle, tokens, kvl, rope, page
     if bad_ones:
         slots[4], slots[7], positions[9], slots[11], positions[11] = -1, n_pages * page, 97, -5, -1
     held = rng.integers(0, 256, (n_pages, page * (width + 4)), dtype=np.uint8)
-    pool, bad, rows = dev(held), dzeros(4), dzeros(tokens * width * 4)
+    pool, bad = dev(held), dzeros(4)
     hip.launch_kv_norm_append_paged(dev(bits(x, bf16)), dev(slots), opt(weight), dev(table), dev(positions), pool, tokens, width, kvl, rope, 97,
                                     page, n_pages, EPS, half, bf16, bad)
-    hip.launch_norm_rope_rows(dev(bits(x, bf16)), rows, opt(weight), None, dev(table), dev(positions), None, tokens, 1, width, kvl, kvl, rope, 97,
-                              0, width, width, width, width, 0, EPS, False, half, bf16, False)
     assert back(bad, np.uint32)[0] == (2 if bad_ones else 0)
     got = back(pool).reshape(n_pages, -1)
-    f32_rows = back(rows, np.float32).reshape(tokens, width)
-    want, far = normed(x, weight, None, table, positions, kvl, kvl, rope, False, half)
-    values = np.sort(e4m3_values()[:127])
+    want, _ = normed(x, weight, None, table, positions, kvl, kvl, rope, False, half)
     expect = held.copy()
     for t in range(tokens):
         if not (0 <= slots[t] < n_pages * page and 0 <= positions[t] < 97):
             continue
         pg, off = divmod(int(slots[t]), page)
-        codes, scale_at = got[pg, off * width:(off + 1) * width], slice(page * width + 4 * off, page * width + 4 * off + 4)
+        scale_at = slice(page * width + 4 * off, page * width + 4 * off + 4)
         scale = got[pg, scale_at].view(np.float32)[0]
-        row = f32_rows[t]
-        top = np.float32(np.abs(row).max())
-        assert scale == (top / np.float32(448) if top > 0 else np.float32(1))
-        expect[pg, off * width:(off + 1) * width] = oracle.f32_to_e4m3(row / scale)
+        v = want[t, 0]
+        top = np.abs(v).max() or 448.0
+        assert abs(float(scale) * 448.0 - top) <= F32 * top * (1 + 2.0 ** -20)
+        expect[pg, off * width:(off + 1) * width] = nearest_codes(v)
         expect[pg, scale_at] = np.float32(scale).reshape(1).view(np.uint8)
-        v, f = want[t, 0], far[t, 0] + F32 * np.abs(want[t, 0])
-        assert abs(scale * 448 - np.abs(v).max()) <= f.max() + 4 * F32 * np.abs(v).max() or not np.abs(v).any()
-        # the nearest code of the exact quotient, or one as near but for what the quotient may be off (half a step of the scale and of itself too)
-        q = np.abs(v) / scale
-        at = np.clip(np.searchsorted(values, q), 1, 126)
-        nearest = np.minimum(np.abs(values[at] - q), np.abs(values[at - 1] - q))
-        assert (np.abs(e4m3_values()[codes] - v / scale) <= nearest + 2 * (f / scale + 4 * F32 * q)).all()
     assert (got == expect).all()
 
 
