@@ -149,26 +149,26 @@ __device__ __forceinline__ float logit_of(u64 place) {
     return __uint_as_float(key ^ (key >> 31 ? 0x80000000u : 0xffffffffu));
 }
 
-// N tokens of a row from `at` on (bf16: eight, f32: four), those at `end` and past it as -inf. A row starts on an element.
+// N tokens of a row from `at` on (bf16: eight, f32: four). A row starts on an element. `some`: those at `end` and past it are -inf (one by one, the last there is again for those).
 template <bool BF16>
 struct Logits;
 template <>
 struct Logits<true> {
     static constexpr int N = 8;
     u32x4 v;
-    __device__ __forceinline__ void load(const void* rows, long long row, int at, int end) {
+    __device__ __forceinline__ void load(const void* from, unsigned at) {
         typedef u32x4 words __attribute__((aligned(2)));
-        const uint16_t* const src = static_cast<const uint16_t*>(rows) + row + at;
-        v = u32x4{0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u};
-        if (at + 8 <= end) {
-            v = *reinterpret_cast<const words*>(src);
-        } else {
-            for (int i = 0; i < end - at; ++i) {
-                const uint32_t one = src[i], shift = 16 * (i & 1);
+        v = *reinterpret_cast<const words*>(static_cast<const char*>(from) + 2u * at);
+    }
+    static __device__ __forceinline__ float one(const void* rows, long long at) { return __uint_as_float((uint32_t)static_cast<const uint16_t*>(rows)[at] << 16); }
+    __device__ __forceinline__ void some(const void* rows, long long row, int at, int end) {
+        uint32_t one[N];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] = j == i >> 1 ? (v[j] & ~(0xffffu << shift)) | (one << shift) : v[j];
-            }
-        }
+        for (int i = 0; i < N; ++i) one[i] = static_cast<const uint16_t*>(rows)[row + min(at + i, end - 1)];
+#pragma unroll
+        for (int i = 0; i < N; ++i) one[i] = at + i < end ? one[i] : 0xff80u;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = one[2 * j] | one[2 * j + 1] << 16;
     }
     __device__ __forceinline__ float operator[](int i) const { return i & 1 ? bf16_hi_to_f32(v[i >> 1]) : bf16_lo_to_f32(v[i >> 1]); }
 };
@@ -177,22 +177,31 @@ struct Logits<false> {
     static constexpr int N = 4;
     typedef float f32x4v __attribute__((ext_vector_type(4)));
     f32x4v v;
-    __device__ __forceinline__ void load(const void* rows, long long row, int at, int end) {
+    __device__ __forceinline__ void load(const void* from, unsigned at) {
         typedef f32x4v words __attribute__((aligned(4)));
-        const float* const src = static_cast<const float*>(rows) + row + at;
-        v = f32x4v{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        if (at + 4 <= end) {
-            v = *reinterpret_cast<const words*>(src);
-        } else {
-            for (int i = 0; i < end - at; ++i) {
-                const float one = src[i];
+        v = *reinterpret_cast<const words*>(static_cast<const char*>(from) + 4u * at);
+    }
+    static __device__ __forceinline__ float one(const void* rows, long long at) { return static_cast<const float*>(rows)[at]; }
+    __device__ __forceinline__ void some(const void* rows, long long row, int at, int end) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] = j == i ? one : v[j];
-            }
-        }
+        for (int i = 0; i < N; ++i) v[i] = static_cast<const float*>(rows)[row + min(at + i, end - 1)];
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = at + i < end ? v[i] : -INFINITY;
     }
     __device__ __forceinline__ float operator[](int i) const { return v[i]; }
 };
+// A thread's K of them, `step` apart from `lane` on, out of `all` tokens that begin at `at` (which is the same for all threads). One branch for all of them, and addresses
+// that are a scalar and the lane's: else every load waited for the one before.
+template <bool BF16, int K>
+__device__ __forceinline__ void load_logits(Logits<BF16> (&v)[K], const void* rows, long long row, int at, int lane, int step, int all, int end) {
+    if (at + all <= end) {
+#pragma unroll
+        for (int j = 0; j < K; ++j) v[j].load(static_cast<const char*>(rows) + (row + at + j * step) * (BF16 ? 2 : 4), (unsigned)lane);
+    } else {
+#pragma unroll
+        for (int j = 0; j < K; ++j) v[j].some(rows, row, at + lane + j * step, end);
+    }
+}
 
 // Sums and maxima over a wave, in every lane, by rotations within sixteen lanes and swaps of those rows: no trip through LDS, which a shuffle is.
 template <int CTRL>
@@ -283,8 +292,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_chunk_kernel(const Samp
     const int row = blockIdx.x / a.chunks, c = blockIdx.x - row * a.chunks, tid = threadIdx.x;
     const int first = c * kSampleChunk + N * tid;
     Logits<BF16> raw[kLoads];
-#pragma unroll
-    for (int j = 0; j < kLoads; ++j) raw[j].load(a.logits, (long long)row * a.stride, first + N * j * kSampleThreads, a.vocab);
+    load_logits(raw, a.logits, (long long)row * a.stride, c * kSampleChunk, N * tid, N * kSampleThreads, kSampleChunk, a.vocab);
     const SampleRow r = sample_row(a, row);
     for (int b = tid; b < kSampleBins; b += kSampleThreads) hist[b] = 0;
     if (tid == 0) n_listed[0] = n_listed[1] = all_count = 0, last_bin[0] = last_bin[1] = -1;
@@ -450,8 +458,7 @@ struct Pick {
         constexpr int kLoads = 4;
         for (int from = 0; from < a.vocab; from += kLoads * N * kPickThreads) {
             Logits<BF16> v[kLoads];
-#pragma unroll
-            for (int j = 0; j < kLoads; ++j) v[j].load(a.logits, (long long)row * a.stride, from + N * ((int)threadIdx.x + j * kPickThreads), a.vocab);
+            load_logits(v, a.logits, (long long)row * a.stride, from, N * (int)threadIdx.x, N * kPickThreads, kLoads * N * kPickThreads, a.vocab);
 #pragma unroll 1
             for (int j = 0; j < kLoads; ++j) {
                 Logits<BF16> one = v[0];
@@ -535,48 +542,54 @@ struct Pick {
                 for (int i = 0; i < kEach; ++i) use(p[i], (unsigned)(kWave * i + lane) < n);
             }
         }
-        // the chunks that have more than is listed, by all threads, two of them on their way at once
+        // the chunks that have more than is listed, by all threads, four of them on their way at once
         // (as they are: a NaN is in no range, what counts as the most is in the top bin, past which nothing is: a NaN)
         const float least_x = fmaxf(least_of(r, lo), __uint_as_float(__float_as_uint(-r.most) - 1)), past_x = hi >= grid.top ? __uint_as_float(0x7fc00000u) : least_of(r, hi + 1);
-        constexpr int kChunks = 2, kLoads = kSampleChunk / (N * kPickThreads);
+        constexpr int kChunks = 4, kLoads = kSampleChunk / (N * kPickThreads);
 #pragma unroll 1
         for (int c0 = 0; c0 < a.chunks; c0 += kChunks) {
             u64 of = raw[0];
 #pragma unroll
             for (int w = 1; w < kSampleMaxChunks / kWave; ++w) of = c0 / kWave == w ? raw[w] : of;
             if ((of >> (c0 % kWave) & ((1 << kChunks) - 1)) == 0) continue;
-            Logits<BF16> v[kChunks][kLoads];
-            bool asked[kChunks];
+            Logits<BF16> v[kChunks * kLoads];
+            load_logits(v, a.logits, (long long)row * a.stride, c0 * kSampleChunk, N * (int)threadIdx.x, N * kPickThreads, kChunks * kSampleChunk, a.vocab);
+            // which of a lane's are: a word's first in its top bit; few, mostly, so that those are read again by themselves rather than looked for among registers
+            static_assert(kChunks == 4 && kLoads * N == 16, "two words of two chunks");
+            uint32_t got[2] = {0, 0};
 #pragma unroll
-            for (int k = 0; k < kChunks; ++k) {
-                asked[k] = of >> ((c0 + k) % kWave) & 1;
-                if (asked[k])
-#pragma unroll
-                    for (int j = 0; j < kLoads; ++j)
-                        v[k][j].load(a.logits, (long long)row * a.stride, (c0 + k) * kSampleChunk + N * ((int)threadIdx.x + j * kPickThreads), a.vocab);
+            for (int i = 0; i < kChunks * kLoads * N; ++i) {
+                const float x = v[i / N][i % N];
+                got[i >> 5] = 2 * got[i >> 5] + (x >= least_x && !(x >= past_x) ? 1u : 0u);
             }
 #pragma unroll
-            for (int k = 0; k < kChunks; ++k) {
-                if (!asked[k]) continue;
-                const auto wanted = [&](int i) {
-                    const float x = v[k][i / N][i % N];
-                    return x >= least_x && !(x >= past_x);
-                };
+            for (int w = 0; w < 2; ++w) {
+                const unsigned asked = (unsigned)(of >> ((c0 + 2 * w) % kWave));
+                got[w] &= (asked & 1 ? 0xffff0000u : 0u) | (asked & 2 ? 0xffffu : 0u);
+            }
+            while (__builtin_amdgcn_ballot_w64((got[0] | got[1]) != 0) != 0) {
+                constexpr int kAgain = 4;
+                int index[kAgain];
+                float x[kAgain];
                 unsigned here = 0;
 #pragma unroll
-                for (int i = 0; i < kLoads * N; ++i) here += wanted(i);
+                for (int q = 0; q < kAgain; ++q) {
+                    const int w = got[0] ? 0 : 1;
+                    const uint32_t left = w ? got[1] : got[0];
+                    const int i = 32 * w + (left ? __builtin_clz(left) : 0);
+                    index[q] = left ? (c0 + (i >> 4)) * kSampleChunk + N * ((int)threadIdx.x + ((i & 15) / N) * kPickThreads) + i % N : 0;
+                    here += left ? 1u : 0u;
+                    const uint32_t rest = left & ~(0x80000000u >> (i & 31));
+                    got[0] = w ? 0u : rest, got[1] = w ? rest : got[1];
+                    x[q] = Logits<BF16>::one(a.logits, (long long)row * a.stride + index[q]);
+                }
                 const unsigned before = wave_inclusive_sum(here);
-                if (__builtin_amdgcn_readlane((int)before, 63) == 0) continue;
                 unsigned base = 0;
                 if (lane == 63) base = atomicAdd(&sh.n, before);
-                unsigned at = (unsigned)__builtin_amdgcn_readlane((int)base, 63) + before - here;
+                const unsigned at = (unsigned)__builtin_amdgcn_readlane((int)base, 63) + before - here;
 #pragma unroll
-                for (int i = 0; i < kLoads * N; ++i)
-                    if (wanted(i)) {
-                        const unsigned index = (unsigned)((c0 + k) * kSampleChunk + N * ((int)threadIdx.x + i / N * kPickThreads) + i % N);
-                        if (at < kPickList) sh.list[at] = place_of(logit(r, v[k][i / N][i % N]), index);
-                        ++at;
-                    }
+                for (int q = 0; q < kAgain; ++q)
+                    if ((unsigned)q < here && at + q < kPickList) sh.list[at + q] = place_of(logit(r, x[q]), (unsigned)index[q]);
             }
         }
         lds_barrier();
@@ -971,7 +984,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
     }
     const u64 hits = __builtin_amdgcn_ballot_w64(c >= 0), lasts = __builtin_amdgcn_ballot_w64(last_c >= 0);
     const int lane = hits ? __builtin_ctzll(hits) : 63 - __builtin_clzll(lasts);
-    c = __shfl(hits ? c : last_c, lane, kWave);
+    c = __builtin_amdgcn_readlane(hits ? c : last_c, lane);
     run_c = __shfl(hits ? run_c : run_last, lane, kWave);
     // ---- the token
     constexpr int kEach = kSampleChunk / kPickThreads, N = Logits<BF16>::N;
@@ -979,13 +992,10 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
     u64 m[kEach];
     sum = 0;
     const int from = c * kSampleChunk + kEach * tid;
+    Logits<BF16> v[kEach / N];
+    load_logits(v, a.logits, (long long)row * a.stride, c * kSampleChunk, kEach * tid, N, kSampleChunk, a.vocab);
 #pragma unroll
-    for (int i = 0; i < kEach; i += N) {
-        Logits<BF16> v;
-        v.load(a.logits, (long long)row * a.stride, from + i, a.vocab);
-#pragma unroll
-        for (int j = 0; j < N; ++j) x[i + j] = logit(r, v[j]);
-    }
+    for (int i = 0; i < kEach; ++i) x[i] = logit(r, v[i / N][i % N]);
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
         m[i] = x[i] != -INFINITY && place_of(x[i], (unsigned)(from + i)) >= cut ? mass_of(pick.weight_of(x[i])) : 0;
@@ -1091,8 +1101,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_probs_kernel(const Samp
         return;
     }
     Logits<BF16> v[kLoads];
-#pragma unroll
-    for (int j = 0; j < kLoads; ++j) v[j].load(a.logits, (long long)row * a.stride, c * kSampleChunk + N * (tid + j * kSampleThreads), a.vocab);
+    load_logits(v, a.logits, (long long)row * a.stride, c * kSampleChunk, N * tid, N * kSampleThreads, kSampleChunk, a.vocab);
     make_table(table, r);
     lds_barrier();
 #pragma unroll
