@@ -160,6 +160,7 @@ struct Logits<true> {
         typedef u32x4 words __attribute__((aligned(2)));
         v = *reinterpret_cast<const words*>(static_cast<const char*>(from) + 2u * at);
     }
+    static __device__ __forceinline__ u32x4 none() { return u32x4{0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u}; }
     static __device__ __forceinline__ float one(const void* rows, long long at) { return __uint_as_float((uint32_t)static_cast<const uint16_t*>(rows)[at] << 16); }
     __device__ __forceinline__ void some(const void* rows, long long row, int at, int end) {
         uint32_t one[N];
@@ -181,6 +182,7 @@ struct Logits<false> {
         typedef f32x4v words __attribute__((aligned(4)));
         v = *reinterpret_cast<const words*>(static_cast<const char*>(from) + 4u * at);
     }
+    static __device__ __forceinline__ f32x4v none() { return f32x4v{-INFINITY, -INFINITY, -INFINITY, -INFINITY}; }
     static __device__ __forceinline__ float one(const void* rows, long long at) { return static_cast<const float*>(rows)[at]; }
     __device__ __forceinline__ void some(const void* rows, long long row, int at, int end) {
 #pragma unroll
@@ -190,17 +192,25 @@ struct Logits<false> {
     }
     __device__ __forceinline__ float operator[](int i) const { return v[i]; }
 };
-// A thread's K of them, `step` apart from `lane` on, out of `all` tokens that begin at `at` (which is the same for all threads). One branch for all of them, and addresses
-// that are a scalar and the lane's: else every load waited for the one before.
+// A thread's K of them out of the tokens from `at` on, a piece of the workgroup's `step` tokens after the other, from its own on. Addresses are a scalar and the lane's, and branches
+// are few: with one each, every load waited for the one before. Of the piece with the row's end a lane reads tokens one by one.
 template <bool BF16, int K>
-__device__ __forceinline__ void load_logits(Logits<BF16> (&v)[K], const void* rows, long long row, int at, int lane, int step, int all, int end) {
-    if (at + all <= end) {
+__device__ __forceinline__ void load_logits(Logits<BF16> (&v)[K], const void* rows, long long row, int at, int own, int step, int end) {
+    const int whole = min((end - at) / step, K);  // pieces
+    const auto load = [&](int j, int from) { v[j].load(static_cast<const char*>(rows) + (row + at + from * step) * (BF16 ? 2 : 4), (unsigned)own); };
+    if (whole == K) {
 #pragma unroll
-        for (int j = 0; j < K; ++j) v[j].load(static_cast<const char*>(rows) + (row + at + j * step) * (BF16 ? 2 : 4), (unsigned)lane);
-    } else {
-#pragma unroll
-        for (int j = 0; j < K; ++j) v[j].some(rows, row, at + lane + j * step, end);
+        for (int j = 0; j < K; ++j) load(j, j);
+        return;
     }
+    Logits<BF16> last;
+    last.some(rows, row, at + whole * step + own, end);
+    if (whole > 0) {
+#pragma unroll
+        for (int j = 0; j < K; ++j) load(j, min(j, whole - 1));
+    }
+#pragma unroll
+    for (int j = 0; j < K; ++j) v[j].v = j < whole ? v[j].v : j == whole ? last.v : Logits<BF16>::none();
 }
 
 // Sums and maxima over a wave, in every lane, by rotations within sixteen lanes and swaps of those rows: no trip through LDS, which a shuffle is.
@@ -292,7 +302,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_chunk_kernel(const Samp
     const int row = blockIdx.x / a.chunks, c = blockIdx.x - row * a.chunks, tid = threadIdx.x;
     const int first = c * kSampleChunk + N * tid;
     Logits<BF16> raw[kLoads];
-    load_logits(raw, a.logits, (long long)row * a.stride, c * kSampleChunk, N * tid, N * kSampleThreads, kSampleChunk, a.vocab);
+    load_logits(raw, a.logits, (long long)row * a.stride, c * kSampleChunk, N * tid, N * kSampleThreads, a.vocab);
     const SampleRow r = sample_row(a, row);
     for (int b = tid; b < kSampleBins; b += kSampleThreads) hist[b] = 0;
     if (tid == 0) n_listed[0] = n_listed[1] = all_count = 0, last_bin[0] = last_bin[1] = -1;
@@ -458,7 +468,7 @@ struct Pick {
         constexpr int kLoads = 4;
         for (int from = 0; from < a.vocab; from += kLoads * N * kPickThreads) {
             Logits<BF16> v[kLoads];
-            load_logits(v, a.logits, (long long)row * a.stride, from, N * (int)threadIdx.x, N * kPickThreads, kLoads * N * kPickThreads, a.vocab);
+            load_logits(v, a.logits, (long long)row * a.stride, from, N * (int)threadIdx.x, N * kPickThreads, a.vocab);
 #pragma unroll 1
             for (int j = 0; j < kLoads; ++j) {
                 Logits<BF16> one = v[0];
@@ -553,7 +563,7 @@ struct Pick {
             for (int w = 1; w < kSampleMaxChunks / kWave; ++w) of = c0 / kWave == w ? raw[w] : of;
             if ((of >> (c0 % kWave) & ((1 << kChunks) - 1)) == 0) continue;
             Logits<BF16> v[kChunks * kLoads];
-            load_logits(v, a.logits, (long long)row * a.stride, c0 * kSampleChunk, N * (int)threadIdx.x, N * kPickThreads, kChunks * kSampleChunk, a.vocab);
+            load_logits(v, a.logits, (long long)row * a.stride, c0 * kSampleChunk, N * (int)threadIdx.x, N * kPickThreads, a.vocab);
             // which of a lane's are: a word's first in its top bit; few, mostly, so that those are read again by themselves rather than looked for among registers
             static_assert(kChunks == 4 && kLoads * N == 16, "two words of two chunks");
             uint32_t got[2] = {0, 0};
@@ -993,7 +1003,11 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
     sum = 0;
     const int from = c * kSampleChunk + kEach * tid;
     Logits<BF16> v[kEach / N];
-    load_logits(v, a.logits, (long long)row * a.stride, c * kSampleChunk, kEach * tid, N, kSampleChunk, a.vocab);
+#pragma unroll
+    for (int i = 0; i < kEach; i += N) {
+        if ((c + 1) * kSampleChunk <= a.vocab) v[i / N].load(static_cast<const char*>(a.logits) + ((long long)row * a.stride + c * kSampleChunk + i) * (BF16 ? 2 : 4), (unsigned)(kEach * tid));
+        else v[i / N].some(a.logits, (long long)row * a.stride, from + i, a.vocab);
+    }
 #pragma unroll
     for (int i = 0; i < kEach; ++i) x[i] = logit(r, v[i / N][i % N]);
 #pragma unroll
@@ -1101,7 +1115,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_probs_kernel(const Samp
         return;
     }
     Logits<BF16> v[kLoads];
-    load_logits(v, a.logits, (long long)row * a.stride, c * kSampleChunk, N * tid, N * kSampleThreads, kSampleChunk, a.vocab);
+    load_logits(v, a.logits, (long long)row * a.stride, c * kSampleChunk, N * tid, N * kSampleThreads, a.vocab);
     make_table(table, r);
     lds_barrier();
 #pragma unroll
