@@ -208,6 +208,9 @@ struct SharedNotes {
     }
 };
 
+// Bound by the issue of a tile's instructions as the tree's kernel is (some 4 300 cycles a tile and workgroup; matrix cores half of them): 64 sequences of 16 heads behind 32 768 rows,
+// 8 192 shared tiles in 16 blocks and 544 of their own, 88 us in a run of such calls; 128 of 32 heads behind four prompts of 65 536 470 us, 0.95 PFLOP/s. FEW: up to 64 groups in lanes, looked up without a
+// chain of loads: the last of these calls 487 us with its merge, by bisection 498; one prompt 103.3 and 103.7.
 template <bool RUNS, bool FEW>
 __global__ __launch_bounds__(kTreeThreads, 1) void mla_attend_shared_kernel(const SharedArgs a) {
     __shared__ __attribute__((aligned(1024))) TreeShared shared;
@@ -291,7 +294,7 @@ struct SharedSums {
     }
 };
 
-// Blocks of the sequences' parts, a column of the launch each, that are not whole without others' records: their own, then those of their group's blocks that have their rows.
+// Bound by a chain of reads, the head, notes, then records: 64 sequences behind one prompt 14 us (17 MB fetched, counted), 128 16. Blocks of the sequences' parts, a column of the launch each, that are not whole without others' records: their own, then those of their group's blocks that have their rows.
 __global__ __launch_bounds__(256) void mla_attend_shared_merge_kernel(const SharedArgs a) {
     const SharedNotes notes(a);
     const SharedHead head = *notes.head;
