@@ -29,7 +29,10 @@ constexpr int kSampleMaxVocab = 1 << 21, kSampleMaxChunks = kSampleMaxVocab / kS
 constexpr int kSampleList = 128, kSampleMore = 512, kSampleListed = kSampleList + kSampleMore;
 constexpr int kPickThreads = 512, kPickWaves = kPickThreads / kWave;
 constexpr int kPickList = 8192;            // tokens in LDS
-constexpr int kPickSubs = kPickThreads, kPickFew = 256;
+constexpr int kPickSubs = kPickThreads, kPickFew = 512;
+// Down to so many tokens that may be kept they are put in order, past them the cut is looked for: 64 rows by k 300 32.1 and 36.6 us, 400 33.8 and 37.0, but 480 37.5 and 37.1; where min-p
+// alone cuts, which needs no order, about 300 36.0 and 32.3.
+constexpr unsigned kPickInOrder = 448, kPickInOrderByM = 256;
 // Up to this k a row's histogram has counts alone, and by min-p alone from this m on: 64 rows of 131 072 by k 50 25.5 us, with weights 31.9, by k 2 000 43.7 and 47.9, but by k 3 000
 // 51.2 and 50.6; by m 0.05 30.4 and 36.7, 0.01 36.5 and 42.2, but by 0.002, where rows may keep more than the list holds, 118 and 54.
 constexpr int kCountedK = 2048;
@@ -626,25 +629,38 @@ struct Pick {
         }
     }
     // Up to kPickFew unlike keys, the largest first, with the masses of theirs (a thread has its own key's) and the sums of those up to each. A key's number is
-    // that of the keys above it: a thread compares two of them with a quarter of all.
-    __device__ __forceinline__ void order(int n, u64* keys, u64 mass, u64* sorted, u64* sorted_mass, u64* upto) const {
-        const int tid = threadIdx.x, part = __builtin_amdgcn_readfirstlane(tid >> 7), first = tid & 127;
-        static_assert(kPickThreads == 512 && kPickFew == 256, "two keys a thread, four parts");
-        const int rounds = (n + 31) / 32;
-        if (tid >= n && tid < 32 * rounds) keys[tid] = 0;  // above none
-        if (tid < kPickFew) rank_of(tid) = 0;
-        lds_barrier();
-        const u64 own = tid < n ? keys[tid] : 0, one = keys[min(first, 32 * rounds - 1)], two = keys[min(first + 128, 32 * rounds - 1)];
-        unsigned above_one = 0, above_two = 0;
+    // that of the keys above it: a thread compares two of them, or four where there are more, with a quarter of all.
+    template <int K>
+    __device__ __forceinline__ void count_above(int n, int rounds, const u64* keys) const {
+        const int part = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 7), first = threadIdx.x & 127;
+        u64 its[K];
+        unsigned above[K] = {};
+#pragma unroll
+        for (int i = 0; i < K; ++i) its[i] = keys[min(first + 128 * i, 32 * rounds - 1)];
+#pragma unroll 1
         for (int j = 0; j < rounds; ++j) {
             u64 k[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) k[i] = keys[32 * j + 8 * part + i];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) above_one += k[i] > one, above_two += k[i] > two;
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int t = 0; t < K; ++t) above[t] += k[i] > its[t];
         }
-        if (first < n) atomicAdd(&sh.rank_of[first], above_one);
-        if (first + 128 < n) atomicAdd(&sh.rank_of[first + 128], above_two);
+#pragma unroll
+        for (int i = 0; i < K; ++i)
+            if (first + 128 * i < n) atomicAdd(&sh.rank_of[first + 128 * i], above[i]);
+    }
+    __device__ __forceinline__ void order(int n, u64* keys, u64 mass, u64* sorted, u64* sorted_mass, u64* upto) const {
+        const int tid = threadIdx.x;
+        static_assert(kPickThreads == 512 && kPickFew == 512, "four keys a thread at most, four parts");
+        const int rounds = (n + 31) / 32;
+        if (tid >= n && tid < 32 * rounds) keys[tid] = 0;  // above none
+        sh.rank_of[tid] = 0;
+        lds_barrier();
+        const u64 own = tid < n ? keys[tid] : 0;
+        if (n <= 256) count_above<2>(n, rounds, keys);
+        else count_above<4>(n, rounds, keys);
         lds_barrier();
         if (tid < n) {
             const unsigned at = sh.rank_of[tid];
@@ -652,16 +668,16 @@ struct Pick {
         }
         lds_barrier();
         if (tid < kWave) {
-            u64 m[4], sum = 0;
+            constexpr int kEach = kPickFew / kWave;
+            u64 m[kEach], sum = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) m[i] = 4 * tid + i < n ? sorted_mass[4 * tid + i] : 0, sum += m[i];
+            for (int i = 0; i < kEach; ++i) m[i] = kEach * tid + i < n ? sorted_mass[kEach * tid + i] : 0, sum += m[i];
             u64 run = wave_upto(sum) - sum;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) upto[4 * tid + i] = run += m[i];
+            for (int i = 0; i < kEach; ++i) upto[kEach * tid + i] = run += m[i];
         }
         lds_barrier();
     }
-    __device__ __forceinline__ unsigned& rank_of(int i) const { return sh.rank_of[i]; }
     // The cut among those: the place of the rank-th, or (by mass) of the last whose tokens before it weigh less than `left`; and what they weigh up to
     // it. Places are sorted out by 512 ranges at a time until few are left, which are compared with each other.
     __device__ __forceinline__ void resolve(bool listed, int b_lo, int b_hi, bool by_mass, unsigned rank, u64 left, u64& cut, u64& upto) const {
@@ -867,7 +883,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
         const unsigned deep = depth < kSampleBins ? sh.count[depth] : ~0u;
         const auto count_in = [&](int b) { return b >= kSampleBins ? ~0u : sh.count[b] - (b ? sh.count[b - 1] : 0u); };
         if (deep <= kPickList) pick.gather(grid.least(depth), INT_MAX, lists);
-        if (deep <= kPickFew) {
+        if (deep <= (r.k_on || r.p_on ? kPickInOrder : kPickInOrderByM)) {
             // ---- few: in order, with what they weigh up to each
             const int n = (int)sh.n;
             pick.order(n, sh.list, tid < n ? mass_of(pick.weight_of(logit_of(sh.list[tid]))) : 0, sh.few, sh.few_mass, sh.few_upto);
@@ -878,10 +894,10 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
                 if (t == 0) return true;
                 return (!r.p_on || sh.few_upto[t - 1] < share(total)) && (!r.m_on || pick.weight_of(logit_of(sh.few[t])) >= pick.least);
             };
-            const bool mine_stays = tid < kPickFew && stays(tid);
+            const bool mine_stays = stays(tid);
             if (mine_stays && !stays(tid + 1)) sh.rank = tid + 1, sh.cut = sh.few[tid], sh.before = sh.few_upto[tid];
             // those by their indexes, with their numbers
-            if (mine_stays) sh.list[tid] = (u64)(kSampleMaxVocab - 1 - index_of(sh.few[tid])) << 8 | (u64)tid;
+            if (mine_stays) sh.list[tid] = (u64)(kSampleMaxVocab - 1 - index_of(sh.few[tid])) << 9 | (u64)tid;
             lds_barrier();
             kept = sh.rank;
             const u64 all = sh.before;
@@ -893,7 +909,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
                 const u64 upto = sh.index_upto[tid], before = tid ? sh.index_upto[tid - 1] : 0;
                 // the first whose sum is past the target; where none's is the last
                 if ((double)upto > target ? tid == 0 || !((double)before > target) : upto == all && (tid == 0 || before != all) && !((double)all > target)) {
-                    const u64 p = sh.few[sh.by_index[tid] & 255];
+                    const u64 p = sh.few[sh.by_index[tid] & (kPickFew - 1)];
 #pragma unroll
                     for (int w = 0; w < kPickFew / kWave; ++w) whole_weight += __builtin_bit_cast(double, sh.room[w]);
                     finish((int)index_of(p), kept, (float)log(pick.weight_of(logit_of(p)) / whole_weight), SampleEnd{1.0 / whole_weight, sh.cut, grid.top, (int)index_of(p), 2});
