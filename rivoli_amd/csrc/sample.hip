@@ -77,6 +77,7 @@ struct SampleRow {
     int k;
     float inv_h, most;           // 1 / h; logits count as this at most, and not at all up to minus it
     double a, p, m;              // a = h / T
+    double c[7];                 // a^k / k! in units of 2^-36, from the first on
     __device__ __forceinline__ bool filtered() const { return k_on || p_on || m_on; }
     // Whether the histogram has weights: not where they are asked for of few tokens alone.
     __device__ __forceinline__ bool weighed() const { return k_on ? k > kCountedK : p_on || !m_on || m < kCountedM; }
@@ -91,6 +92,9 @@ __device__ __forceinline__ SampleRow sample_row(const SampleArgs& a, int row) {
     const int e = (int)((__float_as_uint(tf) >> 23) & 0xff) - 127 - 4;  // (tf is a normal number)
     r.inv_h = __uint_as_float((uint32_t)(127 - e) << 23), r.most = fminf(tf * 33554432.0f, FLT_MAX);
     r.a = 1.0 / ((double)tf * (double)r.inv_h);
+    r.c[0] = r.a * kBinOne;
+#pragma unroll
+    for (int k = 1; k < 7; ++k) r.c[k] = r.c[k - 1] * (r.a * (1.0 / (k + 1)));
     r.k = a.top_ks ? a.top_ks[row] : 0;
     r.p = a.top_ps ? (double)a.top_ps[row] : 1.0;
     r.m = a.min_ps ? (double)a.min_ps[row] : 0.0;
@@ -110,13 +114,14 @@ __device__ __forceinline__ float least_of(const SampleRow& r, int b) {
     return t / r.inv_h;
 }
 __device__ __forceinline__ int bin_of(const SampleRow& r, float x) { return (int)floorf(x * r.inv_h); }
-// exp(place in the bin * a), or of a place in eight bins: arguments up to 1/16 to 2^-47, up to 1/2 to 2^-23.
-__device__ __forceinline__ double weight_in(const SampleRow& r, float place) {
-    const double y = (double)place * r.a;
-    double s = 1.0 / 5040;
-    s = __builtin_fma(s, y, 1.0 / 720), s = __builtin_fma(s, y, 1.0 / 120), s = __builtin_fma(s, y, 1.0 / 24);
-    s = __builtin_fma(s, y, 1.0 / 6), s = __builtin_fma(s, y, 0.5), s = __builtin_fma(s, y, 1.0);
-    return __builtin_fma(s, y, 1.0);
+// exp(place in the bin * a), or of a place in eight bins, in units of 2^-36 and rounded to a whole number, above 2^52: arguments up to 1/16 are right to 2^-47, up to 1/2 to 2^-23. Every
+// weight is one of these, so that sums of either kind agree.
+__device__ __forceinline__ double units_in(const SampleRow& r, float place) {
+    const double y = (double)place;
+    double s = r.c[6];
+#pragma unroll
+    for (int k = 5; k >= 0; --k) s = __builtin_fma(s, y, r.c[k]);
+    return __builtin_fma(s, y, kWhole + kBinOne);
 }
 // A histogram by its top bin.
 struct SampleGrid {
@@ -136,8 +141,7 @@ __device__ __forceinline__ void make_table(SampleTable& t, const SampleRow& r) {
         (threadIdx.x < 64 ? t.fine : t.coarse)[threadIdx.x & 63] = v;
     }
 }
-// The same rounded to 2^-36, as a histogram adds it up: every weight is one of these, so that sums of either kind agree.
-__device__ __forceinline__ double rounded_in(const SampleRow& r, float place) { return __builtin_fma(weight_in(r, place), kBinOne, kWhole) - kWhole; }
+__device__ __forceinline__ double rounded_in(const SampleRow& r, float place) { return units_in(r, place) - kWhole; }
 __device__ __forceinline__ u64 mass_of(double weight) { return __builtin_bit_cast(u64, __builtin_fma(weight, kMassOne, kWhole)) - kWholeBits; }
 // A sum of such numbers times a weight: up to 2^63.
 __device__ __forceinline__ u64 scaled(u64 mass, double by) { return (u64)((double)mass * by + 0.5); }
@@ -296,7 +300,7 @@ __device__ __forceinline__ u64 all_most(u64 x, u64* room) {
 // ---- the first launch: a chunk of a row -----------------------------------------------------------------------
 // Its largest logit, its histogram, and a list of its largest logits, bin by bin as many as there is room for.
 // 64 rows of 131 072 in bf16 14.5 us: of a workgroup's 14 000 cycles loads are 2 000, the largest logit 1 500, the histogram 4 000 (with weights 7 000), the lists 5 500. 256 rows in f32
-// 51 us, 2.6 TB/s, the vector units busy for 70 % of them (counted): 42 instructions a logit with weights, 7 of them the exponential's products in 64 bits.
+// 51 us, 2.6 TB/s, the vector units busy for 70 % of them (counted): 40 instructions a logit with weights, 7 of them the exponential's products in 64 bits.
 template <bool BF16>
 __global__ __launch_bounds__(kSampleThreads) void sample_chunk_kernel(const SampleArgs a) {
     __shared__ u64 hist[kSampleListed + kWave];    // its bins or the list, and a lane's spare place
@@ -349,7 +353,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_chunk_kernel(const Samp
             const float place = t - floor_t + (at < kFine ? 0.0f : (float)(b & 7));
             count += (unsigned)__builtin_popcountll(__builtin_amdgcn_ballot_w64(v[i] > -INFINITY));
             atomicAdd(&hist[at < kSampleBins ? at : spare],
-                      __builtin_bit_cast(u64, __builtin_fma(weight_in(r, place), kBinOne, kWhole)) + ((1ull << kCountShift) - kWholeBits));
+                      __builtin_bit_cast(u64, units_in(r, place)) + ((1ull << kCountShift) - kWholeBits));
         }
     } else {
 #pragma unroll
