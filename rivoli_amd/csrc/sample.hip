@@ -873,9 +873,11 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
         }
         sh.count[tid] = count, sh.mass[tid] = mass;
         // the first bins up to which there is enough, none being the tail; the first whose beginning is too light for min-p
-        const bool by_k = r.k_on && (unsigned)r.k < candidates;
+        // (a k of more tokens than there are cuts nothing, but stands for the weights that the histogram has not)
+        const unsigned k = min((unsigned)r.k, candidates);
+        const bool by_k = r.k_on && (k < candidates || !weighed);
         const auto share = [&](u64 of) -> u64 { return max((u64)ceil(r.p * (double)of), 1ull); };
-        if (by_k && count - count_of < (unsigned)r.k && count >= (unsigned)r.k) sh.k_bin = tid;
+        if (by_k && count - count_of < k && count >= k) sh.k_bin = tid;
         if (!by_k && r.p_on && mass - mass_of_bin < share(total) && mass >= share(total)) sh.p_bin = tid;
         const auto light = [&](int i) { return sh.table.of(grid.top - grid.least(i)) < pick.least; };
         if (r.m_on && light(tid) && (tid == 0 || !light(tid - 1))) sh.m_bin = tid;
@@ -892,9 +894,9 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
             const int n = (int)sh.n;
             pick.order(n, sh.list, tid < n ? mass_of(pick.weight_of(logit_of(sh.list[tid]))) : 0, sh.few, sh.few_mass, sh.few_upto);
             // thread t has the t-th
-            if (by_k && r.p_on) total = sh.few_upto[min(n, r.k) - 1];
+            if (by_k && r.p_on) total = sh.few_upto[min(n, (int)k) - 1];
             const auto stays = [&](int t) {
-                if (t >= n || (by_k && t >= r.k)) return false;
+                if (t >= n || (by_k && t >= (int)k)) return false;
                 if (t == 0) return true;
                 return (!r.p_on || sh.few_upto[t - 1] < share(total)) && (!r.m_on || pick.weight_of(logit_of(sh.few[t])) >= pick.least);
             };
@@ -951,7 +953,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
             const u64 ahead = binned ? mass_before(bin) : 0;
             const unsigned k_ahead = binned && bin ? sh.count[bin - 1] : 0;
             u64 upto, its_cut;
-            pick.resolve(whole_list || binned, lo, hi, by_mass, (unsigned)r.k - k_ahead, by_mass ? (want > ahead ? want - ahead : 1) : 0, its_cut, upto);
+            pick.resolve(whole_list || binned, lo, hi, by_mass, k - k_ahead, by_mass ? (want > ahead ? want - ahead : 1) : 0, its_cut, upto);
             cut = max(cut, its_cut);
             if (!by_mass) total = ahead + upto;
             end_bin = min(end_bin, by_mass ? p_bin : k_bin);

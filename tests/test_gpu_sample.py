@@ -115,6 +115,32 @@ def test_none_of_the_arrays_and_rows_that_start_anywhere():
             check(sample(x, None, [5, 0, 70], [0.9] * 3, None, u, bf16, stride=8201, shift=shift, probs=False), x, None, [5, 0, 70], [0.9] * 3, None, u)
 
 
+@pytest.mark.parametrize("kind", ["normal", "steps", "masked"])
+def test_as_many_as_are_put_in_order_and_more(kind):
+    """Numbers of tokens around those at which the rows' kernel goes another way, by k alone, with top-p and with min-p, and by min-p alone."""
+    rng = np.random.default_rng(60 + len(kind))
+    k = [127, 128, 129, 255, 256, 257, 300, 383, 447, 448, 449, 511, 512, 513, 640, 641]
+    n = len(k)
+    x, u = rows(rng, kind, n, 24001, False), rng.random(n).astype(np.float32)
+    for t, p, m in ((0.25, 1.0, 0.0), (1.0, 0.97, 0.0), (1.0, 1.0, 0.01), (3.0, 0.9, 0.05)):
+        check(sample(x, [t] * n, k, [p] * n, [m] * n, u, False), x, [t] * n, k, [p] * n, [m] * n, u)
+    m = [float(f) for f in np.exp(-np.linspace(2, 9, n))]
+    check(sample(x, None, None, None, m, u, False), x, None, None, None, m, u)
+
+
+def test_what_lies_between_rows_of_shares_is_left_alone():
+    rng = np.random.default_rng(61)
+    n, vocab, apart = 4, 8197, 8200
+    x, u = rows(rng, "model", n, vocab, False), dev(rng.random(n).astype(np.float32))
+    k, p = dev(np.array([0, 20, 0, 1], np.int32)), dev(np.array([1, 1, 0.9, 1], np.float32))
+    out, tokens = dzeros(4 * n * apart, 0xEE), dzeros(4 * n)
+    hip.launch_sample_rows(dev(x), None, k, p, None, u, n, vocab, vocab, False, tokens, probs=out, probs_stride=apart,
+                           workspace=dzeros(hip.sample_rows_workspace_bytes(n, vocab)))
+    out = back(out, np.uint32).reshape(n, apart)
+    assert (out[:, vocab:] == 0xEEEEEEEE).all()
+    assert np.abs(out[:, :vocab].copy().view(np.float32).sum(1, dtype=np.float64) - 1).max() < 2.0 ** -20
+
+
 def test_one_row_for_many_draws():
     """Stride 0: how often a token is drawn is its share, u going evenly through [0, 1)."""
     rng = np.random.default_rng(7)
