@@ -17,8 +17,8 @@ namespace rk {
 
 typedef unsigned long long u64;
 
-// Logits are binned on one grid for all of a row: bins of a power of two's width h, 16 to 32 of them to T, so that x / h, its bin and its place in the bin are exact in f32
-// (logits above 2^25 T count as that, those not above -2^25 T are never drawn: bins have 31 bits). A histogram has some 250 bins from its top on (kFine; 8 T and more), then 256 of eight bins each, another 64 T; what lies
+// Logits are binned on one grid for all of a row: bins of a power of two's width h, 16 to 32 of them to T, so that x / h, its bin and its place in the bin are exact in f32, but for
+// logits just below zero, whose place is right to 2^-25 of a bin, their weight to 2^-29 (logits above 2^25 T count as that, those not above -2^25 T are never drawn: bins have 31 bits). A histogram has some 250 bins from its top on (kFine; 8 T and more), then 256 of eight bins each, another 64 T; what lies
 // deeper weighs less than 2^-92 of the top and is a tail that is only counted. Eights begin at multiples of eight, in every histogram of a row, so that histograms
 // of unlike tops add up exactly: the finer ones' bins are parts of the coarser ones'.
 constexpr int kFine = 256, kSampleBins = 512;
