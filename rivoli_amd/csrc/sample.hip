@@ -7,7 +7,7 @@
 //
 // Which tokens are kept and which one is drawn are decided by sums of up to 2^21 weights next to a border, so that weights and sums have more than 32 bits: over 131 072 tokens
 // sums in f32 would move a draw in some hundred. A weight is made in 64 bits and summed as a whole number of 2^-42 of the largest (in a histogram 2^-36 of
-// its bin's least), so that no sum depends on its order and equal calls give equal tokens.
+// its bin's least), so that no sum depends on its order and equal calls give equal tokens; within the chunk that the draw falls into they are summed as they are, in one order.
 #include <cfloat>
 #include <climits>
 
@@ -273,6 +273,19 @@ __device__ __forceinline__ u64 wave_upto(u64 v) {
     v += before64<0x143, 0xc>(v);
     return v;
 }
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ double before_f64(double v) {
+    return __builtin_bit_cast(double, before64<CTRL, ROW_MASK>(__builtin_bit_cast(u64, v)));  // (no bits are a zero)
+}
+__device__ __forceinline__ double wave_upto_f64(double v) {
+    v += before_f64<0x111, 0xf>(v);
+    v += before_f64<0x112, 0xf>(v);
+    v += before_f64<0x114, 0xf>(v);
+    v += before_f64<0x118, 0xf>(v);
+    v += before_f64<0x142, 0xa>(v);
+    v += before_f64<0x143, 0xc>(v);
+    return v;
+}
 // Of a whole workgroup, in every thread.
 template <int WAVES>
 __device__ __forceinline__ u64 all_sum(u64 x, u64* room) {
@@ -447,6 +460,7 @@ struct PickShared {
     double eighth[8];                      // what a bin weighs more than the first of its eight
     u64 room[kPickWaves];
     u64 chunk_mass[kSampleMaxChunks];
+    unsigned light[kSampleMaxChunks / 32];  // a bit of each chunk: it has kept tokens that count nothing
     int top[kSampleMaxChunks], cover[2][kSampleMaxChunks];
     unsigned listed[2][kSampleMaxChunks];  // the first + 1; 0: a chunk without tokens
     unsigned count[kSampleBins + kWave];   // of the bins, then of all up to them
@@ -475,6 +489,11 @@ struct Pick {
     __device__ __forceinline__ double weight_of(float x) const {
         const float t = x * r.inv_h, floor_t = floorf(t);
         return rounded_in(r, t - floor_t) * (sh.table.of(grid.top - (int)floor_t) * (1 / kBinOne));
+    }
+    // The logarithm of a share; past the table, where a weight is none, by the logits themselves.
+    __device__ __forceinline__ float log_share(float x, double weight, double whole, float most) const {
+        if (weight > 0.0) return (float)log(weight / whole);
+        return (float)(((double)x - (double)most) * r.inv_h * r.a - log(whole / weight_of(most)));
     }
     // f(x, index) of all of a row's; then done(first token) after every piece that the workgroup's threads have together: of one chunk.
     template <class F, class D>
@@ -792,6 +811,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
         sh.top[tid] = mine.top, sh.cover[0][tid] = mine.cover[0], sh.cover[1][tid] = mine.cover[1];
         sh.listed[0][tid] = mine.count ? mine.listed[0] + 1 : 0, sh.listed[1][tid] = mine.listed[1];
     }
+    if (tid < kSampleMaxChunks / 32) sh.light[tid] = 0;
     if (tid == 0) sh.n = 0, sh.k_bin = sh.p_bin = sh.m_bin = kSampleBins;
     u64 best = wave_most64(mine.count ? place_of(mine.most, (unsigned)mine.first) : 0);
     unsigned candidates = (unsigned)wave_sum64(mine.count);
@@ -824,7 +844,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
     double whole_weight = 0.0;             // of what is kept, where it is had but as a whole number
     if (!r.filtered()) {
         const double weight = mine.count ? mine.weight * sh.table.of(grid.top - mine.top) : 0.0;
-        if (mine.count) sh.chunk_mass[tid] = (u64)(weight * kMassOne + 0.5);
+        if (mine.count) sh.chunk_mass[tid] = max((u64)(weight * kMassOne + 0.5), 1ull);  // (every chunk that has tokens is found by some u)
         const double of_wave = wave_sum_f64(weight);
         if ((tid & 63) == 0) sh.few[tid >> 6] = __builtin_bit_cast(u64, of_wave);
         lds_barrier();
@@ -913,12 +933,12 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
             if (tid < (int)kept) {
                 const double target = (double)u * (double)all;
                 const u64 upto = sh.index_upto[tid], before = tid ? sh.index_upto[tid - 1] : 0;
-                // the first whose sum is past the target; where none's is the last
-                if ((double)upto > target ? tid == 0 || !((double)before > target) : upto == all && (tid == 0 || before != all) && !((double)all > target)) {
+                // the first whose sum is past the target, by a u of none the first whatever it weighs; where none's is, the last
+                if (u <= 0.0f ? tid == 0 : (double)all > target ? (double)upto > target && !((double)before > target) : tid == (int)kept - 1) {
                     const u64 p = sh.few[sh.by_index[tid] & (kPickFew - 1)];
 #pragma unroll
                     for (int w = 0; w < kPickFew / kWave; ++w) whole_weight += __builtin_bit_cast(double, sh.room[w]);
-                    finish((int)index_of(p), kept, (float)log(pick.weight_of(logit_of(p)) / whole_weight), SampleEnd{1.0 / whole_weight, sh.cut, grid.top, (int)index_of(p), 2});
+                    finish((int)index_of(p), kept, pick.log_share(logit_of(p), pick.weight_of(logit_of(p)), whole_weight, most), SampleEnd{1.0 / whole_weight, sh.cut, grid.top, (int)index_of(p), 2});
                 }
             }
             return;
@@ -963,13 +983,14 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
         // ---- what is kept, by chunk
         unsigned n = 0;
         u64 end = 0;                       // (inverted: the last kept token's place)
-        const auto keep = [&](u64 p) -> u64 {
-            if (p < cut) return 0;
+        const auto keep = [&](u64 p, u64& mass) -> bool {
+            if (p < cut) return false;
             const double w = pick.weight_of(logit_of(p));
-            if (w < pick.least) return 0;
-            ++n, end = max(end, ~p);
-            return mass_of(w);
+            if (w < pick.least) return false;
+            ++n, end = max(end, ~p), mass = mass_of(w);
+            return true;
         };
+        const auto found_light = [&](int c) { atomicOr(&sh.light[c >> 5], 1u << (c & 31)); };
         if (by_bins) {
             // bins in front of the cut's out of the histograms; its own tokens one by one
             if (held != end_bin) pick.gather(grid.least(end_bin), end_bin < kFine ? grid.least(end_bin) : grid.least(end_bin) + 7, lists);
@@ -977,25 +998,37 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
                 if (sh.listed[0][c] == 0) continue;
                 const SampleGrid of(sh.top[c]);
                 u64 sum = 0;
+                bool some = false;
                 for (int i = tid & 63; i < kSampleBins; i += kWave) {
                     const u64 v = a.masses[((size_t)row * a.chunks + c) * kSampleBins + i];
-                    if (v && grid.of(of.least(i)) < end_bin) sum += scaled(v, sh.table.of(grid.top - of.least(i)) * (kMassOne / kBinOne));
+                    const bool in = v && grid.of(of.least(i)) < end_bin;
+                    if (in) sum += scaled(v, sh.table.of(grid.top - of.least(i)) * (kMassOne / kBinOne));
+                    some |= in;
                 }
-                sum = wave_sum64(sum);
+                sum = wave_sum64(sum), some = __builtin_amdgcn_ballot_w64(some) != 0;
                 if ((tid & 63) == 0 && sum) atomicAdd(&sh.chunk_mass[c], sum);
+                if ((tid & 63) == 0 && some && !sum) found_light(c);
             }
         }
         if (whole_list || by_bins) {
             for (unsigned i = tid; i < sh.n; i += kPickThreads) {
-                const u64 m = keep(sh.list[i]);
-                if (m) atomicAdd(&sh.chunk_mass[index_of(sh.list[i]) / kSampleChunk], m);
+                u64 m;
+                if (!keep(sh.list[i], m)) continue;
+                const int c = (int)(index_of(sh.list[i]) / kSampleChunk);
+                if (m) atomicAdd(&sh.chunk_mass[c], m);
+                else found_light(c);
             }
         } else {
             u64 piece = 0;
-            pick.row_each([&](float x, unsigned i) { piece += keep(place_of(x, i)); }, [&](int from) {
-                piece = wave_sum64(piece);
+            bool some = false;
+            pick.row_each([&](float x, unsigned i) {
+                u64 m;
+                if (keep(place_of(x, i), m)) piece += m, some = true;
+            }, [&](int from) {
+                piece = wave_sum64(piece), some = __builtin_amdgcn_ballot_w64(some) != 0;
                 if (piece && (tid & 63) == 0) atomicAdd(&sh.chunk_mass[from / kSampleChunk], piece);
-                piece = 0;
+                if (some && !piece && (tid & 63) == 0) found_light(from / kSampleChunk);
+                piece = 0, some = false;
             });
         }
         kept = (unsigned)all_sum<kPickWaves>(n, sh.room) + (by_bins && end_bin ? sh.count[end_bin - 1] : 0u);
@@ -1003,10 +1036,16 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
         // (none of the cut's bin kept, by min-p: whatever is in the bins in front of it is)
         cut = last ? ~last : place_of(least_of(r, grid.least(end_bin - 1)), kSampleMaxVocab - 1);
     }
-    // ---- the chunk that the draw falls into, in every wave: a lane has four
+    // ---- the chunk that the draw falls into, in every wave: a lane has four. Chunks' masses are other roundings than their tokens': of the bins' sums, or of the
+    // chunk's; and a chunk that has kept tokens counts as one at least, so that the first and the last of them are in the first and the last chunk that counts.
     u64 mass[4], sum = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) mass[i] = sh.chunk_mass[4 * (tid & 63) + i], sum += mass[i];
+    for (int i = 0; i < 4; ++i) {
+        const int c = 4 * (tid & 63) + i;
+        mass[i] = sh.chunk_mass[c];
+        if (mass[i] == 0) mass[i] = sh.light[c >> 5] >> (c & 31) & 1;
+        sum += mass[i];
+    }
     u64 run = wave_upto(sum);
     const u64 all = ((u64)(uint32_t)__builtin_amdgcn_readlane((int)(run >> 32), 63) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)run, 63);
     run -= sum;
@@ -1025,11 +1064,11 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
     const int lane = hits ? __builtin_ctzll(hits) : 63 - __builtin_clzll(lasts);
     c = __builtin_amdgcn_readlane(hits ? c : last_c, lane);
     run_c = __shfl(hits ? run_c : run_last, lane, kWave);
-    // ---- the token
+    // ---- the token: by running sums of the chunk's weights as they are. (As whole numbers, weights below 2^-43 are none: in a chunk of nothing else none was ever past the target.)
     constexpr int kEach = kSampleChunk / kPickThreads, N = Logits<BF16>::N;
     float x[kEach];
-    u64 m[kEach];
-    sum = 0;
+    double w[kEach], own = 0.0;
+    unsigned in = 0;                       // which of a thread's are kept
     const int from = c * kSampleChunk + kEach * tid;
     Logits<BF16> v[kEach / N];
 #pragma unroll
@@ -1041,35 +1080,44 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
     for (int i = 0; i < kEach; ++i) x[i] = logit(r, v[i / N][i % N]);
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-        m[i] = x[i] != -INFINITY && place_of(x[i], (unsigned)(from + i)) >= cut ? mass_of(pick.weight_of(x[i])) : 0;
-        sum += m[i];
+        const bool kept_one = x[i] != -INFINITY && place_of(x[i], (unsigned)(from + i)) >= cut;
+        in |= kept_one ? 1u << i : 0u;
+        w[i] = kept_one ? pick.weight_of(x[i]) : 0.0;
+        own += w[i];
     }
     // the threads' sums in order
-    const u64 upto = wave_upto(sum);
+    const double upto = wave_upto_f64(own);
     lds_barrier();
-    if ((tid & 63) == 63) sh.room[tid >> 6] = upto;
+    if ((tid & 63) == 63) sh.room[tid >> 6] = __builtin_bit_cast(u64, upto);
     lds_barrier();
-    u64 before = run_c + upto - sum;
-    for (int w = 0; w < tid >> 6; ++w) before += sh.room[w];
-    int hit = -1, last = -1;
+    const double lane_before = __shfl(upto, (tid & 63) - 1, kWave);  // (of the first lane: not used)
+    double before = 0.0, whole_chunk = 0.0;
+#pragma unroll
+    for (int i = 0; i < kPickWaves; ++i) {
+        if (i == tid >> 6) before = whole_chunk;
+        whole_chunk += __builtin_bit_cast(double, sh.room[i]);
+    }
+    if ((tid & 63) != 0) before += lane_before;
+    // What a sum has to be past: less than the chunk's own, whichever rounding found the chunk; nothing where u is none, so that the first is drawn whatever it weighs; more than
+    // any where no chunk was past the target.
+    const double past = u <= 0.0f ? -1.0 : hits ? fmin((target - (double)run_c) / kMassOne, whole_chunk * (1.0 - 0x1p-40)) : (double)INFINITY;
+    int hit = -1;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-        if (m[i]) {
-            if (hit < 0 && (double)(before + m[i]) > target) hit = from + i;
-            last = from + i;
-        }
-        before += m[i];
+        before += w[i];
+        if (hit < 0 && (in >> i & 1) && before > past) hit = from + i;
     }
-    // the first hit; where there is none, the last token that weighs
+    const int last = in ? from + 31 - __builtin_clz(in) : -1;
+    // the first hit; where there is none, the last token
     const u64 hit_lanes = __builtin_amdgcn_ballot_w64(hit >= 0), last_lanes = __builtin_amdgcn_ballot_w64(last >= 0);
     const int wave_hit = hit_lanes ? __builtin_amdgcn_readlane(hit, __builtin_ctzll(hit_lanes)) : -1;
     const int wave_last = last_lanes ? __builtin_amdgcn_readlane(last, 63 - __builtin_clzll(last_lanes)) : -1;
     if ((tid & 63) == 0) sh.few[tid >> 6] = (u64)(uint32_t)wave_hit << 32 | (uint32_t)wave_last;
     lds_barrier();
-    int token = -1, last_token = 0;
+    int token = -1, last_token = -1;
 #pragma unroll
-    for (int w = 0; w < kPickWaves; ++w) {
-        const int h = (int)(sh.few[w] >> 32), l = (int)(uint32_t)sh.few[w];
+    for (int i = 0; i < kPickWaves; ++i) {
+        const int h = (int)(sh.few[i] >> 32), l = (int)(uint32_t)sh.few[i];
         if (token < 0) token = h;
         if (l >= 0) last_token = l;
     }
@@ -1084,7 +1132,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
             whole_weight = (double)all / kMassOne;
             if (weight > 0.25 * whole_weight) weight = (double)mass_of(weight) / kMassOne;
         }
-        finish(token, kept, (float)log(weight / whole_weight), SampleEnd{1.0 / whole_weight, cut, grid.top, token, 2});
+        finish(token, kept, pick.log_share(of, weight, whole_weight, most), SampleEnd{1.0 / whole_weight, cut, grid.top, token, 2});
     }
 }
 
@@ -1136,7 +1184,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_probs_kernel(const Samp
             store(c * kSampleChunk + N * (tid + j * kSampleThreads), zeros);
         }
         __syncthreads();                   // the zeros are there before what comes over them
-        if (end.kind == 1 && tid == 0 && end.token / kSampleChunk == c) out[end.token] = 1.0f;
+        if (end.kind == 1 && tid == 0 && (unsigned)end.token < (unsigned)a.vocab && end.token / kSampleChunk == c) out[end.token] = 1.0f;
         if (none) return;
 #pragma unroll
         for (int k = 0; k < kEach; ++k)
