@@ -75,7 +75,7 @@ struct SampleArgs {
 struct SampleRow {
     bool greedy, k_on, p_on, m_on;
     int k;
-    float inv_h, most;           // 1 / h; logits count as this at most, and not at all up to minus it
+    float inv_h, most, cap;      // 1 / h; logits up to minus `most` do not count at all, those above `cap` as that: as `most`, but where the largest is taken, which needs no bins
     double a, p, m;              // a = h / T
     double c[7];                 // a^k / k! in units of 2^-36, from the first on
     __device__ __forceinline__ bool filtered() const { return k_on || p_on || m_on; }
@@ -91,6 +91,7 @@ __device__ __forceinline__ SampleRow sample_row(const SampleArgs& a, int row) {
     const float tf = r.greedy ? 1.0f : fminf(t, FLT_MAX);
     const int e = (int)((__float_as_uint(tf) >> 23) & 0xff) - 127 - 4;  // (tf is a normal number)
     r.inv_h = __uint_as_float((uint32_t)(127 - e) << 23), r.most = fminf(tf * 33554432.0f, FLT_MAX);
+    r.cap = r.greedy ? INFINITY : r.most;
     r.a = 1.0 / ((double)tf * (double)r.inv_h);
     r.c[0] = r.a * kBinOne;
 #pragma unroll
@@ -105,7 +106,7 @@ __device__ __forceinline__ SampleRow sample_row(const SampleArgs& a, int row) {
     return r;
 }
 // A logit as it counts: what is no number, or further down than all that counts, as -inf, which is never drawn.
-__device__ __forceinline__ float logit(const SampleRow& r, float x) { return x > -r.most ? fminf(x, r.most) : -INFINITY; }
+__device__ __forceinline__ float logit(const SampleRow& r, float x) { return x > -r.most ? fminf(x, r.cap) : -INFINITY; }
 
 // The least logit of a bin's, or of one between it and the next that there is.
 __device__ __forceinline__ float least_of(const SampleRow& r, int b) {
