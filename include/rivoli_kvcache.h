@@ -648,8 +648,8 @@ int rivoli_kv_norm_append_paged(const void* x, const int* slot_mapping, const fl
  * top_ks[r] of them (all when not positive); of those the shortest beginning whose weight reaches top_ps[r] of theirs (all when not below 1, one token when not positive); of those the ones
  * whose w_v is min_ps[r] or more (the first always). The four arrays may each be null: temperature 1, all kept. tokens[r] = the first v, by index, whose running sum
  * of kept weights exceeds uniforms[r] times their whole (the last kept one when none does). A temperature that is not above 2^-16 takes the first in the order. Logits that are NaN or not
- * above -2^25 temperatures (the type's lowest value, -inf; -2^25 where the first is taken) are never drawn nor kept. Those above 2^25 temperatures, where f32 numbers lie more than two
- * temperatures apart, count as that, except where the first is taken. A row without any logit that may be drawn gets token -1. n_kept[r] (nullable) = how many are kept, logprobs[r] (nullable) = the logarithm
+ * above -2^25 temperatures (the type's lowest value, -inf; -2^25 where the first is taken) are never drawn nor kept; infinite ones
+ * count as the largest number, but where the first is taken. A row without any logit that may be drawn gets token -1. n_kept[r] (nullable) = how many are kept, logprobs[r] (nullable) = the logarithm
  * of the token's share of their weight (-inf without a token), probs (nullable) + r * probs_stride = every token's share, zero for those not kept: what rivoli_draft_verify takes; not over the logits. Weights are right to
  * 2^-29 of themselves (in sums those below 2^-11 of the largest to 2^-23), and sums count 2^-42 of the largest a token; what is kept and drawn does not depend on any order of sums: equal calls give equal results.
  * `workspace`: rivoli_sample_rows_workspace_bytes(n_rows, vocab) bytes, 16-byte aligned, nothing to be cleared; two calls in flight need one each. Guards: 1001 null / non-positive; 1002 n_rows >= 2^22,

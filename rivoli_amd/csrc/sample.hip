@@ -18,7 +18,8 @@ namespace rk {
 typedef unsigned long long u64;
 
 // Logits are binned on one grid for all of a row: bins of a power of two's width h, 16 to 32 of them to T, so that x / h, its bin and its place in the bin are exact in f32, but for
-// logits just below zero, whose place is right to 2^-25 of a bin, their weight to 2^-29 (logits above 2^25 T count as that, those not above -2^25 T are never drawn: bins have 31 bits). A histogram has some 250 bins from its top on (kFine; 8 T and more), then 256 of eight bins each, another 64 T; what lies
+// logits just below zero, whose place is right to 2^-25 of a bin, their weight to 2^-29 (bins have 31 bits: logits not above -2^25 T are never drawn, and a row that has some above 2^25 T, which lie
+// two T apart and more, is read by itself, by its logits' distances from the largest). A histogram has some 250 bins from its top on (kFine; 8 T and more), then 256 of eight bins each, another 64 T; what lies
 // deeper weighs less than 2^-92 of the top and is a tail that is only counted. Eights begin at multiples of eight, in every histogram of a row, so that histograms
 // of unlike tops add up exactly: the finer ones' bins are parts of the coarser ones'.
 constexpr int kFine = 256, kSampleBins = 512;
@@ -57,6 +58,7 @@ struct SampleEnd {               // what the third launch writes a row's probabi
     u64 cut;                     // the last kept token's place in the order
     int top;                     // the row's top bin
     int token, kind;             // kind: 0 nothing may be drawn, 1 one token, 2 by weight
+    float base;                  // what its logits are taken from before they are binned: its largest in a row past the bins, else zero
 };
 struct SampleArgs {
     const void* logits;
@@ -75,7 +77,7 @@ struct SampleArgs {
 struct SampleRow {
     bool greedy, k_on, p_on, m_on;
     int k;
-    float inv_h, most, cap;      // 1 / h; logits up to minus `most` do not count at all, those above `cap` as that: as `most`, but where the largest is taken, which needs no bins
+    float inv_h, most, cap;      // 1 / h; logits up to minus `most` do not count at all, those above `cap` as that: as `most`, where there are bins
     double a, p, m;              // a = h / T
     double c[7];                 // a^k / k! in units of 2^-36, from the first on
     __device__ __forceinline__ bool filtered() const { return k_on || p_on || m_on; }
@@ -105,7 +107,7 @@ __device__ __forceinline__ SampleRow sample_row(const SampleArgs& a, int row) {
     r.m_on = r.m > 0.0 && r.m <= 1.0;
     return r;
 }
-// A logit as it counts: what is no number, or further down than all that counts, as -inf, which is never drawn.
+// A logit as it counts: what is no number, or further down than all that counts, as -inf, which is never drawn. (An infinite one past the bins: as the largest number.)
 __device__ __forceinline__ float logit(const SampleRow& r, float x) { return x > -r.most ? fminf(x, r.cap) : -INFINITY; }
 
 // The least logit of a bin's, or of one between it and the next that there is.
@@ -114,6 +116,8 @@ __device__ __forceinline__ float least_of(const SampleRow& r, int b) {
     if ((double)t < (double)b) t = __uint_as_float(__float_as_uint(t) + (t < 0.0f ? -1 : 1));
     return t / r.inv_h;
 }
+// A logit in bins from a row's base: near it exact, far below it, where all weigh nothing, held to the bins' range.
+__device__ __forceinline__ float place_in(const SampleRow& r, float x, float base) { return fmaxf(x - base, -r.most) * r.inv_h; }
 __device__ __forceinline__ int bin_of(const SampleRow& r, float x) { return (int)floorf(x * r.inv_h); }
 // exp(place in the bin * a), or of a place in eight bins, in units of 2^-36 and rounded to a whole number, above 2^52: arguments up to 1/16 are right to 2^-47, up to 1/2 to 2^-23. Every
 // weight is one of these, so that sums of either kind agree.
@@ -485,10 +489,11 @@ struct Pick {
     const int row;
     const SampleGrid grid;
     double least;                          // weight that min-p keeps
+    float base;                            // SampleEnd's
     static constexpr int N = Logits<BF16>::N;
     // The weight of a logit, that of the top bin's beginning being one.
     __device__ __forceinline__ double weight_of(float x) const {
-        const float t = x * r.inv_h, floor_t = floorf(t);
+        const float t = place_in(r, x, base), floor_t = floorf(t);
         return rounded_in(r, t - floor_t) * (sh.table.of(grid.top - (int)floor_t) * (1 / kBinOne));
     }
     // The logarithm of a share; past the table, where a weight is none, by the logits themselves.
@@ -782,7 +787,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
     const SampleChunk* const chunks = a.chunk + (size_t)row * a.chunks;
     SampleChunk mine{0, 0, {0, 0}, -INFINITY, 0, 0, {0, 0}};
     if (tid < a.chunks) mine = chunks[tid];
-    const SampleRow r = sample_row(a, row);
+    SampleRow r = sample_row(a, row);
     const float u = a.uniforms[row];
     // What the chunks have left, all on its way before anything is waited for: their histograms' words of the thread's bin, sixteen chunks at once, and their lists.
     constexpr int kAtOnce = 16;
@@ -800,7 +805,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
     typename Pick<BF16>::Lists lists;
     if (asks) {
         words_of(0);
-        const Pick<BF16> early{a, r, sh, row, SampleGrid(0), 0.0};
+        const Pick<BF16> early{a, r, sh, row, SampleGrid(0), 0.0, 0.0f};
 #pragma unroll
         for (int k = 0; k < Pick<BF16>::kEarly; ++k) early.list_of((tid >> 6) + k * kPickWaves, lists.p[k]);
     }
@@ -829,21 +834,30 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
         a.end[row] = end;
     };
     if (candidates == 0) {
-        if (tid == 0) finish(-1, 0, -INFINITY, SampleEnd{0, 0, 0, -1, 0});
+        if (tid == 0) finish(-1, 0, -INFINITY, SampleEnd{0, 0, 0, -1, 0, 0});
         return;
     }
     if (r.greedy) {
-        if (tid == 0) finish((int)index_of(best), 1, 0.0f, SampleEnd{0, 0, 0, (int)index_of(best), 1});
+        if (tid == 0) finish((int)index_of(best), 1, 0.0f, SampleEnd{0, 0, 0, (int)index_of(best), 1, 0});
         return;
     }
-    const float most = logit_of(best);
-    Pick<BF16> pick{a, r, sh, row, SampleGrid(bin_of(r, most)), 0.0};
+    float most = logit_of(best);
+    // Past the bins: the largest logit out of the row, and nothing of what the chunks left but their numbers of tokens.
+    const bool far = most >= r.most;
+    if (far) {
+        r.cap = FLT_MAX;
+        const Pick<BF16> look{a, r, sh, row, SampleGrid(0), 0.0, 0.0f};
+        u64 top = 0;
+        look.row_each([&](float x, unsigned i) { top = max(top, place_of(x, i)); }, [](int) {});
+        most = logit_of(all_most<kPickWaves>(top, sh.room));
+    }
+    Pick<BF16> pick{a, r, sh, row, SampleGrid(far ? 0 : bin_of(r, most)), 0.0, far ? most : 0.0f};
     const SampleGrid& grid = pick.grid;
     if (r.m_on) pick.least = r.m * pick.weight_of(most);
     u64 cut = 0;
     unsigned kept = candidates;
     double whole_weight = 0.0;             // of what is kept, where it is had but as a whole number
-    if (!r.filtered()) {
+    if (!r.filtered() && !far) {
         const double weight = mine.count ? mine.weight * sh.table.of(grid.top - mine.top) : 0.0;
         if (mine.count) sh.chunk_mass[tid] = max((u64)(weight * kMassOne + 0.5), 1ull);  // (every chunk that has tokens is found by some u)
         const double of_wave = wave_sum_f64(weight);
@@ -854,7 +868,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
     } else {
         // ---- the row's histogram
         // (no branches: what has no bin goes to spare ones, a lane's own)
-        for (int c0 = 0;;) {
+        for (int c0 = 0; !far;) {
             // (a chunk's top is a scalar)
             const int top_of = sh.top[min(c0 + (tid & (kAtOnce - 1)), kSampleMaxChunks - 1)];
             const unsigned there_of = sh.listed[0][min(c0 + (tid & (kAtOnce - 1)), kSampleMaxChunks - 1)];
@@ -901,7 +915,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
         if (by_k && count - count_of < k && count >= k) sh.k_bin = tid;
         if (!by_k && r.p_on && mass - mass_of_bin < share(total) && mass >= share(total)) sh.p_bin = tid;
         const auto light = [&](int i) { return sh.table.of(grid.top - grid.least(i)) < pick.least; };
-        if (r.m_on && light(tid) && (tid == 0 || !light(tid - 1))) sh.m_bin = tid;
+        if (r.m_on && !far && light(tid) && (tid == 0 || !light(tid - 1))) sh.m_bin = tid;
         lds_barrier();
         const int k_bin = sh.k_bin, m_bin = sh.m_bin;
         int p_bin = sh.p_bin;
@@ -939,13 +953,18 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
                     const u64 p = sh.few[sh.by_index[tid] & (kPickFew - 1)];
 #pragma unroll
                     for (int w = 0; w < kPickFew / kWave; ++w) whole_weight += __builtin_bit_cast(double, sh.room[w]);
-                    finish((int)index_of(p), kept, pick.log_share(logit_of(p), pick.weight_of(logit_of(p)), whole_weight, most), SampleEnd{1.0 / whole_weight, sh.cut, grid.top, (int)index_of(p), 2});
+                    finish((int)index_of(p), kept, pick.log_share(logit_of(p), pick.weight_of(logit_of(p)), whole_weight, most), SampleEnd{1.0 / whole_weight, sh.cut, grid.top, (int)index_of(p), 2, 0});
                 }
             }
             return;
         }
         // ---- many: the cuts by themselves. From lists of all down to there, or of the cuts' bins alone, or from the row
         const bool whole_list = deep <= kPickList;
+        if (far && r.p_on && !by_k) {
+            u64 of = 0;
+            pick.row_each([&](float x, unsigned) { of += mass_of(pick.weight_of(x)); }, [](int) {});
+            total = all_sum<kPickWaves>(of, sh.room);
+        }
         const auto mass_before = [&](int b) { return b ? sh.mass[b - 1] : 0ull; };
         int held = -1;                     // the bin that the list is of
         bool by_bins = !whole_list && weighed && depth < kSampleBins && (!by_k || count_in(k_bin) <= kPickList);
@@ -1129,11 +1148,11 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(const SampleA
         for (int i = 1; i < kEach; ++i) of = token - from == i ? x[i] : of;
         // (a whole number's last bits are those of its tokens': where one is nearly all of it, as a whole number too)
         double weight = pick.weight_of(of);
-        if (r.filtered()) {
+        if (r.filtered() || far) {
             whole_weight = (double)all / kMassOne;
             if (weight > 0.25 * whole_weight) weight = (double)mass_of(weight) / kMassOne;
         }
-        finish(token, kept, pick.log_share(of, weight, whole_weight, most), SampleEnd{1.0 / whole_weight, cut, grid.top, token, 2});
+        finish(token, kept, pick.log_share(of, weight, whole_weight, most), SampleEnd{1.0 / whole_weight, cut, grid.top, token, 2, pick.base});
     }
 }
 
@@ -1147,16 +1166,18 @@ __global__ __launch_bounds__(kSampleThreads) void sample_probs_kernel(const Samp
     const int row = blockIdx.x / a.chunks, c = blockIdx.x - row * a.chunks, tid = threadIdx.x;
     const SampleEnd end = a.end[row];
     const SampleChunk of = a.chunk[blockIdx.x];
-    const SampleRow r = sample_row(a, row);
+    SampleRow r = sample_row(a, row);
+    const bool far = end.base != 0.0f;     // (the lists and bins are not its logits')
+    if (far) r.cap = FLT_MAX;
     float* const out = a.probs + (long long)row * a.probs_stride;
     const float least = end.cut ? logit_of(end.cut) : -FLT_MAX;
     const int cut_bin = bin_of(r, least);
-    const bool none = end.kind != 2 || of.count == 0 || (end.cut && of.top < cut_bin);
-    const bool listed = none || (end.cut && of.cover[1] <= cut_bin);
+    const bool none = end.kind != 2 || of.count == 0 || (end.cut && !far && of.top < cut_bin);
+    const bool listed = none || (end.cut && !far && of.cover[1] <= cut_bin);
     typedef float f32x4v __attribute__((ext_vector_type(4)));
     typedef f32x4v words __attribute__((aligned(4)));
     const auto probability = [&](float x) {
-        const float t = x * r.inv_h, floor_t = floorf(t);
+        const float t = place_in(r, x, end.base), floor_t = floorf(t);
         return (float)(rounded_in(r, t - floor_t) * (table.of(end.top - (int)floor_t) * (1 / kBinOne)) * end.inv);
     };
     const auto store = [&](int at, const float* p) {
