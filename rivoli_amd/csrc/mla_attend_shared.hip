@@ -208,8 +208,10 @@ struct SharedNotes {
     }
 };
 
-// Bound by the issue of a tile's instructions as the tree's kernel is (some 4 300 cycles a tile and workgroup; matrix cores half of them): 64 sequences of 16 heads behind 32 768 rows,
-// 8 192 shared tiles in 16 blocks and 544 of their own, 88 us in a run of such calls; 128 of 32 heads behind four prompts of 65 536 470 us, 0.95 PFLOP/s. FEW: up to 64 groups in lanes, looked up without a
+// A tile is bound by the issue of its instructions as the tree kernel's is: 4 430 cycles a workgroup, 2 176 of them matrix cores'. Outside of its tiles a workgroup spends another 37 500: groups and
+// parts looked up by dependent loads, again for a further block, q through LDS, the first tile's way, records (both counted, as the slope and the rest of 64 sequences of 16 heads behind
+// 16 384, 32 768 and 65 536 rows: 117, 188 and 330 thousand cycles a wave for 18, 34 and 66 tiles). Of these 32 768 rows, 8 192 shared tiles in 16 blocks and 519 of the sequences' own, it is a fifth of the launch, 88 us in a
+// run of such calls, matrix cores busy for 39 %; 128 of 32 heads behind four prompts of 65 536 470 us, 0.96 PFLOP/s, 204 tiles a workgroup, matrix cores 48 %. FEW: up to 64 groups in lanes, looked up without a
 // chain of loads: the last of these calls 487 us with its merge, by bisection 498; one prompt 103.3 and 103.7.
 template <bool RUNS, bool FEW>
 __global__ __launch_bounds__(kTreeThreads, 1) void mla_attend_shared_kernel(const SharedArgs a) {
@@ -294,7 +296,8 @@ struct SharedSums {
     }
 };
 
-// Bound by a chain of reads, the head, notes, then records: 64 sequences behind one prompt 14 us (17 MB fetched, counted), 128 16. Blocks of the sequences' parts, a column of the launch each, that are not whole without others' records: their own, then those of their group's blocks that have their rows.
+// Bound by a chain of reads, the head, notes, then records: 64 sequences behind one prompt 14 us, 128 16. (Of the records, 34 and 46 MB as the launch before writes them, 17 and 23 MB are fetched, 1.2 and 1.4 TB/s;
+// the rest is still in the dies' second level. Counted.) Blocks of the sequences' parts, a column of the launch each, that are not whole without others' records: their own, then those of their group's blocks that have their rows.
 __global__ __launch_bounds__(256) void mla_attend_shared_merge_kernel(const SharedArgs a) {
     const SharedNotes notes(a);
     const SharedHead head = *notes.head;

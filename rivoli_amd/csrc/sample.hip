@@ -32,10 +32,12 @@ constexpr int kPickThreads = 512, kPickWaves = kPickThreads / kWave;
 constexpr int kPickList = 8192;            // tokens in LDS
 constexpr int kPickSubs = kPickThreads, kPickFew = 512;
 // Down to so many tokens that may be kept they are put in order, past them the cut is looked for: 64 rows by k 300 32.1 and 36.6 us, 400 33.8 and 37.0, but 480 37.5 and 37.1; where min-p
-// alone cuts, which needs no order, about 300 36.0 and 32.3.
+// alone cuts, which needs no order, about 300 36.0 and 32.3. The lines lie there for one row and for 256 too: by k 400 26.6 and 30.6, 61.3 and 64.5, by k 480 28.7 and 29.7, 63.3 and 65.0; by min-p 200
+// 21.8 and 22.8, 55.8 and 57.5, 300 25.5 and 22.9, 59.4 and 57.6 (bf16).
 constexpr unsigned kPickInOrder = 448, kPickInOrderByM = 256;
 // Up to this k a row's histogram has counts alone, and by min-p alone from this m on: 64 rows of 131 072 by k 50 25.5 us, with weights 31.9, by k 2 000 43.7 and 47.9, but by k 3 000
-// 51.2 and 50.6; by m 0.05 30.4 and 36.7, 0.01 36.5 and 42.2, but by 0.002, where rows may keep more than the list holds, 118 and 54.
+// 51.2 and 50.6; by m 0.05 30.4 and 36.7, 0.01 36.5 and 42.2, but by 0.002, where rows may keep more than the list holds, 118 and 54. One row: by k 50 18.7 and 20.8, 2 000 35.7 and 36.7, by m 0.01 18.9 and
+// 21.0; 256 rows: 50.0 and 66.4, 71.8 and 87.5, 51.4 and 67.4 (bf16, a few dozen tokens far above the others: k 3 000 76.0 and 90.6 there).
 constexpr int kCountedK = 2048;
 constexpr double kCountedM = 1.0 / 128;
 constexpr float kLeastTemperature = 1.0f / 65536;  // up to it the largest logit is taken
@@ -459,7 +461,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_chunk_kernel(const Samp
 // Else the bins of the cuts are sorted out by themselves, by 512 ranges of places at a time, from lists of their tokens or, where even a bin has more than the list has room for, from the row.
 // A chain of short steps by one workgroup a row, mostly waits: 13 us for 64 rows of 16 chunks that keep a few (30 000 cycles: what the chunks left 4 500, their histograms added up 6 500,
 // the lists' tokens 5 000, the two orders 7 000), 25 for a thousand by their order in the list, 37 to 50 for thousands by top-p (a bin's tokens from the row 25 000 cycles, the cut 13 000, the
-// draw 13 000). Rows whose bins have more than the list holds (131 072 logits within a hundredth of the temperature) 230 and more: they are read again for each of some four cuts.
+// draw 13 000). Rows past the bins are read from the first token on for their largest, for each cut and for what is kept: one of 131 072 111 to 640 us. Rows whose bins have more than the list holds (131 072 logits within a hundredth of the temperature) 230 and more: they are read again for each of some four cuts.
 struct PickShared {
     SampleTable table;
     double eighth[8];                      // what a bin weighs more than the first of its eight
