@@ -81,3 +81,26 @@ def test_rows_in_front_of_each_other_write_their_own():
         first = [np.nonzero(np.isfinite(r))[0][0] for r in x]
         for r in range(len(x)):
             assert u[r] != 0.0 or tokens[r] == first[r]
+
+
+@pytest.mark.parametrize("first", [True, False])
+def test_the_longest_rows(first):
+    """2^21 tokens, each next to nothing, half a millionth together: the last numbers in front of one are theirs where they come last."""
+    vocab, gap = 2 ** 21, 29.0
+    u = [0.0, 2.0 ** -33, 0.5, 1 - 2.0 ** -22, 1 - 2.0 ** -23, 1 - 2.0 ** -24, 1.0]
+    x = np.full((len(u), vocab), -gap, np.float32)
+    top = 0 if first else vocab - 1
+    x[:, top] = 0.0
+    tokens, kept, logprobs, _ = sample(x, None, None, None, None, u, False, probs=False)
+    w = np.exp(-np.longdouble(gap))
+    whole = 1 + (vocab - 1) * w
+    assert (kept == vocab).all()
+    for token, number, logprob in zip(tokens, u, logprobs):
+        assert abs(logprob - (float(token != top) * -gap - float(np.log(whole)))) <= F32 * gap + 2.0 ** -29
+        if number in (0.0, 1.0):
+            assert token == (0 if number == 0.0 else vocab - 1)
+        else:
+            # 2^-42 a chunk, 2^-23 of what lies in bins, in tokens of w; where the first outweighs them, it is drawn
+            exact = (np.longdouble(number) * whole - (1 if first else 0)) / w
+            far = float((256 * 2.0 ** -42 + 2.0 ** -23 * vocab * w) / w) + 1
+            assert token == top if exact < 0 or exact >= vocab else abs(float(token - exact)) <= far
